@@ -235,6 +235,125 @@ typedef struct {
 M4_API int m4_bridge_projection_plan(int format, uint32_t M, uint32_t K, const uint32_t* N, uint32_t groups, int swiglu,
                                      m4_projection_plan_t* plan);
 
+/* ---- serving: a paged, quantized KV cache, read and written by batches of
+ *      sequences of any lengths.  No counterpart in the reference, whose cache
+ *      is one prompt's ([Hkv, M, D] Q8_0 blocks).  All buffers are device
+ *      memory of the stream's device; nothing is staged, allocated or waited
+ *      for, so every call can be captured into a graph. ------------------- */
+
+/* A cache of num_pages pages of page_size tokens (16, 32, 64, 128 or 256),
+ * Hkv heads, D = 64 or 128, in format QUANT_Q8_0 (6) or QUANT_Q4_0 (0), one
+ * fp16 scale per 32 dims of a token.  A page holds, for each head, K codes
+ * [page_size][D], V codes [page_size / 4][D][4 tokens], K scales
+ * [page_size][D / 32], V scales [page_size / 4][D / 32][4 tokens].  Q8_0 codes
+ * are stored plus 128; of Q4_0 codes a byte holds two dims: of K, byte 4 m + i
+ * dims 8 m + i (low) and 8 m + 4 + i, of V dims 2 x (low) and 2 x + 1.  Values are
+ * half(q * half(d)) and half((c - 8) * half(d)), as in the router's blocks.
+ * `pages` 16-byte aligned, at least m4_bridge_kv_cache_bytes. */
+typedef struct {
+    void* pages;
+    size_t bytes;
+    int format;
+    uint32_t num_pages, page_size, Hkv, D;
+} m4_kv_cache_t;
+
+/* B sequences.  The T rows of a call's Q, K, V and O are the sequences' new
+ * tokens: rows q_start[b] .. q_start[b + 1] (int32 [B + 1], not decreasing) are
+ * the last keys of sequence b, which has kv_len[b] (int32 [B]) keys with them:
+ * row i of n has position kv_len[b] - n + i.  Position p is token p % page_size
+ * of page page_table[b][p / page_size] (int32 [B][table_stride], table_pages of
+ * a row used).  All three are device memory, read by the kernels: entries out
+ * of range (a page that is not there, more keys than the table holds, a
+ * negative position, rows past T) are never followed -- such a token is not
+ * written and not seen.  Rows behind the last sequence are left as they are.
+ * Two tokens of a call that fall on one place of the cache leave it undefined.
+ * max_new and max_kv are what the caller expects of the longest sequence: they
+ * choose kernels and the size of a workspace; the results hold for any. */
+typedef struct {
+    uint32_t B, T;
+    const int32_t *q_start, *kv_len, *page_table;
+    uint32_t table_pages, table_stride;
+    uint32_t max_new, max_kv;
+} m4_kv_batch_t;
+
+/* fp16 rows [T][heads][D]: element strides of a token and of a head (multiples
+ * of 8; rows of an output must not overlap), D contiguous, 16-byte aligned.
+ * `bytes` is what the buffer holds from ptr on. */
+typedef struct {
+    void* ptr;
+    size_t bytes;
+    int64_t token_stride, head_stride;
+} m4_rows_t;
+
+/* Rotary positions with several axes (time, height, width): pair i of `pairs`
+ * (a multiple of 8, at most 128) turns by positions[pair_axis[i]][token] *
+ * inv_freq[i]; pairs are dims (i, i + pairs), or (2 i, 2 i + 1) when
+ * traditional; dims from 2 * pairs on stay.  Angles keep their precision at any
+ * int32 position. */
+enum { M4_ROPE_MAX_PAIRS = 128 };
+typedef struct {
+    uint32_t pairs, axes;
+    int traditional;
+    uint8_t pair_axis[M4_ROPE_MAX_PAIRS];
+    double inv_freq[M4_ROPE_MAX_PAIRS];
+} m4_rope_axes_t;
+
+/* Bytes of a cache, 0 for a format or dimension that it does not take. */
+M4_API size_t m4_bridge_kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D);
+
+/* Rotates the rows X [T][H][D] (D % 8 == 0, at most 256) into Y, which may be X
+ * itself; positions int32 [axes][position_stride].  Codes: -1, -2 (null,
+ * misaligned, short or not device memory), -4 (dims, strides), -6.  T = 0 is 0. */
+M4_API int m4_bridge_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
+                               const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D);
+
+/* Writes the batch's rows of K and V [T][Hkv][D] to the cache, quantized as
+ * m4_bridge_quantize_kv_q8_0 does (Q8_0) or with d = m / -8 of the value m of
+ * largest magnitude, code floor(x / d + 8.5) (Q4_0).  With `rope`, K is rotated
+ * first, and so are the rows Q [T][H][D] into Q_out (may be Q), in the same
+ * launch; positions NULL with one axis: each token's place in its sequence.
+ * The results are those of m4_bridge_rope_axes followed by a write.  Rows of Q
+ * whose token has no place in the cache are left.  rope NULL: Q must be NULL.
+ * Codes as m4_bridge_rope_axes, and -3 (format). */
+M4_API int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                                     const m4_rows_t* V, const m4_rope_axes_t* rope, const int32_t* positions,
+                                     uint32_t position_stride, const m4_rows_t* Q, const m4_rows_t* Q_out, uint32_t H);
+
+/* The inverse: the values of the batch's rows into K and V [T][Hkv][D] fp16
+ * (with q_start the running sum of kv_len, whole sequences).  Rows that have no
+ * place in the cache are left. */
+M4_API int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                                   const m4_rows_t* V);
+
+/* Causal attention of the batch's rows Q [T][H][D] over the cached keys of their
+ * sequences (their own included: append first), O [T][H][D]: query head h reads
+ * KV head h / (H / Hkv); a row at position p sees keys up to p, and with `window`
+ * > 0 only the last `window` of them.  A row that sees no key, or none that
+ * scores above -infinity, is zero.  Any number of rows a sequence, from one
+ * decoded token to a prompt.  `ws`: m4_bridge_paged_attn_workspace bytes of
+ * device memory, 16-byte aligned, whose contents do not matter; calls that may
+ * run at the same time need one each.  scale finite.  Codes as above. */
+M4_API size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t H,
+                                             uint32_t window);
+M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
+                                         const m4_rows_t* O, uint32_t H, float scale, uint32_t window, void* ws,
+                                         size_t ws_bytes);
+
+/* Validation only, as m4_bridge_validate_gemm: the code that the call would
+ * return on an initialized bridge (0 if it would launch) but for the check that
+ * the pointers are device memory. */
+M4_API int m4_bridge_validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
+                                        const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D);
+M4_API int m4_bridge_validate_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch,
+                                              const m4_rows_t* K, const m4_rows_t* V, const m4_rope_axes_t* rope,
+                                              const int32_t* positions, uint32_t position_stride, const m4_rows_t* Q,
+                                              const m4_rows_t* Q_out, uint32_t H);
+M4_API int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                                            const m4_rows_t* V);
+M4_API int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
+                                         const m4_rows_t* O, uint32_t H, float scale, uint32_t window, const void* ws,
+                                         size_t ws_bytes);
+
 /* Run subsequent work on `stream` (a hipStream_t, e.g. torch's current
  * stream); NULL restores the bridge's own stream.  Returns 0 or -1. */
 M4_API int m4_bridge_set_stream(void* stream);

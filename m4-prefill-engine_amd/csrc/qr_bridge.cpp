@@ -12,6 +12,7 @@
 #include <unistd.h>
 
 #include <cerrno>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -22,6 +23,7 @@
 #include "qr_formats.h"
 #include "qr_host.h"
 #include "qr_kernels.h"
+#include "qr_paged.h"
 #include "qr_registry.h"
 
 namespace {
@@ -372,6 +374,85 @@ constexpr size_t kScratchFloats = (size_t)8 << 20;
 static __device__ __align__(256) float scratch[kScratchFloats];
 constexpr int kMaxDevices = 64;
 float* g_scratch[kMaxDevices] = {};
+
+// ---- serving entry points: device memory only ----
+
+// Makes the stream's device current for a launch, and the caller's again after.
+struct OnStreamDevice {
+    int stream_dev = 0, before = 0;
+    OnStreamDevice() {
+        (void)hipGetDevice(&before);
+        stream_dev = before;
+        hipDevice_t d;
+        if (hipStreamGetDevice(g_stream, &d) == hipSuccess) stream_dev = (int)d;
+        else (void)hipGetLastError();
+        if (stream_dev != before) (void)hipSetDevice(stream_dev);
+    }
+    ~OnStreamDevice() {
+        if (stream_dev != before) (void)hipSetDevice(before);
+    }
+    // memory that kernels on the stream may use as it is
+    bool owns(const void* p) const {
+        hipPointerAttribute_t a;
+        if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+            (void)hipGetLastError();
+            return false;
+        }
+        if (a.type == hipMemoryTypeManaged) return true;
+        return a.type == hipMemoryTypeDevice && a.device == stream_dev;
+    }
+    template <typename... P>
+    bool owns_all(const P*... p) const {
+        if ((true && ... && owns(p))) return true;
+        g_last_error = "a buffer is not memory of the stream's device";
+        return false;
+    }
+};
+
+qr::RowsView rows_view(const m4_rows_t* r) {
+    return {static_cast<_Float16*>(r->ptr), r->token_stride, r->head_stride};
+}
+
+qr::BatchView batch_view(const m4_kv_batch_t* b) {
+    return {b->B, b->T, b->q_start, b->kv_len, b->page_table, b->table_pages, b->table_stride};
+}
+
+qr::PageGeom cache_geom(const m4_kv_cache_t* c) {
+    return qr::page_geom(c->pages, c->format, c->num_pages, c->page_size, c->Hkv, c->D);
+}
+
+// Frequencies in turns, as 64-bit fractions of one: whole turns per position
+// drop out because positions are whole.
+void rope_table(const m4_rope_axes_t* r, const int32_t* positions, uint32_t stride, qr::RopeTable& t) {
+    t.pairs = r->pairs;
+    t.traditional = r->traditional ? 1 : 0;
+    t.positions = positions;
+    t.position_stride = stride;
+    for (uint32_t i = 0; i < r->pairs; i++) {
+        const long double turns = (long double)r->inv_freq[i] / 6.283185307179586476925286766559006L;
+        t.turn[i] = (uint64_t)((turns - floorl(turns)) * 18446744073709551616.0L);
+        t.axis[i] = r->pair_axis[i];
+    }
+}
+
+qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, uint32_t H, uint32_t window) {
+    qr::PagedAttnParams p{};
+    p.H = H;
+    p.D = c->D;
+    p.format = c->format;
+    p.window = window;
+    p.geom = cache_geom(c);
+    p.batch = batch_view(b);
+    p.max_new = b->max_new;
+    p.max_kv = b->max_kv;
+    return p;
+}
+
+int launched(hipError_t e, const char* what) {
+    if (e == hipSuccess) return 0;
+    set_error(what, e);
+    return -6;
+}
 
 }  // namespace
 
@@ -808,6 +889,125 @@ int m4_bridge_rope(void* T, size_t Tb, uint32_t H, uint32_t M, uint32_t D, float
     hipError_t e = qr::launch_rope(static_cast<_Float16*>(dt), H, M, D, theta, offset, traditional, g_stream);
     if (e != hipSuccess) set_error("rope", e);
     return finish(e != hipSuccess ? -6 : 0);
+}
+
+size_t m4_bridge_kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D) {
+    return qr::kv_cache_bytes(format, num_pages, page_size, Hkv, D);
+}
+
+int m4_bridge_validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
+                                 const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D) {
+    bool empty;
+    return qr::validate_rope_axes(rope, positions, position_stride, X, Y, T, H, D, &empty);
+}
+
+int m4_bridge_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
+                        const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_rope_axes(rope, positions, position_stride, X, Y, T, H, D, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(positions, X->ptr, Y->ptr)) return -2;
+    qr::AppendParams p{};
+    p.Q = rows_view(X);
+    p.Qo = rows_view(Y);
+    p.H = H;
+    p.T = T;
+    p.D = D;
+    rope_table(rope, positions, position_stride, p.rope);
+    return launched(qr::launch_kv_append(p, g_stream), "rope_axes");
+}
+
+int m4_bridge_validate_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                                       const m4_rows_t* V, const m4_rope_axes_t* rope, const int32_t* positions,
+                                       uint32_t position_stride, const m4_rows_t* Q, const m4_rows_t* Q_out,
+                                       uint32_t H) {
+    bool empty;
+    return qr::validate_append(cache, batch, K, V, rope, positions, position_stride, Q, Q_out, H, &empty);
+}
+
+int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                              const m4_rows_t* V, const m4_rope_axes_t* rope, const int32_t* positions,
+                              uint32_t position_stride, const m4_rows_t* Q, const m4_rows_t* Q_out, uint32_t H) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_append(cache, batch, K, V, rope, positions, position_stride, Q, Q_out, H, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, K->ptr, V->ptr)) return -2;
+    if (rope && positions && !dev.owns_all(positions)) return -2;
+    if (Q && !dev.owns_all(Q->ptr, Q_out->ptr)) return -2;
+    qr::AppendParams p{};
+    p.K = rows_view(K);
+    p.V = rows_view(V);
+    if (Q) {
+        p.Q = rows_view(Q);
+        p.Qo = rows_view(Q_out);
+        p.H = H;
+    }
+    p.T = batch->T;
+    p.D = cache->D;
+    p.format = cache->format;
+    p.geom = cache_geom(cache);
+    p.batch = batch_view(batch);
+    if (rope) rope_table(rope, positions, position_stride, p.rope);
+    return launched(qr::launch_kv_append(p, g_stream), "kv_cache_append");
+}
+
+int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                                     const m4_rows_t* V) {
+    bool empty;
+    return qr::validate_read(cache, batch, K, V, &empty);
+}
+
+int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+                            const m4_rows_t* V) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_read(cache, batch, K, V, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, K->ptr, V->ptr)) return -2;
+    const qr::ReadParams p{rows_view(K), rows_view(V), cache->D, cache->format, cache_geom(cache), batch_view(batch)};
+    return launched(qr::launch_kv_read(p, g_stream), "kv_cache_read");
+}
+
+size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t H,
+                                      uint32_t window) {
+    if (!cache || !batch || H == 0 || cache->Hkv == 0 || H % cache->Hkv || (cache->D != 64 && cache->D != 128)) return 0;
+    return qr::paged_attn_workspace(attn_params(cache, batch, H, window));
+}
+
+int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
+                                  const m4_rows_t* O, uint32_t H, float scale, uint32_t window, const void* ws,
+                                  size_t ws_bytes) {
+    bool empty;
+    const int rc = qr::validate_attn(cache, batch, Q, O, H, scale, ws, &empty);
+    if (rc || empty) return rc;
+    return ws_bytes < m4_bridge_paged_attn_workspace(cache, batch, H, window) ? -2 : 0;
+}
+
+int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
+                                  const m4_rows_t* O, uint32_t H, float scale, uint32_t window, void* ws,
+                                  size_t ws_bytes) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_attn(cache, batch, Q, O, H, scale, ws, &empty);
+    if (rc || empty) return rc;
+    qr::PagedAttnParams p = attn_params(cache, batch, H, window);
+    if (ws_bytes < qr::paged_attn_workspace(p)) return -2;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, Q->ptr, O->ptr, ws)) return -2;
+    p.Q = rows_view(Q);
+    p.O = rows_view(O);
+    p.scale = scale;
+    p.ws = static_cast<uint8_t*>(ws);
+    return launched(qr::launch_paged_attn(p, g_stream), "paged_attn");
 }
 
 void m4_bridge_synchronize(void) {

@@ -7,6 +7,7 @@
 #include <unistd.h>
 
 #include <cerrno>
+#include <cmath>
 
 namespace qr {
 
@@ -93,6 +94,135 @@ int validate(const void* X, size_t Xb, const void* W, size_t Wb, const void* Y, 
     if (format == qr::QUANT_MLX_4BIT_G64 && (K % 64)) return -4;
     if (Xb < (size_t)M * K * 2 || Yb < (size_t)M * N * 2 || Wb < qr::kernel_weight_bytes(format, K, N))
         return -2;
+    return 0;
+}
+
+// ---- serving: paged cache, batches, rows, rotary tables ----
+
+size_t kv_cache_bytes(int format, uint32_t num_pages, uint32_t P, uint32_t Hkv, uint32_t D) {
+    if (format != QUANT_Q8_0 && format != QUANT_Q4_0) return 0;
+    if (P < 16 || P > 256 || (P & (P - 1)) || (D != 64 && D != 128)) return 0;
+    if (num_pages == 0 || num_pages > 0x7fffffffu || Hkv == 0 || Hkv > 0xffffu) return 0;
+    const size_t row = (size_t)D / 32 * get_quant_info(static_cast<QuantFormat>(format)).block_bytes;
+    return 2 * row * P * Hkv * num_pages;  // at most 2^9 * 2^8 * 2^16 * 2^31 bytes
+}
+
+namespace {
+
+bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+int check_cache(const m4_kv_cache_t* c) {
+    if (!c) return -2;
+    if (c->format != QUANT_Q8_0 && c->format != QUANT_Q4_0) return -3;
+    const size_t need = kv_cache_bytes(c->format, c->num_pages, c->page_size, c->Hkv, c->D);
+    if (need == 0) return -4;
+    if (!c->pages || misaligned(c->pages, 16) || c->bytes < need) return -2;
+    return 0;
+}
+
+// B = 0 or T = 0: no rows, and no pointers needed.
+int check_batch(const m4_kv_batch_t* b, bool* empty) {
+    if (!b) return -2;
+    if (b->B > 0x7fffffffu || b->T > 0x7fffffffu) return -4;
+    *empty = b->B == 0 || b->T == 0;
+    if (*empty) return 0;
+    if (!b->q_start || !b->kv_len || !b->page_table) return -2;
+    if (misaligned(b->q_start, 4) || misaligned(b->kv_len, 4) || misaligned(b->page_table, 4)) return -2;
+    if (b->table_pages == 0 || (b->B > 1 && b->table_stride < b->table_pages)) return -4;
+    return 0;
+}
+
+int check_rows(const m4_rows_t* r, uint32_t T, uint32_t heads, uint32_t D, bool out) {
+    if (!r || !r->ptr || misaligned(r->ptr, 16)) return -2;
+    const int64_t ts = r->token_stride, hs = r->head_stride;
+    if (ts < 0 || hs < 0 || ts % 8 || hs % 8) return -4;
+    if (out) {
+        const bool t_inner = T > 1 && (heads <= 1 || ts < hs);
+        const __int128 inner = t_inner ? ts : hs, outer = t_inner ? hs : ts;
+        const uint32_t n_in = t_inner ? T : heads, n_out = t_inner ? heads : T;
+        if (n_in > 1 && inner < D) return -4;
+        if (n_out > 1 && outer < (n_in > 1 ? inner * (n_in - 1) : 0) + D) return -4;
+    }
+    const __int128 last = (__int128)(T - 1) * ts + (__int128)(heads - 1) * hs + D;
+    if ((__int128)r->bytes < last * 2) return -2;
+    return 0;
+}
+
+int check_rope(const m4_rope_axes_t* r, uint32_t D) {
+    if (r->pairs == 0 || r->pairs > M4_ROPE_MAX_PAIRS || r->pairs % 8 || 2 * r->pairs > D || r->axes == 0) return -4;
+    for (uint32_t i = 0; i < r->pairs; i++)
+        if (r->pair_axis[i] >= r->axes || !std::isfinite(r->inv_freq[i])) return -4;
+    return 0;
+}
+
+int check_positions(const int32_t* positions, uint32_t stride, uint32_t axes, uint32_t T) {
+    if (misaligned(positions, 4)) return -2;
+    return axes > 1 && stride < T ? -4 : 0;
+}
+
+}  // namespace
+
+int validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t stride, const m4_rows_t* X,
+                       const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D, bool* empty) {
+    *empty = false;
+    if (!rope || !X || !Y) return -2;
+    if (H == 0 || H > 0xffffu || D == 0 || D % 8 || D > 256 || T > 0x7fffffffu) return -4;
+    if (int rc = check_rope(rope, D)) return rc;
+    if (T == 0) {
+        *empty = true;
+        return 0;
+    }
+    if (!positions) return -2;
+    if (int rc = check_positions(positions, stride, rope->axes, T)) return rc;
+    if (int rc = check_rows(X, T, H, D, false)) return rc;
+    return check_rows(Y, T, H, D, true);
+}
+
+int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+                    const m4_rope_axes_t* rope, const int32_t* positions, uint32_t stride, const m4_rows_t* Q,
+                    const m4_rows_t* Q_out, uint32_t H, bool* empty) {
+    *empty = false;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(batch, empty)) return rc;
+    if (Q && (!rope || !Q_out)) return -2;
+    if (Q && (H == 0 || H > 0xffffu)) return -4;
+    if (rope) {
+        if (int rc = check_rope(rope, cache->D)) return rc;
+        if (!positions && rope->axes > 1) return -2;
+    }
+    if (*empty) return 0;
+    if (rope && positions)
+        if (int rc = check_positions(positions, stride, rope->axes, batch->T)) return rc;
+    if (int rc = check_rows(K, batch->T, cache->Hkv, cache->D, false)) return rc;
+    if (int rc = check_rows(V, batch->T, cache->Hkv, cache->D, false)) return rc;
+    if (Q) {
+        if (int rc = check_rows(Q, batch->T, H, cache->D, false)) return rc;
+        if (int rc = check_rows(Q_out, batch->T, H, cache->D, true)) return rc;
+    }
+    return 0;
+}
+
+int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+                  bool* empty) {
+    *empty = false;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(batch, empty)) return rc;
+    if (*empty) return 0;
+    if (int rc = check_rows(K, batch->T, cache->Hkv, cache->D, true)) return rc;
+    return check_rows(V, batch->T, cache->Hkv, cache->D, true);
+}
+
+int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q, const m4_rows_t* O,
+                  uint32_t H, float scale, const void* ws, bool* empty) {
+    *empty = false;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(batch, empty)) return rc;
+    if (H == 0 || H > 0xffffu || H % cache->Hkv || !std::isfinite(scale)) return -4;
+    if (*empty) return 0;
+    if ((uint64_t)batch->T * (H / cache->Hkv) > 0x7fffffffu) return -4;  // rows of a KV head are counted in 32 bits
+    if (int rc = check_rows(Q, batch->T, H, cache->D, false)) return rc;
+    if (int rc = check_rows(O, batch->T, H, cache->D, true)) return rc;
+    if (!ws || misaligned(ws, 16)) return -2;
     return 0;
 }
 

@@ -3,6 +3,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/m4_mlx_bridge.h"
 #include "qr_formats.h"
 
 namespace qr {
@@ -20,5 +21,18 @@ bool has_kernels(int f);
 // check); `ext` widens the format range to every format with kernels.
 int validate(const void* X, size_t Xb, const void* W, size_t Wb, const void* Y, size_t Yb, int format,
              uint32_t M, uint32_t K, uint32_t N, bool ext = false);
+
+// Bytes of a paged cache (0: not a cache), and the codes that the serving entry
+// points return for their arguments; *empty: valid, with no rows to work on.
+size_t kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D);
+int validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
+                       const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D, bool* empty);
+int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+                    const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
+                    const m4_rows_t* Q, const m4_rows_t* Q_out, uint32_t H, bool* empty);
+int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+                  bool* empty);
+int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q, const m4_rows_t* O,
+                  uint32_t H, float scale, const void* ws, bool* empty);
 
 }  // namespace qr

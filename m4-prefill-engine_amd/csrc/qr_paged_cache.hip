@@ -1,0 +1,340 @@
+// qr_paged_cache.hip -- rotary positions with several axes, quantizing a paged
+// KV cache as it is written, and reading it back.
+#include "qr_device.h"
+#include "qr_paged.h"
+
+namespace qr {
+
+// Sequence and position of row t (t < T): lanes count the starts at or below it
+// 64 at a time.  Returns false for rows behind the last sequence, rows whose
+// position has no page and tokens before position 0.
+struct Place {
+    uint32_t page, slot;
+    int pos;
+    bool ok;
+};
+__device__ __forceinline__ Place place_of(const BatchView& bv, const PageGeom& g, uint32_t t, int lane) {
+    Place r{0, 0, 0, false};
+    uint32_t before = 0;  // sequences whose first row is at or below t
+    for (uint32_t b0 = 0; b0 < bv.B; b0 += 64) {
+        const uint32_t b = b0 + lane;
+        const bool le = b < bv.B && bv.q_start[b] <= (int)t;
+        const uint32_t n = __popcll(__ballot(le));
+        before += n;
+        if (n < 64) break;
+    }
+    if (before == 0) return r;
+    const uint32_t b = before - 1;
+    const int end = bv.q_start[b + 1];
+    if ((int)t >= end) return r;
+    r.pos = bv.kv_len[b] - (end - (int)t);
+    if (r.pos < 0) return r;
+    const uint32_t pi = (uint32_t)r.pos >> g.log2_page;
+    if (pi >= bv.table_pages) return r;
+    r.page = (uint32_t)bv.table[(size_t)b * bv.table_stride + pi];
+    r.slot = (uint32_t)r.pos & ((1u << g.log2_page) - 1);
+    r.ok = r.page < g.num_pages;
+    return r;
+}
+
+// Codes of 8 dims of a block of 32 that four neighbouring lanes hold (lane & 3
+// the quarter), and the block's scale.  Q8_0 as quantize_block_q8_0: the code
+// rounds x * (1 / d), d = amax / 127 in fp32, half away from zero, and is stored
+// plus 128.  Q4_0: d = m / -8 of the value m of largest magnitude (the first of
+// a tie), code = floor(x (1 / d) + 8.5), product and sum rounded apart.
+template <int FMT>
+__device__ __forceinline__ void quantize8(const float x[8], int lane, uint32_t code[8], uint32_t& d16) {
+    if constexpr (FMT == QUANT_Q8_0) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
+        amax = fmaxf(amax, __shfl_xor(amax, 1));
+        amax = fmaxf(amax, __shfl_xor(amax, 2));
+        const float d = amax / 127.0f;
+        const float id = d > 0.0f ? 1.0f / d : 0.0f;
+        d16 = f2h_bits(d);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            int q = (int)__builtin_roundf(x[e] * id);
+            q = q < -128 ? -128 : (q > 127 ? 127 : q);
+            code[e] = (uint32_t)(q + 128);
+        }
+    } else {
+        // magnitude (15 bits of fp16), then the earliest index, then the sign
+        uint32_t key = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t h = f2h_bits(x[e]);
+            key = max(key, (h & 0x7fffu) << 6 | (uint32_t)(31 - (8 * (lane & 3) + e)) << 1 | h >> 15);
+        }
+        key = max(key, (uint32_t)__shfl_xor((int)key, 1));
+        key = max(key, (uint32_t)__shfl_xor((int)key, 2));
+        const float d = h2f(key >> 6 | (key & 1u) << 15) / -8.0f;
+        const float id = d != 0.0f ? 1.0f / d : 0.0f;
+        d16 = f2h_bits(d);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float c = __builtin_floorf(__fadd_rn(__fmul_rn(x[e], id), 8.5f));
+            code[e] = (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f);
+        }
+    }
+}
+
+// One row of T tokens per LPR lanes, 8 dims a lane; a wave takes 64 / LPR
+// tokens and every `chunks`-th of the heads (Q, then K, then V), so angles are
+// formed once per wave and used for all its heads.  A rotated row is rounded to
+// fp16 before it is quantized, as a rotation and a write apart would.
+template <int LPR, int FMT>
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t chunks) {
+    constexpr int RPW = 64 / LPR;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l = lane % LPR, sub = lane / LPR;
+    const uint32_t t0 = blockIdx.x * RPW, t = t0 + sub;
+    const uint32_t chunk = blockIdx.y * 4 + wave;
+    const bool cached = p.geom.pages != nullptr;
+    const uint32_t items = p.H + (cached ? 2 * p.geom.Hkv : 0);
+    if (chunk >= items) return;
+    const bool live = t < p.T && 8u * l < p.D;
+
+    Place at{0, 0, 0, false};
+    bool row = live;
+    if (p.batch.q_start) {
+        for (int s = 0; s < RPW; s++) {
+            if (t0 + s >= p.T) break;
+            const Place a = place_of(p.batch, p.geom, t0 + s, lane);
+            if (s == sub) at = a;
+        }
+        // rows of Q with no place in the cache (behind the last sequence) stay
+        row = live && at.ok;
+    }
+
+    // angles of this lane's pairs; `turned`: its dims take part, `other`: the
+    // lane that holds the partners of its dims
+    const uint32_t hp = p.rope.pairs / 8;  // lanes of the first halves
+    bool turned;
+    int other = lane;
+    uint32_t pair0;
+    if (p.rope.traditional) {
+        turned = 4u * l < p.rope.pairs;
+        pair0 = 4 * l;
+    } else {
+        turned = (uint32_t)l < 2 * hp;
+        const bool second = (uint32_t)l >= hp;
+        pair0 = 8 * (second ? l - hp : l);
+        if (turned) other = second ? lane - (int)hp : lane + (int)hp;
+    }
+    float cs[8], sn[8];
+    if (turned && row) {
+        const int n = p.rope.traditional ? 4 : 8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (e >= n) break;
+            const int pos = p.rope.positions
+                                ? p.rope.positions[(size_t)p.rope.axis[pair0 + e] * p.rope.position_stride + t]
+                                : at.pos;
+            const uint64_t frac = (uint64_t)(int64_t)pos * p.rope.turn[pair0 + e];
+            const float turn = (float)(int32_t)(frac >> 32) * 0x1p-32f;  // -0.5 .. 0.5
+            sincospif(2.0f * turn, &sn[e], &cs[e]);
+        }
+        if (p.rope.traditional) {
+#pragma unroll
+            for (int e = 3; e >= 0; e--) {  // of dims 2 e and 2 e + 1
+                cs[2 * e + 1] = cs[2 * e] = cs[e];
+                sn[2 * e + 1] = sn[e];
+                sn[2 * e] = -sn[e];
+            }
+        } else if ((uint32_t)l < hp) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) sn[e] = -sn[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            cs[e] = 1.0f;
+            sn[e] = 0.0f;
+        }
+        turned = false;
+    }
+    const bool any_turned = p.rope.pairs != 0;
+
+    for (uint32_t it = chunk; it < items; it += chunks) {
+        const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
+        const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
+        const RowsView& src = is_q ? p.Q : (is_k ? p.K : p.V);
+        h8_t y{};
+        if (row) y = *reinterpret_cast<const h8_t*>(src.p + (int64_t)t * src.ts + (int64_t)h * src.hs + 8 * l);
+        if (any_turned && (is_q || is_k)) {
+            u4_t mine = __builtin_bit_cast(u4_t, y), theirs;
+            if (p.rope.traditional) {
+                theirs = u4_t{mine.x >> 16 | mine.x << 16, mine.y >> 16 | mine.y << 16, mine.z >> 16 | mine.z << 16,
+                              mine.w >> 16 | mine.w << 16};
+            } else {
+                theirs = u4_t{(uint32_t)__shfl((int)mine.x, other), (uint32_t)__shfl((int)mine.y, other),
+                              (uint32_t)__shfl((int)mine.z, other), (uint32_t)__shfl((int)mine.w, other)};
+            }
+            const h8_t z = __builtin_bit_cast(h8_t, theirs);
+            if (turned) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = (_Float16)((float)y[e] * cs[e] + (float)z[e] * sn[e]);
+            }
+        }
+        if (is_q) {
+            if (row) *reinterpret_cast<h8_t*>(p.Qo.p + (int64_t)t * p.Qo.ts + (int64_t)h * p.Qo.hs + 8 * l) = y;
+            continue;
+        }
+        if constexpr (FMT >= 0) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (float)y[e];
+            uint32_t c[8], d16;
+            quantize8<FMT>(x, lane, c, d16);
+            if (!row) continue;
+            constexpr uint32_t D = LPR * 8, NB = D / 32, CB = FMT == QUANT_Q8_0 ? D : D / 2;
+            uint8_t* head = p.geom.pages + ((size_t)at.page * p.geom.Hkv + h) * p.geom.head_bytes;
+            if (is_k) {
+                uint8_t* o = head + at.slot * CB;
+                if constexpr (FMT == QUANT_Q8_0) {
+                    *reinterpret_cast<u2_t*>(o + 8 * l) = u2_t{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
+                                                               c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
+                } else {
+                    *reinterpret_cast<uint32_t*>(o + 4 * l) =
+                        c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24 | c[4] << 4 | c[5] << 12 | c[6] << 20 | c[7] << 28;
+                }
+                if (l % 4 == 0)
+                    *reinterpret_cast<uint16_t*>(head + p.geom.ks_off + (at.slot * NB + l / 4) * 2) = (uint16_t)d16;
+            } else {
+                const uint32_t g4 = at.slot >> 2, k4 = at.slot & 3;
+                uint8_t* o = head + p.geom.v_off + g4 * (4 * CB) + k4;
+                if constexpr (FMT == QUANT_Q8_0) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) o[(8 * l + e) * 4] = (uint8_t)c[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[(4 * l + e) * 4] = (uint8_t)(c[2 * e] | c[2 * e + 1] << 4);
+                }
+                if (l % 4 == 0)
+                    *reinterpret_cast<uint16_t*>(head + p.geom.vs_off + ((g4 * NB + l / 4) * 4 + k4) * 2) = (uint16_t)d16;
+            }
+        }
+    }
+}
+
+hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
+    if (p.T == 0) return hipSuccess;
+    const int lpr = p.D <= 64 ? 8 : (p.D <= 128 ? 16 : 32);
+    if (p.D > 256 || p.D % 8 || p.rope.pairs > kRopeMaxPairs || p.rope.pairs % 8 || 2 * p.rope.pairs > p.D)
+        return hipErrorInvalidValue;
+    if (p.geom.pages && p.D != 64 && p.D != 128) return hipErrorInvalidValue;
+    const uint32_t items = p.H + (p.geom.pages ? 2 * p.geom.Hkv : 0);
+    if (items == 0) return hipSuccess;
+    const uint32_t groups = (p.T + 64 / lpr - 1) / (64 / lpr);
+    uint32_t blocks = (items + 3) / 4;  // one head per wave
+    while (blocks > 1 && (uint64_t)groups * blocks > 1024) blocks = (blocks + 1) / 2;
+    const dim3 grid(groups, blocks);
+    const int fmt = p.geom.pages ? p.format : -1;
+#define QR_APPEND(L, F) hipLaunchKernelGGL((kv_append_kernel<L, F>), grid, dim3(256), 0, st, p, 4 * blocks)
+    if (fmt < 0) {
+        if (lpr == 8) QR_APPEND(8, -1);
+        else if (lpr == 16) QR_APPEND(16, -1);
+        else QR_APPEND(32, -1);
+    } else if (fmt == QUANT_Q8_0) {
+        if (lpr == 8) QR_APPEND(8, QUANT_Q8_0);
+        else QR_APPEND(16, QUANT_Q8_0);
+    } else if (fmt == QUANT_Q4_0) {
+        if (lpr == 8) QR_APPEND(8, QUANT_Q4_0);
+        else QR_APPEND(16, QUANT_Q4_0);
+    } else {
+        return hipErrorInvalidValue;
+    }
+#undef QR_APPEND
+    return hipGetLastError();
+}
+
+// The values of the batch's rows: half(q half(d)), or half((c - 8) half(d)).  A
+// lane reads 8 dims of a token; of V the four tokens of its group, of which it
+// keeps its own (the other three lanes' reads of the same bytes hit the cache).
+template <int LPR, int FMT>
+__global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p, uint32_t chunks) {
+    constexpr int RPW = 64 / LPR;
+    constexpr uint32_t D = LPR * 8, NB = D / 32, CB = FMT == QUANT_Q8_0 ? D : D / 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l = lane % LPR, sub = lane / LPR;
+    const uint32_t t0 = blockIdx.x * RPW, t = t0 + sub;
+    const uint32_t chunk = blockIdx.y * 4 + wave, items = 2 * p.geom.Hkv;
+    if (chunk >= items) return;
+    Place at{0, 0, 0, false};
+    for (int s = 0; s < RPW; s++) {
+        if (t0 + s >= p.batch.T) break;
+        const Place a = place_of(p.batch, p.geom, t0 + s, lane);
+        if (s == sub) at = a;
+    }
+    if (!at.ok) return;
+    for (uint32_t it = chunk; it < items; it += chunks) {
+        const bool is_k = it < p.geom.Hkv;
+        const uint32_t h = is_k ? it : it - p.geom.Hkv;
+        const uint8_t* head = p.geom.pages + ((size_t)at.page * p.geom.Hkv + h) * p.geom.head_bytes;
+        float q[8];
+        uint32_t d16;
+        if (is_k) {
+            const uint8_t* c = head + at.slot * CB;
+            d16 = *reinterpret_cast<const uint16_t*>(head + p.geom.ks_off + (at.slot * NB + l / 4) * 2);
+            if constexpr (FMT == QUANT_Q8_0) {
+                const u2_t w = *reinterpret_cast<const u2_t*>(c + 8 * l);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    q[e] = (float)(int)((w.x >> (8 * e) & 0xffu)) - 128.0f;
+                    q[4 + e] = (float)(int)((w.y >> (8 * e) & 0xffu)) - 128.0f;
+                }
+            } else {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(c + 4 * l);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    q[e] = (float)(int)(w >> (8 * e) & 15u) - 8.0f;
+                    q[4 + e] = (float)(int)(w >> (8 * e + 4) & 15u) - 8.0f;
+                }
+            }
+        } else {
+            const uint32_t g4 = at.slot >> 2, k4 = at.slot & 3;
+            d16 = *reinterpret_cast<const uint16_t*>(head + p.geom.vs_off + ((g4 * NB + l / 4) * 4 + k4) * 2);
+            const u4_t* c = reinterpret_cast<const u4_t*>(head + p.geom.v_off + g4 * (4 * CB) + l * (4 * CB / LPR));
+            const u4_t a = c[0];
+            if constexpr (FMT == QUANT_Q8_0) {
+                const u4_t b = c[1];
+                const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++) q[e] = (float)(int)(w[e] >> (8 * k4) & 0xffu) - 128.0f;
+            } else {
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    q[2 * e] = (float)(int)(w[e] >> (8 * k4) & 15u) - 8.0f;
+                    q[2 * e + 1] = (float)(int)(w[e] >> (8 * k4 + 4) & 15u) - 8.0f;
+                }
+            }
+        }
+        const float d = h2f(d16);
+        h8_t y;
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = (_Float16)(q[e] * d);
+        const RowsView& dst = is_k ? p.K : p.V;
+        *reinterpret_cast<h8_t*>(dst.p + (int64_t)t * dst.ts + (int64_t)h * dst.hs + 8 * l) = y;
+    }
+}
+
+hipError_t launch_kv_read(const ReadParams& p, hipStream_t st) {
+    if (p.batch.T == 0 || p.geom.Hkv == 0) return hipSuccess;
+    if (p.D != 64 && p.D != 128) return hipErrorInvalidValue;
+    const uint32_t rpw = p.D == 64 ? 8 : 4, groups = (p.batch.T + rpw - 1) / rpw;
+    uint32_t blocks = (2 * p.geom.Hkv + 3) / 4;
+    while (blocks > 1 && (uint64_t)groups * blocks > 1024) blocks = (blocks + 1) / 2;
+    const dim3 grid(groups, blocks);
+    switch ((p.D == 128 ? 1 : 0) + (p.format == QUANT_Q8_0 ? 2 : 0)) {
+        case 0: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q4_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
+        case 1: hipLaunchKernelGGL((kv_read_kernel<16, QUANT_Q4_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
+        case 2: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q8_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
+        default: hipLaunchKernelGGL((kv_read_kernel<16, QUANT_Q8_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace qr

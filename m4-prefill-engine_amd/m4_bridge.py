@@ -86,6 +86,16 @@ SIGNATURES = {
     "m4_bridge_prefill_layer_ex_kv": ([_VP] * 13 + [_I, _U32, _U32, _U32, _U32, _U32, _U32, _F, _I, _F, _I, _F,
                                                     _U32, _I], _I),
     "m4_bridge_dequantize": ([_VP, _SZ, _VP, _SZ, _I, _U32, _U32], _I),
+    "m4_bridge_kv_cache_bytes": ([_I, _U32, _U32, _U32, _U32], _SZ),
+    "m4_bridge_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
+    "m4_bridge_kv_cache_append": ([_VP, _VP, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
+    "m4_bridge_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
+    "m4_bridge_paged_attn_workspace": ([_VP, _VP, _U32, _U32], _SZ),
+    "m4_bridge_dispatch_paged_attn": ([_VP, _VP, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_validate_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
+    "m4_bridge_validate_kv_cache_append": ([_VP, _VP, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
+    "m4_bridge_validate_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
+    "m4_bridge_validate_paged_attn": ([_VP, _VP, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
     "m4_bridge_set_stream": ([_VP], _I),
     "m4_bridge_get_stream": ([], _VP),
     "m4_bridge_last_error": ([], ctypes.c_char_p),
@@ -139,6 +149,135 @@ def projection_plan(lib: ctypes.CDLL, format_id: int, M: int, K: int, *N: int, s
     if rc:
         raise ValueError(f"m4_bridge_projection_plan failed with status code {rc}")
     return plan
+
+
+class KVCacheStruct(ctypes.Structure):
+    """m4_kv_cache_t (include/m4_mlx_bridge.h)."""
+    _fields_ = [("pages", _VP), ("bytes", _SZ), ("format", _I), ("num_pages", _U32), ("page_size", _U32),
+                ("Hkv", _U32), ("D", _U32)]
+
+
+class KVBatchStruct(ctypes.Structure):
+    """m4_kv_batch_t (include/m4_mlx_bridge.h)."""
+    _fields_ = [("B", _U32), ("T", _U32), ("q_start", _VP), ("kv_len", _VP), ("page_table", _VP),
+                ("table_pages", _U32), ("table_stride", _U32), ("max_new", _U32), ("max_kv", _U32)]
+
+
+class RowsStruct(ctypes.Structure):
+    """m4_rows_t (include/m4_mlx_bridge.h)."""
+    _fields_ = [("ptr", _VP), ("bytes", _SZ), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class RopeAxesStruct(ctypes.Structure):
+    """m4_rope_axes_t (include/m4_mlx_bridge.h)."""
+    MAX_PAIRS = 128
+    _fields_ = [("pairs", _U32), ("axes", _U32), ("traditional", _I), ("pair_axis", ctypes.c_uint8 * MAX_PAIRS),
+                ("inv_freq", ctypes.c_double * MAX_PAIRS)]
+
+
+def _int32(name: str, t: Any, dims: int) -> Any:
+    import torch
+
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims:
+        raise ValueError(f"{name} must be an int32 tensor with {dims} dimension(s)")
+    if t.numel() and t.stride(-1) != 1:
+        raise ValueError(f"{name} must be contiguous along its last dimension")
+    return t
+
+
+class PagedKVCache:
+    """One layer's paged, quantized KV cache (m4_kv_cache_t): `num_pages` pages of
+    `page_size` tokens (16, 32, 64, 128 or 256), `Hkv` heads of `D` (64 or 128) dims, in
+    format Q8_0 or Q4_0.  `pages` is its memory, a uint8 tensor of any shape (made
+    here when it is None)."""
+
+    def __init__(self, format: Union[int, QuantFormat], num_pages: int, page_size: int, Hkv: int, D: int, pages=None,
+                 device: str = "cuda") -> None:
+        import torch
+
+        self.format, self.num_pages, self.page_size, self.Hkv, self.D = int(format), num_pages, page_size, Hkv, D
+        need = self.nbytes(format, num_pages, page_size, Hkv, D)
+        if need == 0:
+            raise ValueError(f"no paged cache of format {int(format)}, {num_pages} pages of {page_size} tokens, "
+                             f"{Hkv} heads of {D}")
+        if pages is None:
+            pages = torch.zeros(need, dtype=torch.uint8, device=device)
+        if not isinstance(pages, torch.Tensor) or pages.dtype != torch.uint8 or not pages.is_contiguous():
+            raise ValueError("pages must be a contiguous uint8 tensor")
+        if pages.numel() < need:
+            raise ValueError(f"pages holds {pages.numel()} bytes, {need} are needed")
+        self.pages = pages
+        self.struct = KVCacheStruct(pages.data_ptr(), pages.numel(), self.format, num_pages, page_size, Hkv, D)
+        self.ref = ctypes.addressof(self.struct)
+
+    @staticmethod
+    def nbytes(format: Union[int, QuantFormat], num_pages: int, page_size: int, Hkv: int, D: int) -> int:
+        dims = (num_pages, page_size, Hkv, D)
+        if not all(0 <= d < 1 << 32 for d in dims):
+            return 0
+        return int(HIPBridge.get_instance().lib.m4_bridge_kv_cache_bytes(int(format), *dims))
+
+
+class KVBatch:
+    """The sequences of a call (m4_kv_batch_t).  q_start [B + 1], kv_len [B] and
+    page_table [B, pages] are int32 device tensors that the kernels read when they
+    run, so a captured graph follows what is written to them.  The rows
+    q_start[b] .. q_start[b + 1] of a call are the last keys of sequence b, which has
+    kv_len[b] keys with them.  max_new and max_kv: what to expect of the longest
+    sequence (None reads them from the device, which waits for it); they choose
+    kernels and the workspace, results hold for any lengths."""
+
+    def __init__(self, q_start, kv_len, page_table, max_new: Optional[int] = None, max_kv: Optional[int] = None) -> None:
+        self.q_start, self.kv_len = _int32("q_start", q_start, 1), _int32("kv_len", kv_len, 1)
+        self.page_table = _int32("page_table", page_table, 2)
+        B = kv_len.shape[0]
+        if q_start.shape[0] != B + 1 or page_table.shape[0] != B:
+            raise ValueError(f"q_start, kv_len and page_table disagree: {q_start.shape[0]}, {B} and "
+                             f"{page_table.shape[0]} rows (B + 1, B, B)")
+        if max_new is None:
+            max_new = int(q_start.diff().max().item()) if B else 0
+        if max_kv is None:
+            max_kv = int(kv_len.max().item()) if B else 0
+        self.B = B
+        self.struct = KVBatchStruct(B, 0, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+                                    page_table.shape[1], page_table.stride(0), max(int(max_new), 0), max(int(max_kv), 0))
+        self.ref = ctypes.addressof(self.struct)
+
+
+class RotaryAxes:
+    """Rotary embedding of the first `dims` dims of a head (m4_rope_axes_t): pair i turns
+    by positions[pair_axes[i]] * inv_freq[i], inv_freq theta^(-2i / dims) unless given.
+    `sections`: pairs per axis, in runs (time, height, width); `pair_axes`: the axis
+    of each pair, for any other order; neither: one axis.  Pairs are dims
+    (i, i + dims / 2), or (2i, 2i + 1) when traditional."""
+
+    def __init__(self, dims: int, theta: float = 10000.0, sections=None, pair_axes=None, inv_freq=None,
+                 traditional: bool = False) -> None:
+        pairs = dims // 2
+        if dims <= 0 or dims % 16 or pairs > RopeAxesStruct.MAX_PAIRS:
+            raise ValueError(f"dims={dims} must be a positive multiple of 16, at most {2 * RopeAxesStruct.MAX_PAIRS}")
+        if sections is not None and pair_axes is not None:
+            raise ValueError("give sections or pair_axes, not both")
+        if sections is not None:
+            pair_axes = [a for a, n in enumerate(sections) for _ in range(n)]
+        if pair_axes is None:
+            pair_axes = [0] * pairs
+        pair_axes = [int(a) for a in pair_axes]
+        if len(pair_axes) != pairs or min(pair_axes) < 0 or max(pair_axes) > 255:
+            raise ValueError(f"{pairs} pairs need an axis each, got {len(pair_axes)}")
+        if inv_freq is None:
+            if not theta > 0:
+                raise ValueError(f"theta={theta} must be positive")
+            inv_freq = [float(theta) ** (-i / pairs) for i in range(pairs)]
+        inv_freq = [float(f) for f in inv_freq]
+        if len(inv_freq) != pairs:
+            raise ValueError(f"{pairs} pairs need a frequency each, got {len(inv_freq)}")
+        axes = max(pair_axes) + 1 if sections is None else max(len(sections), 1)
+        self.dims, self.axes = dims, axes
+        self.struct = RopeAxesStruct(pairs, axes, int(bool(traditional)))
+        self.struct.pair_axis[:pairs] = pair_axes
+        self.struct.inv_freq[:pairs] = inv_freq
+        self.ref = ctypes.addressof(self.struct)
 
 
 def load_library(path: Optional[Union[str, Path]] = None) -> ctypes.CDLL:
@@ -461,6 +600,127 @@ class HIPBridge:
                                                       int(bool(rope_traditional)))
         self._check("m4_bridge_prefill_layer_ex_kv", ret)
         self._in_flight_tensors.append(bufs)
+        return ret
+
+    # -- serving over a paged KV cache -----------------------------------------
+    def _rows(self, name: str, t: Any, token_major: bool, heads: Optional[int], D: Optional[int], out: bool) -> tuple:
+        """(m4_rows_t, T, heads, tensor) of fp16 rows [heads, T, D], or [T, heads, D] when token_major.
+        Any strides that keep 8 elements together are taken as they are; other inputs
+        are copied (and retained until synchronize())."""
+        import torch
+
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.dim() != 3:
+            raise ValueError(f"{name} must be an fp16 tensor with 3 dimensions")
+        a, b, d = t.shape
+        T, H = (a, b) if token_major else (b, a)
+        if (heads is not None and H != heads) or (D is not None and d != D):
+            raise ValueError(f"{name} has {H} heads of {d}, expected {heads} of {D}")
+        sa, sb, sd = t.stride()
+        if sd != 1 or sa % 8 or sb % 8 or t.data_ptr() % 16:
+            if t.numel() and out:
+                raise ValueError(f"{name} must be contiguous along its last dimension, 16-byte aligned, with strides "
+                                 f"that are multiples of 8")
+            t = t.contiguous() if sd != 1 or sa % 8 or sb % 8 else t.clone(memory_format=torch.contiguous_format)
+            self._retained_contig.append(t)
+            sa, sb, sd = t.stride()
+        ts, hs = (sa, sb) if token_major else (sb, sa)
+        held = ((T - 1) * ts + (H - 1) * hs + d) * 2 if t.numel() else 0
+        return RowsStruct(t.data_ptr(), held, ts, hs), T, H, t
+
+    def _positions(self, positions: Any, rope: "RotaryAxes", T: int) -> tuple:
+        """(pointer, stride) of int32 positions [T] or [axes, T]."""
+        if positions is None:
+            return None, 0
+        p = _int32("positions", positions, positions.dim() if positions.dim() == 1 else 2)
+        axes = 1 if p.dim() == 1 else p.shape[0]
+        if p.shape[-1] != T or axes < rope.axes:
+            raise ValueError(f"positions {tuple(p.shape)} do not give {rope.axes} axes of {T} tokens")
+        return p.data_ptr(), (p.stride(0) if p.dim() == 2 else T)
+
+    def rope_axes(self, X, Y, rope: RotaryAxes, positions, token_major: bool = False) -> int:
+        """Y = X [H, T, D] (or [T, H, D]) turned by positions [T] or [axes, T]; Y may be X."""
+        x, T, H, X = self._rows("X", X, token_major, None, None, False)
+        y, Ty, _, _ = self._rows("Y", Y, token_major, H, X.shape[2], True)
+        if positions is None or Ty != T:
+            raise ValueError("X and Y need the same rows, and positions")
+        pos, stride = self._positions(positions, rope, T)
+        self._bind_stream(X)
+        ret = self._lib.m4_bridge_rope_axes(rope.ref, pos, stride, ctypes.addressof(x), ctypes.addressof(y), T, H,
+                                            X.shape[2])
+        self._check("m4_bridge_rope_axes", ret)
+        self._in_flight_tensors.append((X, Y, positions))
+        return ret
+
+    def kv_cache_append(self, cache: PagedKVCache, batch: KVBatch, K, V, rope: Optional[RotaryAxes] = None,
+                        positions=None, Q=None, Q_out=None, token_major: bool = False) -> int:
+        """Writes the batch's rows of K, V [Hkv, T, D] (or [T, Hkv, D]) to the cache, K turned by `rope` first; Q
+        [H, T, D] is turned into Q_out (Q itself when None) by the same launch.  positions
+        None: each token's place in its sequence."""
+        k, T, _, K = self._rows("K", K, token_major, cache.Hkv, cache.D, False)
+        v, Tv, _, V = self._rows("V", V, token_major, cache.Hkv, cache.D, False)
+        if Tv != T:
+            raise ValueError(f"K has {T} rows, V {Tv}")
+        if Q is None and Q_out is not None:
+            raise ValueError("Q_out without Q")
+        if Q is not None and rope is None:
+            raise ValueError("Q is turned by rope: give both or neither")
+        pos, stride = self._positions(positions, rope, T) if rope is not None else (None, 0)
+        q = qo = None
+        H = 0
+        if Q is not None:
+            Q_out = Q if Q_out is None else Q_out
+            qo, To, H, _ = self._rows("Q_out", Q_out, token_major, None, cache.D, True)
+            q, Tq, _, Q = self._rows("Q", Q, token_major, H, cache.D, False)
+            if Tq != T or To != T:
+                raise ValueError(f"K has {T} rows, Q {Tq} and Q_out {To}")
+        self._bind_stream(K)
+        batch.struct.T = T
+        ref = ctypes.addressof
+        ret = self._lib.m4_bridge_kv_cache_append(cache.ref, batch.ref, ref(k), ref(v), rope.ref if rope else None, pos,
+                                                  stride, ref(q) if q else None, ref(qo) if qo else None, H)
+        self._check("m4_bridge_kv_cache_append", ret)
+        self._in_flight_tensors.append((cache, batch, K, V, Q, Q_out, positions))
+        return ret
+
+    def kv_cache_read(self, cache: PagedKVCache, batch: KVBatch, K, V, token_major: bool = False) -> int:
+        """The cached values of the batch's rows into K, V [Hkv, T, D] (or [T, Hkv, D])."""
+        k, T, _, _ = self._rows("K", K, token_major, cache.Hkv, cache.D, True)
+        v, Tv, _, _ = self._rows("V", V, token_major, cache.Hkv, cache.D, True)
+        if Tv != T:
+            raise ValueError(f"K has {T} rows, V {Tv}")
+        self._bind_stream(K)
+        batch.struct.T = T
+        ret = self._lib.m4_bridge_kv_cache_read(cache.ref, batch.ref, ctypes.addressof(k), ctypes.addressof(v))
+        self._check("m4_bridge_kv_cache_read", ret)
+        self._in_flight_tensors.append((cache, batch, K, V))
+        return ret
+
+    def paged_attn_workspace(self, cache: PagedKVCache, batch: KVBatch, H: int, window: int = 0) -> int:
+        """Bytes of workspace that dispatch_paged_attn needs."""
+        return int(self._lib.m4_bridge_paged_attn_workspace(cache.ref, batch.ref, H, window))
+
+    def dispatch_paged_attn(self, cache: PagedKVCache, batch: KVBatch, Q, O, scale: float, token_major: bool = False,
+                            o_token_major: bool = False, window: int = 0, workspace=None) -> int:
+        """Causal attention of the batch's rows Q [H, T, D] (or [T, H, D]) over their sequences' cached keys (append
+        first); O [H, T, D], or [T, H, D] when o_token_major.  `workspace`: a uint8 device tensor of
+        paged_attn_workspace bytes, not shared with a call that may run at the same time (None: from torch's
+        allocator, on the current stream)."""
+        import torch
+
+        q, T, H, Q = self._rows("Q", Q, token_major, None, cache.D, False)
+        o, To, _, _ = self._rows("O", O, o_token_major, H, cache.D, True)
+        if To != T:
+            raise ValueError(f"Q has {T} rows, O {To}")
+        if window < 0 or window >= 1 << 32:
+            raise ValueError(f"window={window}")
+        self._bind_stream(Q)
+        batch.struct.T = T
+        if workspace is None:
+            workspace = torch.empty(self.paged_attn_workspace(cache, batch, H, window), dtype=torch.uint8, device=Q.device)
+        ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, ctypes.addressof(q), ctypes.addressof(o), H,
+                                                      float(scale), int(window), workspace.data_ptr(), workspace.numel())
+        self._check("m4_bridge_dispatch_paged_attn", ret)
+        self._in_flight_tensors.append((cache, batch, Q, O))
         return ret
 
     def dequantize(self, W, out, format, K, N) -> int:
