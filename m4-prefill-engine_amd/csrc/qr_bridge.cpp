@@ -422,15 +422,17 @@ qr::PageGeom cache_geom(const m4_kv_cache_t* c) {
 }
 
 // Frequencies in turns, as 64-bit fractions of one: whole turns per position
-// drop out because positions are whole.
+// drop out because positions are whole.  Double keeps a turn to 2^-23 at the
+// farthest position.
 void rope_table(const m4_rope_axes_t* r, const int32_t* positions, uint32_t stride, qr::RopeTable& t) {
     t.pairs = r->pairs;
     t.traditional = r->traditional ? 1 : 0;
     t.positions = positions;
     t.position_stride = stride;
     for (uint32_t i = 0; i < r->pairs; i++) {
-        const long double turns = (long double)r->inv_freq[i] / 6.283185307179586476925286766559006L;
-        t.turn[i] = (uint64_t)((turns - floorl(turns)) * 18446744073709551616.0L);
+        const double turns = r->inv_freq[i] * 0.15915494309189533576888376337251;
+        const double part = turns - floor(turns);  // 1 for a tiny negative frequency: no turn
+        t.turn[i] = part < 1.0 ? (uint64_t)(part * 18446744073709551616.0) : 0;
         t.axis[i] = r->pair_axis[i];
     }
 }

@@ -443,35 +443,49 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 }
 
 // Joins the partial rows of the item that begins in worker blockIdx.x's share:
-// its slot 1, then slot 0 of the workers after it.  One wave per row, lanes over dims.
+// its slot 1, then slot 0 of the workers after it.  One wave per row: lanes over
+// the workers for their reference points and sums, then over dims.
 template <int D, int NR>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t workers) {
     constexpr uint32_t R = 16 * NR;
+    constexpr int E = D / 64;
     const uint32_t w = blockIdx.x;
     const ItemNote note = reinterpret_cast<const ItemNote*>(p.ws)[w];
     if (note.workers < 2) return;
-    const Seq s = seq_of(p, note.b, R);
+    const int lane = threadIdx.x & 63;
+    const uint32_t r = blockIdx.y * 4 + (threadIdx.x >> 6);
     const uint32_t G = p.H / p.geom.Hkv;
-    const uint32_t rows = min(R, (uint32_t)s.n * G - note.rt * R);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t r = wave; r < rows; r += 4) {
-        float m = kNone, l = 0.0f, o[D / 64] = {};
-        for (uint32_t k = 0; k < note.workers; k++) {
-            const float* slot = slot_of<D, NR>(p.ws, workers, w + k, k == 0 ? 1 : 0);
-            const float m2 = slot[R * D + r], l2 = slot[R * D + R + r];
-            const float m_new = fmaxf(m, m2);
-            const float fa = __builtin_amdgcn_exp2f(m - m_new), fb = __builtin_amdgcn_exp2f(m2 - m_new);
-            m = m_new;
-            l = l * fa + l2 * fb;
+    const int T = (int)p.batch.T, q0 = min(max(p.batch.q_start[note.b], 0), T);
+    const uint32_t f = note.rt * R + r;
+    if (q0 + (int)(f / G) >= min(max(p.batch.q_start[note.b + 1], 0), T)) return;
+    auto slot = [&](uint32_t k) { return slot_of<D, NR>(p.ws, workers, w + k, k == 0 ? 1 : 0); };
+    float m = kNone;
+    for (uint32_t k = lane; k < note.workers; k += 64) m = fmaxf(m, slot(k)[R * D + r]);
 #pragma unroll
-            for (int e = 0; e < D / 64; e++) o[e] = o[e] * fa + slot[r * D + 64 * e + lane] * fb;
+    for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    float l = 0.0f, o[E] = {};
+    for (uint32_t k0 = 0; k0 < note.workers; k0 += 64) {
+        const uint32_t n = min(64u, note.workers - k0);
+        float weight = 0.0f;
+        if ((uint32_t)lane < n) {
+            const float* s = slot(k0 + lane) + R * D + r;
+            weight = __builtin_amdgcn_exp2f(s[0] - m);
+            l += s[R] * weight;
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const uint32_t f = note.rt * R + r;
-        _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(f / G)) * p.O.ts + (int64_t)(note.hk * G + f % G) * p.O.hs;
+#pragma unroll 4
+        for (uint32_t k = 0; k < n; k++) {
+            const float fa = bits_f32(__builtin_amdgcn_readlane(f32_bits(weight), k));
+            const float* s = slot(k0 + k) + r * D;
 #pragma unroll
-        for (int e = 0; e < D / 64; e++) dst[64 * e + lane] = (_Float16)(o[e] * inv);
+            for (int e = 0; e < E; e++) o[e] += s[64 * e + lane] * fa;
+        }
     }
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    _Float16* dst = p.O.p + (int64_t)(q0 + (int)(f / G)) * p.O.ts + (int64_t)(note.hk * G + f % G) * p.O.hs;
+#pragma unroll
+    for (int e = 0; e < E; e++) dst[64 * e + lane] = (_Float16)(o[e] * inv);
 }
 
 // Row tiles by the rows of the longest chunk, workers by the steps expected.
@@ -505,7 +519,7 @@ static hipError_t launch_rows(const PagedAttnParams& p, uint32_t workers, hipStr
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, NR>), dim3(workers), dim3(256), 0, st, p, workers);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, NR>), dim3(workers), dim3(256), 0, st, p, workers);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, NR>), dim3(workers, 4 * NR), dim3(256), 0, st, p, workers);
     return hipGetLastError();
 }
 

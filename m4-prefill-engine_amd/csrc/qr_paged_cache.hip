@@ -5,29 +5,37 @@
 
 namespace qr {
 
-// Sequence and position of row t (t < T): lanes count the starts at or below it
-// 64 at a time.  Returns false for rows behind the last sequence, rows whose
-// position has no page and tokens before position 0.
+// Where a token lies in the cache.
 struct Place {
     uint32_t page, slot;
     int pos;
     bool ok;
 };
-__device__ __forceinline__ Place place_of(const BatchView& bv, const PageGeom& g, uint32_t t, int lane) {
+// The places of rows t0 .. t0 + RPW - 1, lane's own in row t0 + sub: the lanes
+// count the sequences that begin at or below each row, 64 at a time, and the
+// rest is looked up for all rows at once.  Not ok: rows behind the last
+// sequence, tokens before position 0 and tokens whose page is not there.
+template <int RPW>
+__device__ __forceinline__ Place place_of(const BatchView& bv, const PageGeom& g, uint32_t t0, int sub, int lane) {
     Place r{0, 0, 0, false};
-    uint32_t before = 0;  // sequences whose first row is at or below t
+    uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < bv.B; b0 += 64) {
         const uint32_t b = b0 + lane;
-        const bool le = b < bv.B && bv.q_start[b] <= (int)t;
-        const uint32_t n = __popcll(__ballot(le));
-        before += n;
+        const int start = b < bv.B ? bv.q_start[b] : 0x7fffffff;
+        uint32_t n = 0;
+#pragma unroll
+        for (int s = 0; s < RPW; s++) {
+            n = __popcll(__ballot(start <= (int)(t0 + s)));
+            before += s == sub ? n : 0;
+        }
         if (n < 64) break;
     }
-    if (before == 0) return r;
+    const uint32_t t = t0 + sub;
+    if (before == 0 || t >= bv.T) return r;
     const uint32_t b = before - 1;
-    const int end = bv.q_start[b + 1];
+    const int end = bv.q_start[b + 1], len = bv.kv_len[b];
     if ((int)t >= end) return r;
-    r.pos = bv.kv_len[b] - (end - (int)t);
+    r.pos = len - (end - (int)t);
     if (r.pos < 0) return r;
     const uint32_t pi = (uint32_t)r.pos >> g.log2_page;
     if (pi >= bv.table_pages) return r;
@@ -96,14 +104,25 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
     if (chunk >= items) return;
     const bool live = t < p.T && 8u * l < p.D;
 
+    // the rows of one head ahead of the one at work; the first are under way while
+    // places and angles are found
+    auto fetch = [&](uint32_t it) {
+        h8_t y{};
+        if (it < items && live) {
+            const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
+            const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
+            const _Float16* src = is_q ? p.Q.p : (is_k ? p.K.p : p.V.p);
+            const int64_t ts = is_q ? p.Q.ts : (is_k ? p.K.ts : p.V.ts), hs = is_q ? p.Q.hs : (is_k ? p.K.hs : p.V.hs);
+            y = *reinterpret_cast<const h8_t*>(src + (int64_t)t * ts + (int64_t)h * hs + 8 * l);
+        }
+        return y;
+    };
+    h8_t next = fetch(chunk);
+
     Place at{0, 0, 0, false};
     bool row = live;
     if (p.batch.q_start) {
-        for (int s = 0; s < RPW; s++) {
-            if (t0 + s >= p.T) break;
-            const Place a = place_of(p.batch, p.geom, t0 + s, lane);
-            if (s == sub) at = a;
-        }
+        at = place_of<RPW>(p.batch, p.geom, t0, sub, lane);
         // rows of Q with no place in the cache (behind the last sequence) stay
         row = live && at.ok;
     }
@@ -160,9 +179,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
     for (uint32_t it = chunk; it < items; it += chunks) {
         const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
         const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
-        const RowsView& src = is_q ? p.Q : (is_k ? p.K : p.V);
-        h8_t y{};
-        if (row) y = *reinterpret_cast<const h8_t*>(src.p + (int64_t)t * src.ts + (int64_t)h * src.hs + 8 * l);
+        h8_t y = next;
+        next = fetch(it + chunks);
         if (any_turned && (is_q || is_k)) {
             u4_t mine = __builtin_bit_cast(u4_t, y), theirs;
             if (p.rope.traditional) {
@@ -262,12 +280,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p, uint32_t chu
     const uint32_t t0 = blockIdx.x * RPW, t = t0 + sub;
     const uint32_t chunk = blockIdx.y * 4 + wave, items = 2 * p.geom.Hkv;
     if (chunk >= items) return;
-    Place at{0, 0, 0, false};
-    for (int s = 0; s < RPW; s++) {
-        if (t0 + s >= p.batch.T) break;
-        const Place a = place_of(p.batch, p.geom, t0 + s, lane);
-        if (s == sub) at = a;
-    }
+    const Place at = place_of<RPW>(p.batch, p.geom, t0, sub, lane);
     if (!at.ok) return;
     for (uint32_t it = chunk; it < items; it += chunks) {
         const bool is_k = it < p.geom.Hkv;
