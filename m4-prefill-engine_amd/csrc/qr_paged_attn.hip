@@ -14,18 +14,26 @@
 
 namespace qr {
 
-constexpr int kWaves = 4;
-constexpr uint32_t kUnit = 32 * kWaves;  // keys that a workgroup takes per step
+constexpr uint32_t kWaves = 4;     // of a workgroup
+constexpr uint32_t kStep = 32;     // keys of a step
+// What an item costs beside its steps, in steps: its descriptors, queries and
+// the write of its rows.  64 requests of 1 .. 8192 keys: 4 and 8 the same within
+// noise; shares by steps alone, with a join of four waves an item, 44 us, now 33.
+constexpr uint32_t kItemCost = 4;
+// Waves of a launch: two per SIMD, what the registers allow with the next step's
+// tiles in flight (three without them: 47 us there), at least kMinSteps of the
+// line each.
+constexpr uint32_t kMaxWaves = 2048, kMinSteps = 2;
 constexpr float kNone = -3.402823466e38f;  // reference point of a row that has seen no score above -infinity
 
-// A worker's note of an item that begins in its share of the work and ends in
-// later ones': how many workers took part.
+// A workgroup's note of an item that begins in its share of the work and ends in
+// later ones': how many workgroups took part.
 struct ItemNote {
-    uint32_t b, hk, rt, workers;
+    uint32_t b, hk, rt, parts;
 };
 
 struct WorkPlan {
-    uint32_t nr, workers;
+    uint32_t nr, groups;
 };
 
 // values 1024 + 128 + q of four Q8_0 bytes, as pairs
@@ -51,6 +59,7 @@ struct Tile {
     uint32_t k[W], v[W];
     uint32_t kd;
     u2_t vd;
+    bool there;  // its page is one of the cache's
 
     __device__ __forceinline__ void load(const uint8_t* head, const PageGeom& g, uint32_t slot0, int lane) {
         constexpr uint32_t CB = 4 * W * 4, NB = D / 32;  // bytes of a key's codes, blocks
@@ -110,16 +119,22 @@ template <int D, int NR>
 __host__ __device__ constexpr size_t slot_bytes() {
     return (size_t)16 * NR * (D + 2) * 4;
 }
-// workspace: a note per worker, then two slots per worker of partial rows
+// workspace: a note per workgroup, then two slots per workgroup of partial rows
 // (O [R][D], reference points [R], sums [R], fp32)
 template <int D, int NR>
-__device__ __forceinline__ float* slot_of(uint8_t* ws, uint32_t workers, uint32_t w, int which) {
-    return reinterpret_cast<float*>(ws + (size_t)workers * sizeof(ItemNote) + ((size_t)w * 2 + which) * slot_bytes<D, NR>());
+__device__ __forceinline__ float* slot_of(uint8_t* ws, uint32_t groups, uint32_t w, int which) {
+    return reinterpret_cast<float*>(ws + (size_t)groups * sizeof(ItemNote) + ((size_t)w * 2 + which) * slot_bytes<D, NR>());
+}
+
+// lane `at`'s value, as a wave-uniform one
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int at) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), at) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, at);
 }
 
 struct Seq {
-    int q0, n, len, lo;   // first row, new tokens, keys, first key that any row sees (a multiple of kUnit)
-    uint32_t tiles, units;  // row tiles and key steps per tile
+    int q0, n, len, lo;   // first row, new tokens, keys, first key that any row sees (a multiple of kStep)
+    uint32_t tiles, steps;  // row tiles and key steps per tile
     uint64_t cost;
 };
 __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint32_t R) {
@@ -130,72 +145,71 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
     s.n = max(min(max(p.batch.q_start[b + 1], 0), T) - s.q0, 0);
     s.len = min(max(p.batch.kv_len[b], 0), cap);
     s.lo = 0;
-    if (p.window) s.lo = (int)(max((int64_t)s.len - s.n + 1 - (int64_t)p.window, (int64_t)0) / kUnit * kUnit);
+    if (p.window) s.lo = (int)(max((int64_t)s.len - s.n + 1 - (int64_t)p.window, (int64_t)0) / kStep * kStep);
     const uint32_t G = p.H / p.geom.Hkv;
     s.tiles = (uint32_t)(((uint64_t)s.n * G + R - 1) / R);
-    s.units = max((uint32_t)(s.len - s.lo + (int)kUnit - 1) / kUnit, 1u);
-    s.cost = (uint64_t)p.geom.Hkv * s.tiles * s.units;
+    s.steps = max((uint32_t)(s.len - s.lo + (int)kStep - 1) / kStep, 1u);
+    s.cost = (uint64_t)p.geom.Hkv * s.tiles * (kItemCost + s.steps);
     return s;
 }
 
-// The work is one line of key steps: of every sequence, KV head and row tile.
-// A workgroup takes an even share of it wherever it begins and ends, so batches
-// of any lengths fill the chip alike; items that cross a boundary leave
-// partial rows in the workspace, which paged_attn_join_kernel joins in order.
+// The work is one line: of every sequence, KV head and row tile (an item)
+// kItemCost for its overhead, then its key steps.  A wave takes an even share of
+// the line wherever it begins and ends, so batches of any lengths fill the chip
+// alike and no wave waits for another until the end, when an item that several
+// waves of a workgroup took is gathered by the first of them, through LDS; items
+// of several workgroups leave partial rows in the workspace, which
+// paged_attn_join_kernel joins in order.  The next step's tiles are loaded before
+// the present one is computed, and page numbers 32 steps ahead, a lane each.
+// Bound by the cache's bytes once there are enough of them: four requests of
+// 131072 keys (Q4_0, D = 128, 604 MB) 127 us, 4.8 TB/s; 64 requests of 1 .. 8192
+// keys (Q8_0, 110 MB) 33 us of which 4 are the join; one of 1000 keys 13.6 us, a
+// chain of descriptor, page table, key and join latencies.
 template <int FMT, int D, int NR>
-__global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t workers) {
+__global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
     constexpr int DT = D / 16, KK = D / 32;
     constexpr int RUN = D / 4;  // dims of a lane's run
-    __shared__ uint64_t wave_sum[kWaves];
-    __shared__ uint64_t start_off;
-    __shared__ uint32_t start_b;
-    __shared__ __attribute__((aligned(16))) float xo[2][NR][DT][64][4];
-    __shared__ float xs[2][NR][64][2];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63;
     const int j = lane & 15, g = lane >> 4;
-    const uint32_t w = blockIdx.x;
-    ItemNote* note = reinterpret_cast<ItemNote*>(p.ws) + w;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = blockIdx.x * kWaves + wave;
+    const uint32_t workers = groups * kWaves;
+    ItemNote* note = reinterpret_cast<ItemNote*>(p.ws) + blockIdx.x;
+    // rows of waves 1 .. 3 that finish or carry on an item of the wave before them
+    __shared__ __attribute__((aligned(16))) f4_t xo[kWaves - 1][NR][DT][64];
+    __shared__ float xs[kWaves - 1][NR][64][2];
+    __shared__ int head_of[kWaves];  // 0: none, 1: it ends in that wave's share, 2: it goes on
 
-    // ---- this worker's share [s0, s1) ----
-    const uint32_t per = (p.batch.B + 255) / 256;
-    const uint32_t b_lo = min(tid * per, p.batch.B), b_hi = min(b_lo + per, p.batch.B);
+    // ---- this wave's share [s0, s1) and the item in which it begins ----
+    const uint32_t per = (p.batch.B + 63) / 64;
+    const uint32_t b_lo = min(lane * per, p.batch.B), b_hi = min(b_lo + per, p.batch.B);
     uint64_t mine = 0;
-    for (uint32_t b = b_lo; b < b_hi; b++) mine += seq_of(p, b, R).cost;
+    for (uint32_t x = b_lo; x < b_hi; x++) mine += seq_of(p, x, R).cost;
     uint64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint64_t x = __shfl_up((unsigned long long)incl, o);
         if (lane >= o) incl += x;
     }
-    if (lane == 63) wave_sum[wave] = incl;
-    __syncthreads();
-    uint64_t total = 0, before = incl - mine;
-    for (int k = 0; k < kWaves; k++) {
-        if (k < wave) before += wave_sum[k];
-        total += wave_sum[k];
-    }
+    const uint64_t total = lane_u64(incl, 63);
     const uint64_t nw = min((uint64_t)workers, total);
-    if (tid == 0) *note = ItemNote{0, 0, 0, 0};
-    if (w >= nw) return;
-    const uint64_t s0 = total * w / nw, s1 = total * (w + 1) / nw;
-    if (before <= s0 && s0 < before + mine) {
-        uint64_t at = before;
-        for (uint32_t b = b_lo; b < b_hi; b++) {
-            const uint64_t c = seq_of(p, b, R).cost;
-            if (s0 < at + c) {
-                start_b = b;
-                start_off = s0 - at;
-                break;
-            }
-            at += c;
+    if (threadIdx.x == 0) *note = ItemNote{0, 0, 0, 0};
+    if (lane == 0) head_of[wave] = 0;
+    const uint64_t s0 = w < nw ? total * w / nw : 0, s1 = w < nw ? total * (w + 1) / nw : 0;
+    uint32_t b = 0;
+    uint64_t off = 0;
+    if (incl - mine <= s0 && s0 < incl) {
+        off = s0 - (incl - mine);
+        for (b = b_lo; b + 1 < b_hi; b++) {
+            const uint64_t cost = seq_of(p, b, R).cost;
+            if (off < cost) break;
+            off -= cost;
         }
     }
-    __syncthreads();
-    uint32_t b = __builtin_amdgcn_readfirstlane(start_b);
-    uint64_t off = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(start_off >> 32)) << 32 |
-                   __builtin_amdgcn_readfirstlane((uint32_t)start_off);
+    const int at = max(__ffsll((unsigned long long)__ballot(incl - mine <= s0 && s0 < incl)) - 1, 0);
+    b = __builtin_amdgcn_readlane(b, at);
+    off = lane_u64(off, at);
 
     float c = p.scale * 1.4426950408889634f;  // log2 units
     const bool neg = c < 0.0f;
@@ -205,20 +219,76 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     const h2_t one2 = {(_Float16)1.0f, (_Float16)1.0f};
     const uint32_t pmask = (1u << p.geom.log2_page) - 1;
 
+    // the item at work: its rows, and their running state
+    f4_t o[NR][DT];
+    float m_run[NR], l_run[NR];
+    Seq s{};
+    uint32_t b_open = 0, hk = 0, rt = 0, rows = 0;
+    uint64_t last = 0;            // its last place on the line
+    bool open = false, begun = false;  // it goes on in the next wave's share; its first step was here
+
+    auto row_of = [&](const RowsView& v, uint32_t r) {
+        const uint32_t f = rt * R + r;
+        return v.p + (int64_t)(s.q0 + (int)(f / G)) * v.ts + (int64_t)(hk * G + f % G) * v.hs;
+    };
+    // lane (j, g): row j of each 16, dims RUN g + DT r + dt
+    auto emit = [&]() {
+#pragma unroll
+        for (int q = 0; q < NR; q++) {
+            const uint32_t r = 16 * q + j;
+            if (r >= rows) continue;
+            _Float16* dst = row_of(p.O, r) + g * RUN;
+            const float inv = l_run[q] == 0.0f ? 0.0f : 1.0f / l_run[q];
+#pragma unroll
+            for (int e = 0; e < RUN; e += 8) {
+                h8_t y;
+#pragma unroll
+                for (int x = 0; x < 8; x++) y[x] = (_Float16)(o[q][(e + x) % DT][(e + x) / DT] * inv);
+                *reinterpret_cast<h8_t*>(dst + e) = y;
+            }
+        }
+    };
+    auto leave = [&](int which) {
+        float* slot = slot_of<D, NR>(p.ws, groups, blockIdx.x, which);
+#pragma unroll
+        for (int q = 0; q < NR; q++) {
+            const uint32_t r = 16 * q + j;
+            if (r >= rows) continue;
+#pragma unroll
+            for (int e = 0; e < RUN; e += 4)
+                *reinterpret_cast<f4_t*>(slot + r * D + g * RUN + e) =
+                    f4_t{o[q][e % DT][e / DT], o[q][(e + 1) % DT][(e + 1) / DT], o[q][(e + 2) % DT][(e + 2) / DT],
+                         o[q][(e + 3) % DT][(e + 3) / DT]};
+            if (g == 0) {
+                slot[R * D + r] = m_run[q];
+                slot[R * D + R + r] = l_run[q];
+            }
+        }
+    };
+
     for (uint64_t cur = s0; cur < s1 && b < p.batch.B;) {
-        const Seq s = seq_of(p, b, R);
+        s = seq_of(p, b, R);
         if (off >= s.cost) {
             b++;
             off = 0;
             continue;
         }
-        const uint32_t u0 = (uint32_t)(off % s.units);
-        const uint32_t item = (uint32_t)(off / s.units), hk = item / s.tiles, rt = item % s.tiles;
-        const uint32_t nu = (uint32_t)min((uint64_t)(s.units - u0), s1 - cur);
+        // this share of the item: its line from o0 on, steps u0 .. u0 + nu
+        const uint32_t line = kItemCost + s.steps;
+        const uint32_t o0 = (uint32_t)(off % line), item = (uint32_t)(off / line);
+        const uint32_t o1 = (uint32_t)min((uint64_t)line, o0 + (s1 - cur));
+        cur += o1 - o0;
+        off += o1 - o0;
+        if (o1 <= kItemCost) continue;
+        const uint32_t u0 = o0 > kItemCost ? o0 - kItemCost : 0, nu = o1 - kItemCost - u0;
+        hk = item / s.tiles;
+        rt = item % s.tiles;
+        b_open = b;
+        last = cur - o1 + line - 1;
         const int p0 = s.len - s.n;  // position of the first new token
 
         // ---- rows ----
-        const uint32_t rows = min(R, (uint32_t)s.n * G - rt * R);
+        rows = min(R, (uint32_t)s.n * G - rt * R);
         const int i_first = (int)(rt * R / G), i_last = (int)((rt * R + rows - 1) / G);
         int lim[NR], low[NR];
         h8_t qf[NR][KK];
@@ -241,8 +311,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         const int low_min = p.window ? (int)max((int64_t)lim_min + 1 - (int64_t)p.window, (int64_t)0) : 0;
         const int low_max = p.window ? (int)max((int64_t)lim_max + 1 - (int64_t)p.window, (int64_t)0) : 0;
 
-        f4_t o[NR][DT];
-        float m_run[NR], l_run[NR];
         uint32_t poison = 0;  // bit q: the row saw a V scale that is not finite
 #pragma unroll
         for (int q = 0; q < NR; q++) {
@@ -252,21 +320,33 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             for (int dt = 0; dt < DT; dt++) o[q][dt] = f4_t{};
         }
 
-        for (uint32_t u = u0; u < u0 + nu; u++) {
-            const int key0 = s.lo + (int)(u * kUnit) + 32 * wave;
-            if (key0 > lim_max || key0 + 31 < low_min || key0 >= s.len) continue;
-            Tile<FMT, D> tile[2];
-            bool there[2];
+        // ---- steps that some row sees something of: keys s.lo + kStep u .. + 31 ----
+        const int key_base = s.lo;
+        int ua = (int)u0, ub = (int)(u0 + nu);
+        if (lim_max < key_base) ub = ua;
+        else ub = min(ub, (lim_max - key_base) / (int)kStep + 1);
+        if (low_min > key_base + 31) ua = max(ua, (low_min - key_base - 31 + (int)kStep - 1) / (int)kStep);
+        // page numbers of the next 32 steps, a lane each 16 keys
+        uint32_t page_ids = 0xffffffffu;
+        int ids_from = ua - 32;
+        auto fetch = [&](Tile<FMT, D> tile[2], int u) {
+            if (u >= ids_from + 32) {
+                ids_from = u;
+                const int k0 = key_base + (u + (lane >> 1)) * (int)kStep + 16 * (lane & 1);
+                page_ids = k0 < s.len ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k0 >> p.geom.log2_page)]
+                                      : 0xffffffffu;
+            }
+            const int key0 = key_base + u * (int)kStep;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const int k0 = key0 + 16 * t;
-                const uint32_t pi = (uint32_t)k0 >> p.geom.log2_page;
-                uint32_t page = 0xffffffffu;
-                if (k0 < s.len) page = (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + pi];
-                there[t] = page < p.geom.num_pages;
-                const uint8_t* head = p.geom.pages + ((size_t)(there[t] ? page : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
-                tile[t].load(head, p.geom, (uint32_t)k0 & pmask, lane);
+                const uint32_t page = __builtin_amdgcn_readlane(page_ids, 2 * (u - ids_from) + t);
+                tile[t].there = page < p.geom.num_pages;
+                const uint8_t* head = p.geom.pages + ((size_t)(tile[t].there ? page : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
+                tile[t].load(head, p.geom, (uint32_t)(key0 + 16 * t) & pmask, lane);
             }
+        };
+        auto step = [&](Tile<FMT, D> tile[2], int u) {
+            const int key0 = key_base + u * (int)kStep;
             f4_t sc[NR][2];
 #pragma unroll
             for (int q = 0; q < NR; q++) sc[q][0] = sc[q][1] = f4_t{};
@@ -279,7 +359,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     for (int q = 0; q < NR; q++)
                         sc[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[q][kk], sc[q][t], 0, 0, 0);
                 }
-            if (key0 + 31 > lim_min || key0 < low_max || key0 + 31 >= s.len || !there[0] || !there[1]) {
+            if (key0 + 31 > lim_min || key0 < low_max || key0 + 31 >= s.len || !tile[0].there || !tile[1].there) {
                 // Some row does not see some key.  What such a key's V holds must
                 // not reach that row through 0 times infinity: V scales of keys
                 // that nobody sees are cleared, and scales that are not finite
@@ -291,7 +371,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int key = key0 + 16 * t + 4 * g + r;
-                        const bool dead = !there[t] || key >= s.len;
+                        const bool dead = !tile[t].there || key >= s.len;
                         if (!dead && (e[r] & 0x7c00u) == 0x7c00u) bad |= 1u << r;
                         if (dead || (bad >> r & 1)) e[r] = 0;
                     }
@@ -314,7 +394,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const int key = key0 + 16 * t + 4 * g + r;
-                            if (!there[t] || key > lim[q] || key < low[q]) sc[q][t][r] = -INFINITY;
+                            if (!tile[t].there || key > lim[q] || key < low[q]) sc[q][t][r] = -INFINITY;
                         }
                 }
             }
@@ -354,6 +434,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 #pragma unroll
                 for (int q = 0; q < NR; q++) o[q][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[q], o[q][dt], 0, 0, 0);
             }
+        };
+        Tile<FMT, D> ta[2], tb[2];
+        if (ua < ub) fetch(ta, ua);
+#pragma unroll 1
+        for (int u = ua; u < ub; u++) {
+            if (u + 1 < ub) fetch(tb, u + 1);
+            step(ta, u);
+            ta[0] = tb[0];
+            ta[1] = tb[1];
         }
         if (poison) {
 #pragma unroll
@@ -363,132 +452,126 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     for (int dt = 0; dt < DT; dt++) o[q][dt] = f4_t{NAN, NAN, NAN, NAN};
         }
 
-        // ---- the four waves' rows join: 2, 3 into 0, 1, then 1 into 0 ----
 #pragma unroll
         for (int q = 0; q < NR; q++) {
             l_run[q] += __shfl_xor(l_run[q], 16);
             l_run[q] += __shfl_xor(l_run[q], 32);
         }
+        const bool ends = u0 + nu == s.steps;
+        begun = u0 == 0;
+        open = !ends;
+        if (begun && ends) {
+            emit();
+        } else if (!begun && wave > 0) {
 #pragma unroll
-        for (int half = 2; half >= 1; half /= 2) {
-            __syncthreads();
-            if (wave >= half && wave < 2 * half) {
-                const int x = wave - half;
+            for (int q = 0; q < NR; q++) {
 #pragma unroll
-                for (int q = 0; q < NR; q++) {
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f4_t*>(xo[x][q][dt][lane]) = o[q][dt];
-                    xs[x][q][lane][0] = m_run[q];
-                    xs[x][q][lane][1] = l_run[q];
-                }
+                for (int dt = 0; dt < DT; dt++) xo[wave - 1][q][dt][lane] = o[q][dt];
+                xs[wave - 1][q][lane][0] = m_run[q];
+                xs[wave - 1][q][lane][1] = l_run[q];
             }
-            __syncthreads();
-            if (wave < half) {
-#pragma unroll
-                for (int q = 0; q < NR; q++) {
-                    const float m2 = xs[wave][q][lane][0], l2 = xs[wave][q][lane][1];
-                    const float m = fmaxf(m_run[q], m2);
-                    const float fa = __builtin_amdgcn_exp2f(m_run[q] - m), fb = __builtin_amdgcn_exp2f(m2 - m);
-                    m_run[q] = m;
-                    l_run[q] = l_run[q] * fa + l2 * fb;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++)
-                        o[q][dt] = o[q][dt] * fa + *reinterpret_cast<const f4_t*>(xo[wave][q][dt][lane]) * fb;
-                }
-            }
+            if (lane == 0) head_of[wave] = ends ? 1 : 2;
+            open = false;  // the wave before gathers it
+        } else if (!begun && ends) {
+            leave(0);
         }
-        const bool whole = nu == s.units;
-        if (wave == 0) {
-            // lane (j, g): row j of the tile's 16, dims RUN g + DT r + dt
-            if (whole) {
-#pragma unroll
-                for (int q = 0; q < NR; q++) {
-                    const uint32_t r = 16 * q + j;
-                    if (r >= rows) continue;
-                    const uint32_t f = rt * R + r;
-                    _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(f / G)) * p.O.ts + (int64_t)(hk * G + f % G) * p.O.hs + g * RUN;
-                    const float inv = l_run[q] == 0.0f ? 0.0f : 1.0f / l_run[q];
-#pragma unroll
-                    for (int e = 0; e < RUN; e += 8) {
-                        h8_t y;
-#pragma unroll
-                        for (int x = 0; x < 8; x++) y[x] = (_Float16)(o[q][(e + x) % DT][(e + x) / DT] * inv);
-                        *reinterpret_cast<h8_t*>(dst + e) = y;
-                    }
-                }
-            } else {
-                float* slot = slot_of<D, NR>(p.ws, workers, w, u0 == 0 ? 1 : 0);
-#pragma unroll
-                for (int q = 0; q < NR; q++) {
-                    const uint32_t r = 16 * q + j;
-#pragma unroll
-                    for (int e = 0; e < RUN; e += 4)
-                        *reinterpret_cast<f4_t*>(slot + r * D + g * RUN + e) =
-                            f4_t{o[q][e % DT][e / DT], o[q][(e + 1) % DT][(e + 1) / DT], o[q][(e + 2) % DT][(e + 2) / DT],
-                                 o[q][(e + 3) % DT][(e + 3) / DT]};
-                    if (g == 0) {
-                        slot[R * D + r] = m_run[q];
-                        slot[R * D + R + r] = l_run[q];
-                    }
-                }
-                if (u0 == 0 && lane == 0) {
-                    const uint64_t last = cur + s.units - 1;  // this item's last step, and who takes it
-                    *note = ItemNote{b, hk, rt, (uint32_t)(((last + 1) * nw - 1) / total) - w + 1};
-                }
-            }
-        }
-        cur += nu;
-        off += nu;
     }
+
+    // ---- an item that goes on takes the rows of the waves after this one, in order ----
+    __syncthreads();
+    if (!open) return;
+    bool ended = false;
+    for (uint32_t v = wave + 1; v < kWaves && !ended; v++) {
+#pragma unroll
+        for (int q = 0; q < NR; q++) {
+            const float m2 = xs[v - 1][q][lane][0], l2 = xs[v - 1][q][lane][1];
+            const float m = fmaxf(m_run[q], m2);
+            const float fa = __builtin_amdgcn_exp2f(m_run[q] - m), fb = __builtin_amdgcn_exp2f(m2 - m);
+            m_run[q] = m;
+            l_run[q] = l_run[q] * fa + l2 * fb;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[q][dt] = o[q][dt] * fa + xo[v - 1][q][dt][lane] * fb;
+        }
+        ended = __builtin_amdgcn_readfirstlane(head_of[v]) == 1;
+    }
+    if (ended && begun) {
+        emit();
+        return;
+    }
+    leave(begun ? 1 : 0);
+    if (begun && lane == 0)
+        *note = ItemNote{b_open, hk, rt, (uint32_t)((((last + 1) * nw - 1) / total) / kWaves) - blockIdx.x + 1};
 }
 
-// Joins the partial rows of the item that begins in worker blockIdx.x's share:
-// its slot 1, then slot 0 of the workers after it.  One wave per row: lanes over
-// the workers for their reference points and sums, then over dims.
+// Joins the partial rows of the items that begin in the shares of this block's
+// workgroups: slot 1 of the first, then slot 0 of those after it.  D / 4 lanes hold
+// a row; rows side by side while an item has few parts, else the parts of a row
+// are split over the lane groups, whose sums meet in LDS in a fixed order.
+constexpr uint32_t kJoinBlocks = 512;
 template <int D, int NR>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t workers) {
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
-    constexpr int E = D / 64;
-    const uint32_t w = blockIdx.x;
-    const ItemNote note = reinterpret_cast<const ItemNote*>(p.ws)[w];
-    if (note.workers < 2) return;
-    const int lane = threadIdx.x & 63;
-    const uint32_t r = blockIdx.y * 4 + (threadIdx.x >> 6);
+    constexpr int L = D / 4, GROUPS = 256 / L;
+    __shared__ f4_t part_sum[256];
+    const uint32_t per = (groups + gridDim.x - 1) / gridDim.x, w0 = blockIdx.x * per;
+    const uint32_t w1 = min(w0 + per, groups);
+    const ItemNote* notes = reinterpret_cast<const ItemNote*>(p.ws);
+    const uint32_t tid = threadIdx.x, l4 = tid % L, group = tid / L;
     const uint32_t G = p.H / p.geom.Hkv;
-    const int T = (int)p.batch.T, q0 = min(max(p.batch.q_start[note.b], 0), T);
-    const uint32_t f = note.rt * R + r;
-    if (q0 + (int)(f / G) >= min(max(p.batch.q_start[note.b + 1], 0), T)) return;
-    auto slot = [&](uint32_t k) { return slot_of<D, NR>(p.ws, workers, w + k, k == 0 ? 1 : 0); };
-    float m = kNone;
-    for (uint32_t k = lane; k < note.workers; k += 64) m = fmaxf(m, slot(k)[R * D + r]);
+    for (uint32_t base = w0; base < w1; base += 64) {
+        const uint32_t mine = base + (tid & 63);
+        uint64_t todo = __ballot(mine < w1 && notes[mine].parts >= 2);
+        while (todo) {
+            const uint32_t w = base + __ffsll((unsigned long long)todo) - 1;
+            todo &= todo - 1;
+            const ItemNote note = notes[w];
+            const Seq s = seq_of(p, note.b, R);
+            const uint32_t rows = min(R, (uint32_t)s.n * G - note.rt * R), parts = note.parts;
+            auto slot = [&](uint32_t k) { return slot_of<D, NR>(p.ws, groups, w + k, k == 0 ? 1 : 0); };
+            uint32_t split = 1;
+            while (split < GROUPS && parts > 4 * split) split *= 2;
+            const uint32_t side = GROUPS / split;
+            for (uint32_t r0 = blockIdx.y * side; r0 < rows; r0 += gridDim.y * side) {
+                const uint32_t r = r0 + group / split;
+                const bool live = r < rows;
+                float m = kNone, l = 0.0f;
+                f4_t o{};
+                if (live)
+                    for (uint32_t k = l4; k < parts; k += L) m = fmaxf(m, slot(k)[R * D + r]);
 #pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    float l = 0.0f, o[E] = {};
-    for (uint32_t k0 = 0; k0 < note.workers; k0 += 64) {
-        const uint32_t n = min(64u, note.workers - k0);
-        float weight = 0.0f;
-        if ((uint32_t)lane < n) {
-            const float* s = slot(k0 + lane) + R * D + r;
-            weight = __builtin_amdgcn_exp2f(s[0] - m);
-            l += s[R] * weight;
-        }
+                for (int x = L / 2; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+                if (live) {
+                    for (uint32_t k = l4; k < parts; k += L)
+                        l += slot(k)[R * D + R + r] * __builtin_amdgcn_exp2f(slot(k)[R * D + r] - m);
 #pragma unroll 4
-        for (uint32_t k = 0; k < n; k++) {
-            const float fa = bits_f32(__builtin_amdgcn_readlane(f32_bits(weight), k));
-            const float* s = slot(k0 + k) + r * D;
+                    for (uint32_t k = group % split; k < parts; k += split) {
+                        const float* x = slot(k);
+                        o += *reinterpret_cast<const f4_t*>(x + r * D + 4 * l4) * __builtin_amdgcn_exp2f(x[R * D + r] - m);
+                    }
+                }
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] += s[64 * e + lane] * fa;
+                for (int x = L / 2; x >= 1; x >>= 1) l += __shfl_xor(l, x);
+                if (split > 1) {
+                    __syncthreads();
+                    part_sum[tid] = o;
+                    __syncthreads();
+                    if (group % split == 0)
+                        for (uint32_t k = 1; k < split; k++) o += part_sum[tid + k * L];
+                }
+                if (live && group % split == 0) {
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    const uint32_t f = note.rt * R + r;
+                    _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(f / G)) * p.O.ts + (int64_t)(note.hk * G + f % G) * p.O.hs;
+                    const f2_t a = {o.x * inv, o.y * inv}, b = {o.z * inv, o.w * inv};
+                    *reinterpret_cast<u2_t*>(dst + 4 * l4) =
+                        u2_t{as_u32(__builtin_convertvector(a, h2_t)), as_u32(__builtin_convertvector(b, h2_t))};
+                }
+            }
         }
     }
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    _Float16* dst = p.O.p + (int64_t)(q0 + (int)(f / G)) * p.O.ts + (int64_t)(note.hk * G + f % G) * p.O.hs;
-#pragma unroll
-    for (int e = 0; e < E; e++) dst[64 * e + lane] = (_Float16)(o[e] * inv);
 }
 
-// Row tiles by the rows of the longest chunk, workers by the steps expected.
+// Row tiles by the rows of the longest chunk, workgroups by the length of the line expected.
 static WorkPlan plan_of(const PagedAttnParams& p) {
     const uint64_t G = p.H / p.geom.Hkv, rows = (uint64_t)(p.max_new ? p.max_new : 1) * G;
     WorkPlan w;
@@ -496,17 +579,17 @@ static WorkPlan plan_of(const PagedAttnParams& p) {
     const uint64_t R = 16 * w.nr;
     uint64_t keys = p.max_kv ? p.max_kv : 1;
     if (p.window) keys = keys < (uint64_t)p.window + p.max_new ? keys : (uint64_t)p.window + p.max_new;
-    const uint64_t units = (keys + kUnit - 1) / kUnit + 1;
     const uint64_t tiles = (rows + R - 1) / R;
-    const uint64_t steps = (uint64_t)p.batch.B * p.geom.Hkv * tiles * units;
-    w.workers = (uint32_t)(steps < 512 ? steps : 512);
+    const uint64_t line = (uint64_t)p.batch.B * p.geom.Hkv * tiles * (keys / kStep + 1 + kItemCost);
+    const uint64_t want = (line + kMinSteps - 1) / kMinSteps;
+    w.groups = (uint32_t)((want < kMaxWaves ? want : kMaxWaves) + kWaves - 1) / kWaves;
     return w;
 }
 
 template <int D>
 static size_t ws_bytes(const WorkPlan& w) {
     const size_t slot = w.nr == 1 ? slot_bytes<D, 1>() : slot_bytes<D, 2>();
-    return (size_t)w.workers * (sizeof(ItemNote) + 2 * slot);
+    return (size_t)w.groups * (sizeof(ItemNote) + 2 * slot);
 }
 
 size_t paged_attn_workspace(const PagedAttnParams& p) {
@@ -515,18 +598,20 @@ size_t paged_attn_workspace(const PagedAttnParams& p) {
 }
 
 template <int FMT, int D, int NR>
-static hipError_t launch_rows(const PagedAttnParams& p, uint32_t workers, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, NR>), dim3(workers), dim3(256), 0, st, p, workers);
+static hipError_t launch_rows(const PagedAttnParams& p, uint32_t groups, hipStream_t st) {
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, NR>), dim3(groups), dim3(64 * kWaves), 0, st, p, groups);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, NR>), dim3(workers, 4 * NR), dim3(256), 0, st, p, workers);
+    // four blocks for each few workgroups: the rows of an item in several parts are spread over them
+    const dim3 join(groups < kJoinBlocks ? groups : kJoinBlocks, 4);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, NR>), join, dim3(256), 0, st, p, groups);
     return hipGetLastError();
 }
 
 template <int FMT, int D>
 static hipError_t launch_format(const PagedAttnParams& p, hipStream_t st) {
     const WorkPlan w = plan_of(p);
-    return w.nr == 1 ? launch_rows<FMT, D, 1>(p, w.workers, st) : launch_rows<FMT, D, 2>(p, w.workers, st);
+    return w.nr == 1 ? launch_rows<FMT, D, 1>(p, w.groups, st) : launch_rows<FMT, D, 2>(p, w.groups, st);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) {
