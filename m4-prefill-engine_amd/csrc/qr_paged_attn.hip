@@ -24,16 +24,25 @@ constexpr uint32_t kItemCost = 4;
 // tiles in flight (three without them: 47 us there), at least kMinSteps of the
 // line each.
 constexpr uint32_t kMaxWaves = 2048, kMinSteps = 2;
+// Chunks: rows of a row tile, workgroups (one a CU), what an item costs beside its
+// key tiles and the least of the line that is worth a workgroup.
+constexpr uint32_t kChunkTile = 256, kChunkGroups = 256, kChunkCost = 2, kChunkMin = 4;
+// Rows times keys of all heads from which chunks of rows are worth it, and the
+// tiles through LDS that they share: us of rows / chunks at H = 32, Hkv = 8,
+// D = 128: 128 rows a head and 2^25 53 / 65, 2^26 85 / 86, 2^27 143 / 110; eight
+// requests of 256 x 1024 (2^26) 77 / 57.
+constexpr uint64_t kChunkWork = (uint64_t)1 << 26;
 constexpr float kNone = -3.402823466e38f;  // reference point of a row that has seen no score above -infinity
 
-// A workgroup's note of an item that begins in its share of the work and ends in
-// later ones': how many workgroups took part.
+// A workgroup's note on its partial rows.  tail: an item begins in its share and
+// goes on in the next one's (slot 1, and which it is); head: the first item of
+// its share began before it (slot 0) and ends here (1) or goes on (2).
 struct ItemNote {
-    uint32_t b, hk, rt, parts;
+    uint32_t b, hk, rt, tail, head, pad[3];
 };
 
 struct WorkPlan {
-    uint32_t nr, groups;
+    uint32_t rows, groups, items;  // of a row tile; workgroups; row tiles of all heads, as expected
 };
 
 // values 1024 + 128 + q of four Q8_0 bytes, as pairs
@@ -51,79 +60,118 @@ __device__ __forceinline__ h2_t q4_pair(uint32_t codes, h2_t d) {
     return (code_pair<HI>(codes) - off) * d;
 }
 
+template <int W>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t w[W]) {
+    if constexpr (W == 1) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (W == 2) {
+        const u2_t a = *reinterpret_cast<const u2_t*>(p);
+        w[0] = a.x;
+        w[1] = a.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 4; i++) {
+            const u4_t a = reinterpret_cast<const u4_t*>(p)[i];
+            w[4 * i] = a.x;
+            w[4 * i + 1] = a.y;
+            w[4 * i + 2] = a.z;
+            w[4 * i + 3] = a.w;
+        }
+    }
+}
+
+// the same through a buffer resource: a lane's offset and a wave's
+template <int W>
+__device__ __forceinline__ void fetch_words(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff, uint32_t w[W]) {
+    if constexpr (W == 1) {
+        w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0);
+    } else if constexpr (W == 2) {
+        const u2_t a = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0);
+        w[0] = a.x;
+        w[1] = a.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 4; i++) {
+            const u4_t a = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, soff, 0);
+            w[4 * i] = a.x;
+            w[4 * i + 1] = a.y;
+            w[4 * i + 2] = a.z;
+            w[4 * i + 3] = a.w;
+        }
+    }
+}
+
+// K values of dims 8 kk .. 8 kk + 7 of a run of codes
+template <int FMT>
+__device__ __forceinline__ h8_t k_octet(const uint32_t* k, int kk, h2_t d) {
+    h2_t a, b, c, e;
+    if constexpr (FMT == QUANT_Q8_0) {
+        a = q8_lo(k[2 * kk], d);
+        b = q8_hi(k[2 * kk], d);
+        c = q8_lo(k[2 * kk + 1], d);
+        e = q8_hi(k[2 * kk + 1], d);
+    } else {
+        const uint32_t lo = k[kk] & 0x0f0f0f0fu, hi = k[kk] >> 4 & 0x0f0f0f0fu;
+        a = q4_pair<false>(lo, d);
+        b = q4_pair<true>(lo, d);
+        c = q4_pair<false>(hi, d);
+        e = q4_pair<true>(hi, d);
+    }
+    return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
+}
+// V values of four keys of dim dt of a run of codes, as two pairs
+template <int FMT>
+__device__ __forceinline__ u2_t v_quad(const uint32_t* v, int dt, u2_t d) {
+    const uint32_t s0 = d.x, s1 = d.y;
+    if constexpr (FMT == QUANT_Q8_0) return u2_t{as_u32(q8_lo(v[dt], as_h2(s0))), as_u32(q8_hi(v[dt], as_h2(s1)))};
+    const uint32_t w = (dt & 1 ? v[dt / 2] >> 4 : v[dt / 2]) & 0x0f0f0f0fu;
+    return u2_t{as_u32(q4_pair<false>(w, as_h2(s0))), as_u32(q4_pair<true>(w, as_h2(s1)))};
+}
+
 // A lane's share of 16 keys: W words of K codes (D / 4 dims of one key) and of V
 // codes (D / 16 dims of four keys), its K scale and four V scales.
 template <int FMT, int D>
 struct Tile {
     static constexpr int W = FMT == QUANT_Q8_0 ? D / 16 : D / 32;
+    static constexpr uint32_t CB = 4 * W * 4, NB = D / 32;  // bytes of a key's codes, blocks
     uint32_t k[W], v[W];
     uint32_t kd;
     u2_t vd;
     bool there;  // its page is one of the cache's
 
-    __device__ __forceinline__ void load(const uint8_t* head, const PageGeom& g, uint32_t slot0, int lane) {
-        constexpr uint32_t CB = 4 * W * 4, NB = D / 32;  // bytes of a key's codes, blocks
-        const uint32_t j = lane & 15, q = lane >> 4;
-        const uint8_t* kp = head + (slot0 + j) * CB + q * (W * 4);
-        const uint8_t* vp = head + g.v_off + ((slot0 >> 2) + q) * (4 * CB) + j * (W * 4);
-        load_words(kp, k);
-        load_words(vp, v);
-        kd = *reinterpret_cast<const uint16_t*>(head + g.ks_off + ((slot0 + j) * NB + q * NB / 4) * 2);
-        vd = *reinterpret_cast<const u2_t*>(head + g.vs_off + (((slot0 >> 2) + q) * NB + j * NB / 16) * 8);
-    }
-    __device__ __forceinline__ static void load_words(const uint8_t* p, uint32_t w[W]) {
-        if constexpr (W == 2) {
-            const u2_t a = *reinterpret_cast<const u2_t*>(p);
-            w[0] = a.x;
-            w[1] = a.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < W / 4; i++) {
-                const u4_t a = reinterpret_cast<const u4_t*>(p)[i];
-                w[4 * i] = a.x;
-                w[4 * i + 1] = a.y;
-                w[4 * i + 2] = a.z;
-                w[4 * i + 3] = a.w;
-            }
+    // a lane's byte offsets of those in a page, but for the tile's first slot
+    struct Offsets {
+        uint32_t k, v, ks, vs;
+        __device__ __forceinline__ Offsets(const PageGeom& g, int lane) {
+            const uint32_t j = lane & 15, q = lane >> 4;
+            k = j * CB + q * (W * 4);
+            v = g.v_off + q * (4 * CB) + j * (W * 4);
+            ks = g.ks_off + (j * NB + q * NB / 4) * 2;
+            vs = g.vs_off + (q * NB + j * NB / 16) * 8;
         }
+    };
+    __device__ __forceinline__ void load(const uint8_t* head, const Offsets& at, uint32_t slot0) {
+        // plain loads: through buffer resources the four requests of 131072 keys take 145 us, so 128
+        load_words<W>(head + slot0 * CB + at.k, k);
+        load_words<W>(head + slot0 * CB + at.v, v);
+        kd = *reinterpret_cast<const uint16_t*>(head + slot0 * (NB * 2) + at.ks);
+        vd = *reinterpret_cast<const u2_t*>(head + slot0 * (NB * 2) + at.vs);
     }
     // operand of contraction step kk: dims 8 kk .. 8 kk + 7 of the lane's run
-    __device__ __forceinline__ h8_t k_frag(int kk) const {
-        const h2_t d = as_h2(kd | kd << 16);
-        h2_t a, b, c, e;
-        if constexpr (FMT == QUANT_Q8_0) {
-            a = q8_lo(k[2 * kk], d);
-            b = q8_hi(k[2 * kk], d);
-            c = q8_lo(k[2 * kk + 1], d);
-            e = q8_hi(k[2 * kk + 1], d);
-        } else {
-            const uint32_t lo = k[kk] & 0x0f0f0f0fu, hi = k[kk] >> 4 & 0x0f0f0f0fu;
-            a = q4_pair<false>(lo, d);
-            b = q4_pair<true>(lo, d);
-            c = q4_pair<false>(hi, d);
-            e = q4_pair<true>(hi, d);
-        }
-        return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
-    }
+    __device__ __forceinline__ h8_t k_frag(int kk) const { return k_octet<FMT>(k, kk, as_h2(kd | kd << 16)); }
     // the four keys of dim dt of the lane's run, as two pairs
-    __device__ __forceinline__ u2_t v_pairs(int dt) const {
-        const uint32_t s0 = vd.x, s1 = vd.y;
-        if constexpr (FMT == QUANT_Q8_0)
-            return u2_t{as_u32(q8_lo(v[dt], as_h2(s0))), as_u32(q8_hi(v[dt], as_h2(s1)))};
-        const uint32_t w = (dt & 1 ? v[dt / 2] >> 4 : v[dt / 2]) & 0x0f0f0f0fu;
-        return u2_t{as_u32(q4_pair<false>(w, as_h2(s0))), as_u32(q4_pair<true>(w, as_h2(s1)))};
-    }
+    __device__ __forceinline__ u2_t v_pairs(int dt) const { return v_quad<FMT>(v, dt, vd); }
 };
 
-template <int D, int NR>
+template <int D, int R>
 __host__ __device__ constexpr size_t slot_bytes() {
-    return (size_t)16 * NR * (D + 2) * 4;
+    return (size_t)R * (D + 2) * 4;
 }
 // workspace: a note per workgroup, then two slots per workgroup of partial rows
 // (O [R][D], reference points [R], sums [R], fp32)
-template <int D, int NR>
+template <int D, int R>
 __device__ __forceinline__ float* slot_of(uint8_t* ws, uint32_t groups, uint32_t w, int which) {
-    return reinterpret_cast<float*>(ws + (size_t)groups * sizeof(ItemNote) + ((size_t)w * 2 + which) * slot_bytes<D, NR>());
+    return reinterpret_cast<float*>(ws + (size_t)groups * sizeof(ItemNote) + ((size_t)w * 2 + which) * slot_bytes<D, R>());
 }
 
 // lane `at`'s value, as a wave-uniform one
@@ -194,7 +242,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     }
     const uint64_t total = lane_u64(incl, 63);
     const uint64_t nw = min((uint64_t)workers, total);
-    if (threadIdx.x == 0) *note = ItemNote{0, 0, 0, 0};
+    if (threadIdx.x == 0) *note = ItemNote{};
     if (lane == 0) head_of[wave] = 0;
     const uint64_t s0 = w < nw ? total * w / nw : 0, s1 = w < nw ? total * (w + 1) / nw : 0;
     uint32_t b = 0;
@@ -219,12 +267,13 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     const h2_t one2 = {(_Float16)1.0f, (_Float16)1.0f};
     const uint32_t pmask = (1u << p.geom.log2_page) - 1;
 
+    const typename Tile<FMT, D>::Offsets at_lane(p.geom, lane);
+
     // the item at work: its rows, and their running state
     f4_t o[NR][DT];
     float m_run[NR], l_run[NR];
     Seq s{};
     uint32_t b_open = 0, hk = 0, rt = 0, rows = 0;
-    uint64_t last = 0;            // its last place on the line
     bool open = false, begun = false;  // it goes on in the next wave's share; its first step was here
 
     auto row_of = [&](const RowsView& v, uint32_t r) {
@@ -249,7 +298,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         }
     };
     auto leave = [&](int which) {
-        float* slot = slot_of<D, NR>(p.ws, groups, blockIdx.x, which);
+        float* slot = slot_of<D, R>(p.ws, groups, blockIdx.x, which);
 #pragma unroll
         for (int q = 0; q < NR; q++) {
             const uint32_t r = 16 * q + j;
@@ -284,7 +333,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         hk = item / s.tiles;
         rt = item % s.tiles;
         b_open = b;
-        last = cur - o1 + line - 1;
         const int p0 = s.len - s.n;  // position of the first new token
 
         // ---- rows ----
@@ -342,7 +390,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                 const uint32_t page = __builtin_amdgcn_readlane(page_ids, 2 * (u - ids_from) + t);
                 tile[t].there = page < p.geom.num_pages;
                 const uint8_t* head = p.geom.pages + ((size_t)(tile[t].there ? page : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
-                tile[t].load(head, p.geom, (uint32_t)(key0 + 16 * t) & pmask, lane);
+                tile[t].load(head, at_lane, (uint32_t)(key0 + 16 * t) & pmask);
             }
         };
         auto step = [&](Tile<FMT, D> tile[2], int u) {
@@ -401,10 +449,20 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             h8_t pf[NR];
 #pragma unroll
             for (int q = 0; q < NR; q++) {
-                // the reference point moves only when a score exceeds it by 2^8
-                float mx = fmaxf(fmaxf(fmaxf(sc[q][0].x, sc[q][0].y), fmaxf(sc[q][0].z, sc[q][0].w)),
-                                 fmaxf(fmaxf(sc[q][1].x, sc[q][1].y), fmaxf(sc[q][1].z, sc[q][1].w))) * c;
-                if (__any(mx > m_run[q] + 8.0f)) {
+                // The reference point moves only when an exponent passes 8.  Positive floats
+                // compare as integers do and negative ones are negative integers, so an
+                // integer maximum (three at a time, no quieting of NaNs) tells.
+                float ex[8];
+                int top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) ex[e] = __builtin_fmaf(sc[q][e >> 2][e & 3], c, -m_run[q]);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) top = max(max(top, (int)f32_bits(ex[e])), (int)f32_bits(ex[e + 1]));
+                if (__any(top > 0x41000000)) {
+                    float mx = sc[q][0].x;
+#pragma unroll
+                    for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[q][e >> 2][e & 3]);
+                    mx *= c;
                     mx = fmaxf(mx, __shfl_xor(mx, 16));
                     mx = fmaxf(mx, __shfl_xor(mx, 32));
                     const float m_new = fmaxf(m_run[q], mx);
@@ -413,14 +471,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     l_run[q] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) o[q][dt] *= alpha;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) ex[e] = __builtin_fmaf(sc[q][e >> 2][e & 3], c, -m_run[q]);
                 }
                 uint32_t pk[4];
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int r = 0; r < 4; r += 2) {
-                        const f2_t e = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[q][t][r], c, -m_run[q])),
-                                        __builtin_amdgcn_exp2f(__builtin_fmaf(sc[q][t][r + 1], c, -m_run[q]))};
+                        const f2_t e = {__builtin_amdgcn_exp2f(ex[4 * t + r]), __builtin_amdgcn_exp2f(ex[4 * t + r + 1])};
                         const h2_t pp = __builtin_convertvector(e, h2_t);
                         pk[2 * t + r / 2] = as_u32(pp);
                         l_run[q] = __builtin_amdgcn_fdot2(pp, one2, l_run[q], false);
@@ -474,6 +533,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             open = false;  // the wave before gathers it
         } else if (!begun && ends) {
             leave(0);
+            if (lane == 0) note->head = 1;
         }
     }
 
@@ -499,8 +559,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         return;
     }
     leave(begun ? 1 : 0);
-    if (begun && lane == 0)
-        *note = ItemNote{b_open, hk, rt, (uint32_t)((((last + 1) * nw - 1) / total) / kWaves) - blockIdx.x + 1};
+    if (lane != 0) return;
+    if (begun) {
+        note->b = b_open;
+        note->hk = hk;
+        note->rt = rt;
+        note->tail = 1;
+    } else {
+        note->head = ended ? 1 : 2;
+    }
 }
 
 // Joins the partial rows of the items that begin in the shares of this block's
@@ -508,9 +575,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 // a row; rows side by side while an item has few parts, else the parts of a row
 // are split over the lane groups, whose sums meet in LDS in a fixed order.
 constexpr uint32_t kJoinBlocks = 512;
-template <int D, int NR>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups) {
-    constexpr uint32_t R = 16 * NR;
+template <int D, int R>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups, uint32_t tile_rows) {
     constexpr int L = D / 4, GROUPS = 256 / L;
     __shared__ f4_t part_sum[256];
     const uint32_t per = (groups + gridDim.x - 1) / gridDim.x, w0 = blockIdx.x * per;
@@ -520,14 +586,24 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
     const uint32_t G = p.H / p.geom.Hkv;
     for (uint32_t base = w0; base < w1; base += 64) {
         const uint32_t mine = base + (tid & 63);
-        uint64_t todo = __ballot(mine < w1 && notes[mine].parts >= 2);
+        uint64_t todo = __ballot(mine < w1 && notes[mine].tail);
         while (todo) {
             const uint32_t w = base + __ffsll((unsigned long long)todo) - 1;
             todo &= todo - 1;
             const ItemNote note = notes[w];
+            uint32_t parts = 2;  // up to the first workgroup in which it ends
+            for (uint32_t k = w + 1; k < groups; k += 64) {
+                const uint32_t x = k + (tid & 63);
+                const uint64_t end = __ballot(x >= groups || notes[x].head != 2);
+                if (end) {
+                    parts = k - w + __ffsll((unsigned long long)end);
+                    break;
+                }
+            }
+            parts = min(parts, groups - w);
             const Seq s = seq_of(p, note.b, R);
-            const uint32_t rows = min(R, (uint32_t)s.n * G - note.rt * R), parts = note.parts;
-            auto slot = [&](uint32_t k) { return slot_of<D, NR>(p.ws, groups, w + k, k == 0 ? 1 : 0); };
+            const uint32_t rows = min(tile_rows, (uint32_t)s.n * G - note.rt * tile_rows);
+            auto slot = [&](uint32_t k) { return slot_of<D, R>(p.ws, groups, w + k, k == 0 ? 1 : 0); };
             uint32_t split = 1;
             while (split < GROUPS && parts > 4 * split) split *= 2;
             const uint32_t side = GROUPS / split;
@@ -560,7 +636,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
                 }
                 if (live && group % split == 0) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const uint32_t f = note.rt * R + r;
+                    const uint32_t f = note.rt * tile_rows + r;
                     _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(f / G)) * p.O.ts + (int64_t)(note.hk * G + f % G) * p.O.hs;
                     const f2_t a = {o.x * inv, o.y * inv}, b = {o.z * inv, o.w * inv};
                     *reinterpret_cast<u2_t*>(dst + 4 * l4) =
@@ -571,24 +647,418 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
     }
 }
 
+// ---- chunks: 32 rows a wave, the keys' tiles shared through LDS ----------------
+
+struct Chunk {
+    uint32_t tile_tokens, tiles;  // tokens of a row tile, row tiles
+};
+
+// Steps (key tiles of KT) of row tile rt, and its first key.
+template <int KT>
+__device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq& s, uint32_t tokens, uint32_t rt, int& lo) {
+    const int first = s.len - s.n + (int)(rt * tokens);
+    const int end = min(first + (int)tokens, s.len);
+    lo = p.window ? (int)(max((int64_t)first + 1 - (int64_t)p.window, (int64_t)0) / KT * KT) : 0;
+    return end <= lo ? 1u : (uint32_t)(end - lo + KT - 1) / KT;
+}
+
+// A workgroup of NW waves takes 32 NW rows (whole tokens' query heads) and an even
+// share of the line of all row tiles' key tiles, as above.  Key tiles of 16 NW
+// keys: every thread turns 32 bytes of K and of V codes (Q4_0: 16) into fp16 in a
+// double-buffered LDS tile, the codes loaded two tiles ahead; then each wave
+// takes its rows over the tile, 32 x 32 scores at a time.
+template <int FMT, int D, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
+    constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
+    constexpr int DT = D / 32, KK = D / 16;
+    constexpr int KU = D / 8, VU = KT / 8;       // 16-byte units of a K row (a key), of a V^T row (a dim)
+    constexpr int KB = KT * D * 2, TB = 2 * KB;  // bytes of a K tile, of a tile
+    constexpr int RUN = D / 4;                   // dims of a K task: a quarter of a key
+    constexpr int DV = D / 32;                   // dims of a V task: 8 keys of each
+    constexpr int KW = FMT == QUANT_Q8_0 ? RUN / 4 : RUN / 8, VW = FMT == QUANT_Q8_0 ? DV : DV / 2;
+    constexpr uint32_t CB = 4 * KW * 4, NB = D / 32;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ uint8_t bad_v[2][64 * NW];  // of each thread's V task: keys whose scale is not finite
+    __shared__ int there[2][NW];           // of each 16 keys: their page is one of the cache's
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 5, j = lane & 31;
+    ItemNote* note = reinterpret_cast<ItemNote*>(p.ws) + blockIdx.x;
+    const uint32_t G = p.H / p.geom.Hkv, tokens = R / G;
+    const uint32_t pmask = (1u << p.geom.log2_page) - 1;
+
+    // ---- this workgroup's share [s0, s1) ----
+    auto heads_cost = [&](const Seq& s) {  // of one KV head's row tiles
+        uint64_t c = 0;
+        int lo;
+        const uint32_t tiles = ((uint32_t)s.n + tokens - 1) / tokens;
+        for (uint32_t rt = 0; rt < tiles; rt++) c += kChunkCost + steps_of<KT>(p, s, tokens, rt, lo);
+        return c;
+    };
+    const uint32_t per = (p.batch.B + 63) / 64;
+    const uint32_t b_lo = min(lane * per, p.batch.B), b_hi = min(b_lo + per, p.batch.B);
+    uint64_t mine = 0;
+    for (uint32_t x = b_lo; x < b_hi; x++) mine += heads_cost(seq_of(p, x, R)) * p.geom.Hkv;
+    uint64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t x = __shfl_up((unsigned long long)incl, o);
+        if (lane >= o) incl += x;
+    }
+    const uint64_t total = lane_u64(incl, 63);
+    const uint64_t nw = max(min((uint64_t)groups, total / kChunkMin), (uint64_t)1);
+    if (tid == 0) *note = ItemNote{};
+    if (blockIdx.x >= nw || total == 0) return;
+    const uint64_t s0 = total * blockIdx.x / nw, s1 = total * (blockIdx.x + 1) / nw;
+    uint32_t b = 0;
+    uint64_t off = 0;
+    const bool here = incl - mine <= s0 && s0 < incl;
+    if (here) {
+        off = s0 - (incl - mine);
+        for (b = b_lo; b + 1 < b_hi; b++) {
+            const uint64_t cost = heads_cost(seq_of(p, b, R)) * p.geom.Hkv;
+            if (off < cost) break;
+            off -= cost;
+        }
+    }
+    const int at = max(__ffsll((unsigned long long)__ballot(here)) - 1, 0);
+    b = __builtin_amdgcn_readlane(b, at);
+    off = lane_u64(off, at);
+
+    float c = p.scale * 1.4426950408889634f;  // log2 units
+    const bool neg = c < 0.0f;
+    if (neg) c = -c;
+    c = fmaxf(c, 1.17549435e-38f);
+
+    // Unit u of row r of a tile sits at u ^ swz(r).  A row's units differ from one
+    // base by the exclusive or of 16 times their number: the bases alone are kept
+    // (hidden from the compiler, which would keep every sum).
+    auto swz = [](int units, uint32_t r) -> uint32_t { return units == 16 ? (r & 15u) : ((r ^ (r >> 3)) & 7u); };
+    auto place = [&](int units, uint32_t r, uint32_t u) { return r * (units * 16u) + 16u * (u ^ swz(units, r & 31u)); };
+    uint32_t kof = place(KU, (uint32_t)j, (uint32_t)g), vof = place(VU, (uint32_t)j, (uint32_t)g);
+    // tasks: K, a quarter of key 16 wave + lane / 4; V, dims DV (lane % 32) .. of
+    // unit 2 wave + lane / 32, i.e. keys 16 wave + 4 g + {0 .. 3, 8 .. 11}
+    const uint32_t kkey = lane >> 2, kq = lane & 3, vdim = DV * (uint32_t)j;
+    uint32_t kst = place(KU, 16 * wave + kkey, kq * (RUN / 8)), vst = place(VU, vdim, 2 * wave + g);
+    uint32_t kld = kkey * CB + kq * (KW * 4), vld = p.geom.v_off + g * (4 * CB) + vdim * (4 * CB / D);
+    uint32_t ksl = p.geom.ks_off + (kkey * NB + kq * NB / 4) * 2, vsl = p.geom.vs_off + (g * NB + vdim / 32) * 8;
+    const h2_t one2 = {(_Float16)1.0f, (_Float16)1.0f};
+
+    f16v_t o[DT];
+    float m_run = kNone, l_run = 0.0f;
+    Seq s{};
+    uint64_t row_cost = 0;  // of a KV head of the sequence at work
+    uint32_t at_b = 0xffffffffu;
+
+    for (uint64_t cur = s0; cur < s1 && b < p.batch.B;) {
+        if (b != at_b) {
+            s = seq_of(p, b, R);
+            row_cost = lane_u64(heads_cost(s), 0);
+            at_b = b;
+        }
+        if (off >= row_cost * p.geom.Hkv) {
+            b++;
+            off = 0;
+            continue;
+        }
+        const uint32_t hk = (uint32_t)(off / row_cost);
+        uint64_t in_row = off - hk * row_cost;
+        uint32_t rt = 0, steps;
+        int lo;
+        for (;; rt++) {  // the row tile at this place
+            steps = __builtin_amdgcn_readfirstlane(steps_of<KT>(p, s, tokens, rt, lo));
+            if (in_row < kChunkCost + steps) break;
+            in_row -= kChunkCost + steps;
+        }
+        const uint32_t line = kChunkCost + steps, o0 = (uint32_t)in_row;
+        const uint32_t o1 = (uint32_t)min((uint64_t)line, o0 + (s1 - cur));
+        cur += o1 - o0;
+        off += o1 - o0;
+        if (o1 <= kChunkCost) continue;
+        const int u0 = (int)(o0 > kChunkCost ? o0 - kChunkCost : 0), u1 = (int)(o1 - kChunkCost);
+        const bool begun = u0 == 0, ends = u1 == (int)steps;
+
+        // ---- rows ----
+        const uint32_t rows = min(tokens * G, ((uint32_t)s.n - rt * tokens) * G);
+        const int p0 = s.len - s.n + (int)(rt * tokens);  // position of the tile's first token
+        const uint32_t r = 32 * wave + j, rc = min(r, rows - 1);
+        const bool wave_live = 32u * wave < rows;
+        const int lim = p0 + (int)(rc / G);
+        const int low = p.window ? (int)max((int64_t)lim + 1 - (int64_t)p.window, (int64_t)0) : 0;
+        // of this wave's rows, and of all
+        const int lim0 = p0 + (int)(min(32u * wave, rows - 1) / G), lim1 = p0 + (int)(min(32u * wave + 31, rows - 1) / G);
+        const int all0 = p0, all1 = p0 + (int)((rows - 1) / G);
+        auto lowest = [&](int l) { return p.window ? (int)max((int64_t)l + 1 - (int64_t)p.window, (int64_t)0) : 0; };
+        const int low0 = lowest(lim0), low1 = lowest(lim1), all_low1 = lowest(all1);
+        h8_t qf[KK];
+        {
+            const _Float16* src = p.Q.p + (int64_t)(s.q0 + (int)(rt * tokens + rc / G)) * p.Q.ts +
+                                  (int64_t)(hk * G + rc % G) * p.Q.hs + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                qf[kk] = *reinterpret_cast<const h8_t*>(src + 16 * kk);
+                if (neg) qf[kk] = -qf[kk];
+            }
+        }
+        m_run = kNone;
+        l_run = 0.0f;
+        uint32_t poison = 0;  // bit t: dims 32 t .. saw a V scale that is not finite
+#pragma unroll
+        for (int t = 0; t < DT; t++) o[t] = f16v_t{};
+
+        // ---- codes of a tile into registers, and from there into LDS ----
+        uint32_t kw[KW], vw[2][VW], kd = 0;
+        u2_t vd[2];
+        bool mine_there = false;
+        uint32_t page_ids = 0;
+        int ids_from = u0 - 64;
+        auto fetch = [&](int u) {
+            if (u >= ids_from + 64) {
+                ids_from = u;
+                const int k0 = lo + (u + lane) * KT + 16 * wave;
+                page_ids = k0 < s.len ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k0 >> p.geom.log2_page)]
+                                      : 0xffffffffu;
+            }
+            const uint32_t page = __builtin_amdgcn_readlane(page_ids, u - ids_from);
+            mine_there = page < p.geom.num_pages;
+            const uint32_t slot = (uint32_t)(lo + u * KT + 16 * wave) & pmask;
+            const uint8_t* head = p.geom.pages + ((size_t)(mine_there ? page : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
+            const auto rs = make_rsrc(head, p.geom.head_bytes);
+            fetch_words<KW>(rs, kld, slot * CB, kw);
+            kd = __builtin_amdgcn_raw_buffer_load_b16(rs, ksl, slot * (NB * 2), 0);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                fetch_words<VW>(rs, vld + 2 * h * (4 * CB), slot * CB, vw[h]);
+                vd[h] = __builtin_amdgcn_raw_buffer_load_b64(rs, vsl + 2 * h * NB * 8, slot * (NB * 2), 0);
+            }
+        };
+        auto fill = [&](int u) {
+            uint8_t* buf = smem + (u & 1) * TB;
+            const int k0 = lo + u * KT;
+            asm volatile("" : "+v"(kst), "+v"(vst));
+            const h2_t d = as_h2(kd | kd << 16);
+#pragma unroll
+            for (int kk = 0; kk < RUN / 8; kk++)
+                *reinterpret_cast<h8_t*>(buf + (kst ^ 16u * kk)) = k_octet<FMT>(kw, kk, d);
+            if (lane == 0) there[u & 1][wave] = mine_there || k0 + 16 * wave >= s.len;
+            uint32_t bad = 0;
+            if (k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !mine_there) {
+                // not all rows see all of the tile's keys: V scales of keys that none sees are
+                // cleared, and those that are not finite noted for the rows that do
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t e[4] = {vd[h].x & 0xffffu, vd[h].x >> 16, vd[h].y & 0xffffu, vd[h].y >> 16};
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const bool dead = !mine_there || k0 + 16 * wave + 4 * g + 8 * h + x >= s.len;
+                        if (!dead && (e[x] & 0x7c00u) == 0x7c00u) bad |= 1u << (4 * h + x);
+                        if (dead || (bad >> (4 * h + x) & 1)) e[x] = 0;
+                    }
+                    vd[h] = u2_t{e[0] | e[1] << 16, e[2] | e[3] << 16};
+                }
+            }
+            bad_v[u & 1][tid] = (uint8_t)bad;
+#pragma unroll
+            for (int x = 0; x < DV; x++) {
+                const u2_t a = v_quad<FMT>(vw[0], x, vd[0]), e = v_quad<FMT>(vw[1], x, vd[1]);
+                *reinterpret_cast<u4_t*>(buf + KB + x * (VU * 16) + (vst ^ 16u * x)) = u4_t{a.x, a.y, e.x, e.y};
+            }
+        };
+
+        // ---- this wave's rows over a tile, 32 keys (a unit) at a time ----
+        auto scores = [&](const uint8_t* buf, int x) {
+            const uint8_t* kb = buf + x * 32 * (KU * 16);
+            f16v_t sc{};
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8_t*>(kb + (kof ^ 32u * kk)), qf[kk], sc, 0, 0, 0);
+            return sc;
+        };
+        // Exponents of a unit's weights, beside the reference point.  That moves only
+        // when one passes 8: positive floats compare as integers do, negative ones are
+        // negative integers, so one integer maximum (three at a time, and with no
+        // quieting of NaNs) tells.
+        auto exponents = [&](const f16v_t& sc, float ex[16]) {
+            int top = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) ex[e] = __builtin_fmaf(sc[e], c, -m_run);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) top = max(max(top, (int)f32_bits(ex[e])), (int)f32_bits(ex[e + 1]));
+            if (__any(top > (int)0x41000000)) {
+                float mx = sc[0];
+#pragma unroll
+                for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
+                mx *= c;
+                const float m_new = fmaxf(m_run, fmaxf(mx, __shfl_xor(mx, 32)));
+                const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; t++) o[t] *= alpha;
+#pragma unroll
+                for (int e = 0; e < 16; e++) ex[e] = __builtin_fmaf(sc[e], c, -m_run);
+            }
+        };
+        auto weigh = [&](const float ex[16], uint32_t pk[8]) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const f2_t w = {__builtin_amdgcn_exp2f(ex[e]), __builtin_amdgcn_exp2f(ex[e + 1])};
+                const h2_t pp = __builtin_convertvector(w, h2_t);
+                pk[e >> 1] = as_u32(pp);
+                l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+            }
+        };
+        auto add = [&](const uint8_t* buf, int x, const uint32_t pk[8]) {
+#pragma unroll
+            for (int t2 = 0; t2 < 2; t2++) {
+                const h8_t pf = __builtin_bit_cast(h8_t, u4_t{pk[4 * t2], pk[4 * t2 + 1], pk[4 * t2 + 2], pk[4 * t2 + 3]});
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+                    const h8_t va = *reinterpret_cast<const h8_t*>(buf + KB + t * 32 * (VU * 16) + (vof ^ 32u * (2 * x + t2)));
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pf, o[t], 0, 0, 0);
+                }
+            }
+        };
+        auto attend = [&](int u) {
+            const uint8_t* buf = smem + (u & 1) * TB;
+            asm volatile("" : "+v"(kof), "+v"(vof));
+            const int k0 = lo + u * KT;
+            if (!wave_live || k0 > lim1 || k0 + KT - 1 < low0) return;
+            bool all_there = true;
+#pragma unroll
+            for (int x = 0; x < NW; x++) all_there &= there[u & 1][x] != 0;
+            if (!(k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !all_there)) {
+                // every row sees every key: the next unit's scores are computed beside this
+                // one's weights
+                f16v_t sc = scores(buf, 0);
+#pragma unroll
+                for (int x = 0; x < UNITS; x++) {
+                    float ex[16];
+                    exponents(sc, ex);
+                    uint32_t pk[8];
+                    if (x + 1 < UNITS) sc = scores(buf, x + 1);
+                    weigh(ex, pk);
+                    add(buf, x, pk);
+                }
+                return;
+            }
+            uint32_t any = 0;
+#pragma unroll
+            for (int x = 0; x < NW; x++) any |= bad_v[u & 1][64 * x + lane];
+            if (__any(any != 0)) {
+                for (int x = 0; x < 64 * NW; x++) {
+                    const uint32_t bits = bad_v[u & 1][x];
+                    for (int e = 0; e < 8; e++) {
+                        const int key = k0 + 16 * (x >> 6) + 4 * (x >> 5 & 1) + (e >> 2) * 8 + (e & 3);
+                        if ((bits >> e & 1) && key <= lim && key >= low) poison |= 1u << ((x & 31) * DV / 32);
+                    }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < UNITS; x++) {
+                const int key0 = k0 + 32 * x;
+                if (key0 > lim1 || key0 + 31 < low0) continue;
+                f16v_t sc = scores(buf, x);
+                if (key0 + 31 > lim0 || key0 < low1 || !all_there) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int key = key0 + 8 * (e >> 2) + 4 * g + (e & 3);
+                        if (key > lim || key < low || !there[u & 1][2 * x + (e >> 3)]) sc[e] = -INFINITY;
+                    }
+                }
+                float ex[16];
+                exponents(sc, ex);
+                uint32_t pk[8];
+                weigh(ex, pk);
+                add(buf, x, pk);
+            }
+        };
+
+        fetch(u0);
+        fill(u0);
+        if (u0 + 1 < u1) fetch(u0 + 1);
+        __syncthreads();
+        for (int u = u0; u < u1; u++) {
+            if (u + 1 < u1) fill(u + 1);
+            if (u + 2 < u1) fetch(u + 2);
+            attend(u);
+            __syncthreads();
+        }
+
+        l_run += __shfl_xor(l_run, 32);
+        if (poison) {
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+                if (poison >> t & 1)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[t][e] = NAN;
+        }
+        // lane (j, g): row 32 wave + j, dims 32 t + 8 (e / 4) + 4 g + e % 4
+        if (begun && ends) {
+            if (r < rows) {
+                const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+                _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(rt * tokens + r / G)) * p.O.ts + (int64_t)(hk * G + r % G) * p.O.hs;
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const f2_t x = {o[t][4 * q] * inv, o[t][4 * q + 1] * inv}, y = {o[t][4 * q + 2] * inv, o[t][4 * q + 3] * inv};
+                        *reinterpret_cast<u2_t*>(dst + 32 * t + 8 * q + 4 * g) =
+                            u2_t{as_u32(__builtin_convertvector(x, h2_t)), as_u32(__builtin_convertvector(y, h2_t))};
+                    }
+            }
+        } else {
+            float* slot = slot_of<D, R>(p.ws, groups, blockIdx.x, begun ? 1 : 0);
+            if (r < rows) {
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        *reinterpret_cast<f4_t*>(slot + r * D + 32 * t + 8 * q + 4 * g) =
+                            f4_t{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]};
+                if (g == 0) {
+                    slot[R * D + r] = m_run;
+                    slot[R * D + R + r] = l_run;
+                }
+            }
+            if (tid == 0) {
+                if (begun) {
+                    note->b = b;
+                    note->hk = hk;
+                    note->rt = rt;
+                    note->tail = 1;
+                } else {
+                    note->head = ends ? 1 : 2;
+                }
+            }
+        }
+    }
+}
+
 // Row tiles by the rows of the longest chunk, workgroups by the length of the line expected.
 static WorkPlan plan_of(const PagedAttnParams& p) {
-    const uint64_t G = p.H / p.geom.Hkv, rows = (uint64_t)(p.max_new ? p.max_new : 1) * G;
+    const uint64_t G = p.H / p.geom.Hkv, max_new = p.max_new ? p.max_new : 1, rows = max_new * G;
     WorkPlan w;
-    w.nr = rows <= 16 ? 1 : 2;
-    const uint64_t R = 16 * w.nr;
+    w.rows = rows <= 16 ? 16 : 32;
     uint64_t keys = p.max_kv ? p.max_kv : 1;
-    if (p.window) keys = keys < (uint64_t)p.window + p.max_new ? keys : (uint64_t)p.window + p.max_new;
-    const uint64_t tiles = (rows + R - 1) / R;
-    const uint64_t line = (uint64_t)p.batch.B * p.geom.Hkv * tiles * (keys / kStep + 1 + kItemCost);
-    const uint64_t want = (line + kMinSteps - 1) / kMinSteps;
-    w.groups = (uint32_t)((want < kMaxWaves ? want : kMaxWaves) + kWaves - 1) / kWaves;
+    if (p.window) keys = keys < (uint64_t)p.window + max_new ? keys : (uint64_t)p.window + max_new;
+    if (rows >= kChunkTile / 2 && G <= kChunkTile && (uint64_t)p.batch.T * p.H * keys >= kChunkWork)
+        w.rows = kChunkTile;
+    const uint64_t tiles = (uint64_t)p.batch.B * p.geom.Hkv * ((rows + w.rows - 1) / w.rows);
+    w.items = (uint32_t)(tiles < 0xffffffffu ? tiles : 0xffffffffu);
+    if (w.rows == kChunkTile) {
+        const uint64_t want = tiles * (keys / (kChunkTile / 2) + 1 + kChunkCost) / kChunkMin + 1;
+        w.groups = (uint32_t)(want < kChunkGroups ? want : kChunkGroups);
+    } else {
+        const uint64_t want = (tiles * (keys / kStep + 1 + kItemCost) + kMinSteps - 1) / kMinSteps;
+        w.groups = (uint32_t)((want < kMaxWaves ? want : kMaxWaves) + kWaves - 1) / kWaves;
+    }
     return w;
 }
 
 template <int D>
 static size_t ws_bytes(const WorkPlan& w) {
-    const size_t slot = w.nr == 1 ? slot_bytes<D, 1>() : slot_bytes<D, 2>();
+    const size_t slot = w.rows == 16 ? slot_bytes<D, 16>() : (w.rows == 32 ? slot_bytes<D, 32>() : slot_bytes<D, kChunkTile>());
     return (size_t)w.groups * (sizeof(ItemNote) + 2 * slot);
 }
 
@@ -597,21 +1067,40 @@ size_t paged_attn_workspace(const PagedAttnParams& p) {
     return p.D == 64 ? ws_bytes<64>(w) : ws_bytes<128>(w);
 }
 
-template <int FMT, int D, int NR>
-static hipError_t launch_rows(const PagedAttnParams& p, uint32_t groups, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, NR>), dim3(groups), dim3(64 * kWaves), 0, st, p, groups);
-    hipError_t e = hipGetLastError();
+template <int D, int R>
+static hipError_t launch_join(const PagedAttnParams& p, uint32_t groups, uint32_t items, uint32_t tile_rows, hipStream_t st) {
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // four blocks for each few workgroups: the rows of an item in several parts are spread over them
-    const dim3 join(groups < kJoinBlocks ? groups : kJoinBlocks, 4);
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, NR>), join, dim3(256), 0, st, p, groups);
+    // Blocks for each few workgroups, over which the rows of an item are spread: more
+    // where items have many parts.  us of the whole call with 4 / 16 of them: 64 tokens
+    // over 16384 keys (32 parts an item) 82 / 42, one token 27 / 23, 64 requests (one
+    // part) 34 / 40.
+    const uint32_t parts = groups / items, across = R > 32 ? 32 : (parts >= 16 ? 16 : (parts >= 8 ? 8 : 4));
+    const uint32_t most = 4 * kJoinBlocks / across;
+    const dim3 grid(groups < most ? groups : most, across);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, R>), grid, dim3(256), 0, st, p, groups, tile_rows);
     return hipGetLastError();
 }
 
 template <int FMT, int D>
 static hipError_t launch_format(const PagedAttnParams& p, hipStream_t st) {
     const WorkPlan w = plan_of(p);
-    return w.nr == 1 ? launch_rows<FMT, D, 1>(p, w.groups, st) : launch_rows<FMT, D, 2>(p, w.groups, st);
+    if (w.rows == kChunkTile) {
+        constexpr int NW = kChunkTile / 32;
+        constexpr size_t lds = 2 * 2 * 16 * NW * D * 2;
+        static size_t attr[kMaxDevices] = {};  // more than the default 64 KB of LDS
+        const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW>, lds, attr);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW>), dim3(w.groups), dim3(64 * NW), lds, st, p, w.groups);
+        const uint32_t G = p.H / p.geom.Hkv;
+        return launch_join<D, kChunkTile>(p, w.groups, w.items, kChunkTile / G * G, st);
+    }
+    if (w.rows == 16) {
+        hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1>), dim3(w.groups), dim3(64 * kWaves), 0, st, p, w.groups);
+        return launch_join<D, 16>(p, w.groups, w.items, 16, st);
+    }
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2>), dim3(w.groups), dim3(64 * kWaves), 0, st, p, w.groups);
+    return launch_join<D, 32>(p, w.groups, w.items, 32, st);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) {
