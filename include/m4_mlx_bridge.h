@@ -286,17 +286,25 @@ typedef struct {
 } m4_rows_t;
 
 /* Rotary positions with several axes (time, height, width): pair i of `pairs`
- * (a multiple of 8, at most 128) turns by positions[pair_axis[i]][token] *
- * inv_freq[i]; pairs are dims (i, i + pairs), or (2 i, 2 i + 1) when
- * traditional; dims from 2 * pairs on stay.  Angles keep their precision at any
- * int32 position. */
-enum { M4_ROPE_MAX_PAIRS = 128 };
+ * (a multiple of 8, at most 128) turns by positions[axis of i][token] times its
+ * inverse frequency; pairs are dims (i, i + pairs), or (2 i, 2 i + 1) when
+ * traditional; dims from 2 * pairs on stay.  `table`: device memory, 16-byte
+ * aligned, that holds what m4_bridge_rope_axes_table wrote for these pairs and
+ * axes; a program keeps it as it keeps weights. */
+enum { M4_ROPE_MAX_PAIRS = 128, M4_ROPE_PAIR_BYTES = 12 };
 typedef struct {
     uint32_t pairs, axes;
     int traditional;
-    uint8_t pair_axis[M4_ROPE_MAX_PAIRS];
-    double inv_freq[M4_ROPE_MAX_PAIRS];
+    const void* table;
+    size_t table_bytes;
 } m4_rope_axes_t;
+
+/* Writes the table of `pairs` inverse frequencies (radians per position, finite)
+ * and their axes (each below `axes`) to host memory: M4_ROPE_PAIR_BYTES a pair.
+ * The frequencies come first, in turns as 64-bit fractions, then the axes, 32 bits
+ * each; angles keep their precision at any int32 position.  Host arithmetic only.  0, -2 (null), -4. */
+M4_API int m4_bridge_rope_axes_table(const double* inv_freq, const uint8_t* pair_axis, uint32_t pairs, uint32_t axes,
+                                     void* table);
 
 /* Bytes of a cache, 0 for a format or dimension that it does not take. */
 M4_API size_t m4_bridge_kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D);

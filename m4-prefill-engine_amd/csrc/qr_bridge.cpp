@@ -12,7 +12,6 @@
 #include <unistd.h>
 
 #include <cerrno>
-#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -421,20 +420,8 @@ qr::PageGeom cache_geom(const m4_kv_cache_t* c) {
     return qr::page_geom(c->pages, c->format, c->num_pages, c->page_size, c->Hkv, c->D);
 }
 
-// Frequencies in turns, as 64-bit fractions of one: whole turns per position
-// drop out because positions are whole.  Double keeps a turn to 2^-23 at the
-// farthest position.
-void rope_table(const m4_rope_axes_t* r, const int32_t* positions, uint32_t stride, qr::RopeTable& t) {
-    t.pairs = r->pairs;
-    t.traditional = r->traditional ? 1 : 0;
-    t.positions = positions;
-    t.position_stride = stride;
-    for (uint32_t i = 0; i < r->pairs; i++) {
-        const double turns = r->inv_freq[i] * 0.15915494309189533576888376337251;
-        const double part = turns - floor(turns);  // 1 for a tiny negative frequency: no turn
-        t.turn[i] = part < 1.0 ? (uint64_t)(part * 18446744073709551616.0) : 0;
-        t.axis[i] = r->pair_axis[i];
-    }
+qr::RopeView rope_view(const m4_rope_axes_t* r, const int32_t* positions, uint32_t stride) {
+    return {static_cast<const uint64_t*>(r->table), r->pairs, r->axes, r->traditional ? 1 : 0, positions, stride};
 }
 
 qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, uint32_t H, uint32_t window) {
@@ -897,6 +884,11 @@ size_t m4_bridge_kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_si
     return qr::kv_cache_bytes(format, num_pages, page_size, Hkv, D);
 }
 
+int m4_bridge_rope_axes_table(const double* inv_freq, const uint8_t* pair_axis, uint32_t pairs, uint32_t axes,
+                              void* table) {
+    return qr::rope_axes_table(inv_freq, pair_axis, pairs, axes, table);
+}
+
 int m4_bridge_validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
                                  const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D) {
     bool empty;
@@ -911,14 +903,14 @@ int m4_bridge_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, ui
     if (rc || empty) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
-    if (!dev.owns_all(positions, X->ptr, Y->ptr)) return -2;
+    if (!dev.owns_all(rope->table, positions, X->ptr, Y->ptr)) return -2;
     qr::AppendParams p{};
     p.Q = rows_view(X);
     p.Qo = rows_view(Y);
     p.H = H;
     p.T = T;
     p.D = D;
-    rope_table(rope, positions, position_stride, p.rope);
+    p.rope = rope_view(rope, positions, position_stride);
     return launched(qr::launch_kv_append(p, g_stream), "rope_axes");
 }
 
@@ -940,6 +932,7 @@ int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* b
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
     if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, K->ptr, V->ptr)) return -2;
+    if (rope && !dev.owns_all(rope->table)) return -2;
     if (rope && positions && !dev.owns_all(positions)) return -2;
     if (Q && !dev.owns_all(Q->ptr, Q_out->ptr)) return -2;
     qr::AppendParams p{};
@@ -955,7 +948,7 @@ int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* b
     p.format = cache->format;
     p.geom = cache_geom(cache);
     p.batch = batch_view(batch);
-    if (rope) rope_table(rope, positions, position_stride, p.rope);
+    if (rope) p.rope = rope_view(rope, positions, position_stride);
     return launched(qr::launch_kv_append(p, g_stream), "kv_cache_append");
 }
 

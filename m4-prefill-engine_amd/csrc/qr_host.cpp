@@ -8,6 +8,7 @@
 
 #include <cerrno>
 #include <cmath>
+#include <cstring>
 
 namespace qr {
 
@@ -149,9 +150,9 @@ int check_rows(const m4_rows_t* r, uint32_t T, uint32_t heads, uint32_t D, bool 
 }
 
 int check_rope(const m4_rope_axes_t* r, uint32_t D) {
-    if (r->pairs == 0 || r->pairs > M4_ROPE_MAX_PAIRS || r->pairs % 8 || 2 * r->pairs > D || r->axes == 0) return -4;
-    for (uint32_t i = 0; i < r->pairs; i++)
-        if (r->pair_axis[i] >= r->axes || !std::isfinite(r->inv_freq[i])) return -4;
+    if (r->pairs == 0 || r->pairs > M4_ROPE_MAX_PAIRS || r->pairs % 8 || 2 * r->pairs > D) return -4;
+    if (r->axes == 0 || r->axes > 256) return -4;
+    if (!r->table || misaligned(r->table, 16) || r->table_bytes < (size_t)r->pairs * M4_ROPE_PAIR_BYTES) return -2;
     return 0;
 }
 
@@ -161,6 +162,26 @@ int check_positions(const int32_t* positions, uint32_t stride, uint32_t axes, ui
 }
 
 }  // namespace
+
+// Frequencies in turns, as 64-bit fractions of one: whole turns per position
+// drop out because positions are whole.  Double keeps a turn to 2^-23 at the
+// farthest position.
+int rope_axes_table(const double* inv_freq, const uint8_t* pair_axis, uint32_t pairs, uint32_t axes, void* table) {
+    if (!inv_freq || !pair_axis || !table) return -2;
+    if (pairs == 0 || pairs > M4_ROPE_MAX_PAIRS || pairs % 8 || axes == 0 || axes > 256) return -4;
+    for (uint32_t i = 0; i < pairs; i++)
+        if (pair_axis[i] >= axes || !std::isfinite(inv_freq[i])) return -4;
+    uint8_t* out = static_cast<uint8_t*>(table);
+    for (uint32_t i = 0; i < pairs; i++) {
+        const double turns = inv_freq[i] * 0.15915494309189533576888376337251;
+        const double part = turns - std::floor(turns);  // 1 for a tiny negative frequency: no turn
+        const uint64_t turn = part < 1.0 ? (uint64_t)(part * 18446744073709551616.0) : 0;
+        const uint32_t axis = pair_axis[i];
+        std::memcpy(out + 8 * i, &turn, 8);
+        std::memcpy(out + 8 * pairs + 4 * i, &axis, 4);
+    }
+    return 0;
+}
 
 int validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t stride, const m4_rows_t* X,
                        const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D, bool* empty) {

@@ -22,6 +22,8 @@ bool has_kernels(int f);
 int validate(const void* X, size_t Xb, const void* W, size_t Wb, const void* Y, size_t Yb, int format,
              uint32_t M, uint32_t K, uint32_t N, bool ext = false);
 
+// The table of a rotary embedding (m4_bridge_rope_axes_table).
+int rope_axes_table(const double* inv_freq, const uint8_t* pair_axis, uint32_t pairs, uint32_t axes, void* table);
 // Bytes of a paged cache (0: not a cache), and the codes that the serving entry
 // points return for their arguments; *empty: valid, with no rows to work on.
 size_t kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D);

@@ -3,6 +3,12 @@
 #include "qr_device.h"
 #include "qr_paged.h"
 
+#ifndef QR_GR
+#define QR_GR 1024
+#endif
+#ifndef QR_GB
+#define QR_GB 1024
+#endif
 namespace qr {
 
 // Where a token lies in the cache.
@@ -77,7 +83,9 @@ __device__ __forceinline__ void quantize8(const float x[8], int lane, uint32_t c
         }
         key = max(key, (uint32_t)__shfl_xor((int)key, 1));
         key = max(key, (uint32_t)__shfl_xor((int)key, 2));
-        const float d = h2f(key >> 6 | (key & 1u) << 15) / -8.0f;
+        float d = h2f(key >> 6 | (key & 1u) << 15) / -8.0f;
+        // apart from the rounding below: as one mixed-precision instruction the two lose a zero's sign
+        asm volatile("" : "+v"(d));
         const float id = d != 0.0f ? 1.0f / d : 0.0f;
         d16 = f2h_bits(d);
 #pragma unroll
@@ -93,31 +101,35 @@ __device__ __forceinline__ void quantize8(const float x[8], int lane, uint32_t c
 // formed once per wave and used for all its heads.  A rotated row is rounded to
 // fp16 before it is quantized, as a rotation and a write apart would.
 template <int LPR, int FMT>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t chunks) {
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p) {
     constexpr int RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l = lane % LPR, sub = lane / LPR;
-    const uint32_t t0 = blockIdx.x * RPW, t = t0 + sub;
-    const uint32_t chunk = blockIdx.y * 4 + wave;
+    const uint32_t t0 = (blockIdx.x * 4 + wave) * RPW, t = t0 + sub, chunk = blockIdx.y, chunks = gridDim.y;
     const bool cached = p.geom.pages != nullptr;
     const uint32_t items = p.H + (cached ? 2 * p.geom.Hkv : 0);
-    if (chunk >= items) return;
+    if (t0 >= p.T) return;
     const bool live = t < p.T && 8u * l < p.D;
 
-    // the rows of one head ahead of the one at work; the first are under way while
-    // places and angles are found
-    auto fetch = [&](uint32_t it) {
-        h8_t y{};
-        if (it < items && live) {
+    // Rows of kAhead heads are loaded together, those of the next kAhead while these
+    // are turned and stored; the first are under way while places and angles are found.
+    constexpr int kAhead = 4;
+    h8_t next[kAhead];
+    auto fetch = [&](uint32_t it0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const uint32_t it = it0 + i * chunks;
+            if (it >= items || !live) continue;
             const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
             const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
             const _Float16* src = is_q ? p.Q.p : (is_k ? p.K.p : p.V.p);
             const int64_t ts = is_q ? p.Q.ts : (is_k ? p.K.ts : p.V.ts), hs = is_q ? p.Q.hs : (is_k ? p.K.hs : p.V.hs);
-            y = *reinterpret_cast<const h8_t*>(src + (int64_t)t * ts + (int64_t)h * hs + 8 * l);
+            next[i] = *reinterpret_cast<const h8_t*>(src + (int64_t)t * ts + (int64_t)h * hs + 8 * l);
         }
-        return y;
     };
-    h8_t next = fetch(chunk);
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) next[i] = h8_t{};
+    fetch(chunk);
 
     Place at{0, 0, 0, false};
     bool row = live;
@@ -145,15 +157,28 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
     float cs[8], sn[8];
     if (turned && row) {
         const int n = p.rope.traditional ? 4 : 8;
+        const uint32_t* axis = reinterpret_cast<const uint32_t*>(p.rope.table + p.rope.pairs);
+        // up to four axes' positions are loaded beside the table, more behind it
+        int pos[4] = {at.pos, 0, 0, 0};
+        if (p.rope.positions)
+#pragma unroll
+            for (int a = 0; a < 4; a++)
+                if (a < (int)p.rope.axes) pos[a] = p.rope.positions[(size_t)a * p.rope.position_stride + t];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             if (e >= n) break;
-            const int pos = p.rope.positions
-                                ? p.rope.positions[(size_t)p.rope.axis[pair0 + e] * p.rope.position_stride + t]
-                                : at.pos;
-            const uint64_t frac = (uint64_t)(int64_t)pos * p.rope.turn[pair0 + e];
-            const float turn = (float)(int32_t)(frac >> 32) * 0x1p-32f;  // -0.5 .. 0.5
-            sincospif(2.0f * turn, &sn[e], &cs[e]);
+            int at_axis = pos[0];
+            if (p.rope.axes > 1) {
+                const uint32_t a = min(axis[pair0 + e], p.rope.axes - 1);
+                at_axis = a == 0 ? pos[0] : (a == 1 ? pos[1] : (a == 2 ? pos[2] : pos[3]));
+                if (a > 3) at_axis = p.rope.positions[(size_t)a * p.rope.position_stride + t];
+            }
+            const uint64_t frac = (uint64_t)(int64_t)at_axis * p.rope.table[pair0 + e];
+            // -0.5 .. 0.5 of a turn, which the hardware's sine and cosine take: off by at most
+            // 2^-22.9 there (every 2^-22 of a turn measured)
+            const float turn = (float)(int32_t)(frac >> 32) * 0x1p-32f;
+            sn[e] = __builtin_amdgcn_sinf(turn);
+            cs[e] = __builtin_amdgcn_cosf(turn);
         }
         if (p.rope.traditional) {
 #pragma unroll
@@ -176,11 +201,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
     }
     const bool any_turned = p.rope.pairs != 0;
 
-    for (uint32_t it = chunk; it < items; it += chunks) {
+    auto one = [&](uint32_t it, h8_t y) {
         const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
         const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
-        h8_t y = next;
-        next = fetch(it + chunks);
         if (any_turned && (is_q || is_k)) {
             u4_t mine = __builtin_bit_cast(u4_t, y), theirs;
             if (p.rope.traditional) {
@@ -198,7 +221,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
         }
         if (is_q) {
             if (row) *reinterpret_cast<h8_t*>(p.Qo.p + (int64_t)t * p.Qo.ts + (int64_t)h * p.Qo.hs + 8 * l) = y;
-            continue;
+            return;
         }
         if constexpr (FMT >= 0) {
             float x[8];
@@ -206,7 +229,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
             for (int e = 0; e < 8; e++) x[e] = (float)y[e];
             uint32_t c[8], d16;
             quantize8<FMT>(x, lane, c, d16);
-            if (!row) continue;
+            if (!row) return;
             constexpr uint32_t D = LPR * 8, NB = D / 32, CB = FMT == QUANT_Q8_0 ? D : D / 2;
             uint8_t* head = p.geom.pages + ((size_t)at.page * p.geom.Hkv + h) * p.geom.head_bytes;
             if (is_k) {
@@ -234,23 +257,33 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
                     *reinterpret_cast<uint16_t*>(head + p.geom.vs_off + ((g4 * NB + l / 4) * 4 + k4) * 2) = (uint16_t)d16;
             }
         }
+    };
+    for (uint32_t it0 = chunk; it0 < items; it0 += kAhead * chunks) {
+        h8_t now[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) now[i] = next[i];
+        fetch(it0 + kAhead * chunks);
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            if (it0 + i * chunks < items) one(it0 + i * chunks, now[i]);
     }
 }
 
 hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
     if (p.T == 0) return hipSuccess;
     const int lpr = p.D <= 64 ? 8 : (p.D <= 128 ? 16 : 32);
-    if (p.D > 256 || p.D % 8 || p.rope.pairs > kRopeMaxPairs || p.rope.pairs % 8 || 2 * p.rope.pairs > p.D)
+    if (p.D > 256 || p.D % 8 || p.rope.pairs > 128 || p.rope.pairs % 8 || 2 * p.rope.pairs > p.D)
         return hipErrorInvalidValue;
     if (p.geom.pages && p.D != 64 && p.D != 128) return hipErrorInvalidValue;
     const uint32_t items = p.H + (p.geom.pages ? 2 * p.geom.Hkv : 0);
     if (items == 0) return hipSuccess;
-    const uint32_t groups = (p.T + 64 / lpr - 1) / (64 / lpr);
-    uint32_t blocks = (items + 3) / 4;  // one head per wave
-    while (blocks > 1 && (uint64_t)groups * blocks > 1024) blocks = (blocks + 1) / 2;
+    // four waves of rows side by side, the heads over as many blocks as fill the chip
+    const uint32_t rows = 4 * 64 / lpr, groups = (p.T + rows - 1) / rows;
+    uint32_t blocks = items;
+    while (blocks > 1 && (uint64_t)groups * blocks > QR_GB) blocks = (blocks + 1) / 2;
     const dim3 grid(groups, blocks);
     const int fmt = p.geom.pages ? p.format : -1;
-#define QR_APPEND(L, F) hipLaunchKernelGGL((kv_append_kernel<L, F>), grid, dim3(256), 0, st, p, 4 * blocks)
+#define QR_APPEND(L, F) hipLaunchKernelGGL((kv_append_kernel<L, F>), grid, dim3(256), 0, st, p)
     if (fmt < 0) {
         if (lpr == 8) QR_APPEND(8, -1);
         else if (lpr == 16) QR_APPEND(16, -1);
@@ -272,14 +305,14 @@ hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
 // lane reads 8 dims of a token; of V the four tokens of its group, of which it
 // keeps its own (the other three lanes' reads of the same bytes hit the cache).
 template <int LPR, int FMT>
-__global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p, uint32_t chunks) {
+__global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p) {
     constexpr int RPW = 64 / LPR;
     constexpr uint32_t D = LPR * 8, NB = D / 32, CB = FMT == QUANT_Q8_0 ? D : D / 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l = lane % LPR, sub = lane / LPR;
-    const uint32_t t0 = blockIdx.x * RPW, t = t0 + sub;
-    const uint32_t chunk = blockIdx.y * 4 + wave, items = 2 * p.geom.Hkv;
-    if (chunk >= items) return;
+    const uint32_t t0 = (blockIdx.x * 4 + wave) * RPW, t = t0 + sub;
+    const uint32_t chunk = blockIdx.y, chunks = gridDim.y, items = 2 * p.geom.Hkv;
+    if (t0 >= p.batch.T) return;
     const Place at = place_of<RPW>(p.batch, p.geom, t0, sub, lane);
     if (!at.ok) return;
     for (uint32_t it = chunk; it < items; it += chunks) {
@@ -337,15 +370,15 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p, uint32_t chu
 hipError_t launch_kv_read(const ReadParams& p, hipStream_t st) {
     if (p.batch.T == 0 || p.geom.Hkv == 0) return hipSuccess;
     if (p.D != 64 && p.D != 128) return hipErrorInvalidValue;
-    const uint32_t rpw = p.D == 64 ? 8 : 4, groups = (p.batch.T + rpw - 1) / rpw;
-    uint32_t blocks = (2 * p.geom.Hkv + 3) / 4;
-    while (blocks > 1 && (uint64_t)groups * blocks > 1024) blocks = (blocks + 1) / 2;
+    const uint32_t rows = p.D == 64 ? 32 : 16, groups = (p.batch.T + rows - 1) / rows;
+    uint32_t blocks = 2 * p.geom.Hkv;
+    while (blocks > 1 && (uint64_t)groups * blocks > QR_GR) blocks = (blocks + 1) / 2;
     const dim3 grid(groups, blocks);
     switch ((p.D == 128 ? 1 : 0) + (p.format == QUANT_Q8_0 ? 2 : 0)) {
-        case 0: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q4_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
-        case 1: hipLaunchKernelGGL((kv_read_kernel<16, QUANT_Q4_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
-        case 2: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q8_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
-        default: hipLaunchKernelGGL((kv_read_kernel<16, QUANT_Q8_0>), grid, dim3(256), 0, st, p, 4 * blocks); break;
+        case 0: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q4_0>), grid, dim3(256), 0, st, p); break;
+        case 1: hipLaunchKernelGGL((kv_read_kernel<16, QUANT_Q4_0>), grid, dim3(256), 0, st, p); break;
+        case 2: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q8_0>), grid, dim3(256), 0, st, p); break;
+        default: hipLaunchKernelGGL((kv_read_kernel<16, QUANT_Q8_0>), grid, dim3(256), 0, st, p); break;
     }
     return hipGetLastError();
 }

@@ -87,6 +87,7 @@ SIGNATURES = {
                                                     _U32, _I], _I),
     "m4_bridge_dequantize": ([_VP, _SZ, _VP, _SZ, _I, _U32, _U32], _I),
     "m4_bridge_kv_cache_bytes": ([_I, _U32, _U32, _U32, _U32], _SZ),
+    "m4_bridge_rope_axes_table": ([_VP, _VP, _U32, _U32, _VP], _I),
     "m4_bridge_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
     "m4_bridge_kv_cache_append": ([_VP, _VP, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
     "m4_bridge_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
@@ -151,6 +152,9 @@ def projection_plan(lib: ctypes.CDLL, format_id: int, M: int, K: int, *N: int, s
     return plan
 
 
+_torch: Any = None  # the module, once a library is loaded
+
+
 class KVCacheStruct(ctypes.Structure):
     """m4_kv_cache_t (include/m4_mlx_bridge.h)."""
     _fields_ = [("pages", _VP), ("bytes", _SZ), ("format", _I), ("num_pages", _U32), ("page_size", _U32),
@@ -168,11 +172,15 @@ class RowsStruct(ctypes.Structure):
     _fields_ = [("ptr", _VP), ("bytes", _SZ), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
+_ROWS = ctypes.sizeof(RowsStruct)
+# two and four m4_rows_t as words: one object a call is made faster than one for each
+_ROWS2, _ROWS4 = ctypes.c_uint64 * 8, ctypes.c_uint64 * 16
+
+
 class RopeAxesStruct(ctypes.Structure):
     """m4_rope_axes_t (include/m4_mlx_bridge.h)."""
-    MAX_PAIRS = 128
-    _fields_ = [("pairs", _U32), ("axes", _U32), ("traditional", _I), ("pair_axis", ctypes.c_uint8 * MAX_PAIRS),
-                ("inv_freq", ctypes.c_double * MAX_PAIRS)]
+    MAX_PAIRS, PAIR_BYTES = 128, 12
+    _fields_ = [("pairs", _U32), ("axes", _U32), ("traditional", _I), ("table", _VP), ("table_bytes", _SZ)]
 
 
 def _int32(name: str, t: Any, dims: int) -> Any:
@@ -253,6 +261,8 @@ class RotaryAxes:
 
     def __init__(self, dims: int, theta: float = 10000.0, sections=None, pair_axes=None, inv_freq=None,
                  traditional: bool = False) -> None:
+        import torch
+
         pairs = dims // 2
         if dims <= 0 or dims % 16 or pairs > RopeAxesStruct.MAX_PAIRS:
             raise ValueError(f"dims={dims} must be a positive multiple of 16, at most {2 * RopeAxesStruct.MAX_PAIRS}")
@@ -273,11 +283,28 @@ class RotaryAxes:
         if len(inv_freq) != pairs:
             raise ValueError(f"{pairs} pairs need a frequency each, got {len(inv_freq)}")
         axes = max(pair_axes) + 1 if sections is None else max(len(sections), 1)
-        self.dims, self.axes = dims, axes
-        self.struct = RopeAxesStruct(pairs, axes, int(bool(traditional)))
-        self.struct.pair_axis[:pairs] = pair_axes
-        self.struct.inv_freq[:pairs] = inv_freq
-        self.ref = ctypes.addressof(self.struct)
+        self.dims, self.axes, self.traditional = dims, axes, bool(traditional)
+        self._table = (ctypes.c_uint8 * (pairs * RopeAxesStruct.PAIR_BYTES))()
+        rc = HIPBridge.get_instance().lib.m4_bridge_rope_axes_table((ctypes.c_double * pairs)(*inv_freq),
+                                                                    (ctypes.c_uint8 * pairs)(*pair_axes), pairs, axes,
+                                                                    self._table)
+        if rc:
+            raise ValueError(f"m4_bridge_rope_axes_table failed with status code {rc}")
+        self._on: dict = {}  # device -> (table, struct, its address)
+        if torch.cuda.is_available():
+            self.on(torch.device("cuda", torch.cuda.current_device()))
+
+    def on(self, device) -> int:
+        """Address of the struct for a device, whose copy of the table is made on first use (the current device's with
+        the object; another's before a capture)."""
+        held = self._on.get(device)
+        if held is None:
+            import torch
+
+            t = torch.frombuffer(bytearray(self._table), dtype=torch.uint8).to(device)
+            struct = RopeAxesStruct(self.dims // 2, self.axes, int(self.traditional), t.data_ptr(), t.numel())
+            held = self._on[device] = (t, struct, ctypes.addressof(struct))
+        return held[2]
 
 
 def load_library(path: Optional[Union[str, Path]] = None) -> ctypes.CDLL:
@@ -285,8 +312,9 @@ def load_library(path: Optional[Union[str, Path]] = None) -> ctypes.CDLL:
     # Importing torch first makes the library bind to that already-loaded
     # runtime (same SONAME) instead of loading /opt/rocm's beside it, which
     # would leave torch without a usable device.
+    global _torch
     try:
-        import torch  # noqa: F401
+        import torch as _torch
     except ImportError:
         pass
     lib = ctypes.CDLL(str(Path(path) if path else _find_library_path()))
@@ -305,10 +333,16 @@ def _current_stream(device: int) -> int:
     """Handle of torch's current stream on a device.  The raw getter returns it
     without building a Stream object (0.2 instead of 2.0 us, of ~8 us that an
     eager call takes on the host)."""
-    import torch
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
 
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
+
+
+_raw_stream: Any = None
 
 
 class HIPBridge:
@@ -604,38 +638,44 @@ class HIPBridge:
 
     # -- serving over a paged KV cache -----------------------------------------
     def _rows(self, name: str, t: Any, token_major: bool, heads: Optional[int], D: Optional[int], out: bool) -> tuple:
-        """(m4_rows_t, T, heads, tensor) of fp16 rows [heads, T, D], or [T, heads, D] when token_major.
+        """(m4_rows_t's four words, T, heads, tensor) of fp16 rows [heads, T, D], or [T, heads, D] when token_major.
         Any strides that keep 8 elements together are taken as they are; other inputs
         are copied (and retained until synchronize())."""
-        import torch
-
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.dim() != 3:
+        if not isinstance(t, _torch.Tensor) or t.dtype is not _torch.float16 or len(t.shape) != 3:
             raise ValueError(f"{name} must be an fp16 tensor with 3 dimensions")
         a, b, d = t.shape
         T, H = (a, b) if token_major else (b, a)
         if (heads is not None and H != heads) or (D is not None and d != D):
             raise ValueError(f"{name} has {H} heads of {d}, expected {heads} of {D}")
         sa, sb, sd = t.stride()
-        if sd != 1 or sa % 8 or sb % 8 or t.data_ptr() % 16:
+        ptr = t.data_ptr()
+        if sd != 1 or (sa | sb) & 7 or ptr & 15:
             if t.numel() and out:
                 raise ValueError(f"{name} must be contiguous along its last dimension, 16-byte aligned, with strides "
                                  f"that are multiples of 8")
-            t = t.contiguous() if sd != 1 or sa % 8 or sb % 8 else t.clone(memory_format=torch.contiguous_format)
+            t = t.clone(memory_format=_torch.contiguous_format)
             self._retained_contig.append(t)
             sa, sb, sd = t.stride()
+            ptr = t.data_ptr()
         ts, hs = (sa, sb) if token_major else (sb, sa)
-        held = ((T - 1) * ts + (H - 1) * hs + d) * 2 if t.numel() else 0
-        return RowsStruct(t.data_ptr(), held, ts, hs), T, H, t
+        held = ((T - 1) * ts + (H - 1) * hs + d) * 2 if T and H else 0
+        return (ptr, held, ts, hs), T, H, t
 
     def _positions(self, positions: Any, rope: "RotaryAxes", T: int) -> tuple:
         """(pointer, stride) of int32 positions [T] or [axes, T]."""
         if positions is None:
             return None, 0
-        p = _int32("positions", positions, positions.dim() if positions.dim() == 1 else 2)
-        axes = 1 if p.dim() == 1 else p.shape[0]
-        if p.shape[-1] != T or axes < rope.axes:
-            raise ValueError(f"positions {tuple(p.shape)} do not give {rope.axes} axes of {T} tokens")
-        return p.data_ptr(), (p.stride(0) if p.dim() == 2 else T)
+        shape = positions.shape
+        if positions.dtype is not _torch.int32 or len(shape) not in (1, 2) or (T and positions.stride(-1) != 1):
+            raise ValueError("positions must be int32 [T] or [axes, T], contiguous along T")
+        if shape[-1] != T or (shape[0] if len(shape) == 2 else 1) < rope.axes:
+            raise ValueError(f"positions {tuple(shape)} do not give {rope.axes} axes of {T} tokens")
+        return positions.data_ptr(), (positions.stride(0) if len(shape) == 2 else T)
+
+    def _on_stream_of(self, t: Any) -> None:
+        device = t.get_device()
+        if device >= 0:
+            self._lib.m4_bridge_set_stream(_current_stream(device))
 
     def rope_axes(self, X, Y, rope: RotaryAxes, positions, token_major: bool = False) -> int:
         """Y = X [H, T, D] (or [T, H, D]) turned by positions [T] or [axes, T]; Y may be X."""
@@ -644,9 +684,10 @@ class HIPBridge:
         if positions is None or Ty != T:
             raise ValueError("X and Y need the same rows, and positions")
         pos, stride = self._positions(positions, rope, T)
-        self._bind_stream(X)
-        ret = self._lib.m4_bridge_rope_axes(rope.ref, pos, stride, ctypes.addressof(x), ctypes.addressof(y), T, H,
-                                            X.shape[2])
+        self._on_stream_of(X)
+        rows = _ROWS2(*x, *y)
+        at = ctypes.addressof(rows)
+        ret = self._lib.m4_bridge_rope_axes(rope.on(X.device), pos, stride, at, at + _ROWS, T, H, X.shape[2])
         self._check("m4_bridge_rope_axes", ret)
         self._in_flight_tensors.append((X, Y, positions))
         return ret
@@ -665,19 +706,22 @@ class HIPBridge:
         if Q is not None and rope is None:
             raise ValueError("Q is turned by rope: give both or neither")
         pos, stride = self._positions(positions, rope, T) if rope is not None else (None, 0)
-        q = qo = None
+        q = qo = (0, 0, 0, 0)
         H = 0
         if Q is not None:
             Q_out = Q if Q_out is None else Q_out
             qo, To, H, _ = self._rows("Q_out", Q_out, token_major, None, cache.D, True)
-            q, Tq, _, Q = self._rows("Q", Q, token_major, H, cache.D, False)
+            q, Tq, _, Q = (qo, To, H, Q) if Q is Q_out else self._rows("Q", Q, token_major, H, cache.D, False)
             if Tq != T or To != T:
                 raise ValueError(f"K has {T} rows, Q {Tq} and Q_out {To}")
-        self._bind_stream(K)
+        self._on_stream_of(K)
         batch.struct.T = T
-        ref = ctypes.addressof
-        ret = self._lib.m4_bridge_kv_cache_append(cache.ref, batch.ref, ref(k), ref(v), rope.ref if rope else None, pos,
-                                                  stride, ref(q) if q else None, ref(qo) if qo else None, H)
+        rows = _ROWS4(*k, *v, *q, *qo)
+        at = ctypes.addressof(rows)
+        at_q, at_qo = (at + 2 * _ROWS, at + 3 * _ROWS) if Q is not None else (None, None)
+        ret = self._lib.m4_bridge_kv_cache_append(cache.ref, batch.ref, at, at + _ROWS,
+                                                  rope.on(K.device) if rope is not None else None, pos, stride, at_q,
+                                                  at_qo, H)
         self._check("m4_bridge_kv_cache_append", ret)
         self._in_flight_tensors.append((cache, batch, K, V, Q, Q_out, positions))
         return ret
@@ -688,15 +732,18 @@ class HIPBridge:
         v, Tv, _, _ = self._rows("V", V, token_major, cache.Hkv, cache.D, True)
         if Tv != T:
             raise ValueError(f"K has {T} rows, V {Tv}")
-        self._bind_stream(K)
+        self._on_stream_of(K)
         batch.struct.T = T
-        ret = self._lib.m4_bridge_kv_cache_read(cache.ref, batch.ref, ctypes.addressof(k), ctypes.addressof(v))
+        rows = _ROWS2(*k, *v)
+        at = ctypes.addressof(rows)
+        ret = self._lib.m4_bridge_kv_cache_read(cache.ref, batch.ref, at, at + _ROWS)
         self._check("m4_bridge_kv_cache_read", ret)
         self._in_flight_tensors.append((cache, batch, K, V))
         return ret
 
-    def paged_attn_workspace(self, cache: PagedKVCache, batch: KVBatch, H: int, window: int = 0) -> int:
-        """Bytes of workspace that dispatch_paged_attn needs."""
+    def paged_attn_workspace(self, cache: PagedKVCache, batch: KVBatch, H: int, T: int, window: int = 0) -> int:
+        """Bytes of workspace that dispatch_paged_attn needs for T rows of H heads."""
+        batch.struct.T = T
         return int(self._lib.m4_bridge_paged_attn_workspace(cache.ref, batch.ref, H, window))
 
     def dispatch_paged_attn(self, cache: PagedKVCache, batch: KVBatch, Q, O, scale: float, token_major: bool = False,
@@ -705,20 +752,21 @@ class HIPBridge:
         first); O [H, T, D], or [T, H, D] when o_token_major.  `workspace`: a uint8 device tensor of
         paged_attn_workspace bytes, not shared with a call that may run at the same time (None: from torch's
         allocator, on the current stream)."""
-        import torch
-
         q, T, H, Q = self._rows("Q", Q, token_major, None, cache.D, False)
         o, To, _, _ = self._rows("O", O, o_token_major, H, cache.D, True)
         if To != T:
             raise ValueError(f"Q has {T} rows, O {To}")
-        if window < 0 or window >= 1 << 32:
+        if not 0 <= window < 1 << 32:
             raise ValueError(f"window={window}")
-        self._bind_stream(Q)
-        batch.struct.T = T
+        self._on_stream_of(Q)
         if workspace is None:
-            workspace = torch.empty(self.paged_attn_workspace(cache, batch, H, window), dtype=torch.uint8, device=Q.device)
-        ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, ctypes.addressof(q), ctypes.addressof(o), H,
-                                                      float(scale), int(window), workspace.data_ptr(), workspace.numel())
+            workspace = _torch.empty(self.paged_attn_workspace(cache, batch, H, T, window), dtype=_torch.uint8,
+                                     device=Q.device)
+        batch.struct.T = T
+        rows = _ROWS2(*q, *o)
+        at = ctypes.addressof(rows)
+        ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, at, at + _ROWS, H, float(scale), window,
+                                                      workspace.data_ptr(), workspace.nbytes)
         self._check("m4_bridge_dispatch_paged_attn", ret)
         self._in_flight_tensors.append((cache, batch, Q, O))
         return ret

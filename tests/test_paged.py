@@ -470,7 +470,7 @@ def test_captured_decoding_steps(bridge, fmt):
         batch = m4_bridge.KVBatch(torch.arange(B + 1, dtype=torch.int32, device="cuda"), kv_len, dev(table), 1, 704)
         q, k, v = (torch.zeros_like(t) for t in xs[0])
         o = torch.zeros(B, H, D, dtype=torch.float16, device="cuda")
-        ws = torch.empty(bridge.paged_attn_workspace(cache, batch, H), dtype=torch.uint8, device="cuda")
+        ws = torch.empty(bridge.paged_attn_workspace(cache, batch, H, B), dtype=torch.uint8, device="cuda")
 
         def step():
             bridge.kv_cache_append(cache, batch, k, v, rope=rope, Q=q)
@@ -550,9 +550,7 @@ class Args:
         self.batch = m4_bridge.KVBatchStruct(2, self.T, 0x1000, 0x2000, 0x3000, 4, 4, 5, 60)
         self.kv = m4_bridge.RowsStruct(0x200000, 2 * self.T * 128 * 2, 128, self.T * 128)
         self.q = m4_bridge.RowsStruct(0x300000, 8 * self.T * 128 * 2, 128, self.T * 128)
-        self.rope = m4_bridge.RopeAxesStruct(64, 3, 0)
-        self.rope.pair_axis[:64] = [0] * 16 + [1] * 24 + [2] * 24
-        self.rope.inv_freq[:64] = [1.0] * 64
+        self.rope = m4_bridge.RopeAxesStruct(64, 3, 0, 0x500000, 64 * 12)
         self.positions, self.stride, self.scale, self.ws, self.ws_bytes = 0x4000, self.T, 0.1, 0x400000, 1 << 30
 
     def codes(self, lib):
@@ -609,7 +607,11 @@ def _set(path, value):
     (_set("rope.pairs", 12), (-4, 0, 0, -4)),
     (_set("rope.pairs", 72), (-4, 0, 0, -4)),
     (_set("rope.pairs", 0), (-4, 0, 0, -4)),
-    (_set("rope.axes", 2), (-4, 0, 0, -4)),
+    (_set("rope.axes", 0), (-4, 0, 0, -4)),
+    (_set("rope.axes", 257), (-4, 0, 0, -4)),
+    (_set("rope.table", None), (-2, 0, 0, -2)),
+    (_set("rope.table", 0x500008), (-2, 0, 0, -2)),
+    (_set("rope.table_bytes", 64 * 12 - 1), (-2, 0, 0, -2)),
     (_set("positions", None), (-2, 0, 0, -2)),
     (_set("positions", 0x4002), (-2, 0, 0, -2)),
     (_set("stride", 9), (-4, 0, 0, -4)),
@@ -625,15 +627,33 @@ def test_refusals(lib, change, codes):
     assert a.codes(lib) == codes
 
 
-def test_refusals_of_the_rotary_table(lib):
-    a = Args()
-    a.rope.inv_freq[3] = float("inf")
-    assert a.codes(lib) == (-4, 0, 0, -4)
+def test_rotary_table(lib):
+    """Turns as 64-bit fractions, whole turns dropped; frequencies and axes that are refused."""
+    f = [1.0, -1.0, 2 * np.pi * 3.25, 0.0, 1e-30, -1e-30, 100.0, 2 * np.pi]
+    axes = [0, 1, 2, 0, 1, 2, 0, 1]
+
+    def table(f, axes, n=8, na=3):
+        out = np.zeros(12, np.uint64)
+        rc = lib.m4_bridge_rope_axes_table((ctypes.c_double * 8)(*f), (ctypes.c_uint8 * 8)(*axes), n, na, out.ctypes.data)
+        return rc, out
+
+    rc, out = table(f, axes)
+    assert rc == 0 and list(out[8:].view(np.uint32)) == axes
+    want = np.array(f) / (2 * np.pi)
+    turns = out[:8].astype(np.float64) / 2.0 ** 64
+    off = np.abs(turns - want)
+    assert (np.abs(off - np.round(off)) <= 2.0 ** -51 * np.maximum(np.abs(want), 1)).all()  # double: product and floor
+    assert table([float("inf")] + f[1:], axes)[0] == -4
+    assert table(f, [3] + axes[1:])[0] == -4
+    assert table(f, axes, n=4)[0] == -4 and table(f, axes, n=0)[0] == -4 and table(f, axes, na=0)[0] == -4
+    assert lib.m4_bridge_rope_axes_table(None, None, 8, 3, None) == -2
+
+
+def test_positions_default_to_the_place(lib):
     a = Args()
     a.rope.axes = 1
-    a.rope.pair_axis[:64] = [0] * 64
     a.positions = None
-    assert a.codes(lib) == (0, 0, 0, -2)  # the cache's own places stand in, which a rotation alone has not
+    assert a.codes(lib) == (0, 0, 0, -2)  # a rotation alone has no places to stand in
 
 
 def test_uninitialized_bridge_refuses(lib):
