@@ -35,10 +35,12 @@ constexpr uint64_t kChunkWork = (uint64_t)1 << 26;
 constexpr float kNone = -3.402823466e38f;  // reference point of a row that has seen no score above -infinity
 
 // A workgroup's note on its partial rows.  tail: an item begins in its share and
-// goes on in the next one's (slot 1, and which it is); head: the first item of
-// its share began before it (slot 0) and ends here (1) or goes on (2).
-struct ItemNote {
-    uint32_t b, hk, rt, tail, head, pad[3];
+// goes on in the next one's (slot 1, and which rows they are: the KV head, the
+// first of its sequence's (token, head) pairs and how many, the sequence's first
+// row); head: the first item of its share began before it (slot 0) and ends here
+// (1) or goes on (2).
+struct alignas(16) ItemNote {
+    uint32_t hk, first, rows, q0, tail, head, pad[2];
 };
 
 struct WorkPlan {
@@ -233,14 +235,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     const uint32_t per = (p.batch.B + 63) / 64;
     const uint32_t b_lo = min(lane * per, p.batch.B), b_hi = min(b_lo + per, p.batch.B);
     uint64_t mine = 0;
-    for (uint32_t x = b_lo; x < b_hi; x++) mine += seq_of(p, x, R).cost;
-    uint64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t x = __shfl_up((unsigned long long)incl, o);
-        if (lane >= o) incl += x;
+    Seq held{};  // up to 64 sequences: a lane's own, to be taken from it
+    for (uint32_t x = b_lo; x < b_hi; x++) {
+        held = seq_of(p, x, R);
+        mine += held.cost;
     }
-    const uint64_t total = lane_u64(incl, 63);
+    uint64_t incl = mine;
+    for (uint32_t o = 1; o < min(p.batch.B, 64u); o <<= 1) {
+        const uint64_t x = __shfl_up((unsigned long long)incl, o);
+        if ((uint32_t)lane >= o) incl += x;
+    }
+    const uint64_t total = lane_u64(incl, (int)min(p.batch.B, 64u) - 1);
     const uint64_t nw = min((uint64_t)workers, total);
     if (threadIdx.x == 0) *note = ItemNote{};
     if (lane == 0) head_of[wave] = 0;
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     f4_t o[NR][DT];
     float m_run[NR], l_run[NR];
     Seq s{};
-    uint32_t b_open = 0, hk = 0, rt = 0, rows = 0;
+    uint32_t hk = 0, rt = 0, rows = 0;
     bool open = false, begun = false;  // it goes on in the next wave's share; its first step was here
 
     auto row_of = [&](const RowsView& v, uint32_t r) {
@@ -316,7 +321,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     };
 
     for (uint64_t cur = s0; cur < s1 && b < p.batch.B;) {
-        s = seq_of(p, b, R);
+        if (per == 1) {
+            s.q0 = __builtin_amdgcn_readlane(held.q0, b);
+            s.n = __builtin_amdgcn_readlane(held.n, b);
+            s.len = __builtin_amdgcn_readlane(held.len, b);
+            s.lo = __builtin_amdgcn_readlane(held.lo, b);
+            s.tiles = __builtin_amdgcn_readlane(held.tiles, b);
+            s.steps = __builtin_amdgcn_readlane(held.steps, b);
+            s.cost = lane_u64(held.cost, b);
+        } else {
+            s = seq_of(p, b, R);
+        }
         if (off >= s.cost) {
             b++;
             off = 0;
@@ -332,7 +347,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         const uint32_t u0 = o0 > kItemCost ? o0 - kItemCost : 0, nu = o1 - kItemCost - u0;
         hk = item / s.tiles;
         rt = item % s.tiles;
-        b_open = b;
         const int p0 = s.len - s.n;  // position of the first new token
 
         // ---- rows ----
@@ -561,9 +575,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     leave(begun ? 1 : 0);
     if (lane != 0) return;
     if (begun) {
-        note->b = b_open;
         note->hk = hk;
-        note->rt = rt;
+        note->first = rt * R;
+        note->rows = rows;
+        note->q0 = (uint32_t)s.q0;
         note->tail = 1;
     } else {
         note->head = ended ? 1 : 2;
@@ -576,68 +591,91 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 // are split over the lane groups, whose sums meet in LDS in a fixed order.
 constexpr uint32_t kJoinBlocks = 512;
 template <int D, int R>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups, uint32_t tile_rows) {
-    constexpr int L = D / 4, GROUPS = 256 / L;
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups) {
+    constexpr int L = D / 4, GROUPS = 256 / L, U = 4;
     __shared__ f4_t part_sum[256];
-    const uint32_t per = (groups + gridDim.x - 1) / gridDim.x, w0 = blockIdx.x * per;
-    const uint32_t w1 = min(w0 + per, groups);
+    const uint32_t per = (groups + gridDim.x - 1) / gridDim.x, w1 = min((blockIdx.x + 1) * per, groups);
     const ItemNote* notes = reinterpret_cast<const ItemNote*>(p.ws);
-    const uint32_t tid = threadIdx.x, l4 = tid % L, group = tid / L;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, l4 = tid % L, group = tid / L;
     const uint32_t G = p.H / p.geom.Hkv;
-    for (uint32_t base = w0; base < w1; base += 64) {
-        const uint32_t mine = base + (tid & 63);
-        uint64_t todo = __ballot(mine < w1 && notes[mine].tail);
+    // 32 notes at a time to begin at, and those behind them to end at, a lane each
+    for (uint32_t base = blockIdx.x * per; base < w1; base += 32) {
+        ItemNote mine{};
+        if (base + lane < groups) mine = notes[base + lane];
+        uint64_t todo = __ballot(lane < 32 && base + lane < w1 && mine.tail);
+        const uint64_t stops = __ballot(mine.head != 2);
         while (todo) {
-            const uint32_t w = base + __ffsll((unsigned long long)todo) - 1;
+            const int at = __ffsll((unsigned long long)todo) - 1;
             todo &= todo - 1;
-            const ItemNote note = notes[w];
-            uint32_t parts = 2;  // up to the first workgroup in which it ends
-            for (uint32_t k = w + 1; k < groups; k += 64) {
-                const uint32_t x = k + (tid & 63);
-                const uint64_t end = __ballot(x >= groups || notes[x].head != 2);
-                if (end) {
-                    parts = k - w + __ffsll((unsigned long long)end);
-                    break;
-                }
+            const uint32_t w = base + at;
+            const uint32_t hk = __builtin_amdgcn_readlane(mine.hk, at), first = __builtin_amdgcn_readlane(mine.first, at);
+            const uint32_t rows = __builtin_amdgcn_readlane(mine.rows, at), q0 = __builtin_amdgcn_readlane(mine.q0, at);
+            // parts: up to the first workgroup in which it ends
+            uint32_t parts = 0;
+            const uint64_t behind = at < 63 ? stops >> (at + 1) : 0;
+            if (behind) parts = __ffsll((unsigned long long)behind) + 1;
+            for (uint32_t k = base + 64; parts == 0 && k < groups; k += 64) {
+                const uint64_t end = __ballot(k + lane >= groups || notes[k + lane].head != 2);
+                if (end) parts = k - w + __ffsll((unsigned long long)end);
             }
-            parts = min(parts, groups - w);
-            const Seq s = seq_of(p, note.b, R);
-            const uint32_t rows = min(tile_rows, (uint32_t)s.n * G - note.rt * tile_rows);
+            parts = parts ? min(parts, groups - w) : groups - w;
             auto slot = [&](uint32_t k) { return slot_of<D, R>(p.ws, groups, w + k, k == 0 ? 1 : 0); };
             uint32_t split = 1;
-            while (split < GROUPS && parts > 4 * split) split *= 2;
-            const uint32_t side = GROUPS / split;
+            while (split < GROUPS && parts > U * split) split *= 2;
+            const uint32_t side = GROUPS / split, mine0 = group % split;
             for (uint32_t r0 = blockIdx.y * side; r0 < rows; r0 += gridDim.y * side) {
                 const uint32_t r = r0 + group / split;
                 const bool live = r < rows;
-                float m = kNone, l = 0.0f;
-                f4_t o{};
+                // reference points and sums, a lane each part, and the first rows, all under way together
+                float m = kNone, l = 0.0f, mk[U];
+                f4_t v[U], o{};
+                if (live && l4 < parts) {
+                    m = slot(l4)[R * D + r];
+                    l = slot(l4)[R * D + R + r];
+                }
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    v[i] = f4_t{};
+                    mk[i] = -INFINITY;
+                    const uint32_t k = mine0 + i * split;
+                    if (live && k < parts) {
+                        v[i] = *reinterpret_cast<const f4_t*>(slot(k) + r * D + 4 * l4);
+                        mk[i] = slot(k)[R * D + r];
+                    }
+                }
                 if (live)
-                    for (uint32_t k = l4; k < parts; k += L) m = fmaxf(m, slot(k)[R * D + r]);
+                    for (uint32_t k = l4 + L; k < parts; k += L) {
+                        const float m2 = slot(k)[R * D + r], m_new = fmaxf(m, m2);
+                        l = l * __builtin_amdgcn_exp2f(m - m_new) + slot(k)[R * D + R + r] * __builtin_amdgcn_exp2f(m2 - m_new);
+                        m = m_new;
+                    }
+                const float m_lane = m;
 #pragma unroll
                 for (int x = L / 2; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+                l *= __builtin_amdgcn_exp2f(m_lane - m);
+#pragma unroll
+                for (int x = L / 2; x >= 1; x >>= 1) l += __shfl_xor(l, x);
+#pragma unroll
+                for (int i = 0; i < U; i++)
+                    if (live && mine0 + i * split < parts) o += v[i] * __builtin_amdgcn_exp2f(mk[i] - m);
                 if (live) {
-                    for (uint32_t k = l4; k < parts; k += L)
-                        l += slot(k)[R * D + R + r] * __builtin_amdgcn_exp2f(slot(k)[R * D + r] - m);
 #pragma unroll 4
-                    for (uint32_t k = group % split; k < parts; k += split) {
+                    for (uint32_t k = mine0 + U * split; k < parts; k += split) {
                         const float* x = slot(k);
                         o += *reinterpret_cast<const f4_t*>(x + r * D + 4 * l4) * __builtin_amdgcn_exp2f(x[R * D + r] - m);
                     }
                 }
-#pragma unroll
-                for (int x = L / 2; x >= 1; x >>= 1) l += __shfl_xor(l, x);
                 if (split > 1) {
                     __syncthreads();
                     part_sum[tid] = o;
                     __syncthreads();
-                    if (group % split == 0)
+                    if (mine0 == 0)
                         for (uint32_t k = 1; k < split; k++) o += part_sum[tid + k * L];
                 }
-                if (live && group % split == 0) {
+                if (live && mine0 == 0) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const uint32_t f = note.rt * tile_rows + r;
-                    _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(f / G)) * p.O.ts + (int64_t)(note.hk * G + f % G) * p.O.hs;
+                    const uint32_t f = first + r;
+                    _Float16* dst = p.O.p + (int64_t)(q0 + f / G) * p.O.ts + (int64_t)(hk * G + f % G) * p.O.hs;
                     const f2_t a = {o.x * inv, o.y * inv}, b = {o.z * inv, o.w * inv};
                     *reinterpret_cast<u2_t*>(dst + 4 * l4) =
                         u2_t{as_u32(__builtin_convertvector(a, h2_t)), as_u32(__builtin_convertvector(b, h2_t))};
@@ -1023,9 +1061,10 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             }
             if (tid == 0) {
                 if (begun) {
-                    note->b = b;
                     note->hk = hk;
-                    note->rt = rt;
+                    note->first = rt * tokens * G;
+                    note->rows = rows;
+                    note->q0 = (uint32_t)s.q0;
                     note->tail = 1;
                 } else {
                     note->head = ends ? 1 : 2;
@@ -1068,7 +1107,7 @@ size_t paged_attn_workspace(const PagedAttnParams& p) {
 }
 
 template <int D, int R>
-static hipError_t launch_join(const PagedAttnParams& p, uint32_t groups, uint32_t items, uint32_t tile_rows, hipStream_t st) {
+static hipError_t launch_join(const PagedAttnParams& p, uint32_t groups, uint32_t items, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // Blocks for each few workgroups, over which the rows of an item are spread: more
@@ -1078,7 +1117,7 @@ static hipError_t launch_join(const PagedAttnParams& p, uint32_t groups, uint32_
     const uint32_t parts = groups / items, across = R > 32 ? 32 : (parts >= 16 ? 16 : (parts >= 8 ? 8 : 4));
     const uint32_t most = 4 * kJoinBlocks / across;
     const dim3 grid(groups < most ? groups : most, across);
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, R>), grid, dim3(256), 0, st, p, groups, tile_rows);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, R>), grid, dim3(256), 0, st, p, groups);
     return hipGetLastError();
 }
 
@@ -1092,15 +1131,14 @@ static hipError_t launch_format(const PagedAttnParams& p, hipStream_t st) {
         const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW>, lds, attr);
         if (e != hipSuccess) return e;
         hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW>), dim3(w.groups), dim3(64 * NW), lds, st, p, w.groups);
-        const uint32_t G = p.H / p.geom.Hkv;
-        return launch_join<D, kChunkTile>(p, w.groups, w.items, kChunkTile / G * G, st);
+        return launch_join<D, kChunkTile>(p, w.groups, w.items, st);
     }
     if (w.rows == 16) {
         hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1>), dim3(w.groups), dim3(64 * kWaves), 0, st, p, w.groups);
-        return launch_join<D, 16>(p, w.groups, w.items, 16, st);
+        return launch_join<D, 16>(p, w.groups, w.items, st);
     }
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2>), dim3(w.groups), dim3(64 * kWaves), 0, st, p, w.groups);
-    return launch_join<D, 32>(p, w.groups, w.items, 32, st);
+    return launch_join<D, 32>(p, w.groups, w.items, st);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) {
