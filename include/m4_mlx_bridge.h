@@ -347,6 +347,22 @@ M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv
                                          const m4_rows_t* O, uint32_t H, float scale, uint32_t window, void* ws,
                                          size_t ws_bytes);
 
+/* A transformer block over the cache: m4_bridge_prefill_layer_ex with the
+ * batch's rows as its prompt and the paged cache in place of one call's keys --
+ * RMSNorm -> Q, K, V -> m4_bridge_kv_cache_append (K and Q turned by `rope`, NULL:
+ * not) -> m4_bridge_dispatch_paged_attn -> O-projection + residual -> RMSNorm ->
+ * SwiGLU -> down-projection + residual.  X, X_out fp16 [T, d_model], X_out not
+ * X; weights as there, in `format`; KV heads and head width are the cache's.
+ * Device pointers, 16-byte aligned.  Scratch is the bridge's: a size must have
+ * run once before it is captured, and calls run one after the other.  Rows of
+ * X_out behind the last sequence hold nothing of use.  Codes as
+ * m4_bridge_prefill_layer_ex. */
+M4_API int m4_bridge_paged_layer(void* X_ptr, void* w_attn, void* Wq, void* Wk, void* Wv, void* Wo, void* w_ffn,
+                                 void* Wg, void* Wu, void* Wd, void* X_out, const m4_kv_cache_t* cache,
+                                 const m4_kv_batch_t* batch, const m4_rope_axes_t* rope, const int32_t* positions,
+                                 uint32_t position_stride, int format, uint32_t d_model, uint32_t Hq, uint32_t N_mlp,
+                                 float attn_scale, uint32_t window, int norm_type, float norm_eps);
+
 /* Validation only, as m4_bridge_validate_gemm: the code that the call would
  * return on an initialized bridge (0 if it would launch) but for the check that
  * the pointers are device memory. */

@@ -443,6 +443,64 @@ int launched(hipError_t e, const char* what) {
     return -6;
 }
 
+// A transformer block's parts around its attention: norm and the Q, K and V
+// projections (head-major, one grouped launch), and what follows it.
+struct LayerCall {
+    const void *X, *w_attn, *Wq, *Wk, *Wv, *Wo, *w_ffn, *Wg, *Wu, *Wd;
+    void* Xout;
+    int format;
+    uint32_t M, dm, Hq, Hkv, D, Nm;
+    int norm_type;
+    float eps;
+};
+
+int layer_qkv(const LayerCall& c, _Float16* q, _Float16* k, _Float16* v, _Float16* xn) {
+    const void* a = c.X;
+    if (c.w_attn) {
+        const int rc = launched(qr::launch_rmsnorm(static_cast<const _Float16*>(c.X), static_cast<const _Float16*>(c.w_attn),
+                                                   xn, c.M, c.dm, c.eps, c.norm_type, g_stream), "layer rmsnorm");
+        if (rc) return rc;
+        a = xn;
+    }
+    const uint32_t HQ = c.Hq * c.D, HK = c.Hkv * c.D;
+    qr::GemmParams g{};
+    g.format = c.format;
+    g.X = static_cast<const _Float16*>(a);
+    g.W = static_cast<const uint8_t*>(c.Wq);
+    g.Y = q;
+    g.M = c.M; g.N = HQ; g.K = c.dm;
+    g.head_D = c.D;
+    g.col_bytes = qr::kernel_weight_bytes(c.format, c.dm, HQ) / HQ;
+    g.ngroups = 3;
+    g.Wx[0] = static_cast<const uint8_t*>(c.Wk); g.Yx[0] = k; g.Nx[0] = HK;
+    g.Wx[1] = static_cast<const uint8_t*>(c.Wv); g.Yx[1] = v; g.Nx[1] = HK;
+    return launch(g);
+}
+
+int layer_rest(const LayerCall& c, const _Float16* o, _Float16* xm, _Float16* s, _Float16* xn) {
+    auto proj = [&](const void* A, const void* W, const void* W2, void* Y, const void* R, uint32_t N, uint32_t Kd) {
+        qr::GemmParams p{};
+        p.format = c.format;
+        p.X = static_cast<const _Float16*>(A);
+        p.W = static_cast<const uint8_t*>(W);
+        p.W2 = static_cast<const uint8_t*>(W2);
+        p.Y = static_cast<_Float16*>(Y);
+        p.R = static_cast<const _Float16*>(R);
+        p.M = c.M; p.N = N; p.K = Kd;
+        p.col_bytes = qr::kernel_weight_bytes(c.format, Kd, N) / N;
+        return launch(p);
+    };
+    int rc = proj(o, c.Wo, nullptr, xm, c.X, c.dm, c.Hq * c.D);
+    const void* a = xm;
+    if (!rc && c.w_ffn) {
+        rc = launched(qr::launch_rmsnorm(xm, static_cast<const _Float16*>(c.w_ffn), xn, c.M, c.dm, c.eps, c.norm_type,
+                                         g_stream), "layer rmsnorm");
+        a = xn;
+    }
+    rc = rc ? rc : proj(a, c.Wg, c.Wu, s, nullptr, c.Nm, c.dm);
+    return rc ? rc : proj(s, c.Wd, nullptr, c.Xout, xm, c.dm, c.Nm);
+}
+
 }  // namespace
 
 extern "C" {
@@ -782,49 +840,10 @@ int m4_bridge_prefill_layer_ex_kv(void* X, void* w_attn, void* Wq, void* Wk, voi
     _Float16* s = reinterpret_cast<_Float16*>(take((size_t)M * Nm * 2));
     _Float16* xn = norms ? reinterpret_cast<_Float16*>(take((size_t)M * dm * 2)) : nullptr;
 
-    auto proj = [&](const void* A, const void* W, const void* W2, _Float16* Y, const _Float16* R, uint32_t N,
-                    uint32_t Kd, uint32_t headD) {
-        qr::GemmParams p{};
-        p.format = format;
-        p.X = static_cast<const _Float16*>(A);
-        p.W = static_cast<const uint8_t*>(W);
-        p.W2 = static_cast<const uint8_t*>(W2);
-        p.Y = Y;
-        p.R = R;
-        p.M = M; p.N = N; p.K = Kd;
-        p.head_D = headD;
-        p.col_bytes = qr::kernel_weight_bytes(format, Kd, N) / N;
-        return launch(p);
-    };
-    auto check = [&](hipError_t e, const char* what) {
-        if (e == hipSuccess) return 0;
-        set_error(what, e);
-        return -6;
-    };
-    int rc = 0;
-    const void* a = X;
-    if (w_attn) {
-        rc = check(qr::launch_rmsnorm(static_cast<const _Float16*>(X), static_cast<const _Float16*>(w_attn), xn, M, dm,
-                                      eps, norm_type, g_stream), "layer rmsnorm");
-        a = xn;
-    }
-    // Q, K, V: one grouped launch
-    if (!rc) {
-        qr::GemmParams g{};
-        g.format = format;
-        g.X = static_cast<const _Float16*>(a);
-        g.W = static_cast<const uint8_t*>(Wq);
-        g.Y = q;
-        g.M = M; g.N = HQ; g.K = dm;
-        g.head_D = D;
-        g.col_bytes = qr::kernel_weight_bytes(format, dm, HQ) / HQ;
-        g.ngroups = 3;
-        g.Wx[0] = static_cast<const uint8_t*>(Wk); g.Yx[0] = k; g.Nx[0] = HK;
-        g.Wx[1] = static_cast<const uint8_t*>(Wv); g.Yx[1] = v; g.Nx[1] = HK;
-        rc = launch(g);
-    }
+    const LayerCall lc{X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, Xout, format, M, dm, Hq, Hkv, D, Nm, norm_type, eps};
+    int rc = layer_qkv(lc, q, k, v, xn);
     if (!rc && rope) {
-        rc = check(qr::launch_rope(q, Hq, M, D, theta, offset, traditional, g_stream, k, Hkv), "layer rope");
+        rc = launched(qr::launch_rope(q, Hq, M, D, theta, offset, traditional, g_stream, k, Hkv), "layer rope");
     }
     if (!rc) {
         // The Q8_0 KV cache (unified_prefill_engine.mm:548-572), written in
@@ -833,18 +852,9 @@ int m4_bridge_prefill_layer_ex_kv(void* X, void* w_attn, void* Wq, void* Wk, voi
         hipError_t e = qr::launch_kv_prep(k, v, false, kf, vtf, Hkv, M, D, g_stream, kq, vq);
         qr::AttnParams ap{q, o, Hq, M, D, scale, 1, Hkv, kf, vtf, Mp};
         if (e == hipSuccess) e = qr::launch_flash_attn_q8_0(ap, g_stream);
-        rc = check(e, "layer attention");
+        rc = launched(e, "layer attention");
     }
-    rc = rc ? rc : proj(o, Wo, nullptr, xm, static_cast<const _Float16*>(X), dm, HQ, 0);
-    a = xm;
-    if (!rc && w_ffn) {
-        rc = check(qr::launch_rmsnorm(xm, static_cast<const _Float16*>(w_ffn), xn, M, dm, eps, norm_type, g_stream),
-                   "layer rmsnorm");
-        a = xn;
-    }
-    rc = rc ? rc : proj(a, Wg, Wu, s, nullptr, Nm, dm, 0);
-    rc = rc ? rc : proj(s, Wd, nullptr, static_cast<_Float16*>(Xout), xm, dm, Nm, 0);
-    return rc;
+    return rc ? rc : layer_rest(lc, o, xm, s, xn);
 }
 
 int m4_bridge_rmsnorm(void* X, size_t Xb, void* W, size_t Wb, void* Y, size_t Yb, uint32_t M, uint32_t D, float eps,
@@ -1003,6 +1013,76 @@ int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_
     p.scale = scale;
     p.ws = static_cast<uint8_t*>(ws);
     return launched(qr::launch_paged_attn(p, g_stream), "paged_attn");
+}
+
+int m4_bridge_paged_layer(void* X, void* w_attn, void* Wq, void* Wk, void* Wv, void* Wo, void* w_ffn, void* Wg,
+                          void* Wu, void* Wd, void* Xout, const m4_kv_cache_t* cache, const m4_kv_batch_t* batch,
+                          const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride, int format,
+                          uint32_t dm, uint32_t Hq, uint32_t Nm, float scale, uint32_t window, int norm_type,
+                          float eps) {
+    if (!g_initialized) return -1;
+    bool empty;
+    int rc = qr::validate_layer(cache, batch, rope, positions, position_stride, format, dm, Hq, Nm, scale,
+                                w_attn || w_ffn, norm_type, &empty);
+    if (rc || empty) return rc;
+    void* ptrs[9] = {X, Wq, Wk, Wv, Wo, Wg, Wu, Wd, Xout};
+    for (void* q : ptrs)
+        if (!q || reinterpret_cast<uintptr_t>(q) % 16) return -2;
+    for (void* q : {w_attn, w_ffn})
+        if (q && reinterpret_cast<uintptr_t>(q) % 16) return -2;
+    if (X == Xout) return -2;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    for (void* q : ptrs)
+        if (!dev.owns_all(q)) return -2;
+    for (void* q : {w_attn, w_ffn})
+        if (q && !dev.owns_all(q)) return -2;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table)) return -2;
+    if (rope && (!dev.owns_all(rope->table) || (positions && !dev.owns_all(positions)))) return -2;
+    const uint32_t M = batch->T, Hkv = cache->Hkv, D = cache->D;
+    const size_t nq = (size_t)M * Hq * D, nk = (size_t)M * Hkv * D;
+    qr::PagedAttnParams ap = attn_params(cache, batch, Hq, window);
+    const size_t part = qr::paged_attn_workspace(ap);
+    auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const bool norms = w_attn || w_ffn;
+    const size_t need = 2 * al(nq * 2) + 2 * al(nk * 2) + al(part) + (norms ? 2 : 1) * al((size_t)M * dm * 2) +
+                        al((size_t)M * Nm * 2);
+    if (grow(&g_ws, &g_ws_bytes, need, false, "layer scratch") != hipSuccess) return -5;
+    uint8_t* w = static_cast<uint8_t*>(g_ws);
+    auto take = [&](size_t b) { uint8_t* r = w; w += al(b); return r; };
+    _Float16* q = reinterpret_cast<_Float16*>(take(nq * 2));
+    _Float16* k = reinterpret_cast<_Float16*>(take(nk * 2));
+    _Float16* v = reinterpret_cast<_Float16*>(take(nk * 2));
+    _Float16* o = reinterpret_cast<_Float16*>(take(nq * 2));
+    ap.ws = take(part);
+    _Float16* xm = reinterpret_cast<_Float16*>(take((size_t)M * dm * 2));
+    _Float16* s = reinterpret_cast<_Float16*>(take((size_t)M * Nm * 2));
+    _Float16* xn = norms ? reinterpret_cast<_Float16*>(take((size_t)M * dm * 2)) : nullptr;
+    const LayerCall lc{X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, Xout, format, M, dm, Hq, Hkv, D, Nm, norm_type, eps};
+    rc = layer_qkv(lc, q, k, v, xn);
+    if (!rc) {
+        qr::AppendParams p{};
+        p.K = {k, D, (int64_t)M * D};
+        p.V = {v, D, (int64_t)M * D};
+        if (rope) {
+            p.Q = p.Qo = {q, D, (int64_t)M * D};
+            p.H = Hq;
+            p.rope = rope_view(rope, positions, position_stride);
+        }
+        p.T = M;
+        p.D = D;
+        p.format = cache->format;
+        p.geom = ap.geom;
+        p.batch = ap.batch;
+        rc = launched(qr::launch_kv_append(p, g_stream), "layer append");
+    }
+    if (!rc) {
+        ap.Q = {q, D, (int64_t)M * D};
+        ap.O = {o, (int64_t)Hq * D, D};
+        ap.scale = scale;
+        rc = launched(qr::launch_paged_attn(ap, g_stream), "layer attention");
+    }
+    return rc ? rc : layer_rest(lc, o, xm, s, xn);
 }
 
 void m4_bridge_synchronize(void) {

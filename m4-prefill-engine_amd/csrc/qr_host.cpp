@@ -247,4 +247,27 @@ int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const 
     return 0;
 }
 
+int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rope_axes_t* rope,
+                   const int32_t* positions, uint32_t stride, int format, uint32_t dm, uint32_t Hq, uint32_t Nm,
+                   float scale, bool norms, int norm_type, bool* empty) {
+    *empty = false;
+    if (!cache || !batch) return -2;
+    if (!has_kernels(format) || (norms && norm_type != 1 && norm_type != 2)) return -3;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(batch, empty)) return rc;
+    if (dm == 0 || Nm == 0 || Hq == 0 || Hq > 0xffffu || Hq % cache->Hkv || !std::isfinite(scale)) return -4;
+    const uint64_t HQ = (uint64_t)Hq * cache->D;
+    const uint32_t bs = get_quant_info(static_cast<QuantFormat>(format)).block_size;
+    if (dm % bs || HQ % bs || Nm % bs || dm % 32 || Nm % 32) return -4;
+    if (rope) {
+        if (int rc = check_rope(rope, cache->D)) return rc;
+        if (!positions && rope->axes > 1) return -2;
+    }
+    if (*empty) return 0;
+    if (rope && positions)
+        if (int rc = check_positions(positions, stride, rope->axes, batch->T)) return rc;
+    if ((uint64_t)batch->T * (Hq / cache->Hkv) > 0x7fffffffu) return -4;
+    return 0;
+}
+
 }  // namespace qr

@@ -36,5 +36,9 @@ int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const 
                   bool* empty);
 int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q, const m4_rows_t* O,
                   uint32_t H, float scale, const void* ws, bool* empty);
+// all of a layer's arguments but its tensors
+int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rope_axes_t* rope,
+                   const int32_t* positions, uint32_t position_stride, int format, uint32_t d_model, uint32_t Hq,
+                   uint32_t N_mlp, float scale, bool norms, int norm_type, bool* empty);
 
 }  // namespace qr

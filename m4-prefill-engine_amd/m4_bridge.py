@@ -93,6 +93,7 @@ SIGNATURES = {
     "m4_bridge_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
     "m4_bridge_paged_attn_workspace": ([_VP, _VP, _U32, _U32], _SZ),
     "m4_bridge_dispatch_paged_attn": ([_VP, _VP, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_paged_layer": ([_VP] * 15 + [_U32, _I, _U32, _U32, _U32, _F, _U32, _I, _F], _I),
     "m4_bridge_validate_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
     "m4_bridge_validate_kv_cache_append": ([_VP, _VP, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
     "m4_bridge_validate_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
@@ -769,6 +770,27 @@ class HIPBridge:
                                                       workspace.data_ptr(), workspace.nbytes)
         self._check("m4_bridge_dispatch_paged_attn", ret)
         self._in_flight_tensors.append((cache, batch, Q, O))
+        return ret
+
+    def paged_layer(self, X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, X_out, format, d_model, Hq, N_mlp, attn_scale,
+                    cache: PagedKVCache, batch: KVBatch, rope: Optional[RotaryAxes] = None, positions=None,
+                    norm_type: int = 1, norm_eps: float = 1e-5, window: int = 0) -> int:
+        """prefill_layer_ex over a paged cache: X, X_out [T, d_model] are the batch's rows, whose keys are appended and
+        whose queries see their sequences' (positions None: each token's place)."""
+        bufs = (X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, X_out)
+        T = X.shape[0]
+        for name, t in (("X", X), ("X_out", X_out)):
+            if t.dtype is not _torch.float16 or tuple(t.shape) != (T, d_model) or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous fp16 [{T}, {d_model}]")
+        ptrs = [None if t is None else self.extract_buffer_address_and_size(t)[0] for t in bufs]
+        pos, stride = self._positions(positions, rope, T) if rope is not None else (None, 0)
+        self._on_stream_of(X)
+        batch.struct.T = T
+        ret = self._lib.m4_bridge_paged_layer(*ptrs, cache.ref, batch.ref, rope.on(X.device) if rope is not None else None,
+                                              pos, stride, int(format), d_model, Hq, N_mlp, float(attn_scale), window,
+                                              int(norm_type), float(norm_eps))
+        self._check("m4_bridge_paged_layer", ret)
+        self._in_flight_tensors.append((*bufs, cache, batch, positions))
         return ret
 
     def dequantize(self, W, out, format, K, N) -> int:

@@ -510,6 +510,95 @@ def test_captured_decoding_steps(bridge, fmt):
 
 
 @gpu
+@pytest.mark.parametrize("norm_type,traditional,Hq,Hkv,D,wfmt", [(1, False, 4, 2, 64, 0), (2, True, 4, 1, 128, 3)])
+def test_paged_layer_in_chunks_and_steps(bridge, oracle, norm_type, traditional, Hq, Hkv, D, wfmt):
+    """The layer over two prompts that arrive in chunks beside each other, ending with single tokens, against the
+    oracle's layer of each whole prompt: causal attention makes a row's result the same either way.  Tolerance as for
+    the prefill layer: fp16 in between on both sides, a tie upstream moves a value by about one output step."""
+    import synth
+    import torch
+    from tolerance import TOL
+
+    dm, Nm, P = 256, 512, 16
+    lens = [90, 41]
+    rng = np.random.default_rng(72)
+    Xs = [synth.activations(n, dm, 71 + n) for n in lens]
+    na, nf = ((1 + 0.1 * rng.standard_normal(dm)).astype(np.float16) for _ in range(2))
+    if norm_type == 2:
+        na, nf = (na - 1).astype(np.float16), (nf - 1).astype(np.float16)
+    shapes = [(Hq * D, dm), (Hkv * D, dm), (Hkv * D, dm), (dm, Hq * D), (Nm, dm), (Nm, dm), (dm, Nm)]
+    Ws = [synth.quantized_weights(wfmt, n, k, 80 + i) for i, (n, k) in enumerate(shapes)]
+    table, num = table_of(rng, lens, P)
+    cache = m4_bridge.PagedKVCache(Q8_0, num, P, Hkv, D)
+    rope = m4_bridge.RotaryAxes(D, traditional=traditional)
+    scale = D ** -0.5
+    W = [dev(w) for w in Ws]
+    got = [np.zeros((0, dm), np.float16) for _ in lens]
+    done = np.zeros(2, np.int64)
+    for new in ([50, 7], [0, 33], [39, 0], [1, 1]):
+        x = np.concatenate([Xs[b][done[b]:done[b] + n] for b, n in enumerate(new)])
+        done += new
+        batch = m4_bridge.KVBatch(dev(np.array([0, new[0], sum(new)], np.int32)), dev(done.astype(np.int32)), dev(table))
+        out = torch.empty(len(x), dm, dtype=torch.float16, device="cuda")
+        bridge.paged_layer(dev(x), dev(na), *W[:4], dev(nf), *W[4:], out, wfmt, dm, Hq, Nm, scale, cache, batch, rope,
+                           norm_type=norm_type)
+        bridge.synchronize()
+        o = out.cpu().numpy()
+        got = [np.concatenate([got[0], o[:new[0]]]), np.concatenate([got[1], o[new[0]:]])]
+    for b, n in enumerate(lens):
+        want = oracle.layer_ex(wfmt, Xs[b], na, *Ws[:4], nf, *Ws[4:], Hq, Hkv, D, Nm, scale, norm_type=norm_type, eps=1e-5,
+                               rope=True, theta=10000.0, offset=0, traditional=traditional)
+        d = np.abs(got[b].astype(np.float64) - want.astype(np.float64)).max()
+        say(f"paged layer, sequence {b}: max|diff| {d:.3g}")
+        assert d <= 2 * TOL
+    with pytest.raises(RuntimeError, match="-2"):  # in place
+        x = dev(Xs[0][:1])
+        bridge.paged_layer(x, dev(na), *W[:4], dev(nf), *W[4:], x, wfmt, dm, Hq, Nm, scale, cache,
+                           m4_bridge.KVBatch(dev(np.array([0, 1, 1], np.int32)), dev(np.array(lens, np.int32)), dev(table)))
+
+
+@gpu
+def test_paged_layer_captured(bridge):
+    """A layer's decoding step, replayed as the sequence grows, against the eager calls."""
+    import synth
+    import torch
+
+    dm, Nm, Hq, Hkv, D, P, steps = 256, 512, 4, 2, 64, 16, 4
+    shapes = [(Hq * D, dm), (Hkv * D, dm), (Hkv * D, dm), (dm, Hq * D), (Nm, dm), (Nm, dm), (dm, Nm)]
+    W = [dev(synth.quantized_weights(0, n, k, 80 + i)) for i, (n, k) in enumerate(shapes)]
+    na = dev(np.ones(dm, np.float16))
+    rope = m4_bridge.RotaryAxes(D)
+    xs = [dev(synth.activations(2, dm, 90 + i)) for i in range(steps)]
+
+    def lane():
+        cache = m4_bridge.PagedKVCache(Q4_0, 4, P, Hkv, D)
+        kv_len = torch.zeros(2, dtype=torch.int32, device="cuda")
+        table = dev(np.array([[0, 1], [2, 3]], np.int32))
+        batch = m4_bridge.KVBatch(dev(np.array([0, 1, 2], np.int32)), kv_len, table, 1, 32)
+        x, out = torch.zeros(2, dm, dtype=torch.float16, device="cuda"), torch.zeros(2, dm, dtype=torch.float16, device="cuda")
+        return cache, kv_len, x, out, lambda: bridge.paged_layer(x, na, *W[:4], na, *W[4:], out, 0, dm, Hq, Nm, 0.125, cache,
+                                                                  batch, rope)
+
+    eager, graphed, first = lane(), lane(), lane()
+    first[4]()  # the bridge's scratch grows to this size before the capture (no keys yet: nothing is written)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        graphed[4]()
+    for i in range(steps):
+        for l in (eager, graphed):
+            l[1].copy_(dev(np.array([i + 1, i + 14], np.int32)))
+            l[2].copy_(xs[i])
+        eager[4]()
+        bridge.synchronize()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager[3].view(torch.int16), graphed[3].view(torch.int16)), f"step {i}"
+        assert torch.equal(eager[0].pages, graphed[0].pages), f"step {i}"
+
+
+@gpu
 def test_on_another_stream(bridge):
     import torch
 
@@ -665,6 +754,8 @@ def test_uninitialized_bridge_refuses(lib):
     assert lib.m4_bridge_rope_axes(r(a.rope), 0x4000, 10, r(a.q), r(a.q), 10, 8, 128) == -1
     assert lib.m4_bridge_kv_cache_append(r(a.cache), r(a.batch), r(a.kv), r(a.kv), None, None, 0, None, None, 0) == -1
     assert lib.m4_bridge_kv_cache_read(r(a.cache), r(a.batch), r(a.kv), r(a.kv)) == -1
+    assert lib.m4_bridge_paged_layer(*[0x600000] * 11, r(a.cache), r(a.batch), None, None, 0, 0, 256, 8, 512, 0.1, 0, 1,
+                                     1e-5) == -1
     assert lib.m4_bridge_dispatch_paged_attn(r(a.cache), r(a.batch), r(a.q), r(a.q), 8, 0.1, 0, 0x400000, 1 << 30) == -1
 
 
@@ -697,6 +788,28 @@ def test_python_refusals(libpath):
         b.dispatch_paged_attn(cache, batch, kv, kv[:, :1], 0.1)
     with pytest.raises(ValueError):
         b.rope_axes(kv, kv, m4_bridge.RotaryAxes(128, sections=(16, 24, 24)), i32(3))
+
+
+@gpu
+@pytest.mark.parametrize("change,code", [
+    ({"fmt": 9}, -3), ({"norm_type": 3}, -3), ({"Hq": 3}, -4), ({"dm": 100}, -4), ({"Nm": 0}, -4), ({"cache_fmt": 1}, -3),
+    ({"ptr": None}, -2), ({"ptr": 8}, -2), ({"B": 0}, 0),
+])
+def test_paged_layer_refusals(bridge, change, code):
+    import torch
+
+    v = {"fmt": 0, "norm_type": 1, "Hq": 4, "dm": 256, "Nm": 512, "cache_fmt": 6, "ptr": 0, "B": 2, **change}
+    lib, a = bridge.lib, Args()
+    buf = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    a.cache.pages, a.cache.format = buf.data_ptr(), v["cache_fmt"]
+    a.batch.q_start = a.batch.kv_len = a.batch.page_table = buf.data_ptr()
+    a.batch.B = v["B"]
+    x = None if v["ptr"] is None else buf.data_ptr() + v["ptr"]
+    r = ctypes.addressof
+    # a well-formed call is not made here: B = 0 is the only one that passes
+    assert lib.m4_bridge_paged_layer(x, *[buf.data_ptr() + 512] * 9, buf.data_ptr() + 1024, r(a.cache), r(a.batch), None, None, 0, v["fmt"],
+                                     v["dm"], v["Hq"], v["Nm"], 0.1, 0, v["norm_type"], 1e-5) == code
+    bridge.synchronize()
 
 
 @gpu
