@@ -427,6 +427,7 @@ qr::RopeView rope_view(const m4_rope_axes_t* r, const int32_t* positions, uint32
 qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, uint32_t H, uint32_t window) {
     qr::PagedAttnParams p{};
     p.H = H;
+    p.G = H / c->Hkv;
     p.D = c->D;
     p.format = c->format;
     p.window = window;

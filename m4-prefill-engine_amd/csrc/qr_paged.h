@@ -89,7 +89,7 @@ hipError_t launch_kv_read(const ReadParams& p, hipStream_t st);
 
 struct PagedAttnParams {
     RowsView Q, O;
-    uint32_t H, D;
+    uint32_t H, G, D;  // query heads, those of a KV head, head width
     int format;
     float scale;
     uint32_t window;  // keys a row sees at most (the newest), 0: all

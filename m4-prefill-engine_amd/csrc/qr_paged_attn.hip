@@ -182,6 +182,19 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int at) {
            (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, at);
 }
 
+// a / b of wave-uniform numbers that nearly always fit in 32 bits, where a
+// division takes a fifth of the time
+__device__ __forceinline__ uint64_t udiv(uint64_t a, uint64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
+}
+// share w of nw of a line of `total`: the remainder goes to the first ones
+__device__ __forceinline__ void share_of(uint64_t total, uint64_t nw, uint32_t w, uint64_t& s0, uint64_t& s1) {
+    const uint64_t each = udiv(total, nw), more = total - each * nw;
+    s0 = each * w + min((uint64_t)w, more);
+    s1 = s0 + each + (w < more ? 1 : 0);
+}
+
 struct Seq {
     int q0, n, len, lo;   // first row, new tokens, keys, first key that any row sees (a multiple of kStep)
     uint32_t tiles, steps;  // row tiles and key steps per tile
@@ -196,7 +209,7 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
     s.len = min(max(p.batch.kv_len[b], 0), cap);
     s.lo = 0;
     if (p.window) s.lo = (int)(max((int64_t)s.len - s.n + 1 - (int64_t)p.window, (int64_t)0) / kStep * kStep);
-    const uint32_t G = p.H / p.geom.Hkv;
+    const uint32_t G = p.G;
     s.tiles = (uint32_t)(((uint64_t)s.n * G + R - 1) / R);
     s.steps = max((uint32_t)(s.len - s.lo + (int)kStep - 1) / kStep, 1u);
     s.cost = (uint64_t)p.geom.Hkv * s.tiles * (kItemCost + s.steps);
@@ -249,7 +262,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     const uint64_t nw = min((uint64_t)workers, total);
     if (threadIdx.x == 0) *note = ItemNote{};
     if (lane == 0) head_of[wave] = 0;
-    const uint64_t s0 = w < nw ? total * w / nw : 0, s1 = w < nw ? total * (w + 1) / nw : 0;
+    uint64_t s0 = 0, s1 = 0;
+    if (w < nw) share_of(total, nw, w, s0, s1);
     uint32_t b = 0;
     uint64_t off = 0;
     if (incl - mine <= s0 && s0 < incl) {
@@ -268,7 +282,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     const bool neg = c < 0.0f;
     if (neg) c = -c;
     c = fmaxf(c, 1.17549435e-38f);  // a scale of zero weighs seen keys alike, and hidden ones (-infinity times it) not
-    const uint32_t G = p.H / p.geom.Hkv;
+    const uint32_t G = p.G;
     const h2_t one2 = {(_Float16)1.0f, (_Float16)1.0f};
     const uint32_t pmask = (1u << p.geom.log2_page) - 1;
 
@@ -339,14 +353,14 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         }
         // this share of the item: its line from o0 on, steps u0 .. u0 + nu
         const uint32_t line = kItemCost + s.steps;
-        const uint32_t o0 = (uint32_t)(off % line), item = (uint32_t)(off / line);
+        const uint32_t item = (uint32_t)udiv(off, line), o0 = (uint32_t)(off - (uint64_t)item * line);
         const uint32_t o1 = (uint32_t)min((uint64_t)line, o0 + (s1 - cur));
         cur += o1 - o0;
         off += o1 - o0;
         if (o1 <= kItemCost) continue;
         const uint32_t u0 = o0 > kItemCost ? o0 - kItemCost : 0, nu = o1 - kItemCost - u0;
-        hk = item / s.tiles;
-        rt = item % s.tiles;
+        hk = s.tiles == 1 ? item : item / s.tiles;
+        rt = item - hk * s.tiles;
         const int p0 = s.len - s.n;  // position of the first new token
 
         // ---- rows ----
@@ -597,7 +611,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
     const uint32_t per = (groups + gridDim.x - 1) / gridDim.x, w1 = min((blockIdx.x + 1) * per, groups);
     const ItemNote* notes = reinterpret_cast<const ItemNote*>(p.ws);
     const uint32_t tid = threadIdx.x, lane = tid & 63, l4 = tid % L, group = tid / L;
-    const uint32_t G = p.H / p.geom.Hkv;
+    const uint32_t G = p.G;
     // 32 notes at a time to begin at, and those behind them to end at, a lane each
     for (uint32_t base = blockIdx.x * per; base < w1; base += 32) {
         ItemNote mine{};
@@ -722,7 +736,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 5, j = lane & 31;
     ItemNote* note = reinterpret_cast<ItemNote*>(p.ws) + blockIdx.x;
-    const uint32_t G = p.H / p.geom.Hkv, tokens = R / G;
+    const uint32_t G = p.G, tokens = R / G;
     const uint32_t pmask = (1u << p.geom.log2_page) - 1;
 
     // ---- this workgroup's share [s0, s1) ----
@@ -747,7 +761,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
     const uint64_t nw = max(min((uint64_t)groups, total / kChunkMin), (uint64_t)1);
     if (tid == 0) *note = ItemNote{};
     if (blockIdx.x >= nw || total == 0) return;
-    const uint64_t s0 = total * blockIdx.x / nw, s1 = total * (blockIdx.x + 1) / nw;
+    uint64_t s0, s1;
+    share_of(total, nw, blockIdx.x, s0, s1);
     uint32_t b = 0;
     uint64_t off = 0;
     const bool here = incl - mine <= s0 && s0 < incl;
@@ -799,7 +814,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             off = 0;
             continue;
         }
-        const uint32_t hk = (uint32_t)(off / row_cost);
+        const uint32_t hk = (uint32_t)udiv(off, row_cost);
         uint64_t in_row = off - hk * row_cost;
         uint32_t rt = 0, steps;
         int lo;
@@ -1076,7 +1091,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
 
 // Row tiles by the rows of the longest chunk, workgroups by the length of the line expected.
 static WorkPlan plan_of(const PagedAttnParams& p) {
-    const uint64_t G = p.H / p.geom.Hkv, max_new = p.max_new ? p.max_new : 1, rows = max_new * G;
+    const uint64_t G = p.G, max_new = p.max_new ? p.max_new : 1, rows = max_new * G;
     WorkPlan w;
     w.rows = rows <= 16 ? 16 : 32;
     uint64_t keys = p.max_kv ? p.max_kv : 1;
