@@ -12,18 +12,27 @@
 #include "qr_device.h"
 #include "qr_paged.h"
 
+#ifndef QR_WPE
+#define QR_WPE
+#endif
+#ifndef QR_WPR
+#define QR_WPR
+#endif
 namespace qr {
 
 constexpr uint32_t kWaves = 4;     // of a workgroup
 constexpr uint32_t kStep = 32;     // keys of a step
 // What an item costs beside its steps, in steps: its descriptors, queries and
-// the write of its rows.  64 requests of 1 .. 8192 keys: 4 and 8 the same within
-// noise; shares by steps alone, with a join of four waves an item, 44 us, now 33.
-constexpr uint32_t kItemCost = 4;
-// Waves of a launch: two per SIMD, what the registers allow with the next step's
-// tiles in flight (three without them: 47 us there), at least kMinSteps of the
-// line each.
-constexpr uint32_t kMaxWaves = 2048, kMinSteps = 2;
+// the write of its rows.  us with 2 / 3 / 4: drafted tokens 19.3 / 18.2 / 18.9, a
+// chunk of 300 among single tokens 23.7 / 25.3 / 25.0, 64 requests of D = 64
+// 21.7 / 19.1 / 19.0.
+constexpr uint32_t kItemCost = 3;
+// Waves: two per SIMD where they get kLongShare of the line each (four requests of
+// 131072 keys: 132 us on one, 118 on two), else up to one per SIMD: fewer items
+// are cut and fewer parts joined (drafted tokens 18.2 us, on two 19.8; one token
+// over 16384 keys 16.8 and 19.5).  Three are slower, 145 us and more: with the next
+// step's tiles in flight the registers hold two.
+constexpr uint32_t kMaxWaves = 2048, kFewWaves = 1024, kLongShare = 16, kMinSteps = 2;
 // Chunks: rows of a row tile, workgroups (one a CU), what an item costs beside its
 // key tiles and the least of the line that is worth a workgroup.
 constexpr uint32_t kChunkTile = 256, kChunkGroups = 256, kChunkCost = 2, kChunkMin = 4;
@@ -229,7 +238,7 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // keys (Q8_0, 110 MB) 33 us of which 4 are the join; one of 1000 keys 13.6 us, a
 // chain of descriptor, page table, key and join latencies.
 template <int FMT, int D, int NR>
-__global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
+__global__ void __launch_bounds__(256, 2) QR_WPR paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
     constexpr int DT = D / 16, KK = D / 32;
     constexpr int RUN = D / 4;  // dims of a lane's run
@@ -259,7 +268,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         if ((uint32_t)lane >= o) incl += x;
     }
     const uint64_t total = lane_u64(incl, (int)min(p.batch.B, 64u) - 1);
-    const uint64_t nw = min((uint64_t)workers, total);
+    const uint64_t nw = min((uint64_t)workers, max(min(total, (uint64_t)kFewWaves), total / kLongShare));
     if (threadIdx.x == 0) *note = ItemNote{};
     if (lane == 0) head_of[wave] = 0;
     uint64_t s0 = 0, s1 = 0;
@@ -720,7 +729,7 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
 // double-buffered LDS tile, the codes loaded two tiles ahead; then each wave
 // takes its rows over the tile, 32 x 32 scores at a time.
 template <int FMT, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
+__global__ void __launch_bounds__(64 * NW, 2) QR_WPE paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
     constexpr int DT = D / 32, KK = D / 16;
     constexpr int KU = D / 8, VU = KT / 8;       // 16-byte units of a K row (a key), of a V^T row (a dim)

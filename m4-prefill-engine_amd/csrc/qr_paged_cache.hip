@@ -3,13 +3,9 @@
 #include "qr_device.h"
 #include "qr_paged.h"
 
-#ifndef QR_GR
-#define QR_GR 1024
-#endif
-#ifndef QR_GB
-#define QR_GB 1024
-#endif
 namespace qr {
+
+constexpr uint64_t kBlocks = 1024;  // that fill the chip
 
 // Where a token lies in the cache.
 struct Place {
@@ -96,40 +92,58 @@ __device__ __forceinline__ void quantize8(const float x[8], int lane, uint32_t c
     }
 }
 
-// One row of T tokens per LPR lanes, 8 dims a lane; a wave takes 64 / LPR
-// tokens and every `chunks`-th of the heads (Q, then K, then V), so angles are
-// formed once per wave and used for all its heads.  A rotated row is rounded to
-// fp16 before it is quantized, as a rotation and a write apart would.
+// One row of T tokens per LPR lanes, 8 dims a lane; a wave takes 64 / LPR tokens
+// and every so many of the heads, of Q (the first q_blocks of a row of blocks) or
+// of K and V, so angles are formed once per wave and used for all its heads.  A
+// rotated row is rounded to fp16 before it is quantized, as a rotation and a write
+// apart would.  Bound by bytes once there are enough: 8100 tokens of 32 heads
+// (133 MB) 30 us, 4.4 TB/s; 64 tokens 5 us, a chain of table and angle latencies.
 template <int LPR, int FMT>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t q_blocks) {
     constexpr int RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l = lane % LPR, sub = lane / LPR;
-    const uint32_t t0 = (blockIdx.x * 4 + wave) * RPW, t = t0 + sub, chunk = blockIdx.y, chunks = gridDim.y;
-    const bool cached = p.geom.pages != nullptr;
-    const uint32_t items = p.H + (cached ? 2 * p.geom.Hkv : 0);
+    const uint32_t t0 = (blockIdx.x * 4 + wave) * RPW, t = t0 + sub;
+    const bool of_q = blockIdx.y < q_blocks;
+    const uint32_t chunk = of_q ? blockIdx.y : blockIdx.y - q_blocks, chunks = of_q ? q_blocks : gridDim.y - q_blocks;
+    const uint32_t heads = of_q ? p.H : p.geom.Hkv;
     if (t0 >= p.T) return;
     const bool live = t < p.T && 8u * l < p.D;
 
-    // Rows of kAhead heads are loaded together, those of the next kAhead while these
-    // are turned and stored; the first are under way while places and angles are found.
+    // Heads chunk, chunk + chunks, ...: kAhead rows of Q, or kAhead / 2 of K and of V,
+    // are loaded together, the next while these are turned and stored; the first are
+    // under way while places and angles are found.
     constexpr int kAhead = 4;
     h8_t next[kAhead];
-    auto fetch = [&](uint32_t it0) {
-#pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const uint32_t it = it0 + i * chunks;
-            if (it >= items || !live) continue;
-            const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
-            const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
-            const _Float16* src = is_q ? p.Q.p : (is_k ? p.K.p : p.V.p);
-            const int64_t ts = is_q ? p.Q.ts : (is_k ? p.K.ts : p.V.ts), hs = is_q ? p.Q.hs : (is_k ? p.K.hs : p.V.hs);
-            next[i] = *reinterpret_cast<const h8_t*>(src + (int64_t)t * ts + (int64_t)h * hs + 8 * l);
-        }
-    };
 #pragma unroll
     for (int i = 0; i < kAhead; i++) next[i] = h8_t{};
-    fetch(chunk);
+    const _Float16 *src = nullptr, *src2 = nullptr;  // the next row to load, of V too
+    int64_t step, step2 = 0;
+    if (of_q) {
+        src = p.Q.p + (int64_t)t * p.Q.ts + (int64_t)chunk * p.Q.hs + 8 * l;
+        step = (int64_t)chunks * p.Q.hs;
+    } else {
+        src = p.K.p + (int64_t)t * p.K.ts + (int64_t)chunk * p.K.hs + 8 * l;
+        src2 = p.V.p + (int64_t)t * p.V.ts + (int64_t)chunk * p.V.hs + 8 * l;
+        step = (int64_t)chunks * p.K.hs;
+        step2 = (int64_t)chunks * p.V.hs;
+    }
+    uint32_t ahead = chunk;  // its head
+    auto fetch = [&]() {
+        if (of_q) {
+#pragma unroll
+            for (int i = 0; i < kAhead; i++, ahead += chunks, src += step)
+                if (ahead < heads && live) next[i] = *reinterpret_cast<const h8_t*>(src);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kAhead; i += 2, ahead += chunks, src += step, src2 += step2)
+                if (ahead < heads && live) {
+                    next[i] = *reinterpret_cast<const h8_t*>(src);
+                    next[i + 1] = *reinterpret_cast<const h8_t*>(src2);
+                }
+        }
+    };
+    fetch();
 
     Place at{0, 0, 0, false};
     bool row = live;
@@ -201,71 +215,86 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p) {
     }
     const bool any_turned = p.rope.pairs != 0;
 
-    auto one = [&](uint32_t it, h8_t y) {
-        const bool is_q = it < p.H, is_k = !is_q && it < p.H + p.geom.Hkv;
-        const uint32_t h = is_q ? it : (is_k ? it - p.H : it - p.H - p.geom.Hkv);
-        if (any_turned && (is_q || is_k)) {
-            u4_t mine = __builtin_bit_cast(u4_t, y), theirs;
-            if (p.rope.traditional) {
-                theirs = u4_t{mine.x >> 16 | mine.x << 16, mine.y >> 16 | mine.y << 16, mine.z >> 16 | mine.z << 16,
-                              mine.w >> 16 | mine.w << 16};
-            } else {
-                theirs = u4_t{(uint32_t)__shfl((int)mine.x, other), (uint32_t)__shfl((int)mine.y, other),
-                              (uint32_t)__shfl((int)mine.z, other), (uint32_t)__shfl((int)mine.w, other)};
-            }
-            const h8_t z = __builtin_bit_cast(h8_t, theirs);
-            if (turned) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = (_Float16)((float)y[e] * cs[e] + (float)z[e] * sn[e]);
-            }
+    auto turn = [&](h8_t y) {
+        u4_t mine = __builtin_bit_cast(u4_t, y), theirs;
+        if (p.rope.traditional) {
+            theirs = u4_t{mine.x >> 16 | mine.x << 16, mine.y >> 16 | mine.y << 16, mine.z >> 16 | mine.z << 16,
+                          mine.w >> 16 | mine.w << 16};
+        } else {
+            theirs = u4_t{(uint32_t)__shfl((int)mine.x, other), (uint32_t)__shfl((int)mine.y, other),
+                          (uint32_t)__shfl((int)mine.z, other), (uint32_t)__shfl((int)mine.w, other)};
         }
-        if (is_q) {
-            if (row) *reinterpret_cast<h8_t*>(p.Qo.p + (int64_t)t * p.Qo.ts + (int64_t)h * p.Qo.hs + 8 * l) = y;
-            return;
+        const h8_t z = __builtin_bit_cast(h8_t, theirs);
+        if (turned) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = (_Float16)((float)y[e] * cs[e] + (float)z[e] * sn[e]);
         }
-        if constexpr (FMT >= 0) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = (float)y[e];
-            uint32_t c[8], d16;
-            quantize8<FMT>(x, lane, c, d16);
-            if (!row) return;
-            constexpr uint32_t D = LPR * 8, NB = D / 32, CB = FMT == QUANT_Q8_0 ? D : D / 2;
-            uint8_t* head = p.geom.pages + ((size_t)at.page * p.geom.Hkv + h) * p.geom.head_bytes;
-            if (is_k) {
-                uint8_t* o = head + at.slot * CB;
-                if constexpr (FMT == QUANT_Q8_0) {
-                    *reinterpret_cast<u2_t*>(o + 8 * l) = u2_t{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
-                                                               c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
-                } else {
-                    *reinterpret_cast<uint32_t*>(o + 4 * l) =
-                        c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24 | c[4] << 4 | c[5] << 12 | c[6] << 20 | c[7] << 28;
-                }
-                if (l % 4 == 0)
-                    *reinterpret_cast<uint16_t*>(head + p.geom.ks_off + (at.slot * NB + l / 4) * 2) = (uint16_t)d16;
-            } else {
-                const uint32_t g4 = at.slot >> 2, k4 = at.slot & 3;
-                uint8_t* o = head + p.geom.v_off + g4 * (4 * CB) + k4;
-                if constexpr (FMT == QUANT_Q8_0) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) o[(8 * l + e) * 4] = (uint8_t)c[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[(4 * l + e) * 4] = (uint8_t)(c[2 * e] | c[2 * e + 1] << 4);
-                }
-                if (l % 4 == 0)
-                    *reinterpret_cast<uint16_t*>(head + p.geom.vs_off + ((g4 * NB + l / 4) * 4 + k4) * 2) = (uint16_t)d16;
-            }
-        }
+        return y;
     };
-    for (uint32_t it0 = chunk; it0 < items; it0 += kAhead * chunks) {
-        h8_t now[kAhead];
+
+    if (of_q) {
+        _Float16* dst = p.Qo.p + (int64_t)t * p.Qo.ts + (int64_t)chunk * p.Qo.hs + 8 * l;
+        for (uint32_t h = chunk; h < heads;) {
+            h8_t now[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) now[i] = next[i];
-        fetch(it0 + kAhead * chunks);
+            for (int i = 0; i < kAhead; i++) now[i] = next[i];
+            fetch();
 #pragma unroll
-        for (int i = 0; i < kAhead; i++)
-            if (it0 + i * chunks < items) one(it0 + i * chunks, now[i]);
+            for (int i = 0; i < kAhead; i++, h += chunks, dst += (int64_t)chunks * p.Qo.hs) {
+                if (h >= heads) break;
+                const h8_t y = any_turned ? turn(now[i]) : now[i];
+                if (row) *reinterpret_cast<h8_t*>(dst) = y;
+            }
+        }
+        return;
+    }
+    if constexpr (FMT >= 0) {
+        constexpr uint32_t D = LPR * 8, NB = D / 32, CB = FMT == QUANT_Q8_0 ? D : D / 2;
+        const uint32_t g4 = at.slot >> 2, k4 = at.slot & 3;
+        for (uint32_t h = chunk; h < heads;) {
+            h8_t now[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) now[i] = next[i];
+            fetch();
+#pragma unroll
+            for (int i = 0; i < kAhead; i += 2, h += chunks) {
+                if (h >= heads) break;
+                const h8_t k = any_turned ? turn(now[i]) : now[i], v = now[i + 1];
+                float x[8];
+                uint32_t c[8], d16;
+                uint8_t* head = p.geom.pages + ((size_t)at.page * p.geom.Hkv + h) * p.geom.head_bytes;
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = (float)k[e];
+                quantize8<FMT>(x, lane, c, d16);
+                if (row) {
+                    uint8_t* o = head + at.slot * CB;
+                    if constexpr (FMT == QUANT_Q8_0) {
+                        *reinterpret_cast<u2_t*>(o + 8 * l) = u2_t{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
+                                                                   c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
+                    } else {
+                        *reinterpret_cast<uint32_t*>(o + 4 * l) =
+                            c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24 | c[4] << 4 | c[5] << 12 | c[6] << 20 | c[7] << 28;
+                    }
+                    if (l % 4 == 0)
+                        *reinterpret_cast<uint16_t*>(head + p.geom.ks_off + (at.slot * NB + l / 4) * 2) = (uint16_t)d16;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = (float)v[e];
+                quantize8<FMT>(x, lane, c, d16);
+                if (row) {
+                    uint8_t* o = head + p.geom.v_off + g4 * (4 * CB) + k4;
+                    if constexpr (FMT == QUANT_Q8_0) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) o[(8 * l + e) * 4] = (uint8_t)c[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[(4 * l + e) * 4] = (uint8_t)(c[2 * e] | c[2 * e + 1] << 4);
+                    }
+                    if (l % 4 == 0)
+                        *reinterpret_cast<uint16_t*>(head + p.geom.vs_off + ((g4 * NB + l / 4) * 4 + k4) * 2) = (uint16_t)d16;
+                }
+            }
+        }
     }
 }
 
@@ -275,15 +304,21 @@ hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
     if (p.D > 256 || p.D % 8 || p.rope.pairs > 128 || p.rope.pairs % 8 || 2 * p.rope.pairs > p.D)
         return hipErrorInvalidValue;
     if (p.geom.pages && p.D != 64 && p.D != 128) return hipErrorInvalidValue;
-    const uint32_t items = p.H + (p.geom.pages ? 2 * p.geom.Hkv : 0);
-    if (items == 0) return hipSuccess;
-    // four waves of rows side by side, the heads over as many blocks as fill the chip
+    // four waves of rows side by side; the heads of Q, and those of K and V, over as
+    // many blocks as fill the chip (8100 x 32 heads: 1024 blocks 30.3 us, 4096 39.9)
     const uint32_t rows = 4 * 64 / lpr, groups = (p.T + rows - 1) / rows;
-    uint32_t blocks = items;
-    while (blocks > 1 && (uint64_t)groups * blocks > QR_GB) blocks = (blocks + 1) / 2;
-    const dim3 grid(groups, blocks);
+    uint32_t q_blocks = p.H, kv_blocks = p.geom.pages ? p.geom.Hkv : 0;
+    if (q_blocks + kv_blocks == 0) return hipSuccess;
+    // a head of K and V takes longer than eight of Q (three prompts of a 1B model, with
+    // the read back: counted as 2 / 4 / 8 of Q 21.4 / 20.3 / 19.4 us)
+    for (uint32_t each = 1; (uint64_t)groups * (q_blocks + kv_blocks) > kBlocks && each < 0x10000; each *= 2) {
+        const uint32_t of_kv = each > 8 ? each / 8 : 1;
+        q_blocks = (p.H + each - 1) / each;
+        kv_blocks = p.geom.pages ? (p.geom.Hkv + of_kv - 1) / of_kv : 0;
+    }
+    const dim3 grid(groups, q_blocks + kv_blocks);
     const int fmt = p.geom.pages ? p.format : -1;
-#define QR_APPEND(L, F) hipLaunchKernelGGL((kv_append_kernel<L, F>), grid, dim3(256), 0, st, p)
+#define QR_APPEND(L, F) hipLaunchKernelGGL((kv_append_kernel<L, F>), grid, dim3(256), 0, st, p, q_blocks)
     if (fmt < 0) {
         if (lpr == 8) QR_APPEND(8, -1);
         else if (lpr == 16) QR_APPEND(16, -1);
@@ -372,7 +407,7 @@ hipError_t launch_kv_read(const ReadParams& p, hipStream_t st) {
     if (p.D != 64 && p.D != 128) return hipErrorInvalidValue;
     const uint32_t rows = p.D == 64 ? 32 : 16, groups = (p.batch.T + rows - 1) / rows;
     uint32_t blocks = 2 * p.geom.Hkv;
-    while (blocks > 1 && (uint64_t)groups * blocks > QR_GR) blocks = (blocks + 1) / 2;
+    while (blocks > 1 && (uint64_t)groups * blocks > kBlocks) blocks = (blocks + 1) / 2;
     const dim3 grid(groups, blocks);
     switch ((p.D == 128 ? 1 : 0) + (p.format == QUANT_Q8_0 ? 2 : 0)) {
         case 0: hipLaunchKernelGGL((kv_read_kernel<8, QUANT_Q4_0>), grid, dim3(256), 0, st, p); break;
