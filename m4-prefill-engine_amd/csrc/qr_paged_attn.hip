@@ -12,12 +12,6 @@
 #include "qr_device.h"
 #include "qr_paged.h"
 
-#ifndef QR_WPE
-#define QR_WPE
-#endif
-#ifndef QR_WPR
-#define QR_WPR
-#endif
 namespace qr {
 
 constexpr uint32_t kWaves = 4;     // of a workgroup
@@ -197,11 +191,13 @@ __device__ __forceinline__ uint64_t udiv(uint64_t a, uint64_t b) {
     if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
     return a / b;
 }
-// share w of nw of a line of `total`: the remainder goes to the first ones
-__device__ __forceinline__ void share_of(uint64_t total, uint64_t nw, uint32_t w, uint64_t& s0, uint64_t& s1) {
-    const uint64_t each = udiv(total, nw), more = total - each * nw;
-    s0 = each * w + min((uint64_t)w, more);
-    s1 = s0 + each + (w < more ? 1 : 0);
+// share w of nw (at most 2^16) of a line of `total`: total w / nw on, in whole
+// places, so that as many items as shares, alike in cost, are not cut
+__device__ __forceinline__ void share_of(uint64_t total, uint32_t nw, uint32_t w, uint64_t& s0, uint64_t& s1) {
+    const uint64_t each = udiv(total, nw);
+    const uint32_t more = (uint32_t)(total - each * nw);
+    s0 = each * w + more * w / nw;
+    s1 = each * (w + 1) + more * (w + 1) / nw;
 }
 
 struct Seq {
@@ -238,7 +234,7 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // keys (Q8_0, 110 MB) 33 us of which 4 are the join; one of 1000 keys 13.6 us, a
 // chain of descriptor, page table, key and join latencies.
 template <int FMT, int D, int NR>
-__global__ void __launch_bounds__(256, 2) QR_WPR paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
+__global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
     constexpr int DT = D / 16, KK = D / 32;
     constexpr int RUN = D / 4;  // dims of a lane's run
@@ -272,7 +268,7 @@ __global__ void __launch_bounds__(256, 2) QR_WPR paged_attn_kernel(PagedAttnPara
     if (threadIdx.x == 0) *note = ItemNote{};
     if (lane == 0) head_of[wave] = 0;
     uint64_t s0 = 0, s1 = 0;
-    if (w < nw) share_of(total, nw, w, s0, s1);
+    if (w < nw) share_of(total, (uint32_t)nw, w, s0, s1);
     uint32_t b = 0;
     uint64_t off = 0;
     if (incl - mine <= s0 && s0 < incl) {
@@ -729,7 +725,7 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
 // double-buffered LDS tile, the codes loaded two tiles ahead; then each wave
 // takes its rows over the tile, 32 x 32 scores at a time.
 template <int FMT, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) QR_WPE paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
+__global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
     constexpr int DT = D / 32, KK = D / 16;
     constexpr int KU = D / 8, VU = KT / 8;       // 16-byte units of a K row (a key), of a V^T row (a dim)
@@ -771,7 +767,7 @@ __global__ void __launch_bounds__(64 * NW, 2) QR_WPE paged_attn_chunk_kernel(Pag
     if (tid == 0) *note = ItemNote{};
     if (blockIdx.x >= nw || total == 0) return;
     uint64_t s0, s1;
-    share_of(total, nw, blockIdx.x, s0, s1);
+    share_of(total, (uint32_t)nw, blockIdx.x, s0, s1);
     uint32_t b = 0;
     uint64_t off = 0;
     const bool here = incl - mine <= s0 && s0 < incl;
@@ -940,12 +936,7 @@ __global__ void __launch_bounds__(64 * NW, 2) QR_WPE paged_attn_chunk_kernel(Pag
         // when one passes 8: positive floats compare as integers do, negative ones are
         // negative integers, so one integer maximum (three at a time, and with no
         // quieting of NaNs) tells.
-        auto exponents = [&](const f16v_t& sc, float ex[16]) {
-            int top = 0;
-#pragma unroll
-            for (int e = 0; e < 16; e++) ex[e] = __builtin_fmaf(sc[e], c, -m_run);
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) top = max(max(top, (int)f32_bits(ex[e])), (int)f32_bits(ex[e + 1]));
+        auto settle = [&](const f16v_t& sc, float ex[16], int top) {
             if (__any(top > (int)0x41000000)) {
                 float mx = sc[0];
 #pragma unroll
@@ -960,6 +951,14 @@ __global__ void __launch_bounds__(64 * NW, 2) QR_WPE paged_attn_chunk_kernel(Pag
 #pragma unroll
                 for (int e = 0; e < 16; e++) ex[e] = __builtin_fmaf(sc[e], c, -m_run);
             }
+        };
+        auto exponents = [&](const f16v_t& sc, float ex[16]) {
+            int top = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) ex[e] = __builtin_fmaf(sc[e], c, -m_run);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) top = max(max(top, (int)f32_bits(ex[e])), (int)f32_bits(ex[e + 1]));
+            settle(sc, ex, top);
         };
         auto weigh = [&](const float ex[16], uint32_t pk[8]) {
 #pragma unroll
@@ -990,17 +989,75 @@ __global__ void __launch_bounds__(64 * NW, 2) QR_WPE paged_attn_chunk_kernel(Pag
 #pragma unroll
             for (int x = 0; x < NW; x++) all_there &= there[u & 1][x] != 0;
             if (!(k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !all_there)) {
-                // every row sees every key: the next unit's scores are computed beside this
-                // one's weights
-                f16v_t sc = scores(buf, 0);
+                // every row sees every key.  Each line below ends at a barrier for the scheduler:
+                // one MFMA, the loads of operands four MFMAs ahead, and the vector work that
+                // runs beside it -- a unit's exponentials beside the next one's scores (the
+                // matrix pipe leaves the transcendental unit free), the next one's exponents
+                // beside this one's values.
+                auto key = [&](int x, int kk) {
+                    return *reinterpret_cast<const h8_t*>(buf + x * 32 * (KU * 16) + (kof ^ 32u * kk));
+                };
+                auto value = [&](int x, int i) {
+                    return *reinterpret_cast<const h8_t*>(buf + KB + (i % DT) * 32 * (VU * 16) + (vof ^ 32u * (2 * x + i / DT)));
+                };
+                constexpr int NV = 2 * DT;
+                h8_t kf[4], vf[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) kf[i] = key(0, i);
+                f16v_t sc{};
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) {
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk & 3], qf[kk], sc, 0, 0, 0);
+                    kf[kk & 3] = kk + 4 < KK ? key(0, kk + 4) : key(1, kk + 4 - KK);
+                }
+                float ex[16];
+                exponents(sc, ex);
 #pragma unroll
                 for (int x = 0; x < UNITS; x++) {
-                    float ex[16];
-                    exponents(sc, ex);
                     uint32_t pk[8];
-                    if (x + 1 < UNITS) sc = scores(buf, x + 1);
-                    weigh(ex, pk);
-                    add(buf, x, pk);
+                    auto pair = [&](int e) {
+                        const f2_t w = {__builtin_amdgcn_exp2f(ex[2 * e]), __builtin_amdgcn_exp2f(ex[2 * e + 1])};
+                        const h2_t pp = __builtin_convertvector(w, h2_t);
+                        pk[e] = as_u32(pp);
+                        l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                    };
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (x + 1 < UNITS) {
+                        sc = f16v_t{};
+#pragma unroll
+                        for (int kk = 0; kk < KK; kk++) {
+                            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk & 3], qf[kk], sc, 0, 0, 0);
+                            if (kk + 4 < KK) kf[kk & 3] = key(x + 1, kk + 4);
+                            else vf[kk + 4 - KK] = value(x, kk + 4 - KK);
+#pragma unroll
+                            for (int e = 0; e < 8 / KK; e++) pair(kk * (8 / KK) + e);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) vf[i] = value(x, i);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) pair(e);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    int top = 0;
+#pragma unroll
+                    for (int i = 0; i < NV; i++) {
+                        const int t2 = i / DT, t = i % DT;
+                        const h8_t pf = __builtin_bit_cast(h8_t, u4_t{pk[4 * t2], pk[4 * t2 + 1], pk[4 * t2 + 2], pk[4 * t2 + 3]});
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i & 3], pf, o[t], 0, 0, 0);
+                        if (i + 4 < NV) vf[i & 3] = value(x, i + 4);
+                        else if (x + 2 < UNITS) kf[i + 4 - NV] = key(x + 2, i + 4 - NV);
+                        if (x + 1 < UNITS)
+#pragma unroll
+                            for (int e = i * (16 / NV); e < (i + 1) * (16 / NV); e += 2) {
+                                ex[e] = __builtin_fmaf(sc[e], c, -m_run);
+                                ex[e + 1] = __builtin_fmaf(sc[e + 1], c, -m_run);
+                                top = max(max(top, (int)f32_bits(ex[e])), (int)f32_bits(ex[e + 1]));
+                            }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (x + 1 < UNITS) settle(sc, ex, top);
                 }
                 return;
             }
