@@ -21,19 +21,21 @@ constexpr uint32_t kStep = 32;     // keys of a step
 // chunk of 300 among single tokens 23.7 / 25.3 / 25.0, 64 requests of D = 64
 // 21.7 / 19.1 / 19.0.
 constexpr uint32_t kItemCost = 3;
-// Waves: two per SIMD where they get kLongShare of the line each (four requests of
-// 131072 keys: 132 us on one, 118 on two), else up to one per SIMD: fewer items
-// are cut and fewer parts joined (drafted tokens 18.2 us, on two 19.8; one token
-// over 16384 keys 16.8 and 19.5).  Three are slower, 145 us and more: with the next
-// step's tiles in flight the registers hold two.
+// Waves: two per SIMD where each gets kLongShare of the line (four requests of
+// 131072 keys: 132 us on one, 118 on two), else one: fewer items are cut and fewer
+// parts joined (drafted tokens 18.7 us, on two 19.8; one token over 16384 keys 16.7
+// and 19.5).  A count between the two leaves some SIMDs with two and the rest
+// waiting.  Three are slower: with the next step's tiles in flight the registers
+// of most variants hold two.
 constexpr uint32_t kMaxWaves = 2048, kFewWaves = 1024, kLongShare = 16, kMinSteps = 2;
 // Chunks: rows of a row tile, workgroups (one a CU), what an item costs beside its
 // key tiles and the least of the line that is worth a workgroup.
 constexpr uint32_t kChunkTile = 256, kChunkGroups = 256, kChunkCost = 2, kChunkMin = 4;
 // Rows times keys of all heads from which chunks of rows are worth it, and the
 // tiles through LDS that they share: us of rows / chunks at H = 32, Hkv = 8,
-// D = 128: 128 rows a head and 2^25 53 / 65, 2^26 85 / 86, 2^27 143 / 110; eight
-// requests of 256 x 1024 (2^26) 77 / 57.
+// D = 128, one request unless said: 2^25 64 tokens over 16384 keys 49 / 76, 256
+// over 4096 48 / 50, eight of 32 over 4096 57 / 45; 2^26 512 over 4096 72 / 70,
+// eight of 256 over 1024 70 / 57; 2^27 256 over 16384 130 / 102.
 constexpr uint64_t kChunkWork = (uint64_t)1 << 26;
 constexpr float kNone = -3.402823466e38f;  // reference point of a row that has seen no score above -infinity
 
@@ -208,7 +210,7 @@ struct Seq {
 __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint32_t R) {
     Seq s;
     const int T = (int)p.batch.T;
-    const int cap = (int)min((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)0x7fffffff);
+    const int cap = (int)min((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)0x7fffff00);  // + a tile fits
     s.q0 = min(max(p.batch.q_start[b], 0), T);
     s.n = max(min(max(p.batch.q_start[b + 1], 0), T) - s.q0, 0);
     s.len = min(max(p.batch.kv_len[b], 0), cap);
@@ -230,9 +232,10 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // paged_attn_join_kernel joins in order.  The next step's tiles are loaded before
 // the present one is computed, and page numbers 32 steps ahead, a lane each.
 // Bound by the cache's bytes once there are enough of them: four requests of
-// 131072 keys (Q4_0, D = 128, 604 MB) 127 us, 4.8 TB/s; 64 requests of 1 .. 8192
-// keys (Q8_0, 110 MB) 33 us of which 4 are the join; one of 1000 keys 13.6 us, a
-// chain of descriptor, page table, key and join latencies.
+// 131072 keys (Q4_0, D = 128, 604 MB) 118 .. 122 us, 5.0 TB/s; 64 requests of 1 .. 8192
+// keys (Q8_0, 110 MB) 30 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
+// of descriptor, page table, key and join latencies; drafted tokens and short
+// chunks (two row blocks) by turning codes into fp16 on one wave per SIMD.
 template <int FMT, int D, int NR>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         if ((uint32_t)lane >= o) incl += x;
     }
     const uint64_t total = lane_u64(incl, (int)min(p.batch.B, 64u) - 1);
-    const uint64_t nw = min((uint64_t)workers, max(min(total, (uint64_t)kFewWaves), total / kLongShare));
+    const uint64_t nw = min((uint64_t)workers, total >= (uint64_t)kLongShare * kMaxWaves ? kMaxWaves : min(total, (uint64_t)kFewWaves));
     if (threadIdx.x == 0) *note = ItemNote{};
     if (lane == 0) head_of[wave] = 0;
     uint64_t s0 = 0, s1 = 0;
@@ -723,7 +726,11 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
 // share of the line of all row tiles' key tiles, as above.  Key tiles of 16 NW
 // keys: every thread turns 32 bytes of K and of V codes (Q4_0: 16) into fp16 in a
 // double-buffered LDS tile, the codes loaded two tiles ahead; then each wave
-// takes its rows over the tile, 32 x 32 scores at a time.
+// takes its rows over the tile, 32 x 32 scores at a time.  256 rows share the work
+// of turning codes (128 rows: 1306 us where 256 take 1140).  2048 tokens over 30000
+// keys (D = 128, 972 GFLOP) 1080 us with the join, 0.90 PFLOP/s; counters: the
+// matrix pipe 46% busy, 7.5 vector operations per MFMA, at 1.94 GHz: cycles saved
+// since (2.38 M a CU to 2.03 M) came back as a lower clock, so power bounds it.
 template <int FMT, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
