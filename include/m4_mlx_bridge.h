@@ -257,8 +257,8 @@ typedef struct {
     uint32_t num_pages, page_size, Hkv, D;
 } m4_kv_cache_t;
 
-/* B sequences.  The T rows of a call's Q, K, V and O are the sequences' new
- * tokens: rows q_start[b] .. q_start[b + 1] (int32 [B + 1], not decreasing) are
+/* B sequences.  The rows of a call's Q, K, V and O (T of them) are the sequences'
+ * new tokens: rows q_start[b] .. q_start[b + 1] (int32 [B + 1], not decreasing) are
  * the last keys of sequence b, which has kv_len[b] (int32 [B]) keys with them:
  * row i of n has position kv_len[b] - n + i.  Position p is token p % page_size
  * of page page_table[b][p / page_size] (int32 [B][table_stride], table_pages of
@@ -270,7 +270,7 @@ typedef struct {
  * max_new and max_kv are what the caller expects of the longest sequence: they
  * choose kernels and the size of a workspace; the results hold for any. */
 typedef struct {
-    uint32_t B, T;
+    uint32_t B;
     const int32_t *q_start, *kv_len, *page_table;
     uint32_t table_pages, table_stride;
     uint32_t max_new, max_kv;
@@ -323,15 +323,16 @@ M4_API int m4_bridge_rope_axes(const m4_rope_axes_t* rope, const int32_t* positi
  * The results are those of m4_bridge_rope_axes followed by a write.  Rows of Q
  * whose token has no place in the cache are left.  rope NULL: Q must be NULL.
  * Codes as m4_bridge_rope_axes, and -3 (format). */
-M4_API int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
-                                     const m4_rows_t* V, const m4_rope_axes_t* rope, const int32_t* positions,
-                                     uint32_t position_stride, const m4_rows_t* Q, const m4_rows_t* Q_out, uint32_t H);
+M4_API int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                     const m4_rows_t* K, const m4_rows_t* V, const m4_rope_axes_t* rope,
+                                     const int32_t* positions, uint32_t position_stride, const m4_rows_t* Q,
+                                     const m4_rows_t* Q_out, uint32_t H);
 
 /* The inverse: the values of the batch's rows into K and V [T][Hkv][D] fp16
  * (with q_start the running sum of kv_len, whole sequences).  Rows that have no
  * place in the cache are left. */
-M4_API int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
-                                   const m4_rows_t* V);
+M4_API int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                   const m4_rows_t* K, const m4_rows_t* V);
 
 /* Causal attention of the batch's rows Q [T][H][D] over the cached keys of their
  * sequences (their own included: append first), O [T][H][D]: query head h reads
@@ -341,11 +342,11 @@ M4_API int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch
  * decoded token to a prompt.  `ws`: m4_bridge_paged_attn_workspace bytes of
  * device memory, 16-byte aligned, whose contents do not matter; calls that may
  * run at the same time need one each.  scale finite.  Codes as above. */
-M4_API size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t H,
-                                             uint32_t window);
-M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
-                                         const m4_rows_t* O, uint32_t H, float scale, uint32_t window, void* ws,
-                                         size_t ws_bytes);
+M4_API size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                             uint32_t H, uint32_t window);
+M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                         const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
+                                         uint32_t window, void* ws, size_t ws_bytes);
 
 /* A transformer block over the cache: m4_bridge_prefill_layer_ex with the
  * batch's rows as its prompt and the paged cache in place of one call's keys --
@@ -359,24 +360,25 @@ M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv
  * m4_bridge_prefill_layer_ex. */
 M4_API int m4_bridge_paged_layer(void* X_ptr, void* w_attn, void* Wq, void* Wk, void* Wv, void* Wo, void* w_ffn,
                                  void* Wg, void* Wu, void* Wd, void* X_out, const m4_kv_cache_t* cache,
-                                 const m4_kv_batch_t* batch, const m4_rope_axes_t* rope, const int32_t* positions,
-                                 uint32_t position_stride, int format, uint32_t d_model, uint32_t Hq, uint32_t N_mlp,
-                                 float attn_scale, uint32_t window, int norm_type, float norm_eps);
+                                 const m4_kv_batch_t* batch, uint32_t T, const m4_rope_axes_t* rope,
+                                 const int32_t* positions, uint32_t position_stride, int format, uint32_t d_model,
+                                 uint32_t Hq, uint32_t N_mlp, float attn_scale, uint32_t window, int norm_type,
+                                 float norm_eps);
 
 /* Validation only, as m4_bridge_validate_gemm: the code that the call would
  * return on an initialized bridge (0 if it would launch) but for the check that
  * the pointers are device memory. */
 M4_API int m4_bridge_validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
                                         const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D);
-M4_API int m4_bridge_validate_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch,
+M4_API int m4_bridge_validate_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
                                               const m4_rows_t* K, const m4_rows_t* V, const m4_rope_axes_t* rope,
                                               const int32_t* positions, uint32_t position_stride, const m4_rows_t* Q,
                                               const m4_rows_t* Q_out, uint32_t H);
-M4_API int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
-                                            const m4_rows_t* V);
-M4_API int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
-                                         const m4_rows_t* O, uint32_t H, float scale, uint32_t window, const void* ws,
-                                         size_t ws_bytes);
+M4_API int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                            const m4_rows_t* K, const m4_rows_t* V);
+M4_API int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                         const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
+                                         uint32_t window, const void* ws, size_t ws_bytes);
 
 /* Run subsequent work on `stream` (a hipStream_t, e.g. torch's current
  * stream); NULL restores the bridge's own stream.  Returns 0 or -1. */

@@ -412,8 +412,8 @@ qr::RowsView rows_view(const m4_rows_t* r) {
     return {static_cast<_Float16*>(r->ptr), r->token_stride, r->head_stride};
 }
 
-qr::BatchView batch_view(const m4_kv_batch_t* b) {
-    return {b->B, b->T, b->q_start, b->kv_len, b->page_table, b->table_pages, b->table_stride};
+qr::BatchView batch_view(const m4_kv_batch_t* b, uint32_t T) {
+    return {b->B, T, b->q_start, b->kv_len, b->page_table, b->table_pages, b->table_stride};
 }
 
 qr::PageGeom cache_geom(const m4_kv_cache_t* c) {
@@ -424,7 +424,7 @@ qr::RopeView rope_view(const m4_rope_axes_t* r, const int32_t* positions, uint32
     return {static_cast<const uint64_t*>(r->table), r->pairs, r->axes, r->traditional ? 1 : 0, positions, stride};
 }
 
-qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, uint32_t H, uint32_t window) {
+qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, uint32_t T, uint32_t H, uint32_t window) {
     qr::PagedAttnParams p{};
     p.H = H;
     p.G = H / c->Hkv;
@@ -432,7 +432,7 @@ qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, 
     p.format = c->format;
     p.window = window;
     p.geom = cache_geom(c);
-    p.batch = batch_view(b);
+    p.batch = batch_view(b, T);
     p.max_new = b->max_new;
     p.max_kv = b->max_kv;
     return p;
@@ -925,20 +925,20 @@ int m4_bridge_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, ui
     return launched(qr::launch_kv_append(p, g_stream), "rope_axes");
 }
 
-int m4_bridge_validate_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+int m4_bridge_validate_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K,
                                        const m4_rows_t* V, const m4_rope_axes_t* rope, const int32_t* positions,
                                        uint32_t position_stride, const m4_rows_t* Q, const m4_rows_t* Q_out,
                                        uint32_t H) {
     bool empty;
-    return qr::validate_append(cache, batch, K, V, rope, positions, position_stride, Q, Q_out, H, &empty);
+    return qr::validate_append(cache, batch, T, K, V, rope, positions, position_stride, Q, Q_out, H, &empty);
 }
 
-int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K,
                               const m4_rows_t* V, const m4_rope_axes_t* rope, const int32_t* positions,
                               uint32_t position_stride, const m4_rows_t* Q, const m4_rows_t* Q_out, uint32_t H) {
     if (!g_initialized) return -1;
     bool empty;
-    const int rc = qr::validate_append(cache, batch, K, V, rope, positions, position_stride, Q, Q_out, H, &empty);
+    const int rc = qr::validate_append(cache, batch, T, K, V, rope, positions, position_stride, Q, Q_out, H, &empty);
     if (rc || empty) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
@@ -954,57 +954,57 @@ int m4_bridge_kv_cache_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* b
         p.Qo = rows_view(Q_out);
         p.H = H;
     }
-    p.T = batch->T;
+    p.T = T;
     p.D = cache->D;
     p.format = cache->format;
     p.geom = cache_geom(cache);
-    p.batch = batch_view(batch);
+    p.batch = batch_view(batch, T);
     if (rope) p.rope = rope_view(rope, positions, position_stride);
     return launched(qr::launch_kv_append(p, g_stream), "kv_cache_append");
 }
 
-int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K,
                                      const m4_rows_t* V) {
     bool empty;
-    return qr::validate_read(cache, batch, K, V, &empty);
+    return qr::validate_read(cache, batch, T, K, V, &empty);
 }
 
-int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K,
+int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K,
                             const m4_rows_t* V) {
     if (!g_initialized) return -1;
     bool empty;
-    const int rc = qr::validate_read(cache, batch, K, V, &empty);
+    const int rc = qr::validate_read(cache, batch, T, K, V, &empty);
     if (rc || empty) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
     if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, K->ptr, V->ptr)) return -2;
-    const qr::ReadParams p{rows_view(K), rows_view(V), cache->D, cache->format, cache_geom(cache), batch_view(batch)};
+    const qr::ReadParams p{rows_view(K), rows_view(V), cache->D, cache->format, cache_geom(cache), batch_view(batch, T)};
     return launched(qr::launch_kv_read(p, g_stream), "kv_cache_read");
 }
 
-size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t H,
+size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, uint32_t H,
                                       uint32_t window) {
     if (!cache || !batch || H == 0 || cache->Hkv == 0 || H % cache->Hkv || (cache->D != 64 && cache->D != 128)) return 0;
-    return qr::paged_attn_workspace(attn_params(cache, batch, H, window));
+    return qr::paged_attn_workspace(attn_params(cache, batch, T, H, window));
 }
 
-int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
+int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
                                   const m4_rows_t* O, uint32_t H, float scale, uint32_t window, const void* ws,
                                   size_t ws_bytes) {
     bool empty;
-    const int rc = qr::validate_attn(cache, batch, Q, O, H, scale, ws, &empty);
+    const int rc = qr::validate_attn(cache, batch, T, Q, O, H, scale, ws, &empty);
     if (rc || empty) return rc;
-    return ws_bytes < m4_bridge_paged_attn_workspace(cache, batch, H, window) ? -2 : 0;
+    return ws_bytes < m4_bridge_paged_attn_workspace(cache, batch, T, H, window) ? -2 : 0;
 }
 
-int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q,
+int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
                                   const m4_rows_t* O, uint32_t H, float scale, uint32_t window, void* ws,
                                   size_t ws_bytes) {
     if (!g_initialized) return -1;
     bool empty;
-    const int rc = qr::validate_attn(cache, batch, Q, O, H, scale, ws, &empty);
+    const int rc = qr::validate_attn(cache, batch, T, Q, O, H, scale, ws, &empty);
     if (rc || empty) return rc;
-    qr::PagedAttnParams p = attn_params(cache, batch, H, window);
+    qr::PagedAttnParams p = attn_params(cache, batch, T, H, window);
     if (ws_bytes < qr::paged_attn_workspace(p)) return -2;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
@@ -1017,13 +1017,13 @@ int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_
 }
 
 int m4_bridge_paged_layer(void* X, void* w_attn, void* Wq, void* Wk, void* Wv, void* Wo, void* w_ffn, void* Wg,
-                          void* Wu, void* Wd, void* Xout, const m4_kv_cache_t* cache, const m4_kv_batch_t* batch,
+                          void* Wu, void* Wd, void* Xout, const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
                           const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride, int format,
                           uint32_t dm, uint32_t Hq, uint32_t Nm, float scale, uint32_t window, int norm_type,
                           float eps) {
     if (!g_initialized) return -1;
     bool empty;
-    int rc = qr::validate_layer(cache, batch, rope, positions, position_stride, format, dm, Hq, Nm, scale,
+    int rc = qr::validate_layer(cache, batch, T, rope, positions, position_stride, format, dm, Hq, Nm, scale,
                                 w_attn || w_ffn, norm_type, &empty);
     if (rc || empty) return rc;
     void* ptrs[9] = {X, Wq, Wk, Wv, Wo, Wg, Wu, Wd, Xout};
@@ -1040,9 +1040,9 @@ int m4_bridge_paged_layer(void* X, void* w_attn, void* Wq, void* Wk, void* Wv, v
         if (q && !dev.owns_all(q)) return -2;
     if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table)) return -2;
     if (rope && (!dev.owns_all(rope->table) || (positions && !dev.owns_all(positions)))) return -2;
-    const uint32_t M = batch->T, Hkv = cache->Hkv, D = cache->D;
+    const uint32_t M = T, Hkv = cache->Hkv, D = cache->D;
     const size_t nq = (size_t)M * Hq * D, nk = (size_t)M * Hkv * D;
-    qr::PagedAttnParams ap = attn_params(cache, batch, Hq, window);
+    qr::PagedAttnParams ap = attn_params(cache, batch, T, Hq, window);
     const size_t part = qr::paged_attn_workspace(ap);
     auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const bool norms = w_attn || w_ffn;

@@ -122,10 +122,10 @@ int check_cache(const m4_kv_cache_t* c) {
 }
 
 // B = 0 or T = 0: no rows, and no pointers needed.
-int check_batch(const m4_kv_batch_t* b, bool* empty) {
+int check_batch(const m4_kv_batch_t* b, uint32_t T, bool* empty) {
     if (!b) return -2;
-    if (b->B > 0x7fffffffu || b->T > 0x7fffffffu) return -4;
-    *empty = b->B == 0 || b->T == 0;
+    if (b->B > 0x7fffffffu || T > 0x7fffffffu) return -4;
+    *empty = b->B == 0 || T == 0;
     if (*empty) return 0;
     if (!b->q_start || !b->kv_len || !b->page_table) return -2;
     if (misaligned(b->q_start, 4) || misaligned(b->kv_len, 4) || misaligned(b->page_table, 4)) return -2;
@@ -199,12 +199,12 @@ int validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uin
     return check_rows(Y, T, H, D, true);
 }
 
-int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K, const m4_rows_t* V,
                     const m4_rope_axes_t* rope, const int32_t* positions, uint32_t stride, const m4_rows_t* Q,
                     const m4_rows_t* Q_out, uint32_t H, bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, empty)) return rc;
+    if (int rc = check_batch(batch, T, empty)) return rc;
     if (Q && (!rope || !Q_out)) return -2;
     if (Q && (H == 0 || H > 0xffffu)) return -4;
     if (rope) {
@@ -213,48 +213,48 @@ int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, cons
     }
     if (*empty) return 0;
     if (rope && positions)
-        if (int rc = check_positions(positions, stride, rope->axes, batch->T)) return rc;
-    if (int rc = check_rows(K, batch->T, cache->Hkv, cache->D, false)) return rc;
-    if (int rc = check_rows(V, batch->T, cache->Hkv, cache->D, false)) return rc;
+        if (int rc = check_positions(positions, stride, rope->axes, T)) return rc;
+    if (int rc = check_rows(K, T, cache->Hkv, cache->D, false)) return rc;
+    if (int rc = check_rows(V, T, cache->Hkv, cache->D, false)) return rc;
     if (Q) {
-        if (int rc = check_rows(Q, batch->T, H, cache->D, false)) return rc;
-        if (int rc = check_rows(Q_out, batch->T, H, cache->D, true)) return rc;
+        if (int rc = check_rows(Q, T, H, cache->D, false)) return rc;
+        if (int rc = check_rows(Q_out, T, H, cache->D, true)) return rc;
     }
     return 0;
 }
 
-int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K, const m4_rows_t* V,
                   bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, empty)) return rc;
+    if (int rc = check_batch(batch, T, empty)) return rc;
     if (*empty) return 0;
-    if (int rc = check_rows(K, batch->T, cache->Hkv, cache->D, true)) return rc;
-    return check_rows(V, batch->T, cache->Hkv, cache->D, true);
+    if (int rc = check_rows(K, T, cache->Hkv, cache->D, true)) return rc;
+    return check_rows(V, T, cache->Hkv, cache->D, true);
 }
 
-int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q, const m4_rows_t* O,
+int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* O,
                   uint32_t H, float scale, const void* ws, bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, empty)) return rc;
+    if (int rc = check_batch(batch, T, empty)) return rc;
     if (H == 0 || H > 0xffffu || H % cache->Hkv || !std::isfinite(scale)) return -4;
     if (*empty) return 0;
-    if ((uint64_t)batch->T * (H / cache->Hkv) > 0x7fffffffu) return -4;  // rows of a KV head are counted in 32 bits
-    if (int rc = check_rows(Q, batch->T, H, cache->D, false)) return rc;
-    if (int rc = check_rows(O, batch->T, H, cache->D, true)) return rc;
+    if ((uint64_t)T * (H / cache->Hkv) > 0x7fffffffu) return -4;  // rows of a KV head are counted in 32 bits
+    if (int rc = check_rows(Q, T, H, cache->D, false)) return rc;
+    if (int rc = check_rows(O, T, H, cache->D, true)) return rc;
     if (!ws || misaligned(ws, 16)) return -2;
     return 0;
 }
 
-int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rope_axes_t* rope,
+int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rope_axes_t* rope,
                    const int32_t* positions, uint32_t stride, int format, uint32_t dm, uint32_t Hq, uint32_t Nm,
                    float scale, bool norms, int norm_type, bool* empty) {
     *empty = false;
     if (!cache || !batch) return -2;
     if (!has_kernels(format) || (norms && norm_type != 1 && norm_type != 2)) return -3;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, empty)) return rc;
+    if (int rc = check_batch(batch, T, empty)) return rc;
     if (dm == 0 || Nm == 0 || Hq == 0 || Hq > 0xffffu || Hq % cache->Hkv || !std::isfinite(scale)) return -4;
     const uint64_t HQ = (uint64_t)Hq * cache->D;
     const uint32_t bs = get_quant_info(static_cast<QuantFormat>(format)).block_size;
@@ -265,8 +265,8 @@ int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const
     }
     if (*empty) return 0;
     if (rope && positions)
-        if (int rc = check_positions(positions, stride, rope->axes, batch->T)) return rc;
-    if ((uint64_t)batch->T * (Hq / cache->Hkv) > 0x7fffffffu) return -4;
+        if (int rc = check_positions(positions, stride, rope->axes, T)) return rc;
+    if ((uint64_t)T * (Hq / cache->Hkv) > 0x7fffffffu) return -4;
     return 0;
 }
 

@@ -29,15 +29,15 @@ int rope_axes_table(const double* inv_freq, const uint8_t* pair_axis, uint32_t p
 size_t kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D);
 int validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
                        const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D, bool* empty);
-int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K, const m4_rows_t* V,
                     const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
                     const m4_rows_t* Q, const m4_rows_t* Q_out, uint32_t H, bool* empty);
-int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* K, const m4_rows_t* V,
+int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* K, const m4_rows_t* V,
                   bool* empty);
-int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rows_t* Q, const m4_rows_t* O,
+int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* O,
                   uint32_t H, float scale, const void* ws, bool* empty);
 // all of a layer's arguments but its tensors
-int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const m4_rope_axes_t* rope,
+int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rope_axes_t* rope,
                    const int32_t* positions, uint32_t position_stride, int format, uint32_t d_model, uint32_t Hq,
                    uint32_t N_mlp, float scale, bool norms, int norm_type, bool* empty);
 

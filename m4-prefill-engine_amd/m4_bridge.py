@@ -89,15 +89,15 @@ SIGNATURES = {
     "m4_bridge_kv_cache_bytes": ([_I, _U32, _U32, _U32, _U32], _SZ),
     "m4_bridge_rope_axes_table": ([_VP, _VP, _U32, _U32, _VP], _I),
     "m4_bridge_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
-    "m4_bridge_kv_cache_append": ([_VP, _VP, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
-    "m4_bridge_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
-    "m4_bridge_paged_attn_workspace": ([_VP, _VP, _U32, _U32], _SZ),
-    "m4_bridge_dispatch_paged_attn": ([_VP, _VP, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
-    "m4_bridge_paged_layer": ([_VP] * 15 + [_U32, _I, _U32, _U32, _U32, _F, _U32, _I, _F], _I),
+    "m4_bridge_kv_cache_append": ([_VP, _VP, _U32, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
+    "m4_bridge_kv_cache_read": ([_VP, _VP, _U32, _VP, _VP], _I),
+    "m4_bridge_paged_attn_workspace": ([_VP, _VP, _U32, _U32, _U32], _SZ),
+    "m4_bridge_dispatch_paged_attn": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_paged_layer": ([_VP] * 13 + [_U32, _VP, _VP, _U32, _I, _U32, _U32, _U32, _F, _U32, _I, _F], _I),
     "m4_bridge_validate_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
-    "m4_bridge_validate_kv_cache_append": ([_VP, _VP, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
-    "m4_bridge_validate_kv_cache_read": ([_VP, _VP, _VP, _VP], _I),
-    "m4_bridge_validate_paged_attn": ([_VP, _VP, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_validate_kv_cache_append": ([_VP, _VP, _U32, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
+    "m4_bridge_validate_kv_cache_read": ([_VP, _VP, _U32, _VP, _VP], _I),
+    "m4_bridge_validate_paged_attn": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
     "m4_bridge_set_stream": ([_VP], _I),
     "m4_bridge_get_stream": ([], _VP),
     "m4_bridge_last_error": ([], ctypes.c_char_p),
@@ -164,7 +164,7 @@ class KVCacheStruct(ctypes.Structure):
 
 class KVBatchStruct(ctypes.Structure):
     """m4_kv_batch_t (include/m4_mlx_bridge.h)."""
-    _fields_ = [("B", _U32), ("T", _U32), ("q_start", _VP), ("kv_len", _VP), ("page_table", _VP),
+    _fields_ = [("B", _U32), ("q_start", _VP), ("kv_len", _VP), ("page_table", _VP),
                 ("table_pages", _U32), ("table_stride", _U32), ("max_new", _U32), ("max_kv", _U32)]
 
 
@@ -248,7 +248,7 @@ class KVBatch:
         if max_kv is None:
             max_kv = int(kv_len.max().item()) if B else 0
         self.B = B
-        self.struct = KVBatchStruct(B, 0, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+        self.struct = KVBatchStruct(B, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
                                     page_table.shape[1], page_table.stride(0), max(int(max_new), 0), max(int(max_kv), 0))
         self.ref = ctypes.addressof(self.struct)
 
@@ -716,11 +716,10 @@ class HIPBridge:
             if Tq != T or To != T:
                 raise ValueError(f"K has {T} rows, Q {Tq} and Q_out {To}")
         self._on_stream_of(K)
-        batch.struct.T = T
         rows = _ROWS4(*k, *v, *q, *qo)
         at = ctypes.addressof(rows)
         at_q, at_qo = (at + 2 * _ROWS, at + 3 * _ROWS) if Q is not None else (None, None)
-        ret = self._lib.m4_bridge_kv_cache_append(cache.ref, batch.ref, at, at + _ROWS,
+        ret = self._lib.m4_bridge_kv_cache_append(cache.ref, batch.ref, T, at, at + _ROWS,
                                                   rope.on(K.device) if rope is not None else None, pos, stride, at_q,
                                                   at_qo, H)
         self._check("m4_bridge_kv_cache_append", ret)
@@ -734,18 +733,16 @@ class HIPBridge:
         if Tv != T:
             raise ValueError(f"K has {T} rows, V {Tv}")
         self._on_stream_of(K)
-        batch.struct.T = T
         rows = _ROWS2(*k, *v)
         at = ctypes.addressof(rows)
-        ret = self._lib.m4_bridge_kv_cache_read(cache.ref, batch.ref, at, at + _ROWS)
+        ret = self._lib.m4_bridge_kv_cache_read(cache.ref, batch.ref, T, at, at + _ROWS)
         self._check("m4_bridge_kv_cache_read", ret)
         self._in_flight_tensors.append((cache, batch, K, V))
         return ret
 
     def paged_attn_workspace(self, cache: PagedKVCache, batch: KVBatch, H: int, T: int, window: int = 0) -> int:
         """Bytes of workspace that dispatch_paged_attn needs for T rows of H heads."""
-        batch.struct.T = T
-        return int(self._lib.m4_bridge_paged_attn_workspace(cache.ref, batch.ref, H, window))
+        return int(self._lib.m4_bridge_paged_attn_workspace(cache.ref, batch.ref, T, H, window))
 
     def dispatch_paged_attn(self, cache: PagedKVCache, batch: KVBatch, Q, O, scale: float, token_major: bool = False,
                             o_token_major: bool = False, window: int = 0, workspace=None) -> int:
@@ -763,10 +760,9 @@ class HIPBridge:
         if workspace is None:
             workspace = _torch.empty(self.paged_attn_workspace(cache, batch, H, T, window), dtype=_torch.uint8,
                                      device=Q.device)
-        batch.struct.T = T
         rows = _ROWS2(*q, *o)
         at = ctypes.addressof(rows)
-        ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, at, at + _ROWS, H, float(scale), window,
+        ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, T, at, at + _ROWS, H, float(scale), window,
                                                       workspace.data_ptr(), workspace.nbytes)
         self._check("m4_bridge_dispatch_paged_attn", ret)
         self._in_flight_tensors.append((cache, batch, Q, O))
@@ -785,10 +781,10 @@ class HIPBridge:
         ptrs = [None if t is None else self.extract_buffer_address_and_size(t)[0] for t in bufs]
         pos, stride = self._positions(positions, rope, T) if rope is not None else (None, 0)
         self._on_stream_of(X)
-        batch.struct.T = T
-        ret = self._lib.m4_bridge_paged_layer(*ptrs, cache.ref, batch.ref, rope.on(X.device) if rope is not None else None,
-                                              pos, stride, int(format), d_model, Hq, N_mlp, float(attn_scale), window,
-                                              int(norm_type), float(norm_eps))
+        ret = self._lib.m4_bridge_paged_layer(*ptrs, cache.ref, batch.ref, T,
+                                              rope.on(X.device) if rope is not None else None, pos, stride, int(format),
+                                              d_model, Hq, N_mlp, float(attn_scale), window, int(norm_type),
+                                              float(norm_eps))
         self._check("m4_bridge_paged_layer", ret)
         self._in_flight_tensors.append((*bufs, cache, batch, positions))
         return ret

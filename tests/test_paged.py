@@ -248,7 +248,8 @@ def test_fused_rope_append_is_rope_then_append(bridge, fmt, D, dims, axes, tradi
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_bad_metadata_is_not_followed(bridge, fmt):
+@pytest.mark.parametrize("max_new,max_kv", [(20, 60), (4096, 10 ** 8)], ids=["rows", "chunks"])
+def test_bad_metadata_is_not_followed(bridge, fmt, max_new, max_kv):
     """Pages that are not there, more keys than the table holds, starts past the rows: such tokens are not written, not
     read and not seen, and nothing outside the buffers is touched."""
     import torch
@@ -258,7 +259,7 @@ def test_bad_metadata_is_not_followed(bridge, fmt):
     table = s.table.copy()
     table[0, 1] = 10 ** 9      # keys 16 .. 31 of sequence 0
     table[1, 2] = -1           # keys 32 .. 39 of sequence 1: its new tokens
-    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array([60, 40], np.int32)), dev(table), 20, 60)
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array([60, 40], np.int32)), dev(table), max_new, max_kv)
     cache = s.cache()
     q = half(s.rng, H, s.T, D)
     O = torch.full((H, s.T, D), 5.0, dtype=torch.float16, device="cuda")
@@ -282,7 +283,7 @@ def test_bad_metadata_is_not_followed(bridge, fmt):
     np.testing.assert_array_equal(cache.pages.cpu().numpy(), s.pages.raw)
     # lengths past the table and starts past the rows: no fault, rows in range still written
     wild = m4_bridge.KVBatch(dev(np.array([0, 10 ** 6, 5], np.int32)), dev(np.array([2 ** 31 - 1, -5], np.int32)),
-                             dev(s.table), 20, 60)
+                             dev(s.table), max_new, max_kv)
     bridge.dispatch_paged_attn(cache, wild, dev(q), O, 0.125)
     bridge.kv_cache_append(cache, wild, dev(k), dev(k), token_major=True)
     bridge.synchronize()
@@ -334,8 +335,11 @@ def check_attention(bridge, s, H, window=0, scale=None, token_major=False, infin
     ([300], [200], 160, 1, 64, 16, 0),                        # a group wider than a row tile
     ([5000], [70], 8, 8, 128, 64, 0),
 ])
-def test_paged_attention(bridge, fmt, lens, new, H, Hkv, D, P, window):
-    check_attention(bridge, Setup(fmt, lens, new, Hkv, D, P, seed=sum(lens) + H), H, window)
+@pytest.mark.parametrize("kernels", ["as_planned", "rows", "chunks"])
+def test_paged_attention(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
+    # what is expected of the lengths chooses the kernels: every case runs on both
+    kw = {"as_planned": {}, "rows": {"max_new": 1, "max_kv": 1}, "chunks": {"max_new": 4096, "max_kv": 10 ** 8}}[kernels]
+    check_attention(bridge, Setup(fmt, lens, new, Hkv, D, P, seed=sum(lens) + H), H, window, **kw)
 
 
 @gpu
@@ -354,8 +358,9 @@ def test_paged_attention_scales(bridge, scale):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("new", [[60, 3], [2, 3], [15, 3]])  # by chunks, and by rows of 16 and 32
-def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(bridge, fmt, D, new):
+@pytest.mark.parametrize("new,kw", [([60, 3], {"max_new": 4096, "max_kv": 10 ** 8}), ([2, 3], {}), ([15, 3], {})],
+                         ids=["chunks", "rows_of_16", "rows_of_32"])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(bridge, fmt, D, new, kw):
     """A key whose V scale is infinite reaches the rows that see it, in its 32 dims, and no other; what was never written
     (all-ones bytes: NaN scales) reaches none.  Its values are its codes times infinity, so a row's result there is an
     infinity or NaN: `infinite` takes the two alike."""
@@ -365,7 +370,7 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(bridge, fmt
         avs = s.pages._places(p % 16)[3]
         raw[1, avs[1]], raw[1, avs[1] + 1] = 0x00, 0x7C  # +inf, dims 32 .. 63 of head 1
         s.v[b][1, p, 32:64] = np.nan
-    check_attention(bridge, s, 4, infinite=True)
+    check_attention(bridge, s, 4, infinite=True, **kw)
 
 
 @gpu
@@ -450,8 +455,8 @@ def test_chunks_and_steps_of_a_growing_batch(bridge, fmt):
 
 
 @gpu
-@pytest.mark.parametrize("fmt", FORMATS)
-def test_captured_decoding_steps(bridge, fmt):
+@pytest.mark.parametrize("fmt,own_workspace", [(Q8_0, True), (Q4_0, False)])
+def test_captured_decoding_steps(bridge, fmt, own_workspace):
     """A step captured once and replayed as the sequences grow, with the program's own work and waits in between,
     equals the eager calls bit for bit; two graphs with a workspace each replay side by side on their streams."""
     import torch
@@ -470,7 +475,7 @@ def test_captured_decoding_steps(bridge, fmt):
         batch = m4_bridge.KVBatch(torch.arange(B + 1, dtype=torch.int32, device="cuda"), kv_len, dev(table), 1, 704)
         q, k, v = (torch.zeros_like(t) for t in xs[0])
         o = torch.zeros(B, H, D, dtype=torch.float16, device="cuda")
-        ws = torch.empty(bridge.paged_attn_workspace(cache, batch, H, B), dtype=torch.uint8, device="cuda")
+        ws = torch.empty(bridge.paged_attn_workspace(cache, batch, H, B), dtype=torch.uint8, device="cuda") if own_workspace else None
 
         def step():
             bridge.kv_cache_append(cache, batch, k, v, rope=rope, Q=q)
@@ -636,7 +641,7 @@ class Args:
     def __init__(self):
         self.T, self.H = 10, 8
         self.cache = m4_bridge.KVCacheStruct(0x100000, 4 * 16 * 2 * 2 * 4 * 34, 6, 4, 16, 2, 128)
-        self.batch = m4_bridge.KVBatchStruct(2, self.T, 0x1000, 0x2000, 0x3000, 4, 4, 5, 60)
+        self.batch = m4_bridge.KVBatchStruct(2, 0x1000, 0x2000, 0x3000, 4, 4, 5, 60)
         self.kv = m4_bridge.RowsStruct(0x200000, 2 * self.T * 128 * 2, 128, self.T * 128)
         self.q = m4_bridge.RowsStruct(0x300000, 8 * self.T * 128 * 2, 128, self.T * 128)
         self.rope = m4_bridge.RopeAxesStruct(64, 3, 0, 0x500000, 64 * 12)
@@ -644,10 +649,10 @@ class Args:
 
     def codes(self, lib):
         r = lambda x: None if x is None else ctypes.addressof(x)  # noqa: E731
-        return (lib.m4_bridge_validate_kv_cache_append(r(self.cache), r(self.batch), r(self.kv), r(self.kv), r(self.rope),
+        return (lib.m4_bridge_validate_kv_cache_append(r(self.cache), r(self.batch), self.T, r(self.kv), r(self.kv), r(self.rope),
                                                        self.positions, self.stride, r(self.q), r(self.q), self.H),
-                lib.m4_bridge_validate_kv_cache_read(r(self.cache), r(self.batch), r(self.kv), r(self.kv)),
-                lib.m4_bridge_validate_paged_attn(r(self.cache), r(self.batch), r(self.q), r(self.q), self.H, self.scale, 0,
+                lib.m4_bridge_validate_kv_cache_read(r(self.cache), r(self.batch), self.T, r(self.kv), r(self.kv)),
+                lib.m4_bridge_validate_paged_attn(r(self.cache), r(self.batch), self.T, r(self.q), r(self.q), self.H, self.scale, 0,
                                                   self.ws, self.ws_bytes),
                 lib.m4_bridge_validate_rope_axes(r(self.rope), self.positions, self.stride, r(self.q), r(self.q), self.T,
                                                  self.H, 128))
@@ -678,7 +683,8 @@ def _set(path, value):
     (_set("batch.kv_len", 0x2002), (-2, -2, -2, 0)),
     (_set("batch.table_pages", 0), (-4, -4, -4, 0)),
     (_set("batch.table_stride", 3), (-4, -4, -4, 0)),
-    (_set("batch.T", 0), (0, 0, 0, 0)),
+    (_set("T", 0), (0, 0, 0, 0)),
+    (_set("T", 1 << 31), (-4, -4, -4, -4)),
     (_set("batch.B", 0), (0, 0, 0, 0)),
     (_set("kv", None), (-2, -2, 0, 0)),
     (_set("kv.ptr", 0x200002), (-2, -2, 0, 0)),
@@ -752,11 +758,11 @@ def test_uninitialized_bridge_refuses(lib):
         pytest.skip("a GPU is present")
     a, r = Args(), ctypes.addressof
     assert lib.m4_bridge_rope_axes(r(a.rope), 0x4000, 10, r(a.q), r(a.q), 10, 8, 128) == -1
-    assert lib.m4_bridge_kv_cache_append(r(a.cache), r(a.batch), r(a.kv), r(a.kv), None, None, 0, None, None, 0) == -1
-    assert lib.m4_bridge_kv_cache_read(r(a.cache), r(a.batch), r(a.kv), r(a.kv)) == -1
-    assert lib.m4_bridge_paged_layer(*[0x600000] * 11, r(a.cache), r(a.batch), None, None, 0, 0, 256, 8, 512, 0.1, 0, 1,
+    assert lib.m4_bridge_kv_cache_append(r(a.cache), r(a.batch), 10, r(a.kv), r(a.kv), None, None, 0, None, None, 0) == -1
+    assert lib.m4_bridge_kv_cache_read(r(a.cache), r(a.batch), 10, r(a.kv), r(a.kv)) == -1
+    assert lib.m4_bridge_paged_layer(*[0x600000] * 11, r(a.cache), r(a.batch), 10, None, None, 0, 0, 256, 8, 512, 0.1, 0, 1,
                                      1e-5) == -1
-    assert lib.m4_bridge_dispatch_paged_attn(r(a.cache), r(a.batch), r(a.q), r(a.q), 8, 0.1, 0, 0x400000, 1 << 30) == -1
+    assert lib.m4_bridge_dispatch_paged_attn(r(a.cache), r(a.batch), 10, r(a.q), r(a.q), 8, 0.1, 0, 0x400000, 1 << 30) == -1
 
 
 def test_python_refusals(libpath):
@@ -807,7 +813,8 @@ def test_paged_layer_refusals(bridge, change, code):
     x = None if v["ptr"] is None else buf.data_ptr() + v["ptr"]
     r = ctypes.addressof
     # a well-formed call is not made here: B = 0 is the only one that passes
-    assert lib.m4_bridge_paged_layer(x, *[buf.data_ptr() + 512] * 9, buf.data_ptr() + 1024, r(a.cache), r(a.batch), None, None, 0, v["fmt"],
+    assert lib.m4_bridge_paged_layer(x, *[buf.data_ptr() + 512] * 9, buf.data_ptr() + 1024, r(a.cache), r(a.batch), 10,
+                                     None, None, 0, v["fmt"],
                                      v["dm"], v["Hq"], v["Nm"], 0.1, 0, v["norm_type"], 1e-5) == code
     bridge.synchronize()
 
