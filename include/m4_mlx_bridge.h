@@ -239,7 +239,8 @@ M4_API int m4_bridge_projection_plan(int format, uint32_t M, uint32_t K, const u
  *      sequences of any lengths.  No counterpart in the reference, whose cache
  *      is one prompt's ([Hkv, M, D] Q8_0 blocks).  All buffers are device
  *      memory of the stream's device; nothing is staged, allocated or waited
- *      for, so every call can be captured into a graph. ------------------- */
+ *      for, so every call can be captured into a graph.  A call's outputs do
+ *      not overlap its other buffers, but where one may be the other. ------ */
 
 /* A cache of num_pages pages of page_size tokens (16, 32, 64, 128 or 256),
  * Hkv heads, D = 64 or 128, in format QUANT_Q8_0 (6) or QUANT_Q4_0 (0), one
@@ -268,7 +269,8 @@ typedef struct {
  * written and not seen.  Rows behind the last sequence are left as they are.
  * Two tokens of a call that fall on one place of the cache leave it undefined.
  * max_new and max_kv are what the caller expects of the longest sequence: they
- * choose kernels and the size of a workspace; the results hold for any. */
+ * choose kernels and the size of a workspace; the results hold for any.  T at
+ * most 2^26, a table row's pages at most 0x7fff0000 tokens (else -4). */
 typedef struct {
     uint32_t B;
     const int32_t *q_start, *kv_len, *page_table;

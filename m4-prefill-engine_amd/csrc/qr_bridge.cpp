@@ -984,7 +984,9 @@ int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* bat
 
 size_t m4_bridge_paged_attn_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, uint32_t H,
                                       uint32_t window) {
-    if (!cache || !batch || H == 0 || cache->Hkv == 0 || H % cache->Hkv || (cache->D != 64 && cache->D != 128)) return 0;
+    if (!cache || !batch || H == 0 || H > 0xffffu) return 0;
+    if (!qr::kv_cache_bytes(cache->format, cache->num_pages, cache->page_size, cache->Hkv, cache->D) || H % cache->Hkv)
+        return 0;
     return qr::paged_attn_workspace(attn_params(cache, batch, T, H, window));
 }
 

@@ -121,15 +121,20 @@ int check_cache(const m4_kv_cache_t* c) {
     return 0;
 }
 
-// B = 0 or T = 0: no rows, and no pointers needed.
-int check_batch(const m4_kv_batch_t* b, uint32_t T, bool* empty) {
+// Rows of a call: what a launch of one thread per eight dims of a row can number.
+constexpr uint32_t kMaxRows = 1u << 26;
+
+// B = 0 or T = 0: no rows, and no pointers needed.  Positions are 32-bit, with
+// room for a stretch of pages on top.
+int check_batch(const m4_kv_cache_t* c, const m4_kv_batch_t* b, uint32_t T, bool* empty) {
     if (!b) return -2;
-    if (b->B > 0x7fffffffu || T > 0x7fffffffu) return -4;
+    if (b->B > 0x7fffffffu || T > kMaxRows) return -4;
     *empty = b->B == 0 || T == 0;
     if (*empty) return 0;
     if (!b->q_start || !b->kv_len || !b->page_table) return -2;
     if (misaligned(b->q_start, 4) || misaligned(b->kv_len, 4) || misaligned(b->page_table, 4)) return -2;
     if (b->table_pages == 0 || (b->B > 1 && b->table_stride < b->table_pages)) return -4;
+    if ((uint64_t)b->table_pages * c->page_size > 0x7fff0000u) return -4;
     return 0;
 }
 
@@ -187,7 +192,7 @@ int validate_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uin
                        const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D, bool* empty) {
     *empty = false;
     if (!rope || !X || !Y) return -2;
-    if (H == 0 || H > 0xffffu || D == 0 || D % 8 || D > 256 || T > 0x7fffffffu) return -4;
+    if (H == 0 || H > 0xffffu || D == 0 || D % 8 || D > 256 || T > kMaxRows) return -4;
     if (int rc = check_rope(rope, D)) return rc;
     if (T == 0) {
         *empty = true;
@@ -204,7 +209,7 @@ int validate_append(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint
                     const m4_rows_t* Q_out, uint32_t H, bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, T, empty)) return rc;
+    if (int rc = check_batch(cache, batch, T, empty)) return rc;
     if (Q && (!rope || !Q_out)) return -2;
     if (Q && (H == 0 || H > 0xffffu)) return -4;
     if (rope) {
@@ -227,7 +232,7 @@ int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32
                   bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, T, empty)) return rc;
+    if (int rc = check_batch(cache, batch, T, empty)) return rc;
     if (*empty) return 0;
     if (int rc = check_rows(K, T, cache->Hkv, cache->D, true)) return rc;
     return check_rows(V, T, cache->Hkv, cache->D, true);
@@ -237,7 +242,7 @@ int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32
                   uint32_t H, float scale, const void* ws, bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, T, empty)) return rc;
+    if (int rc = check_batch(cache, batch, T, empty)) return rc;
     if (H == 0 || H > 0xffffu || H % cache->Hkv || !std::isfinite(scale)) return -4;
     if (*empty) return 0;
     if ((uint64_t)T * (H / cache->Hkv) > 0x7fffffffu) return -4;  // rows of a KV head are counted in 32 bits
@@ -254,7 +259,7 @@ int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint3
     if (!cache || !batch) return -2;
     if (!has_kernels(format) || (norms && norm_type != 1 && norm_type != 2)) return -3;
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = check_batch(batch, T, empty)) return rc;
+    if (int rc = check_batch(cache, batch, T, empty)) return rc;
     if (dm == 0 || Nm == 0 || Hq == 0 || Hq > 0xffffu || Hq % cache->Hkv || !std::isfinite(scale)) return -4;
     const uint64_t HQ = (uint64_t)Hq * cache->D;
     const uint32_t bs = get_quant_info(static_cast<QuantFormat>(format)).block_size;

@@ -38,6 +38,13 @@ constexpr uint32_t kChunkTile = 256, kChunkGroups = 256, kChunkCost = 2, kChunkM
 // eight of 256 over 1024 70 / 57; 2^27 256 over 16384 130 / 102.
 constexpr uint64_t kChunkWork = (uint64_t)1 << 26;
 constexpr float kNone = -3.402823466e38f;  // reference point of a row that has seen no score above -infinity
+// Weights are rounded to fp16 for the second product, 2^-11 of each; those below
+// 2^-14 lose more.  So a row's reference point is kLift below its largest exponent:
+// beside a largest weight of 2^7 or more the small ones keep 2^-32 of it, where
+// beside 1 it would be 2^-25, and many light keys next to a heavy one count.  It
+// moves when an exponent passes 15 (kTop, as bits), so no weight passes 2^15.
+constexpr float kLift = 7.0f;
+constexpr int kTop = 0x41700000;
 
 // A workgroup's note on its partial rows.  tail: an item begins in its share and
 // goes on in the next one's (slot 1, and which rows they are: the KV head, the
@@ -210,7 +217,7 @@ struct Seq {
 __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint32_t R) {
     Seq s;
     const int T = (int)p.batch.T;
-    const int cap = (int)min((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)0x7fffff00);  // + a tile fits
+    const int cap = (int)min((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)0x7fff0000);  // a stretch of pages on top fits
     s.q0 = min(max(p.batch.q_start[b], 0), T);
     s.n = max(min(max(p.batch.q_start[b + 1], 0), T) - s.q0, 0);
     s.len = min(max(p.batch.kv_len[b], 0), cap);
@@ -485,20 +492,20 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             h8_t pf[NR];
 #pragma unroll
             for (int q = 0; q < NR; q++) {
-                // The reference point moves only when an exponent passes 8.  Positive floats
-                // compare as integers do and negative ones are negative integers, so an
-                // integer maximum (three at a time, no quieting of NaNs) tells.
+                // Positive floats compare as integers do and negative ones are negative
+                // integers, so an integer maximum (three at a time, no quieting of NaNs) tells
+                // whether the reference point has to move.
                 float ex[8];
                 int top = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) ex[e] = __builtin_fmaf(sc[q][e >> 2][e & 3], c, -m_run[q]);
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) top = max(max(top, (int)f32_bits(ex[e])), (int)f32_bits(ex[e + 1]));
-                if (__any(top > 0x41000000)) {
+                if (__any(top > kTop)) {
                     float mx = sc[q][0].x;
 #pragma unroll
                     for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[q][e >> 2][e & 3]);
-                    mx *= c;
+                    mx = __builtin_fmaf(mx, c, -kLift);
                     mx = fmaxf(mx, __shfl_xor(mx, 16));
                     mx = fmaxf(mx, __shfl_xor(mx, 32));
                     const float m_new = fmaxf(m_run[q], mx);
@@ -939,16 +946,14 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8_t*>(kb + (kof ^ 32u * kk)), qf[kk], sc, 0, 0, 0);
             return sc;
         };
-        // Exponents of a unit's weights, beside the reference point.  That moves only
-        // when one passes 8: positive floats compare as integers do, negative ones are
-        // negative integers, so one integer maximum (three at a time, and with no
-        // quieting of NaNs) tells.
+        // Exponents of a unit's weights, beside the reference point; whether that has to
+        // move, an integer maximum tells, as above.
         auto settle = [&](const f16v_t& sc, float ex[16], int top) {
-            if (__any(top > (int)0x41000000)) {
+            if (__any(top > kTop)) {
                 float mx = sc[0];
 #pragma unroll
                 for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
-                mx *= c;
+                mx = __builtin_fmaf(mx, c, -kLift);
                 const float m_new = fmaxf(m_run, fmaxf(mx, __shfl_xor(mx, 32)));
                 const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
                 m_run = m_new;
@@ -1162,23 +1167,26 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
     }
 }
 
-// Row tiles by the rows of the longest chunk, workgroups by the length of the line expected.
+// Row tiles by the rows of the longest chunk, workgroups by the length of the line
+// expected.  Any expectation is right, so every product stays within 64 bits.
 static WorkPlan plan_of(const PagedAttnParams& p) {
+    auto at_most = [](uint64_t a, uint64_t b) { return a < b ? a : b; };
     const uint64_t G = p.G, max_new = p.max_new ? p.max_new : 1, rows = max_new * G;
     WorkPlan w;
     w.rows = rows <= 16 ? 16 : 32;
     uint64_t keys = p.max_kv ? p.max_kv : 1;
-    if (p.window) keys = keys < (uint64_t)p.window + max_new ? keys : (uint64_t)p.window + max_new;
-    if (rows >= kChunkTile / 2 && G <= kChunkTile && (uint64_t)p.batch.T * p.H * keys >= kChunkWork)
+    if (p.window) keys = at_most(keys, (uint64_t)p.window + max_new);
+    if (rows >= kChunkTile / 2 && G <= kChunkTile && (uint64_t)p.batch.T * p.H >= (kChunkWork + keys - 1) / keys)
         w.rows = kChunkTile;
-    const uint64_t tiles = (uint64_t)p.batch.B * p.geom.Hkv * ((rows + w.rows - 1) / w.rows);
-    w.items = (uint32_t)(tiles < 0xffffffffu ? tiles : 0xffffffffu);
+    const uint64_t tiles = at_most((uint64_t)p.batch.B * p.geom.Hkv, 1u << 31) * at_most((rows + w.rows - 1) / w.rows, 1u << 31);
+    w.items = (uint32_t)at_most(tiles, 0xffffffffu);
+    const uint64_t many = at_most(tiles, kMaxWaves * kMinSteps);  // of one step: as many groups as are of use
     if (w.rows == kChunkTile) {
-        const uint64_t want = tiles * (keys / (kChunkTile / 2) + 1 + kChunkCost) / kChunkMin + 1;
-        w.groups = (uint32_t)(want < kChunkGroups ? want : kChunkGroups);
+        const uint64_t want = many * (keys / (kChunkTile / 2) + 1 + kChunkCost) / kChunkMin + 1;
+        w.groups = (uint32_t)at_most(want, kChunkGroups);
     } else {
-        const uint64_t want = (tiles * (keys / kStep + 1 + kItemCost) + kMinSteps - 1) / kMinSteps;
-        w.groups = (uint32_t)((want < kMaxWaves ? want : kMaxWaves) + kWaves - 1) / kWaves;
+        const uint64_t want = (many * (keys / kStep + 1 + kItemCost) + kMinSteps - 1) / kMinSteps;
+        w.groups = (uint32_t)(at_most(want, kMaxWaves) + kWaves - 1) / kWaves;
     }
     return w;
 }

@@ -775,6 +775,8 @@ class HIPBridge:
         whose queries see their sequences' (positions None: each token's place)."""
         bufs = (X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, X_out)
         T = X.shape[0]
+        if not 0 <= window < 1 << 32:
+            raise ValueError(f"window={window}")
         for name, t in (("X", X), ("X_out", X_out)):
             if t.dtype is not _torch.float16 or tuple(t.shape) != (T, d_model) or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous fp16 [{T}, {d_model}]")

@@ -96,7 +96,7 @@ def attention(q, k, v, first, window, scale, valid=None):
     [H, n, D] and a bound on what a kernel may be off it by, from these roundings:
       * scores in fp32: (D + 8) 2^-24 of the sum of |q k|, the product with the scale and the base-2 exponent 2^-22
         relative to the exponent, so weights are off by e = 2 (that) + 2^-21 relatively;
-      * each weight rounds to fp16 once (2^-11, or 2^-25 absolutely beside the largest, which is at least 1) and
+      * each weight rounds to fp16 once (2^-11, or 2^-25 absolutely beside the largest, which is at least 2^7) and
         the sum is of the rounded ones, so a weight's error multiplies v - o;
       * fp32 sums over the keys: (keys + 8) 2^-24 of the sum of |w v|;
       * the result rounds to fp16: 2^-11 |o|, or 2^-25 where it is subnormal."""
@@ -126,7 +126,7 @@ def attention(q, k, v, first, window, scale, valid=None):
             e = 2 * np.where(seen, a * ((D + 8) * 2.0 ** -24 + 2.0 ** -22), 0).max(-1, initial=0)[:, None] + 2.0 ** -21
             big = w @ np.abs(fin)
             top = np.abs(fin).max(0, initial=0)[None, :]
-            bound[h] = ((2.0 ** -11 + e) * (big + np.abs(o[h])) + seen.sum(-1, keepdims=True) * 2.0 ** -25 * (top + np.abs(o[h]))
+            bound[h] = ((2.0 ** -11 + e) * (big + np.abs(o[h])) + seen.sum(-1, keepdims=True) * 2.0 ** -32 * (top + np.abs(o[h]))
                         + (L + 8) * 2.0 ** -24 * big + 2.0 ** -11 * np.abs(o[h]) + 2.0 ** -25)
             for key in np.nonzero(~np.isfinite(vv).all(-1))[0]:  # a value that is not finite reaches the rows that see it
                 rows = seen[:, key]

@@ -3,6 +3,7 @@ plain implementations in 64 bits, and their refusals."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -290,6 +291,24 @@ def test_bad_metadata_is_not_followed(bridge, fmt, max_new, max_kv):
     assert bool(torch.isfinite(O).all())
 
 
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_negative_lengths_hold_nothing(bridge, fmt):
+    """However far below zero: positions are not formed from such a length past 32 bits."""
+    import torch
+
+    s = Setup(fmt, [40, 40], [3, 3], 2, 64, 16, seed=3)
+    cache, x = s.cache(), dev(half(s.rng, 2, 6, 64))
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array([-2 ** 31, -1], np.int32)), dev(s.table), 3, 40)
+    bridge.kv_cache_append(cache, batch, x, x)
+    out, O = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    bridge.kv_cache_read(cache, batch, out, out.clone())
+    bridge.dispatch_paged_attn(cache, batch, x, O, 0.125)
+    bridge.synchronize()
+    np.testing.assert_array_equal(cache.pages.cpu().numpy(), s.pages.raw)
+    assert (out == 7.0).all() and (O == 0.0).all()
+
+
 # ---- attention ----------------------------------------------------------------------------------------------------
 
 def check_attention(bridge, s, H, window=0, scale=None, token_major=False, infinite=False, **kw):
@@ -347,6 +366,42 @@ def test_paged_attention(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
 def test_paged_attention_holds_for_any_expectation(bridge, max_new, max_kv):
     check_attention(bridge, Setup(Q8_0, [800, 5, 77], [60, 5, 1], 2, 64, 16, seed=4), 8, max_new=max_new, max_kv=max_kv,
                     token_major=True)
+
+
+@gpu
+@pytest.mark.parametrize("max_new,max_kv", [(2 ** 32 - 1, 2 ** 32 - 1), (2 ** 32 - 1, 1), (1, 2 ** 32 - 1)])
+def test_expectations_past_any_length(bridge, max_new, max_kv):
+    s = Setup(Q4_0, [70] * 5, [3] * 5, 2, 64, 16, seed=5)
+    assert 0 < bridge.paged_attn_workspace(s.cache(), s.batch(max_new=max_new, max_kv=max_kv), 8, s.T) < 1 << 28
+    check_attention(bridge, s, 8, max_new=max_new, max_kv=max_kv)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,kw", [(1, {"max_new": 1}), (8, {"max_new": 8}), (60, {"max_new": 4096, "max_kv": 10 ** 8})],
+                         ids=["rows_of_16", "rows_of_32", "chunks"])
+def test_many_light_keys_beside_a_heavy_one(bridge, D, n, kw):
+    """Weights of 2^-24.4 beside one of 1: fp16 has two bits at most for them, and 40000 of them count."""
+    import torch
+
+    L, P = 40000, 256
+    k, v = np.zeros((1, L, D), np.float16), np.ones((1, L, D), np.float16)
+    k[0, 0], v[0, 0] = 24.4 * math.log(2) * 8 / D, 0.0
+    q = np.ones((4, n, D), np.float16)
+    pages = -(-L // P)
+    cache = m4_bridge.PagedKVCache(Q8_0, pages, P, 1, D)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    kv_len = dev(np.array([L], np.int32))
+    bridge.kv_cache_append(cache, m4_bridge.KVBatch(dev(np.array([0, L], np.int32)), kv_len, table, L, L), dev(k), dev(v))
+    O = torch.zeros(4, n, D, dtype=torch.float16, device="cuda")
+    batch = m4_bridge.KVBatch(dev(np.array([0, n], np.int32)), kv_len, table, **{"max_kv": L, **kw})
+    say("light keys", D, n)
+    bridge.dispatch_paged_attn(cache, batch, dev(q), O, 0.125)
+    bridge.synchronize()
+    kx, vx = (ref.values(*ref.quantize(Q8_0, x[0])) for x in (k, v))
+    want, bound = ref.attention(q, kx[None], vx[None], L - n, 0, 0.125)
+    assert 0.001 < want.min() and want.max() < 0.01
+    close(O.cpu().numpy(), want, bound, "light keys")
 
 
 @gpu
@@ -684,7 +739,9 @@ def _set(path, value):
     (_set("batch.table_pages", 0), (-4, -4, -4, 0)),
     (_set("batch.table_stride", 3), (-4, -4, -4, 0)),
     (_set("T", 0), (0, 0, 0, 0)),
-    (_set("T", 1 << 31), (-4, -4, -4, -4)),
+    (_set("T", (1 << 26) + 1), (-4, -4, -4, -4)),
+    (lambda a: (setattr(a.batch, "table_pages", 0x7fff0000 // 16 + 1), setattr(a.batch, "table_stride", 1 << 28)),
+     (-4, -4, -4, 0)),
     (_set("batch.B", 0), (0, 0, 0, 0)),
     (_set("kv", None), (-2, -2, 0, 0)),
     (_set("kv.ptr", 0x200002), (-2, -2, 0, 0)),
@@ -765,6 +822,15 @@ def test_uninitialized_bridge_refuses(lib):
     assert lib.m4_bridge_dispatch_paged_attn(r(a.cache), r(a.batch), 10, r(a.q), r(a.q), 8, 0.1, 0, 0x400000, 1 << 30) == -1
 
 
+@pytest.mark.parametrize("change", [_set("cache.page_size", 0xffffffff), _set("cache.page_size", 24), _set("cache.D", 32),
+                                    _set("cache.Hkv", 3), _set("cache.format", 1), _set("H", 0), _set("H", 1 << 16)])
+def test_no_workspace_for_what_is_refused(lib, change):
+    a = Args()
+    assert lib.m4_bridge_paged_attn_workspace(ctypes.addressof(a.cache), ctypes.addressof(a.batch), a.T, a.H, 0) > 0
+    change(a)
+    assert lib.m4_bridge_paged_attn_workspace(ctypes.addressof(a.cache), ctypes.addressof(a.batch), a.T, a.H, 0) == 0
+
+
 def test_python_refusals(libpath):
     import torch
 
@@ -794,6 +860,9 @@ def test_python_refusals(libpath):
         b.dispatch_paged_attn(cache, batch, kv, kv[:, :1], 0.1)
     with pytest.raises(ValueError):
         b.rope_axes(kv, kv, m4_bridge.RotaryAxes(128, sections=(16, 24, 24)), i32(3))
+    x = torch.zeros(3, 256, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        b.paged_layer(x, None, *[x] * 4, None, *[x] * 3, x.clone(), 0, 256, 2, 512, 0.1, cache, batch, window=-1)
 
 
 @gpu
