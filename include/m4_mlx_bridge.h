@@ -249,7 +249,8 @@ M4_API int m4_bridge_projection_plan(int format, uint32_t M, uint32_t K, const u
  * [page_size][D / 32], V scales [page_size / 4][D / 32][4 tokens].  Q8_0 codes
  * are stored plus 128; of Q4_0 codes a byte holds two dims: of K, byte 4 m + i
  * dims 8 m + i (low) and 8 m + 4 + i, of V dims 2 x (low) and 2 x + 1.  Values are
- * half(q * half(d)) and half((c - 8) * half(d)), as in the router's blocks.
+ * half(q * half(d)) and half((c - 8) * half(d)), as in the router's blocks; scales
+ * of Q4_0 at most 8188, as those of fp16 rows are.
  * `pages` 16-byte aligned, at least m4_bridge_kv_cache_bytes. */
 typedef struct {
     void* pages;

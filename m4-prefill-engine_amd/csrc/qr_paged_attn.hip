@@ -22,7 +22,7 @@ constexpr uint32_t kStep = 32;     // keys of a step
 // 21.7 / 19.1 / 19.0.
 constexpr uint32_t kItemCost = 3;
 // Waves: two per SIMD where each gets kLongShare of the line (four requests of
-// 131072 keys: 132 us on one, 118 on two), else one: fewer items are cut and fewer
+// 131072 keys: 132 us on one, 118 on two when this was chosen), else one: fewer items are cut and fewer
 // parts joined (drafted tokens 18.7 us, on two 19.8; one token over 16384 keys 16.7
 // and 19.5).  A count between the two leaves some SIMDs with two and the rest
 // waiting.  Three are slower: with the next step's tiles in flight the registers
@@ -68,10 +68,15 @@ __device__ __forceinline__ h2_t q8_hi(uint32_t w, h2_t d) {
     const h2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
     return (as_h2(nib_pair_hi(w)) - off) * d;
 }
+// values c d - 8 d of Q4_0 codes, n8 = -8 d: one instruction, and one rounding as in
+// (c - 8) d since 8 d is exact for scales up to 8188, which fp16 rows do not pass
 template <bool HI>
-__device__ __forceinline__ h2_t q4_pair(uint32_t codes, h2_t d) {
-    const h2_t off = {(_Float16)8.0f, (_Float16)8.0f};
-    return (code_pair<HI>(codes) - off) * d;
+__device__ __forceinline__ h2_t q4_pair(uint32_t codes, h2_t d, h2_t n8) {
+    return __builtin_elementwise_fma(code_pair<HI>(codes), d, n8);
+}
+__device__ __forceinline__ h2_t q4_offset(h2_t d) {
+    const h2_t m8 = {(_Float16)-8.0f, (_Float16)-8.0f};
+    return d * m8;
 }
 
 template <int W>
@@ -126,20 +131,21 @@ __device__ __forceinline__ h8_t k_octet(const uint32_t* k, int kk, h2_t d) {
         e = q8_hi(k[2 * kk + 1], d);
     } else {
         const uint32_t lo = k[kk] & 0x0f0f0f0fu, hi = k[kk] >> 4 & 0x0f0f0f0fu;
-        a = q4_pair<false>(lo, d);
-        b = q4_pair<true>(lo, d);
-        c = q4_pair<false>(hi, d);
-        e = q4_pair<true>(hi, d);
+        const h2_t n8 = q4_offset(d);
+        a = q4_pair<false>(lo, d, n8);
+        b = q4_pair<true>(lo, d, n8);
+        c = q4_pair<false>(hi, d, n8);
+        e = q4_pair<true>(hi, d, n8);
     }
     return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
 }
 // V values of four keys of dim dt of a run of codes, as two pairs
 template <int FMT>
 __device__ __forceinline__ u2_t v_quad(const uint32_t* v, int dt, u2_t d) {
-    const uint32_t s0 = d.x, s1 = d.y;
-    if constexpr (FMT == QUANT_Q8_0) return u2_t{as_u32(q8_lo(v[dt], as_h2(s0))), as_u32(q8_hi(v[dt], as_h2(s1)))};
+    const h2_t s0 = as_h2((uint32_t)d.x), s1 = as_h2((uint32_t)d.y);
+    if constexpr (FMT == QUANT_Q8_0) return u2_t{as_u32(q8_lo(v[dt], s0)), as_u32(q8_hi(v[dt], s1))};
     const uint32_t w = (dt & 1 ? v[dt / 2] >> 4 : v[dt / 2]) & 0x0f0f0f0fu;
-    return u2_t{as_u32(q4_pair<false>(w, as_h2(s0))), as_u32(q4_pair<true>(w, as_h2(s1)))};
+    return u2_t{as_u32(q4_pair<false>(w, s0, q4_offset(s0))), as_u32(q4_pair<true>(w, s1, q4_offset(s1)))};
 }
 
 // A lane's share of 16 keys: W words of K codes (D / 4 dims of one key) and of V
@@ -239,7 +245,8 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // paged_attn_join_kernel joins in order.  The next step's tiles are loaded before
 // the present one is computed, and page numbers 32 steps ahead, a lane each.
 // Bound by the cache's bytes once there are enough of them: four requests of
-// 131072 keys (Q4_0, D = 128, 604 MB) 118 .. 122 us, 5.0 TB/s; 64 requests of 1 .. 8192
+// 131072 keys (Q4_0, D = 128, 604 MB) 116 us, 5.2 TB/s (122 with codes less 8, then
+// times the scale: vector instructions count there too); 64 requests of 1 .. 8192
 // keys (Q8_0, 110 MB) 30 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
 // of descriptor, page table, key and join latencies; drafted tokens and short
 // chunks (two row blocks) by turning codes into fp16 on one wave per SIMD.
