@@ -79,18 +79,23 @@ __device__ __forceinline__ h2_t q4_offset(h2_t d) {
     return d * m8;
 }
 
-template <int W>
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load_of(const uint8_t* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+    return *reinterpret_cast<const T*>(p);
+}
+template <int W, bool ONCE>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t w[W]) {
     if constexpr (W == 1) {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
+        w[0] = load_of<ONCE, uint32_t>(p);
     } else if constexpr (W == 2) {
-        const u2_t a = *reinterpret_cast<const u2_t*>(p);
+        const u2_t a = load_of<ONCE, u2_t>(p);
         w[0] = a.x;
         w[1] = a.y;
     } else {
 #pragma unroll
         for (int i = 0; i < W / 4; i++) {
-            const u4_t a = reinterpret_cast<const u4_t*>(p)[i];
+            const u4_t a = load_of<ONCE, u4_t>(p + 16 * i);
             w[4 * i] = a.x;
             w[4 * i + 1] = a.y;
             w[4 * i + 2] = a.z;
@@ -170,10 +175,12 @@ struct Tile {
             vs = g.vs_off + (q * NB + j * NB / 16) * 8;
         }
     };
+    // ONCE: codes that no other wave reads pass the caches by
+    template <bool ONCE>
     __device__ __forceinline__ void load(const uint8_t* head, const Offsets& at, uint32_t slot0) {
-        // plain loads: through buffer resources the four requests of 131072 keys take 145 us, so 128
-        load_words<W>(head + slot0 * CB + at.k, k);
-        load_words<W>(head + slot0 * CB + at.v, v);
+        // no buffer resources: through them the four requests of 131072 keys took 145 us, so 128
+        load_words<W, ONCE>(head + slot0 * CB + at.k, k);
+        load_words<W, ONCE>(head + slot0 * CB + at.v, v);
         kd = *reinterpret_cast<const uint16_t*>(head + slot0 * (NB * 2) + at.ks);
         vd = *reinterpret_cast<const u2_t*>(head + slot0 * (NB * 2) + at.vs);
     }
@@ -245,8 +252,8 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // paged_attn_join_kernel joins in order.  The next step's tiles are loaded before
 // the present one is computed, and page numbers 32 steps ahead, a lane each.
 // Bound by the cache's bytes once there are enough of them: four requests of
-// 131072 keys (Q4_0, D = 128, 604 MB) 116 us, 5.2 TB/s (122 with codes less 8, then
-// times the scale: vector instructions count there too); 64 requests of 1 .. 8192
+// 131072 keys (Q4_0, D = 128, 604 MB) 109 us, 5.5 TB/s (with codes less 8, then times
+// the scale, 6 more: vector instructions count there too); 64 requests of 1 .. 8192
 // keys (Q8_0, 110 MB) 30 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
 // of descriptor, page table, key and join latencies; drafted tokens and short
 // chunks (two row blocks) by turning codes into fp16 on one wave per SIMD.
@@ -255,6 +262,11 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     constexpr uint32_t R = 16 * NR;
     constexpr int DT = D / 16, KK = D / 32;
     constexpr int RUN = D / 4;  // dims of a lane's run
+    // Codes past the caches: one row tile, Q4_0.  us without / with: four requests of
+    // 131072 keys 113.5 / 109, one 40 / 37.6, 64 of 8192 113 / 108.5.  Q8_0, whose lines
+    // are longer runs: 64 of 1 .. 8192 30.4 / 31.0, 64 of 1024 36.0 / 35.3, one of 131072
+    // 62.7 / 63.6.  Two row blocks (more tiles that read them again): Q4_0 24.4 / 24.8.
+    constexpr bool kOnce = FMT == QUANT_Q4_0 && NR == 1;
 
     const int lane = threadIdx.x & 63;
     const int j = lane & 15, g = lane >> 4;
@@ -440,7 +452,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                 const uint32_t page = __builtin_amdgcn_readlane(page_ids, 2 * (u - ids_from) + t);
                 tile[t].there = page < p.geom.num_pages;
                 const uint8_t* head = p.geom.pages + ((size_t)(tile[t].there ? page : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
-                tile[t].load(head, at_lane, (uint32_t)(key0 + 16 * t) & pmask);
+                tile[t].template load<kOnce>(head, at_lane, (uint32_t)(key0 + 16 * t) & pmask);
             }
         };
         auto step = [&](Tile<FMT, D> tile[2], int u) {

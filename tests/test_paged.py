@@ -196,6 +196,31 @@ def test_append_and_read(bridge, fmt, lens, new, Hkv, D, P):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_reads_are_short_ones(bridge, fmt, D):
+    """Results that pass the caches by, bit for bit those of parts that do not."""
+    import torch
+
+    T, Hkv, P, parts = 8192 * 128 // D + 77, 16, 256, 3
+    pages = -(-T // P)
+    cache = m4_bridge.PagedKVCache(fmt, pages, P, Hkv, D)
+    x = torch.randn(2, Hkv, T, D, device="cuda").half()
+    table = torch.randperm(pages, device="cuda").int()[None]
+    batch = lambda a, b: m4_bridge.KVBatch(dev(np.array([0, b - a], np.int32)), dev(np.array([b], np.int32)),  # noqa: E731
+                                           table, T, T)
+    bridge.kv_cache_append(cache, batch(0, T), x[0], x[1])
+    long, short = torch.zeros_like(x), torch.zeros_like(x)
+    assert long.numel() * 2 > 64 << 20
+    bridge.kv_cache_read(cache, batch(0, T), long[0], long[1])
+    for i in range(parts):
+        a, b = T * i // parts, T * (i + 1) // parts
+        bridge.kv_cache_read(cache, batch(a, b), short[0, :, a:b], short[1, :, a:b])
+    bridge.synchronize()
+    assert torch.equal(long, short) and (long != 0).any()
+
+
+@gpu
 def test_append_matches_quantize_kv_q8_0(bridge):
     """The cache holds what m4_bridge_quantize_kv_q8_0 makes of the same rows, scale and code for code."""
     import torch
