@@ -6,6 +6,9 @@
 namespace qr {
 
 constexpr uint64_t kBlocks = 1024;  // that fill the chip
+// Bytes from which rows that are read once are loaded past the caches (what the L2
+// caches hold together), and results stored past them.
+constexpr uint64_t kLoadPast = (uint64_t)32 << 20, kStorePast = (uint64_t)64 << 20;
 
 // Where a token lies in the cache.
 struct Place {
@@ -121,8 +124,11 @@ __device__ __forceinline__ void quantize8(const float x[8], int lane, uint32_t c
 // of K and V, so angles are formed once per wave and used for all its heads.  A
 // rotated row is rounded to fp16 before it is quantized, as a rotation and a write
 // apart would.  Bound by bytes once there are enough: 8100 tokens of 32 heads
-// (133 MB) 30 us, 4.4 TB/s; 64 tokens 5 us, a chain of table and angle latencies.
-template <int LPR, int FMT>
+// (133 MB) 27 us, 4.9 TB/s; 64 tokens 5 us, a chain of table and angle latencies.
+// PAST: rows of Q, kLoadPast bytes and more, are loaded past the caches, which keep
+// the turned ones: 30 us without; then attention over as many keys 710 us with both.
+// Stored past them too it is 25, and the attention that reads them longer by more.
+template <int LPR, int FMT, bool PAST>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t q_blocks) {
     constexpr int RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -157,7 +163,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, uint32_t
         if (of_q) {
 #pragma unroll
             for (int i = 0; i < kAhead; i++, ahead += chunks, src += step)
-                if (ahead < heads && live) next[i] = *reinterpret_cast<const h8_t*>(src);
+                if (ahead < heads && live) {
+                    if constexpr (PAST) next[i] = __builtin_nontemporal_load(reinterpret_cast<const h8_t*>(src));
+                    else next[i] = *reinterpret_cast<const h8_t*>(src);
+                }
         } else {
 #pragma unroll
             for (int i = 0; i < kAhead; i += 2, ahead += chunks, src += step, src2 += step2)
@@ -338,19 +347,19 @@ hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
     }
     const dim3 grid(groups, q_blocks + kv_blocks);
     const int fmt = p.geom.pages ? p.format : -1;
-#define QR_APPEND(L, F) hipLaunchKernelGGL((kv_append_kernel<L, F>), grid, dim3(256), 0, st, p, q_blocks)
-    if (fmt < 0) {
-        if (lpr == 8) QR_APPEND(8, -1);
-        else if (lpr == 16) QR_APPEND(16, -1);
-        else QR_APPEND(32, -1);
-    } else if (fmt == QUANT_Q8_0) {
-        if (lpr == 8) QR_APPEND(8, QUANT_Q8_0);
-        else QR_APPEND(16, QUANT_Q8_0);
-    } else if (fmt == QUANT_Q4_0) {
-        if (lpr == 8) QR_APPEND(8, QUANT_Q4_0);
-        else QR_APPEND(16, QUANT_Q4_0);
-    } else {
-        return hipErrorInvalidValue;
+    const bool past = (uint64_t)p.T * p.H * p.D * 2 >= kLoadPast;
+#define QR_APPEND(L, F)                                                                              \
+    if (past) hipLaunchKernelGGL((kv_append_kernel<L, F, true>), grid, dim3(256), 0, st, p, q_blocks); \
+    else hipLaunchKernelGGL((kv_append_kernel<L, F, false>), grid, dim3(256), 0, st, p, q_blocks)
+    switch (fmt * 32 + lpr) {
+        case -32 + 8: QR_APPEND(8, -1); break;
+        case -32 + 16: QR_APPEND(16, -1); break;
+        case -32 + 32: QR_APPEND(32, -1); break;
+        case QUANT_Q8_0 * 32 + 8: QR_APPEND(8, QUANT_Q8_0); break;
+        case QUANT_Q8_0 * 32 + 16: QR_APPEND(16, QUANT_Q8_0); break;
+        case QUANT_Q4_0 * 32 + 8: QR_APPEND(8, QUANT_Q4_0); break;
+        case QUANT_Q4_0 * 32 + 16: QR_APPEND(16, QUANT_Q4_0); break;
+        default: return hipErrorInvalidValue;
     }
 #undef QR_APPEND
     return hipGetLastError();
@@ -359,10 +368,9 @@ hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
 // The values of the batch's rows: half(q half(d)), or half((c - 8) half(d)).  A
 // lane reads 8 dims of a token; of V the four tokens of its group, of which it
 // keeps its own (the other three lanes' reads of the same bytes hit the cache).
-// PAST: stores that do not stay in the caches, from kPastCaches bytes of results
+// PAST: stores that do not stay in the caches, from kStorePast bytes of results
 // on.  us without / with: 91 MB 36.7 / 25.0 (5.7 TB/s), and with a copy of the
 // results behind it 85 MB 71 / 78, 195 MB 159 / 158; 39 MB 46.7 / 50.0.
-constexpr uint64_t kPastCaches = (uint64_t)64 << 20;
 template <int LPR, int FMT, bool PAST>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p) {
     constexpr int RPW = 64 / LPR;
@@ -435,7 +443,7 @@ hipError_t launch_kv_read(const ReadParams& p, hipStream_t st) {
     uint32_t blocks = 2 * p.geom.Hkv;
     while (blocks > 1 && (uint64_t)groups * blocks > kBlocks) blocks = (blocks + 1) / 2;
     const dim3 grid(groups, blocks);
-    const bool past = (uint64_t)p.batch.T * p.geom.Hkv * p.D * 4 >= kPastCaches;
+    const bool past = (uint64_t)p.batch.T * p.geom.Hkv * p.D * 4 >= kStorePast;
 #define QR_READ(L, F)                                                                        \
     if (past) hipLaunchKernelGGL((kv_read_kernel<L, F, true>), grid, dim3(256), 0, st, p);   \
     else hipLaunchKernelGGL((kv_read_kernel<L, F, false>), grid, dim3(256), 0, st, p);       \

@@ -152,6 +152,39 @@ def test_rope_axes_matches_rope_and_takes_strides(bridge):
     assert bool((rest == 9.0).all())
 
 
+@gpu
+@pytest.mark.parametrize("D,fmt", [(64, None), (128, None), (256, None), (64, Q8_0), (128, Q8_0), (64, Q4_0), (128, Q4_0)])
+def test_long_rows_turn_as_short_ones(bridge, D, fmt):
+    """64 MB of rows and more, which are loaded another way, alone and beside an append, bit for bit those of parts."""
+    import torch
+
+    H, Hkv, T, P, parts = 64, 2, 4096 * 128 // D + 33, 256, 3
+    x, kv = torch.randn(H, T, D, device="cuda").half(), torch.randn(Hkv, T, D, device="cuda").half()
+    assert x.numel() * 2 > 64 << 20
+    rope = m4_bridge.RotaryAxes(D, theta=1e6)
+    long, short = torch.zeros_like(x), torch.zeros_like(x)
+    places = torch.arange(T, dtype=torch.int32, device="cuda")
+    pages = -(-T // P)
+    cache = m4_bridge.PagedKVCache(fmt, pages, P, Hkv, D) if fmt is not None else None
+    say("long rows", D, fmt)
+
+    def turn(a, b, y):
+        if fmt is None:
+            return bridge.rope_axes(x[:, a:b], y[:, a:b], rope, places[a:b])
+        batch = m4_bridge.KVBatch(dev(np.array([0, b - a], np.int32)), dev(np.array([b], np.int32)),
+                                  torch.arange(pages, dtype=torch.int32, device="cuda")[None], b - a, b)
+        bridge.kv_cache_append(cache, batch, kv[:, a:b], kv[:, a:b], rope=rope, Q=x[:, a:b], Q_out=y[:, a:b])
+
+    turn(0, T, long)
+    for i in range(parts):
+        turn(T * i // parts, T * (i + 1) // parts, short)
+    bridge.synchronize()
+    assert torch.equal(long, short) and (long != x).any()
+    turn(0, T, x)  # in place
+    bridge.synchronize()
+    assert torch.equal(long, x)
+
+
 # ---- the cache ----------------------------------------------------------------------------------------------------
 
 @gpu
