@@ -755,7 +755,7 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
 // takes its rows over the tile, 32 x 32 scores at a time.  256 rows share the work
 // of turning codes (128 rows: 1306 us where 256 take 1140).  2048 tokens over 30000
 // keys (D = 128, 972 GFLOP) 1080 us with the join, 0.90 PFLOP/s; counters: the
-// matrix pipe 46% busy, 7.5 vector operations per MFMA, at 1.94 GHz: cycles saved
+// matrix pipe 44% busy, 7.5 vector operations per MFMA, at 1.94 GHz: cycles saved
 // since (2.38 M a CU to 2.03 M) came back as a lower clock, so power bounds it.
 template <int FMT, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
