@@ -96,6 +96,8 @@ struct PagedAttnParams {
     PageGeom geom;
     BatchView batch;
     uint32_t max_new, max_kv;  // what the plan expects; any value is right
+    // a launch's: sequences of that many rows a KV head, [min_rows, max_rows)
+    uint32_t min_rows, max_rows;
     uint8_t* ws;
 };
 size_t paged_attn_workspace(const PagedAttnParams& p);

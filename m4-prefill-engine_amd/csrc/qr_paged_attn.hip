@@ -58,6 +58,10 @@ struct alignas(16) ItemNote {
 struct WorkPlan {
     uint32_t rows, groups, items;  // of a row tile; workgroups; row tiles of all heads, as expected
 };
+struct AttnPlan {
+    WorkPlan few, many;  // of the sequences of few rows and of those of chunks; no groups: no launch
+    bool both;
+};
 
 // values 1024 + 128 + q of four Q8_0 bytes, as pairs
 __device__ __forceinline__ h2_t q8_lo(uint32_t w, h2_t d) {
@@ -233,6 +237,7 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
     const int cap = (int)min((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)0x7fff0000);  // a stretch of pages on top fits
     s.q0 = min(max(p.batch.q_start[b], 0), T);
     s.n = max(min(max(p.batch.q_start[b + 1], 0), T) - s.q0, 0);
+    if ((uint32_t)s.n * p.G < p.min_rows || (uint32_t)s.n * p.G >= p.max_rows) s.n = 0;  // another launch's
     s.len = min(max(p.batch.kv_len[b], 0), cap);
     s.lo = 0;
     if (p.window) s.lo = (int)(max((int64_t)s.len - s.n + 1 - (int64_t)p.window, (int64_t)0) / kStep * kStep);
@@ -1187,27 +1192,39 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
 }
 
 // Row tiles by the rows of the longest chunk, workgroups by the length of the line
-// expected.  Any expectation is right, so every product stays within 64 bits.
-static WorkPlan plan_of(const PagedAttnParams& p) {
+// expected.  Any expectation is right, so every product stays within 64 bits.  A
+// batch whose chunks are worth theirs, but not all of whose sequences are as long (T
+// says so), is taken apart, sequences of kChunkTile / 2 rows and more for chunks: a
+// row tile there is as much work for one token as for 64.  us of chunks alone / both:
+// 2048 tokens beside 63 single ones 523 / 387, four of 512 beside 60 270 / 178, 512
+// beside 31 (Q4_0) 199 / 113; three prompts of 700 .. 2048, for which the other
+// kernels run in vain, 119 / 124.  From a little more work than chunks alone: 512
+// beside 63 (9/8 of kChunkWork) by rows altogether 100, both 116; prompts of 1500
+// and 700 (12/8) 99 and 82.
+static AttnPlan plan_of(const PagedAttnParams& p) {
     auto at_most = [](uint64_t a, uint64_t b) { return a < b ? a : b; };
     const uint64_t G = p.G, max_new = p.max_new ? p.max_new : 1, rows = max_new * G;
-    WorkPlan w;
-    w.rows = rows <= 16 ? 16 : 32;
     uint64_t keys = p.max_kv ? p.max_kv : 1;
     if (p.window) keys = at_most(keys, (uint64_t)p.window + max_new);
-    if (rows >= kChunkTile / 2 && G <= kChunkTile && (uint64_t)p.batch.T * p.H >= (kChunkWork + keys - 1) / keys)
-        w.rows = kChunkTile;
-    const uint64_t tiles = at_most((uint64_t)p.batch.B * p.geom.Hkv, 1u << 31) * at_most((rows + w.rows - 1) / w.rows, 1u << 31);
-    w.items = (uint32_t)at_most(tiles, 0xffffffffu);
-    const uint64_t many = at_most(tiles, kMaxWaves * kMinSteps);  // of one step: as many groups as are of use
-    if (w.rows == kChunkTile) {
-        const uint64_t want = many * (keys / (kChunkTile / 2) + 1 + kChunkCost) / kChunkMin + 1;
-        w.groups = (uint32_t)at_most(want, kChunkGroups);
-    } else {
-        const uint64_t want = (many * (keys / kStep + 1 + kItemCost) + kMinSteps - 1) / kMinSteps;
-        w.groups = (uint32_t)(at_most(want, kMaxWaves) + kWaves - 1) / kWaves;
+    const bool mixed = p.batch.T < p.batch.B * max_new && p.batch.B > 1;
+    const uint64_t least = mixed ? kChunkWork * 5 / 4 : kChunkWork;
+    const bool chunks = rows >= kChunkTile / 2 && G <= kChunkTile && (uint64_t)p.batch.T * p.H >= (least + keys - 1) / keys;
+    const uint64_t heads = at_most((uint64_t)p.batch.B * p.geom.Hkv, 1u << 31);
+    auto tiles_of = [&](uint32_t of) { return heads * at_most((rows + of - 1) / of, 1u << 31); };
+    AttnPlan a{};
+    a.both = chunks && mixed;
+    if (chunks) {
+        const uint64_t tiles = tiles_of(kChunkTile), some = at_most(tiles, kChunkGroups * kChunkMin);
+        const uint64_t want = some * (keys / (kChunkTile / 2) + 1 + kChunkCost) / kChunkMin + 1;
+        a.many = {kChunkTile, (uint32_t)at_most(want, kChunkGroups), (uint32_t)at_most(tiles, 0xffffffffu)};
     }
-    return w;
+    if (!chunks || mixed) {
+        const uint32_t of = (chunks ? G : rows) <= 16 ? 16 : 32;
+        const uint64_t tiles = chunks ? heads : tiles_of(of), some = at_most(tiles, kMaxWaves * kMinSteps);
+        const uint64_t want = (some * (keys / kStep + 1 + kItemCost) + kMinSteps - 1) / kMinSteps;
+        a.few = {of, (uint32_t)(at_most(want, kMaxWaves) + kWaves - 1) / kWaves, (uint32_t)at_most(tiles, 0xffffffffu)};
+    }
+    return a;
 }
 
 template <int D>
@@ -1217,43 +1234,54 @@ static size_t ws_bytes(const WorkPlan& w) {
 }
 
 size_t paged_attn_workspace(const PagedAttnParams& p) {
-    const WorkPlan w = plan_of(p);
-    return p.D == 64 ? ws_bytes<64>(w) : ws_bytes<128>(w);
+    const AttnPlan a = plan_of(p);
+    return p.D == 64 ? ws_bytes<64>(a.few) + ws_bytes<64>(a.many) : ws_bytes<128>(a.few) + ws_bytes<128>(a.many);
 }
 
 template <int D, int R>
-static hipError_t launch_join(const PagedAttnParams& p, uint32_t groups, uint32_t items, hipStream_t st) {
+static hipError_t launch_join(const PagedAttnParams& p, const WorkPlan& w, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // Blocks for each few workgroups, over which the rows of an item are spread: more
     // where items have many parts.  us of the whole call with 4 / 16 of them: 64 tokens
     // over 16384 keys (32 parts an item) 82 / 42, one token 27 / 23, 64 requests (one
     // part) 34 / 40.
-    const uint32_t parts = groups / items, across = R > 32 ? 32 : (parts >= 16 ? 16 : (parts >= 8 ? 8 : 4));
+    const uint32_t parts = w.groups / w.items, across = R > 32 ? 32 : (parts >= 16 ? 16 : (parts >= 8 ? 8 : 4));
     const uint32_t most = 4 * kJoinBlocks / across;
-    const dim3 grid(groups < most ? groups : most, across);
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, R>), grid, dim3(256), 0, st, p, groups);
+    const dim3 grid(w.groups < most ? w.groups : most, across);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, R>), grid, dim3(256), 0, st, p, w.groups);
     return hipGetLastError();
 }
 
 template <int FMT, int D>
-static hipError_t launch_format(const PagedAttnParams& p, hipStream_t st) {
-    const WorkPlan w = plan_of(p);
-    if (w.rows == kChunkTile) {
-        constexpr int NW = kChunkTile / 32;
-        constexpr size_t lds = 2 * 2 * 16 * NW * D * 2;
-        static size_t attr[kMaxDevices] = {};  // more than the default 64 KB of LDS
-        const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW>, lds, attr);
+static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
+    const AttnPlan a = plan_of(p);
+    constexpr uint32_t cut = kChunkTile / 2;
+    p.min_rows = 0;
+    p.max_rows = a.both ? cut : 0xffffffffu;
+    if (a.few.groups) {
+        const dim3 grid(a.few.groups), block(64 * kWaves);
+        hipError_t e;
+        if (a.few.rows == 16) {
+            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1>), grid, block, 0, st, p, a.few.groups);
+            e = launch_join<D, 16>(p, a.few, st);
+        } else {
+            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2>), grid, block, 0, st, p, a.few.groups);
+            e = launch_join<D, 32>(p, a.few, st);
+        }
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW>), dim3(w.groups), dim3(64 * NW), lds, st, p, w.groups);
-        return launch_join<D, kChunkTile>(p, w.groups, w.items, st);
     }
-    if (w.rows == 16) {
-        hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1>), dim3(w.groups), dim3(64 * kWaves), 0, st, p, w.groups);
-        return launch_join<D, 16>(p, w.groups, w.items, st);
-    }
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2>), dim3(w.groups), dim3(64 * kWaves), 0, st, p, w.groups);
-    return launch_join<D, 32>(p, w.groups, w.items, st);
+    if (!a.many.groups) return hipSuccess;
+    p.ws += ws_bytes<D>(a.few);
+    p.min_rows = a.both ? cut : 0;
+    p.max_rows = 0xffffffffu;
+    constexpr int NW = kChunkTile / 32;
+    constexpr size_t lds = 2 * 2 * 16 * NW * D * 2;
+    static size_t attr[kMaxDevices] = {};  // more than the default 64 KB of LDS
+    const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW>, lds, attr);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW>), dim3(a.many.groups), dim3(64 * NW), lds, st, p, a.many.groups);
+    return launch_join<D, kChunkTile>(p, a.many, st);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) {

@@ -307,13 +307,14 @@ def test_fused_rope_append_is_rope_then_append(bridge, fmt, D, dims, axes, tradi
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("max_new,max_kv", [(20, 60), (4096, 10 ** 8)], ids=["rows", "chunks"])
-def test_bad_metadata_is_not_followed(bridge, fmt, max_new, max_kv):
+@pytest.mark.parametrize("H,max_new,max_kv", [(4, 20, 60), (32, 8, 10 ** 8), (32, 4096, 10 ** 8)],
+                         ids=["rows", "chunks", "both"])
+def test_bad_metadata_is_not_followed(bridge, fmt, H, max_new, max_kv):
     """Pages that are not there, more keys than the table holds, starts past the rows: such tokens are not written, not
     read and not seen, and nothing outside the buffers is touched."""
     import torch
 
-    P, Hkv, H, D = 16, 2, 4, 64
+    P, Hkv, D = 16, 2, 64
     s = Setup(fmt, [60, 40], [20, 6], Hkv, D, P, seed=9, fill=0)
     table = s.table.copy()
     table[0, 1] = 10 ** 9      # keys 16 .. 31 of sequence 0
@@ -411,11 +412,14 @@ def check_attention(bridge, s, H, window=0, scale=None, token_major=False, infin
     ([700, 1], [333, 1], 10, 2, 128, 256, 100),               # groups of 5: row tiles that are not full
     ([300], [200], 160, 1, 64, 16, 0),                        # a group wider than a row tile
     ([5000], [70], 8, 8, 128, 64, 0),
+    ([700, 90, 40, 33, 500], [300, 1, 2, 17, 128], 8, 2, 128, 16, 0),  # chunks and steps in any order
 ])
-@pytest.mark.parametrize("kernels", ["as_planned", "rows", "chunks"])
+@pytest.mark.parametrize("kernels", ["as_planned", "rows", "chunks", "both"])
 def test_paged_attention(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
-    # what is expected of the lengths chooses the kernels: every case runs on both
-    kw = {"as_planned": {}, "rows": {"max_new": 1, "max_kv": 1}, "chunks": {"max_new": 4096, "max_kv": 10 ** 8}}[kernels]
+    # what is expected of the lengths chooses the kernels: every case runs on each, and with its longer sequences on
+    # one and the others on the other
+    kw = {"as_planned": {}, "rows": {"max_new": 1, "max_kv": 1}, "both": {"max_new": 4096, "max_kv": 10 ** 8},
+          "chunks": {"max_new": -(-128 // (H // Hkv)), "max_kv": 10 ** 8}}[kernels]
     check_attention(bridge, Setup(fmt, lens, new, Hkv, D, P, seed=sum(lens) + H), H, window, **kw)
 
 
@@ -471,9 +475,10 @@ def test_paged_attention_scales(bridge, scale):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("new,kw", [([60, 3], {"max_new": 4096, "max_kv": 10 ** 8}), ([2, 3], {}), ([15, 3], {})],
-                         ids=["chunks", "rows_of_16", "rows_of_32"])
-def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(bridge, fmt, D, new, kw):
+@pytest.mark.parametrize("new,H,kw", [([60, 3], 16, {"max_new": 16, "max_kv": 10 ** 8}),
+                                      ([60, 3], 16, {"max_new": 4096, "max_kv": 10 ** 8}), ([2, 3], 4, {}), ([15, 3], 4, {})],
+                         ids=["chunks", "both", "rows_of_16", "rows_of_32"])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(bridge, fmt, D, new, H, kw):
     """A key whose V scale is infinite reaches the rows that see it, in its 32 dims, and no other; what was never written
     (all-ones bytes: NaN scales) reaches none.  Its values are its codes times infinity, so a row's result there is an
     infinity or NaN: `infinite` takes the two alike."""
@@ -483,7 +488,7 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(bridge, fmt
         avs = s.pages._places(p % 16)[3]
         raw[1, avs[1]], raw[1, avs[1] + 1] = 0x00, 0x7C  # +inf, dims 32 .. 63 of head 1
         s.v[b][1, p, 32:64] = np.nan
-    check_attention(bridge, s, 4, infinite=True, **kw)
+    check_attention(bridge, s, H, infinite=True, **kw)
 
 
 @gpu
