@@ -573,6 +573,46 @@ def test_chunks_and_steps_of_a_growing_batch(bridge, fmt):
 
 
 @gpu
+@pytest.mark.parametrize("fmt,D", [(Q8_0, 64), (Q4_0, 128)])
+def test_captured_chunks_among_steps(bridge, fmt, D):
+    """A batch for both kernels, captured once: replays follow lengths, starts and pages that change on the device, so
+    that a sequence goes from one kernel to the other, and equal the eager calls bit for bit."""
+    import torch
+
+    H, Hkv, P = 8, 2, 16
+    s = Setup(fmt, [400, 300, 350], [90, 2, 7], Hkv, D, P, seed=31)
+    cache, q = s.cache(), dev(half(s.rng, H, s.T, D))
+    q_start, kv_len, table = dev(s.q_start), dev(np.array(s.lens, np.int32)), dev(s.table)
+    batch = m4_bridge.KVBatch(q_start, kv_len, table, 4096, 10 ** 8)
+    eager, graphed = torch.zeros_like(q), torch.zeros_like(q)
+    ws = torch.empty(bridge.paged_attn_workspace(cache, batch, H, s.T), dtype=torch.uint8, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        bridge.dispatch_paged_attn(cache, batch, q, graphed, 0.125, workspace=ws)
+    for starts, lens in (([0, 90, 92, 99], [400, 300, 350]), ([0, 3, 80, 99], [50, 290, 19]), ([0, 0, 99, 99], [7, 200, 1]),
+                         ([0, 90, 92, 95], [399, 300, 350])):
+        q_start.copy_(dev(np.array(starts, np.int32)))
+        kv_len.copy_(dev(np.array(lens, np.int32)))
+        eager.fill_(3.0)
+        graphed.fill_(3.0)
+        ws.fill_(0x7F)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        bridge.dispatch_paged_attn(cache, batch, q, eager, 0.125)
+        bridge.synchronize()
+        assert torch.equal(eager.view(torch.int16), graphed.view(torch.int16)), f"{starts} {lens}"
+        assert bool((graphed[:, starts[-1]:] == 3.0).all()) and not bool((graphed[:, :starts[-1]] == 3.0).all())
+        s.q_start, s.new = np.array(starts, np.int32), [b - a for a, b in zip(starts, starts[1:])]
+        n = starts[-1]
+        want = [np.concatenate(x, 1) for x in zip(*[
+            ref.attention(q.cpu().numpy()[:, a:a + m], k[:, :L], v[:, :L], L - m, 0, 0.125)
+            for a, m, L, k, v in zip(starts, s.new, lens, s.k, s.v)])]
+        close(graphed.cpu().numpy()[:, :n], want[0], want[1], f"replay of {starts} {lens}")
+
+
+@gpu
 @pytest.mark.parametrize("fmt,own_workspace", [(Q8_0, True), (Q4_0, False)])
 def test_captured_decoding_steps(bridge, fmt, own_workspace):
     """A step captured once and replayed as the sequences grow, with the program's own work and waits in between,
