@@ -341,7 +341,9 @@ M4_API int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch
  * sequences (their own included: append first), O [T][H][D]: query head h reads
  * KV head h / (H / Hkv); a row at position p sees keys up to p, and with `window`
  * > 0 only the last `window` of them.  A row that sees no key, or none that
- * scores above -infinity, is zero.  Any number of rows a sequence, from one
+ * scores above -infinity, is zero.  A cached value that is not finite (of a
+ * row with 65504 in it, half(127 half(65504 / 127)) is infinity) reaches its
+ * dim of the rows that see its key, and no others.  Any number of rows a sequence, from one
  * decoded token to a prompt.  `ws`: m4_bridge_paged_attn_workspace bytes of
  * device memory, 16-byte aligned, whose contents do not matter; calls that may
  * run at the same time need one each.  scale finite.  Codes as above. */

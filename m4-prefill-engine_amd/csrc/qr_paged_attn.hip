@@ -83,6 +83,44 @@ __device__ __forceinline__ h2_t q4_offset(h2_t d) {
     return d * m8;
 }
 
+// Smallest V scale (fp16 bits, without the sign) whose values may not be finite: 512,
+// -128 of which is -65536, or 8192, -8 of which is (q4_offset; past what such a cache
+// holds).  A row of fp16 reaches 516 in Q8_0: half(127 half(65504 / 127)) is infinite.
+template <int FMT>
+constexpr uint32_t kOddScale = FMT == QUANT_Q8_0 ? 0x6000u : 0x7000u;
+
+// Hidden keys have weight 0, and 0 times a value that is not finite is NaN.  Where such
+// values meet rows that do not see them, the product takes their finite part, and two
+// more, in bfloat16, add what is left out: 2^127 or -2^127 for an infinity, both for NaN,
+// times 4 for a row that sees the key, which fp32 does not hold, and times 0 for others.
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ h8_t finite_part(h8_t v) {
+    u4_t w = __builtin_bit_cast(u4_t, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t lo = (w[i] & 0x7c00u) == 0x7c00u ? 0xffff0000u : 0xffffffffu;
+        w[i] &= (w[i] & 0x7c000000u) == 0x7c000000u ? lo & 0xffffu : lo;
+    }
+    return __builtin_bit_cast(h8_t, w);
+}
+// DOWN: of -infinities, else of infinities
+template <bool DOWN>
+__device__ __forceinline__ b8_t marks_of(h8_t v) {
+    u4_t w = __builtin_bit_cast(u4_t, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 32; e += 16) {
+            const uint32_t h = w[i] >> e & 0xffffu;
+            if (h == (DOWN ? 0xfc00u : 0x7c00u) || (h & 0x7fffu) > 0x7c00u) m |= (DOWN ? 0xff00u : 0x7f00u) << e;
+        }
+        w[i] = m;
+    }
+    return __builtin_bit_cast(b8_t, w);
+}
+constexpr uint32_t kSeen = 0x4080u;  // bfloat16 4
+
 template <bool ONCE, typename T>
 __device__ __forceinline__ T load_of(const uint8_t* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
@@ -192,6 +230,25 @@ struct Tile {
     __device__ __forceinline__ h8_t k_frag(int kk) const { return k_octet<FMT>(k, kk, as_h2(kd | kd << 16)); }
     // the four keys of dim dt of the lane's run, as two pairs
     __device__ __forceinline__ u2_t v_pairs(int dt) const { return v_quad<FMT>(v, dt, vd); }
+    // of those, `y`, the ones that are not finite become zero: the codes of Q8_0 by finite
+    // scales here, the others by their scales
+    __device__ __forceinline__ void clear_odd(int dt, u2_t y) {
+        if constexpr (FMT == QUANT_Q8_0) {
+            const uint32_t h[4] = {y.x & 0x7fffu, y.x >> 16 & 0x7fffu, y.y & 0x7fffu, y.y >> 16 & 0x7fffu};
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (h[r] >= 0x7c00u) v[dt] = (v[dt] & ~(0xffu << 8 * r)) | 0x80u << 8 * r;
+        }
+    }
+    __device__ __forceinline__ void clear_scales() {
+        constexpr uint32_t least = FMT == QUANT_Q8_0 ? 0x7c00u : kOddScale<FMT>;
+        const uint32_t e[2] = {vd.x, vd.y};
+        uint32_t y[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            y[i] = ((e[i] & 0x7fffu) >= least ? 0 : e[i] & 0xffffu) | ((e[i] >> 16 & 0x7fffu) >= least ? 0 : e[i] & 0xffff0000u);
+        vd = u2_t{y[0], y[1]};
+    }
 };
 
 template <int D, int R>
@@ -426,7 +483,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         const int low_min = p.window ? (int)max((int64_t)lim_min + 1 - (int64_t)p.window, (int64_t)0) : 0;
         const int low_max = p.window ? (int)max((int64_t)lim_max + 1 - (int64_t)p.window, (int64_t)0) : 0;
 
-        uint32_t poison = 0;  // bit q: the row saw a V scale that is not finite
 #pragma unroll
         for (int q = 0; q < NR; q++) {
             m_run[q] = kNone;
@@ -462,6 +518,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         };
         auto step = [&](Tile<FMT, D> tile[2], int u) {
             const int key0 = key_base + u * (int)kStep;
+            bool odd = false;  // some row does not see all keys, and some V value may not be finite
             f4_t sc[NR][2];
 #pragma unroll
             for (int q = 0; q < NR; q++) sc[q][0] = sc[q][1] = f4_t{};
@@ -475,35 +532,18 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                         sc[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[q][kk], sc[q][t], 0, 0, 0);
                 }
             if (key0 + 31 > lim_min || key0 < low_max || key0 + 31 >= s.len || !tile[0].there || !tile[1].there) {
-                // Some row does not see some key.  What such a key's V holds must
-                // not reach that row through 0 times infinity: V scales of keys
-                // that nobody sees are cleared, and scales that are not finite
-                // are cleared and noted for the rows that do see them.
+                // Some row does not see some key.  V scales of keys that nobody sees are
+                // cleared: what was never written may be anything.
+                uint32_t large = 0;
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    uint32_t bad = 0;
                     uint32_t e[4] = {tile[t].vd.x & 0xffffu, tile[t].vd.x >> 16, tile[t].vd.y & 0xffffu, tile[t].vd.y >> 16};
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int key = key0 + 16 * t + 4 * g + r;
-                        const bool dead = !tile[t].there || key >= s.len;
-                        if (!dead && (e[r] & 0x7c00u) == 0x7c00u) bad |= 1u << r;
-                        if (dead || (bad >> r & 1)) e[r] = 0;
+                        if (!tile[t].there || key0 + 16 * t + 4 * g + r >= s.len) e[r] = 0;
+                        large = max(large, e[r] & 0x7fffu);
                     }
                     tile[t].vd = u2_t{e[0] | e[1] << 16, e[2] | e[3] << 16};
-                    if (__any(bad != 0)) {
-                        // lane (j, g) owns output dims of block g NB / 4 of its row; the scales
-                        // of block i are lanes j = i * 16 / NB's
-                        constexpr int NB = D / 32;
-                        for (int key = 0; key < 16; key++) {
-                            const uint32_t theirs = (uint32_t)__shfl((int)bad, (key >> 2) * 16 + (g * NB / 4) * (16 / NB));
-                            if (!(theirs >> (key & 3) & 1)) continue;
-                            const int at = key0 + 16 * t + key;
-#pragma unroll
-                            for (int q = 0; q < NR; q++)
-                                if (at <= lim[q] && at >= low[q]) poison |= 1u << q;
-                        }
-                    }
 #pragma unroll
                     for (int q = 0; q < NR; q++)
 #pragma unroll
@@ -512,6 +552,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                             if (!tile[t].there || key > lim[q] || key < low[q]) sc[q][t][r] = -INFINITY;
                         }
                 }
+                odd = __any(large >= kOddScale<FMT>);
             }
             h8_t pf[NR];
 #pragma unroll
@@ -553,6 +594,36 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     }
                 pf[q] = __builtin_bit_cast(h8_t, u4_t{pk[0], pk[1], pk[2], pk[3]});
             }
+            if (__builtin_expect(odd, 0)) {
+                auto seen = [&](int q) {
+                    u4_t w{};
+                    int l = lim[q] - key0, f = low[q] - key0;
+                    asm volatile("" : "+v"(l), "+v"(f));  // formed anew for each dt: kept, registers would spill
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        const int key = 16 * (x >> 2) + 4 * g + (x & 3);
+                        if (tile[x >> 2].there && key <= l && key >= f) w[x / 2] |= kSeen << (x & 1) * 16;
+                    }
+                    return __builtin_bit_cast(b8_t, w);
+                };
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    const u2_t a = tile[0].v_pairs(dt), e = tile[1].v_pairs(dt);
+                    const h8_t vf = __builtin_bit_cast(h8_t, u4_t{a.x, a.y, e.x, e.y});
+#pragma unroll
+                    for (int q = 0; q < NR; q++) {
+                        o[q][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks_of<false>(vf), seen(q), o[q][dt], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        o[q][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks_of<true>(vf), seen(q), o[q][dt], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    tile[0].clear_odd(dt, a);
+                    tile[1].clear_odd(dt, e);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                tile[0].clear_scales();
+                tile[1].clear_scales();
+            }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
                 const u2_t a = tile[0].v_pairs(dt), e = tile[1].v_pairs(dt);
@@ -570,14 +641,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             ta[0] = tb[0];
             ta[1] = tb[1];
         }
-        if (poison) {
-#pragma unroll
-            for (int q = 0; q < NR; q++)
-                if (poison >> q & 1)
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) o[q][dt] = f4_t{NAN, NAN, NAN, NAN};
-        }
-
 #pragma unroll
         for (int q = 0; q < NR; q++) {
             l_run[q] += __shfl_xor(l_run[q], 16);
@@ -773,8 +836,9 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
     constexpr int KW = FMT == QUANT_Q8_0 ? RUN / 4 : RUN / 8, VW = FMT == QUANT_Q8_0 ? DV : DV / 2;
     constexpr uint32_t CB = 4 * KW * 4, NB = D / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    __shared__ uint8_t bad_v[2][64 * NW];  // of each thread's V task: keys whose scale is not finite
-    __shared__ int there[2][NW];           // of each 16 keys: their page is one of the cache's
+    // of each 16 keys: 1, their page is one of the cache's; 2, not all rows see all keys of
+    // the tile, and some V value of these may not be finite
+    __shared__ int there[2][NW];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 5, j = lane & 31;
@@ -898,7 +962,6 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         }
         m_run = kNone;
         l_run = 0.0f;
-        uint32_t poison = 0;  // bit t: dims 32 t .. saw a V scale that is not finite
 #pragma unroll
         for (int t = 0; t < DT; t++) o[t] = f16v_t{};
 
@@ -936,24 +999,23 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
 #pragma unroll
             for (int kk = 0; kk < RUN / 8; kk++)
                 *reinterpret_cast<h8_t*>(buf + (kst ^ 16u * kk)) = k_octet<FMT>(kw, kk, d);
-            if (lane == 0) there[u & 1][wave] = mine_there || k0 + 16 * wave >= s.len;
-            uint32_t bad = 0;
+            int odd = 0;
             if (k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !mine_there) {
-                // not all rows see all of the tile's keys: V scales of keys that none sees are
-                // cleared, and those that are not finite noted for the rows that do
+                // not all rows see all of the tile's keys: V scales of keys that none sees are cleared
+                uint32_t large = 0;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t e[4] = {vd[h].x & 0xffffu, vd[h].x >> 16, vd[h].y & 0xffffu, vd[h].y >> 16};
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
-                        const bool dead = !mine_there || k0 + 16 * wave + 4 * g + 8 * h + x >= s.len;
-                        if (!dead && (e[x] & 0x7c00u) == 0x7c00u) bad |= 1u << (4 * h + x);
-                        if (dead || (bad >> (4 * h + x) & 1)) e[x] = 0;
+                        if (!mine_there || k0 + 16 * wave + 4 * g + 8 * h + x >= s.len) e[x] = 0;
+                        large = max(large, e[x] & 0x7fffu);
                     }
                     vd[h] = u2_t{e[0] | e[1] << 16, e[2] | e[3] << 16};
                 }
+                odd = __any(large >= kOddScale<FMT>) ? 2 : 0;
             }
-            bad_v[u & 1][tid] = (uint8_t)bad;
+            if (lane == 0) there[u & 1][wave] = odd | (mine_there || k0 + 16 * wave >= s.len);
 #pragma unroll
             for (int x = 0; x < DV; x++) {
                 const u2_t a = v_quad<FMT>(vw[0], x, vd[0]), e = v_quad<FMT>(vw[1], x, vd[1]);
@@ -1016,14 +1078,42 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 }
             }
         };
+        // the same where some values may not be finite, and rows do not see all keys
+        auto add_marked = [&](const uint8_t* buf, int x, const uint32_t pk[8], int u) {
+            const int key0 = lo + u * KT + 32 * x;
+#pragma unroll
+            for (int t2 = 0; t2 < 2; t2++) {
+                const h8_t pf = __builtin_bit_cast(h8_t, u4_t{pk[4 * t2], pk[4 * t2 + 1], pk[4 * t2 + 2], pk[4 * t2 + 3]});
+                u4_t seen{};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + 16 * t2 + 8 * (e >> 2) + 4 * g + (e & 3);
+                    if ((there[u & 1][2 * x + t2] & 1) && key <= lim && key >= low) seen[e / 2] |= kSeen << (e & 1) * 16;
+                }
+                const b8_t sf = __builtin_bit_cast(b8_t, seen);
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+                    const h8_t va = *reinterpret_cast<const h8_t*>(buf + KB + t * 32 * (VU * 16) + (vof ^ 32u * (2 * x + t2)));
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(marks_of<false>(va), sf, o[t], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(marks_of<true>(va), sf, o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_part(va), pf, o[t], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        };
         auto attend = [&](int u) {
             const uint8_t* buf = smem + (u & 1) * TB;
             asm volatile("" : "+v"(kof), "+v"(vof));
             const int k0 = lo + u * KT;
             if (!wave_live || k0 > lim1 || k0 + KT - 1 < low0) return;
-            bool all_there = true;
+            int every = 1, some = 0;
 #pragma unroll
-            for (int x = 0; x < NW; x++) all_there &= there[u & 1][x] != 0;
+            for (int x = 0; x < NW; x++) {
+                every &= there[u & 1][x];
+                some |= there[u & 1][x];
+            }
+            const bool all_there = every & 1;
             if (!(k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !all_there)) {
                 // every row sees every key.  Each line below ends at a barrier for the scheduler:
                 // one MFMA, the loads of operands four MFMAs ahead, and the vector work that
@@ -1097,36 +1187,31 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 }
                 return;
             }
-            uint32_t any = 0;
-#pragma unroll
-            for (int x = 0; x < NW; x++) any |= bad_v[u & 1][64 * x + lane];
-            if (__any(any != 0)) {
-                for (int x = 0; x < 64 * NW; x++) {
-                    const uint32_t bits = bad_v[u & 1][x];
-                    for (int e = 0; e < 8; e++) {
-                        const int key = k0 + 16 * (x >> 6) + 4 * (x >> 5 & 1) + (e >> 2) * 8 + (e & 3);
-                        if ((bits >> e & 1) && key <= lim && key >= low) poison |= 1u << ((x & 31) * DV / 32);
-                    }
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < UNITS; x++) {
+            auto unit = [&](int x, bool marks) {
                 const int key0 = k0 + 32 * x;
-                if (key0 > lim1 || key0 + 31 < low0) continue;
+                if (key0 > lim1 || key0 + 31 < low0) return;
                 f16v_t sc = scores(buf, x);
                 if (key0 + 31 > lim0 || key0 < low1 || !all_there) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const int key = key0 + 8 * (e >> 2) + 4 * g + (e & 3);
-                        if (key > lim || key < low || !there[u & 1][2 * x + (e >> 3)]) sc[e] = -INFINITY;
+                        if (key > lim || key < low || !(there[u & 1][2 * x + (e >> 3)] & 1)) sc[e] = -INFINITY;
                     }
                 }
                 float ex[16];
                 exponents(sc, ex);
                 uint32_t pk[8];
                 weigh(ex, pk);
-                add(buf, x, pk);
+                if (marks) add_marked(buf, x, pk, u);
+                else add(buf, x, pk);
+            };
+            if (__builtin_amdgcn_readfirstlane(some) & 2) {
+#pragma unroll 1
+                for (int x = 0; x < UNITS; x++) unit(x, true);
+                return;
             }
+#pragma unroll
+            for (int x = 0; x < UNITS; x++) unit(x, false);
         };
 
         fetch(u0);
@@ -1141,13 +1226,6 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         }
 
         l_run += __shfl_xor(l_run, 32);
-        if (poison) {
-#pragma unroll
-            for (int t = 0; t < DT; t++)
-                if (poison >> t & 1)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[t][e] = NAN;
-        }
         // lane (j, g): row 32 wave + j, dims 32 t + 8 (e / 4) + 4 g + e % 4
         if (begun && ends) {
             if (r < rows) {

@@ -1,0 +1,75 @@
+"""The serving operators at the limits of what a batch and its cache may hold.  References and their bounds are those of
+paged_reference.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import m4_bridge
+import paged_reference as ref
+from paged_reference import Q8_0
+from test_paged import FORMATS, Setup, close, dev, half, say
+
+gpu = pytest.mark.gpu
+
+# what is expected of the lengths chooses the kernels: for 8 query heads a KV head, rows alone, chunks alone (no window,
+# and rows enough for 16 tokens of each sequence) and sequences of 16 tokens and more on the one, the others on the other
+KERNELS = {"rows": {"max_new": 1, "max_kv": 1}, "chunks": {"max_new": 16, "max_kv": 10 ** 8},
+           "both": {"max_new": 2 ** 31 - 1, "max_kv": 10 ** 8}}
+
+
+def takes(bridge, cache, batch, H, T, window):
+    """The kernels of a call, by the workspace that they need: of a group of workgroups two row tiles and 32 bytes."""
+    D = cache.D
+    ws = bridge.paged_attn_workspace(cache, batch, H, T, window)
+    tile = lambda rows: 32 + 2 * rows * (D + 2) * 4  # noqa: E731
+    few = [a for a in (16, 32) if ws % tile(a) == 0 and ws // tile(a) <= 512]
+    if ws % tile(256) == 0 and ws // tile(256) <= 256:
+        return "chunks"
+    return "rows" if few else "both"
+
+
+def attend(bridge, s, q, starts, lens, window, kernels):
+    """The call's results [H, T, D] over s's cache, for starts and lengths given apart."""
+    import torch
+
+    H, T, D = q.shape
+    cache = s.cache()
+    batch = m4_bridge.KVBatch(dev(np.array(starts, np.int32)), dev(np.array(lens, np.int32)), dev(s.table), **KERNELS[kernels])
+    assert takes(bridge, cache, batch, H, T, window) == kernels
+    O = torch.full((H, T, D), 6.0, dtype=torch.float16, device="cuda")
+    say("paged limits", s.fmt, starts, lens, H, s.Hkv, D, s.P, window, kernels)
+    bridge.dispatch_paged_attn(cache, batch, dev(q), O, D ** -0.5, window=window)
+    bridge.synchronize()
+    return O.cpu().numpy()
+
+
+# ---- values that are not finite -----------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,kernels,new", [
+    (0, "rows", [2, 5, 1]), (0, "rows", [40, 20, 30]), (0, "chunks", [40, 20, 30]), (0, "both", [40, 20, 3]),
+    (20, "rows", [2, 5, 1]), (20, "rows", [40, 20, 30]), (20, "both", [40, 20, 3])])
+def test_largest_values_stay_with_the_rows_that_see_them(bridge, fmt, D, window, kernels, new):
+    """V rows of +-65504, finite in fp16, whose Q8_0 value half(127 half(65504 / 127)) is infinite: rows that see the key
+    get what that gives in its dim and finite results in the 31 that share its scale; the others do not notice."""
+    s = Setup(fmt, [100, 60, 75], new, 2, D, 16, seed=40)
+    big = {0: [(70, 1, 33, 65504), (99, 0, 5, -65504), (83, 1, 2, 65504), (84, 1, 2, -65504)], 1: [(58, 0, D - 1, -65504), (30, 1, 0, 65504)],
+           2: [(74, 0, 40, 65504)]}
+    for b, places in big.items():
+        for p, h, dim, x in places:
+            v = half(s.rng, s.Hkv, D)
+            v[h, dim] = x
+            k = half(s.rng, s.Hkv, D)
+            (kq, kd), (vq, vd) = ref.quantize(fmt, k), ref.quantize(fmt, v)
+            s.pages.write(s.table[b, p // 16], p % 16, kq, kd, vq, vd)
+            s.k[b][:, p], s.v[b][:, p] = ref.values(kq, kd), ref.values(vq, vd)
+            assert np.isinf(s.v[b][h, p, dim]) == (fmt == Q8_0)
+    q = half(s.rng, 16, s.T, D)
+    got = attend(bridge, s, q, s.q_start, s.lens, window, kernels)
+    if fmt == Q8_0:  # the last rows of two sequences
+        assert (got[:8, s.q_start[3] - 1, 40] == np.inf).all() and (got[:8, s.q_start[2] - 1, D - 1] == -np.inf).all()
+    got = np.where(np.isfinite(got), got, np.float16("nan"))  # an infinity or, of two, NaN: taken alike
+    close(got, *s.expected(q, window, D ** -0.5), "largest values")
