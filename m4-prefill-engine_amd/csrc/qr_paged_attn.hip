@@ -284,7 +284,8 @@ __device__ __forceinline__ void share_of(uint64_t total, uint32_t nw, uint32_t w
 }
 
 struct Seq {
-    int q0, n, len, lo;   // first row, new tokens, keys, first key that any row sees (a multiple of kStep)
+    int q0, n, first;     // first row, new tokens, position of the first of them
+    int keys, lo;         // keys that the table holds and a row may see, first that one sees (a multiple of kStep)
     uint32_t tiles, steps;  // row tiles and key steps per tile
     uint64_t cost;
 };
@@ -295,12 +296,15 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
     s.q0 = min(max(p.batch.q_start[b], 0), T);
     s.n = max(min(max(p.batch.q_start[b + 1], 0), T) - s.q0, 0);
     if ((uint32_t)s.n * p.G < p.min_rows || (uint32_t)s.n * p.G >= p.max_rows) s.n = 0;  // another launch's
-    s.len = min(max(p.batch.kv_len[b], 0), cap);
+    // a sequence may be longer than its row of the table: its tokens have the positions
+    // that its length gives them, its keys end where the table does
+    s.first = max(p.batch.kv_len[b], 0) - s.n;
+    s.keys = min(max(s.first + s.n, 0), cap);
     s.lo = 0;
-    if (p.window) s.lo = (int)(max((int64_t)s.len - s.n + 1 - (int64_t)p.window, (int64_t)0) / kStep * kStep);
+    if (p.window) s.lo = (int)min(max((int64_t)s.first + 1 - (int64_t)p.window, (int64_t)0), (int64_t)s.keys) / (int)kStep * (int)kStep;
     const uint32_t G = p.G;
     s.tiles = (uint32_t)(((uint64_t)s.n * G + R - 1) / R);
-    s.steps = max((uint32_t)(s.len - s.lo + (int)kStep - 1) / kStep, 1u);
+    s.steps = max((uint32_t)(s.keys - s.lo + (int)kStep - 1) / kStep, 1u);
     s.cost = (uint64_t)p.geom.Hkv * s.tiles * (kItemCost + s.steps);
     return s;
 }
@@ -434,7 +438,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         if (per == 1) {
             s.q0 = __builtin_amdgcn_readlane(held.q0, b);
             s.n = __builtin_amdgcn_readlane(held.n, b);
-            s.len = __builtin_amdgcn_readlane(held.len, b);
+            s.first = __builtin_amdgcn_readlane(held.first, b);
+            s.keys = __builtin_amdgcn_readlane(held.keys, b);
             s.lo = __builtin_amdgcn_readlane(held.lo, b);
             s.tiles = __builtin_amdgcn_readlane(held.tiles, b);
             s.steps = __builtin_amdgcn_readlane(held.steps, b);
@@ -457,9 +462,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         const uint32_t u0 = o0 > kItemCost ? o0 - kItemCost : 0, nu = o1 - kItemCost - u0;
         hk = s.tiles == 1 ? item : item / s.tiles;
         rt = item - hk * s.tiles;
-        const int p0 = s.len - s.n;  // position of the first new token
 
-        // ---- rows ----
+        // ---- rows: the last key that each sees (none behind the table), and the first ----
+        auto last_seen = [&](int i) { return min(s.first + i, s.keys - 1); };
+        auto first_seen = [&](int i) { return p.window ? (int)max((int64_t)s.first + i + 1 - (int64_t)p.window, (int64_t)0) : 0; };
         rows = min(R, (uint32_t)s.n * G - rt * R);
         const int i_first = (int)(rt * R / G), i_last = (int)((rt * R + rows - 1) / G);
         int lim[NR], low[NR];
@@ -470,8 +476,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             const uint32_t f = rt * R + min(r, rows - 1);
             const int i = (int)(f / G);
             const uint32_t h = hk * G + f % G;
-            lim[q] = p0 + i;
-            low[q] = p.window ? (int)max((int64_t)lim[q] + 1 - (int64_t)p.window, (int64_t)0) : 0;
+            lim[q] = last_seen(i);
+            low[q] = first_seen(i);
             const _Float16* src = p.Q.p + (int64_t)(s.q0 + i) * p.Q.ts + (int64_t)h * p.Q.hs + g * RUN;
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
@@ -479,9 +485,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                 if (neg) qf[q][kk] = -qf[q][kk];
             }
         }
-        const int lim_min = p0 + i_first, lim_max = p0 + i_last;
-        const int low_min = p.window ? (int)max((int64_t)lim_min + 1 - (int64_t)p.window, (int64_t)0) : 0;
-        const int low_max = p.window ? (int)max((int64_t)lim_max + 1 - (int64_t)p.window, (int64_t)0) : 0;
+        const int lim_min = last_seen(i_first), lim_max = last_seen(i_last);
+        const int low_min = first_seen(i_first), low_max = first_seen(i_last);
 
 #pragma unroll
         for (int q = 0; q < NR; q++) {
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             if (u >= ids_from + 32) {
                 ids_from = u;
                 const int k0 = key_base + (u + (lane >> 1)) * (int)kStep + 16 * (lane & 1);
-                page_ids = k0 < s.len ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k0 >> p.geom.log2_page)]
+                page_ids = k0 < s.keys ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k0 >> p.geom.log2_page)]
                                       : 0xffffffffu;
             }
             const int key0 = key_base + u * (int)kStep;
@@ -531,7 +536,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     for (int q = 0; q < NR; q++)
                         sc[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[q][kk], sc[q][t], 0, 0, 0);
                 }
-            if (key0 + 31 > lim_min || key0 < low_max || key0 + 31 >= s.len || !tile[0].there || !tile[1].there) {
+            if (key0 + 31 > lim_min || key0 < low_max || !tile[0].there || !tile[1].there) {
                 // Some row does not see some key.  V scales of keys that nobody sees are
                 // cleared: what was never written may be anything.
                 uint32_t large = 0;
@@ -540,7 +545,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     uint32_t e[4] = {tile[t].vd.x & 0xffffu, tile[t].vd.x >> 16, tile[t].vd.y & 0xffffu, tile[t].vd.y >> 16};
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        if (!tile[t].there || key0 + 16 * t + 4 * g + r >= s.len) e[r] = 0;
+                        if (!tile[t].there || key0 + 16 * t + 4 * g + r >= s.keys) e[r] = 0;
                         large = max(large, e[r] & 0x7fffu);
                     }
                     tile[t].vd = u2_t{e[0] | e[1] << 16, e[2] | e[3] << 16};
@@ -810,9 +815,9 @@ struct Chunk {
 // Steps (key tiles of KT) of row tile rt, and its first key.
 template <int KT>
 __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq& s, uint32_t tokens, uint32_t rt, int& lo) {
-    const int first = s.len - s.n + (int)(rt * tokens);
-    const int end = min(first + (int)tokens, s.len);
-    lo = p.window ? (int)(max((int64_t)first + 1 - (int64_t)p.window, (int64_t)0) / KT * KT) : 0;
+    const int64_t first = (int64_t)s.first + rt * tokens;
+    const int end = (int)min(first + tokens, (int64_t)s.keys);
+    lo = p.window ? (int)min(max(first + 1 - (int64_t)p.window, (int64_t)0), (int64_t)s.keys) / KT * KT : 0;
     return end <= lo ? 1u : (uint32_t)(end - lo + KT - 1) / KT;
 }
 
@@ -940,16 +945,19 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
 
         // ---- rows ----
         const uint32_t rows = min(tokens * G, ((uint32_t)s.n - rt * tokens) * G);
-        const int p0 = s.len - s.n + (int)(rt * tokens);  // position of the tile's first token
+        const int i0 = (int)(rt * tokens);  // the tile's first token
         const uint32_t r = 32 * wave + j, rc = min(r, rows - 1);
         const bool wave_live = 32u * wave < rows;
-        const int lim = p0 + (int)(rc / G);
-        const int low = p.window ? (int)max((int64_t)lim + 1 - (int64_t)p.window, (int64_t)0) : 0;
+        // the last key that a row sees (none behind the table), and the first
+        auto last_seen = [&](uint32_t r) { return min(s.first + i0 + (int)(r / G), s.keys - 1); };
+        auto first_seen = [&](uint32_t r) {
+            return p.window ? (int)max((int64_t)s.first + i0 + (int)(r / G) + 1 - (int64_t)p.window, (int64_t)0) : 0;
+        };
+        const int lim = last_seen(rc), low = first_seen(rc);
         // of this wave's rows, and of all
-        const int lim0 = p0 + (int)(min(32u * wave, rows - 1) / G), lim1 = p0 + (int)(min(32u * wave + 31, rows - 1) / G);
-        const int all0 = p0, all1 = p0 + (int)((rows - 1) / G);
-        auto lowest = [&](int l) { return p.window ? (int)max((int64_t)l + 1 - (int64_t)p.window, (int64_t)0) : 0; };
-        const int low0 = lowest(lim0), low1 = lowest(lim1), all_low1 = lowest(all1);
+        const uint32_t r0 = min(32u * wave, rows - 1), r1 = min(32u * wave + 31, rows - 1);
+        const int lim0 = last_seen(r0), lim1 = last_seen(r1), low0 = first_seen(r0), low1 = first_seen(r1);
+        const int all0 = last_seen(0), all_low1 = first_seen(rows - 1);
         h8_t qf[KK];
         {
             const _Float16* src = p.Q.p + (int64_t)(s.q0 + (int)(rt * tokens + rc / G)) * p.Q.ts +
@@ -975,7 +983,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             if (u >= ids_from + 64) {
                 ids_from = u;
                 const int k0 = lo + (u + lane) * KT + 16 * wave;
-                page_ids = k0 < s.len ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k0 >> p.geom.log2_page)]
+                page_ids = k0 < s.keys ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k0 >> p.geom.log2_page)]
                                       : 0xffffffffu;
             }
             const uint32_t page = __builtin_amdgcn_readlane(page_ids, u - ids_from);
@@ -1000,7 +1008,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             for (int kk = 0; kk < RUN / 8; kk++)
                 *reinterpret_cast<h8_t*>(buf + (kst ^ 16u * kk)) = k_octet<FMT>(kw, kk, d);
             int odd = 0;
-            if (k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !mine_there) {
+            if (k0 + KT - 1 > all0 || k0 < all_low1 || !mine_there) {
                 // not all rows see all of the tile's keys: V scales of keys that none sees are cleared
                 uint32_t large = 0;
 #pragma unroll
@@ -1008,14 +1016,14 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                     uint32_t e[4] = {vd[h].x & 0xffffu, vd[h].x >> 16, vd[h].y & 0xffffu, vd[h].y >> 16};
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
-                        if (!mine_there || k0 + 16 * wave + 4 * g + 8 * h + x >= s.len) e[x] = 0;
+                        if (!mine_there || k0 + 16 * wave + 4 * g + 8 * h + x >= s.keys) e[x] = 0;
                         large = max(large, e[x] & 0x7fffu);
                     }
                     vd[h] = u2_t{e[0] | e[1] << 16, e[2] | e[3] << 16};
                 }
                 odd = __any(large >= kOddScale<FMT>) ? 2 : 0;
             }
-            if (lane == 0) there[u & 1][wave] = odd | (mine_there || k0 + 16 * wave >= s.len);
+            if (lane == 0) there[u & 1][wave] = odd | (mine_there || k0 + 16 * wave >= s.keys);
 #pragma unroll
             for (int x = 0; x < DV; x++) {
                 const u2_t a = v_quad<FMT>(vw[0], x, vd[0]), e = v_quad<FMT>(vw[1], x, vd[1]);
@@ -1114,7 +1122,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 some |= there[u & 1][x];
             }
             const bool all_there = every & 1;
-            if (!(k0 + KT - 1 > all0 || k0 < all_low1 || k0 + KT > s.len || !all_there)) {
+            if (!(k0 + KT - 1 > all0 || k0 < all_low1 || !all_there)) {
                 // every row sees every key.  Each line below ends at a barrier for the scheduler:
                 // one MFMA, the loads of operands four MFMAs ahead, and the vector work that
                 // runs beside it -- a unit's exponentials beside the next one's scores (the

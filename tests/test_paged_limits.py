@@ -73,3 +73,25 @@ def test_largest_values_stay_with_the_rows_that_see_them(bridge, fmt, D, window,
         assert (got[:8, s.q_start[3] - 1, 40] == np.inf).all() and (got[:8, s.q_start[2] - 1, D - 1] == -np.inf).all()
     got = np.where(np.isfinite(got), got, np.float16("nan"))  # an infinity or, of two, NaN: taken alike
     close(got, *s.expected(q, window, D ** -0.5), "largest values")
+
+
+# ---- lengths past the table and starts past the rows ---------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,kernels,new", [
+    (0, "rows", [5, 3, 2]), (0, "rows", [40, 3, 30]), (0, "chunks", [40, 3, 30]), (0, "both", [40, 3, 30]),
+    (9, "rows", [5, 3, 2]), (37, "rows", [40, 3, 30]), (9, "both", [40, 3, 30]), (37, "both", [40, 3, 30])])
+@pytest.mark.parametrize("past", [1, 2, 30, 2 ** 31 - 1 - 160])
+def test_lengths_past_the_table(bridge, fmt, D, window, kernels, new, past):
+    """A sequence that is longer than its row of the table: its tokens keep their positions, and see those keys of theirs
+    that the table holds."""
+    s = Setup(fmt, [160, 40, 160], new, 2, D, 16, seed=41)
+    assert s.table.shape[1] * 16 == 160
+    lens = [160 + past, 40, 160 + min(past, 5)]
+    q = half(s.rng, 16, s.T, D)
+    got = attend(bridge, s, q, s.q_start, lens, window, kernels)
+    for b, (a, n, L) in enumerate(zip(s.q_start, new, lens)):
+        want, bound = ref.attention(q[:, a:a + n], s.k[b], s.v[b], L - n, window, D ** -0.5)
+        close(got[:, a:a + n], want, bound, f"sequence {b} of {L}")
