@@ -267,7 +267,8 @@ typedef struct {
  * a row used).  All three are device memory, read by the kernels: entries out
  * of range (a page that is not there, more keys than the table holds, a
  * negative position, rows past T) are never followed -- such a token is not
- * written and not seen, and the others keep the positions that this gives them.
+ * written and not seen, and the others keep the positions that this gives them
+ * (a start below 0 or past T counts rows that the call does not have).
  * Rows behind the last sequence are left as they are.
  * Two tokens of a call that fall on one place of the cache leave it undefined.
  * max_new and max_kv are what the caller expects of the longest sequence: they

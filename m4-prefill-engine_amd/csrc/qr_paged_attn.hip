@@ -294,11 +294,12 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
     const int T = (int)p.batch.T;
     const int cap = (int)min((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)0x7fff0000);  // a stretch of pages on top fits
     s.q0 = min(max(p.batch.q_start[b], 0), T);
-    s.n = max(min(max(p.batch.q_start[b + 1], 0), T) - s.q0, 0);
+    const int end = p.batch.q_start[b + 1];  // past T: its last rows are not there
+    s.n = max(min(max(end, 0), T) - s.q0, 0);
     if ((uint32_t)s.n * p.G < p.min_rows || (uint32_t)s.n * p.G >= p.max_rows) s.n = 0;  // another launch's
     // a sequence may be longer than its row of the table: its tokens have the positions
     // that its length gives them, its keys end where the table does
-    s.first = max(p.batch.kv_len[b], 0) - s.n;
+    s.first = s.n ? max(p.batch.kv_len[b], 0) - (end - s.q0) : 0;
     s.keys = min(max(s.first + s.n, 0), cap);
     s.lo = 0;
     if (p.window) s.lo = (int)min(max((int64_t)s.first + 1 - (int64_t)p.window, (int64_t)0), (int64_t)s.keys) / (int)kStep * (int)kStep;

@@ -38,7 +38,7 @@ __device__ __forceinline__ Place place_of(const BatchView& bv, const PageGeom& g
     const uint32_t t = t0 + sub;
     if (before == 0 || t >= bv.T) return r;
     const uint32_t b = before - 1;
-    const int end = min(bv.q_start[b + 1], (int)bv.T), len = max(bv.kv_len[b], 0);
+    const int end = bv.q_start[b + 1], len = max(bv.kv_len[b], 0);  // an end past T: rows that are not there
     if ((int)t >= end) return r;
     r.pos = len - (end - (int)t);
     if (r.pos < 0) return r;

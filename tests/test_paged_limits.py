@@ -95,3 +95,40 @@ def test_lengths_past_the_table(bridge, fmt, D, window, kernels, new, past):
     for b, (a, n, L) in enumerate(zip(s.q_start, new, lens)):
         want, bound = ref.attention(q[:, a:a + n], s.k[b], s.v[b], L - n, window, D ** -0.5)
         close(got[:, a:a + n], want, bound, f"sequence {b} of {L}")
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("window,kernels", [(0, "rows"), (0, "chunks"), (0, "both"), (9, "rows"), (9, "both")])
+@pytest.mark.parametrize("before,past", [(0, 1), (3, 7), (40, 200), (2 ** 31, 2 ** 31 - 1 - 72)])
+def test_starts_past_the_rows(bridge, fmt, window, kernels, before, past):
+    """Starts below zero and past T stand for rows that a call does not have.  Those that it has keep their positions,
+    kv_len less the rows from them to the sequence's end, wherever they are written, read and attended."""
+    import torch
+
+    D, P = 64, 16
+    s = Setup(fmt, [90, 130, 300], [30, 12, 30], 2, D, P, seed=42)
+    starts = [-before, 30, 42, 72 + past]
+    first = [60, 118, 300 - 30 - past]  # positions of the first rows that are there
+    q = half(s.rng, 16, s.T, D)
+    got = attend(bridge, s, q, starts, s.lens, window, kernels)
+    for b, (a, n, p0) in enumerate(zip(s.q_start, s.new, first)):
+        want, bound = ref.attention(q[:, a:a + n], s.k[b], s.v[b], p0, window, D ** -0.5)
+        close(got[:, a:a + n], want, bound, f"sequence {b}")
+    cache = s.cache()
+    batch = m4_bridge.KVBatch(dev(np.array(starts, np.int32)), dev(np.array(s.lens, np.int32)), dev(s.table), **KERNELS[kernels])
+    k, v = half(s.rng, s.T, 2, D), half(s.rng, s.T, 2, D)
+    bridge.kv_cache_append(cache, batch, dev(k), dev(v), token_major=True)
+    ko, vo = (torch.full((s.T, 2, D), 3.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    bridge.kv_cache_read(cache, batch, ko, vo, token_major=True)
+    bridge.synchronize()
+    (kq, kd), (vq, vd) = ref.quantize(fmt, k), ref.quantize(fmt, v)
+    ek, ev = np.full((s.T, 2, D), 3, np.float16), np.full((s.T, 2, D), 3, np.float16)
+    for b, (a, n, p0) in enumerate(zip(s.q_start, s.new, first)):
+        for i in range(n):
+            if p0 + i >= 0:
+                s.pages.write(s.table[b, (p0 + i) // P], (p0 + i) % P, kq[a + i], kd[a + i], vq[a + i], vd[a + i])
+                ek[a + i], ev[a + i] = s.pages.read(s.table[b, (p0 + i) // P], (p0 + i) % P)
+    np.testing.assert_array_equal(cache.pages.cpu().numpy(), s.pages.raw)
+    np.testing.assert_array_equal(ko.cpu().numpy().view(np.uint16), ek.view(np.uint16))
+    np.testing.assert_array_equal(vo.cpu().numpy().view(np.uint16), ev.view(np.uint16))
