@@ -315,7 +315,8 @@ M4_API int m4_bridge_rope_axes_table(const double* inv_freq, const uint8_t* pair
 M4_API size_t m4_bridge_kv_cache_bytes(int format, uint32_t num_pages, uint32_t page_size, uint32_t Hkv, uint32_t D);
 
 /* Rotates the rows X [T][H][D] (D % 8 == 0, at most 256) into Y, which may be X
- * itself; positions int32 [axes][position_stride].  Codes: -1, -2 (null,
+ * itself; positions int32 [axes][position_stride], a stride of 0 for one row
+ * that all axes read.  Codes: -1, -2 (null,
  * misaligned, short or not device memory), -4 (dims, strides), -6.  T = 0 is 0. */
 M4_API int m4_bridge_rope_axes(const m4_rope_axes_t* rope, const int32_t* positions, uint32_t position_stride,
                                const m4_rows_t* X, const m4_rows_t* Y, uint32_t T, uint32_t H, uint32_t D);

@@ -161,9 +161,10 @@ int check_rope(const m4_rope_axes_t* r, uint32_t D) {
     return 0;
 }
 
+// A stride of 0 is one row for all axes, as text has.
 int check_positions(const int32_t* positions, uint32_t stride, uint32_t axes, uint32_t T) {
     if (misaligned(positions, 4)) return -2;
-    return axes > 1 && stride < T ? -4 : 0;
+    return axes > 1 && stride != 0 && stride < T ? -4 : 0;
 }
 
 }  // namespace

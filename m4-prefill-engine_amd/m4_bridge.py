@@ -663,7 +663,7 @@ class HIPBridge:
         return (ptr, held, ts, hs), T, H, t
 
     def _positions(self, positions: Any, rope: "RotaryAxes", T: int) -> tuple:
-        """(pointer, stride) of int32 positions [T] or [axes, T]."""
+        """(pointer, stride) of int32 positions [T] or [axes, T], expanded over the axes (stride 0) included."""
         if positions is None:
             return None, 0
         shape = positions.shape

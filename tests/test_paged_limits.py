@@ -132,3 +132,41 @@ def test_starts_past_the_rows(bridge, fmt, window, kernels, before, past):
     np.testing.assert_array_equal(cache.pages.cpu().numpy(), s.pages.raw)
     np.testing.assert_array_equal(ko.cpu().numpy().view(np.uint16), ek.view(np.uint16))
     np.testing.assert_array_equal(vo.cpu().numpy().view(np.uint16), ev.view(np.uint16))
+
+
+# ---- positions that repeat ------------------------------------------------------------------------------------------
+
+def test_positions_of_all_axes_may_be_one_row(libpath):
+    """A stride of 0: every axis reads the same positions.  Other strides below the number of tokens stay refused."""
+    import ctypes
+
+    lib, T = m4_bridge.load_library(libpath), 10
+    rows = m4_bridge.RowsStruct(0x300000, 8 * T * 128 * 2, 128, T * 128)
+    rope = m4_bridge.RopeAxesStruct(64, 3, 0, 0x500000, 64 * 12)
+    cache = m4_bridge.KVCacheStruct(0x100000, 4 * 16 * 2 * 2 * 4 * 34, 6, 4, 16, 2, 128)
+    batch = m4_bridge.KVBatchStruct(2, 0x1000, 0x2000, 0x3000, 4, 4, 5, 60)
+    r = ctypes.addressof
+    for stride, code in ((0, 0), (1, -4), (T - 1, -4), (T, 0)):
+        assert lib.m4_bridge_validate_rope_axes(r(rope), 0x4000, stride, r(rows), r(rows), T, 8, 128) == code
+        assert lib.m4_bridge_validate_kv_cache_append(r(cache), r(batch), T, r(rows), r(rows), r(rope), 0x4000, stride, r(rows),
+                                                      r(rows), 8) == code
+
+
+@gpu
+def test_expanded_positions_are_repeated_ones(bridge):
+    """Text positions expanded over the axes, as they stand, alone and beside an append."""
+    import torch
+
+    s = Setup(Q8_0, [70, 9], [41, 9], 2, 64, 16, seed=43)
+    rope = m4_bridge.RotaryAxes(64, sections=(8, 12, 12))
+    text = torch.arange(1000, 1000 + s.T, dtype=torch.int32, device="cuda")
+    q, k = dev(half(s.rng, 4, s.T, 64)), dev(half(s.rng, 2, s.T, 64))
+    results = []
+    for positions in (text.expand(3, s.T), text.repeat(3, 1)):
+        y, qo, cache = torch.empty_like(q), torch.empty_like(q), s.cache()
+        bridge.rope_axes(q, y, rope, positions)
+        bridge.kv_cache_append(cache, s.batch(), k, k, rope=rope, positions=positions, Q=q, Q_out=qo)
+        bridge.synchronize()
+        results.append((y, qo, cache.pages))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*results))
+    assert not torch.equal(results[0][0], q)
