@@ -690,7 +690,7 @@ class HIPBridge:
         at = ctypes.addressof(rows)
         ret = self._lib.m4_bridge_rope_axes(rope.on(X.device), pos, stride, at, at + _ROWS, T, H, X.shape[2])
         self._check("m4_bridge_rope_axes", ret)
-        self._in_flight_tensors.append((X, Y, positions))
+        self._in_flight_tensors.append((X, Y, rope, positions))
         return ret
 
     def kv_cache_append(self, cache: PagedKVCache, batch: KVBatch, K, V, rope: Optional[RotaryAxes] = None,
@@ -723,7 +723,7 @@ class HIPBridge:
                                                   rope.on(K.device) if rope is not None else None, pos, stride, at_q,
                                                   at_qo, H)
         self._check("m4_bridge_kv_cache_append", ret)
-        self._in_flight_tensors.append((cache, batch, K, V, Q, Q_out, positions))
+        self._in_flight_tensors.append((cache, batch, K, V, rope, Q, Q_out, positions))
         return ret
 
     def kv_cache_read(self, cache: PagedKVCache, batch: KVBatch, K, V, token_major: bool = False) -> int:
@@ -757,6 +757,7 @@ class HIPBridge:
         if not 0 <= window < 1 << 32:
             raise ValueError(f"window={window}")
         self._on_stream_of(Q)
+        given = workspace  # one made here goes back to the stream that the kernels are on, behind them
         if workspace is None:
             workspace = _torch.empty(self.paged_attn_workspace(cache, batch, H, T, window), dtype=_torch.uint8,
                                      device=Q.device)
@@ -765,7 +766,7 @@ class HIPBridge:
         ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, T, at, at + _ROWS, H, float(scale), window,
                                                       workspace.data_ptr(), workspace.nbytes)
         self._check("m4_bridge_dispatch_paged_attn", ret)
-        self._in_flight_tensors.append((cache, batch, Q, O))
+        self._in_flight_tensors.append((cache, batch, Q, O, given))
         return ret
 
     def paged_layer(self, X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, X_out, format, d_model, Hq, N_mlp, attn_scale,
@@ -788,7 +789,7 @@ class HIPBridge:
                                               d_model, Hq, N_mlp, float(attn_scale), window, int(norm_type),
                                               float(norm_eps))
         self._check("m4_bridge_paged_layer", ret)
-        self._in_flight_tensors.append((*bufs, cache, batch, positions))
+        self._in_flight_tensors.append((*bufs, cache, batch, rope, positions))
         return ret
 
     def dequantize(self, W, out, format, K, N) -> int:

@@ -170,3 +170,75 @@ def test_expanded_positions_are_repeated_ones(bridge):
         results.append((y, qo, cache.pages))
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*results))
     assert not torch.equal(results[0][0], q)
+
+
+# ---- what a call holds, and the workspace that it takes ---------------------------------------------------------------
+
+class Launched:
+    """The library, but for the calls that need a device, which launch nothing and succeed."""
+
+    def __init__(self, lib):
+        self._lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        if name in ("m4_bridge_rope_axes", "m4_bridge_kv_cache_append", "m4_bridge_dispatch_paged_attn", "m4_bridge_paged_layer",
+                    "m4_bridge_synchronize"):
+            self.calls.append(name)
+            return lambda *a: 0
+        return getattr(self._lib, name)
+
+
+@pytest.fixture
+def launched(libpath, monkeypatch):
+    b = m4_bridge.HIPBridge.get_instance(libpath)
+    lib = Launched(b.lib)
+    monkeypatch.setattr(b, "_lib", lib)
+    monkeypatch.setattr(b, "_in_flight_tensors", [])
+    yield b
+
+
+def host_batch():
+    import torch
+
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    return (m4_bridge.PagedKVCache(Q8_0, 4, 16, 2, 64, device="cpu"), m4_bridge.KVBatch(i32(3), i32(2), i32(2, 4), 1, 64))
+
+
+@pytest.mark.parametrize("call", ["rope_axes", "append", "layer", "attention"])
+def test_rotary_tables_and_workspaces_are_held(launched, call):
+    """Until synchronize(), as the tensors of a call are: a table or workspace that the caller lets go of while the kernel
+    waits would go back to its stream's memory."""
+    import weakref
+
+    import torch
+
+    cache, batch = host_batch()
+    rope, ws = m4_bridge.RotaryAxes(64), torch.zeros(1 << 20, dtype=torch.uint8)
+    x, positions = torch.zeros(2, 3, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32)
+    held = weakref.ref(ws if call == "attention" else rope)
+    if call == "rope_axes":
+        launched.rope_axes(x, x, rope, positions)
+    elif call == "append":
+        launched.kv_cache_append(cache, batch, x, x, rope=rope)
+    elif call == "layer":
+        X, W = torch.zeros(3, 256, dtype=torch.float16), torch.zeros(64, dtype=torch.uint8)
+        launched.paged_layer(X, None, *[W] * 4, None, *[W] * 3, X.clone(), 0, 256, 2, 512, 0.1, cache, batch, rope)
+    else:
+        launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125, workspace=ws)
+    assert len(launched.lib.calls) == 1
+    del rope, ws
+    assert held() is not None
+    launched.synchronize()
+    assert held() is None
+
+
+def test_a_workspace_of_the_calls_own_is_not_held(launched):
+    """It is torch's memory of the stream that the kernels run on: held, a loop of eager steps would take one a step."""
+    import torch
+
+    cache, batch = host_batch()
+    x = torch.zeros(2, 3, 64, dtype=torch.float16)
+    launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125)
+    assert launched.lib.calls == ["m4_bridge_dispatch_paged_attn"]
+    (held,) = launched._in_flight_tensors
+    assert not any(isinstance(t, torch.Tensor) and t.dtype == torch.uint8 for t in held)
