@@ -756,6 +756,8 @@ class HIPBridge:
             raise ValueError(f"Q has {T} rows, O {To}")
         if not 0 <= window < 1 << 32:
             raise ValueError(f"window={window}")
+        if workspace is not None and not (isinstance(workspace, _torch.Tensor) and workspace.is_contiguous()):
+            raise ValueError("workspace must be a contiguous tensor")  # its bytes are counted from its address on
         self._on_stream_of(Q)
         given = workspace  # one made here goes back to the stream that the kernels are on, behind them
         if workspace is None:

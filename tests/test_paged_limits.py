@@ -242,3 +242,18 @@ def test_a_workspace_of_the_calls_own_is_not_held(launched):
     assert launched.lib.calls == ["m4_bridge_dispatch_paged_attn"]
     (held,) = launched._in_flight_tensors
     assert not any(isinstance(t, torch.Tensor) and t.dtype == torch.uint8 for t in held)
+
+
+def test_workspaces_that_are_refused(launched):
+    """One whose elements share their bytes, or have others' between them: the kernels would write past it or there."""
+    import torch
+
+    cache, batch = host_batch()
+    x = torch.zeros(2, 3, 64, dtype=torch.float16)
+    n = launched.paged_attn_workspace(cache, batch, 2, 3)
+    assert n > 0
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(2 * n), torch.zeros(4 * n, dtype=torch.uint8)[::2], bytearray(2 * n)):
+        with pytest.raises(ValueError, match="workspace"):
+            launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125, workspace=ws)
+    assert launched.lib.calls == []
+    launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125, workspace=torch.zeros(n, dtype=torch.uint8))
