@@ -416,8 +416,8 @@ def check_attention(bridge, s, H, window=0, scale=None, token_major=False, infin
 ])
 @pytest.mark.parametrize("kernels", ["as_planned", "rows", "chunks", "both"])
 def test_paged_attention(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
-    # what is expected of the lengths chooses the kernels: every case runs on each, and with its longer sequences on
-    # one and the others on the other
+    # what is expected of the lengths chooses the kernels, as far as the batch allows: one of which most sequences have
+    # few rows goes to the kernel for rows, or with its longer sequences to the other
     kw = {"as_planned": {}, "rows": {"max_new": 1, "max_kv": 1}, "both": {"max_new": 4096, "max_kv": 10 ** 8},
           "chunks": {"max_new": -(-128 // (H // Hkv)), "max_kv": 10 ** 8}}[kernels]
     check_attention(bridge, Setup(fmt, lens, new, Hkv, D, P, seed=sum(lens) + H), H, window, **kw)

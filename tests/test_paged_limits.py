@@ -257,3 +257,27 @@ def test_workspaces_that_are_refused(launched):
             launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125, workspace=ws)
     assert launched.lib.calls == []
     launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125, workspace=torch.zeros(n, dtype=torch.uint8))
+
+
+# ---- batches that the kernel for chunks takes alone ------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lens,new,H,Hkv,D,P,window,kernels", [
+    ([40 + 3 * (i % 50) for i in range(100)], [20 + i % 21 for i in range(100)], 8, 1, 64, 16, 0, "chunks"),  # more than one a lane
+    ([40 + 3 * (i % 50) for i in range(100)], [20 + i % 21 for i in range(100)], 8, 1, 64, 16, 25, "both"),
+    ([30] * 70, [30 if i % 3 else 0 for i in range(70)], 16, 2, 64, 32, 0, "chunks"),                      # some without rows
+    ([3, 200, 10], [40, 30, 20], 16, 2, 64, 16, 0, "chunks"),                                             # rows that see nothing
+    ([0, 17, 0], [30, 30, 30], 16, 2, 128, 16, 0, "chunks"),
+    ([0, 17, 0], [30, 30, 30], 16, 2, 128, 16, 5, "both"),
+    ([100, 0, 300, 8, 25], [40, 0, 60, 0, 25], 8, 1, 128, 64, 0, "chunks"),                                # and none at all
+    ([700, 1, 0, 0, 90], [64, 1, 0, 0, 40], 32, 4, 64, 256, 0, "chunks"),
+    ([300, 4, 90], [64, 24, 40], 32, 4, 64, 256, 100, "both"),
+])
+def test_batches_of_chunks(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
+    """No sequence of these is the rows kernel's: with both, each has the 128 rows a KV head that make a chunk."""
+    assert kernels == "chunks" or min(n * H // Hkv for n in new) >= 128
+    s = Setup(fmt, lens, new, Hkv, D, P, seed=len(lens) + H)
+    q = half(s.rng, H, s.T, D)
+    got = attend(bridge, s, q, s.q_start, lens, window, kernels)
+    close(got, *s.expected(q, window, D ** -0.5), "chunks")
