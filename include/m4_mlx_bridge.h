@@ -363,7 +363,8 @@ M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv
  * SwiGLU -> down-projection + residual.  X, X_out fp16 [T, d_model], X_out not
  * X; weights as there, in `format`; KV heads and head width are the cache's.
  * Device pointers, 16-byte aligned.  Scratch is the bridge's: a size must have
- * run once before it is captured, and calls run one after the other.  Rows of
+ * run once before it is captured, calls run one after the other, and the stream
+ * is of the device that was current at m4_bridge_init (else -2).  Rows of
  * X_out behind the last sequence hold nothing of use.  Codes as
  * m4_bridge_prefill_layer_ex. */
 M4_API int m4_bridge_paged_layer(void* X_ptr, void* w_attn, void* Wq, void* Wk, void* Wv, void* Wo, void* w_ffn,

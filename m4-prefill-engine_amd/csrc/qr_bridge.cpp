@@ -1036,6 +1036,10 @@ int m4_bridge_paged_layer(void* X, void* w_attn, void* Wq, void* Wk, void* Wv, v
     if (X == Xout) return -2;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
+    if (dev.stream_dev != g_device) {
+        g_last_error = "the layer's scratch is on the device that the bridge was initialized on, the stream on another";
+        return -2;
+    }
     for (void* q : ptrs)
         if (!dev.owns_all(q)) return -2;
     for (void* q : {w_attn, w_ffn})
@@ -1051,6 +1055,8 @@ int m4_bridge_paged_layer(void* X, void* w_attn, void* Wq, void* Wk, void* Wv, v
     const size_t need = 2 * al(nq * 2) + 2 * al(nk * 2) + al(part) + (norms ? 2 : 1) * al((size_t)M * dm * 2) +
                         al((size_t)M * Nm * 2);
     if (grow(&g_ws, &g_ws_bytes, need, false, "layer scratch") != hipSuccess) return -5;
+    // grown by a call that was made with another device current
+    if (!dev.owns_all(g_ws) || (g_sk_ws && !dev.owns_all(g_sk_ws))) return -2;
     uint8_t* w = static_cast<uint8_t*>(g_ws);
     auto take = [&](size_t b) { uint8_t* r = w; w += al(b); return r; };
     _Float16* q = reinterpret_cast<_Float16*>(take(nq * 2));

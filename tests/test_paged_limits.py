@@ -259,6 +259,31 @@ def test_workspaces_that_are_refused(launched):
     launched.dispatch_paged_attn(cache, batch, x, x.clone(), 0.125, workspace=torch.zeros(n, dtype=torch.uint8))
 
 
+# ---- another device -------------------------------------------------------------------------------------------------
+
+@gpu
+def test_layers_of_another_device_are_refused(bridge):
+    """The layer's scratch is on the device that the bridge was initialized on; the other calls have none of the bridge's."""
+    import torch
+
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    with torch.cuda.device(1), torch.cuda.stream(torch.cuda.Stream(1)):
+        s = Setup(Q8_0, [40], [2], 2, 64, 16, seed=44)
+        one = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to("cuda:1")  # noqa: E731
+        cache = m4_bridge.PagedKVCache(Q8_0, s.num_pages, 16, 2, 64, pages=one(s.pages.raw))
+        batch = m4_bridge.KVBatch(one(s.q_start), one(np.array(s.lens, np.int32)), one(s.table), 2, 40)
+        q = half(s.rng, 4, s.T, 64)
+        O = torch.empty(4, s.T, 64, dtype=torch.float16, device="cuda:1")
+        bridge.dispatch_paged_attn(cache, batch, one(q), O, 0.125)
+        bridge.synchronize()
+        close(O.cpu().numpy(), *s.expected(q, 0, 0.125), "attention")
+        X, W = torch.zeros(2, 256, dtype=torch.float16, device="cuda:1"), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda:1")
+        with pytest.raises(RuntimeError, match="-2"):
+            bridge.paged_layer(X, None, *[W] * 4, None, *[W] * 3, X.clone(), 0, 256, 4, 512, 0.125, cache, batch)
+        assert "initialized" in bridge.last_error()
+
+
 # ---- batches that the kernel for chunks takes alone ------------------------------------------------------------------
 
 @gpu
