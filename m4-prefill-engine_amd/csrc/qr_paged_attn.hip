@@ -42,7 +42,9 @@ constexpr float kNone = -3.402823466e38f;  // reference point of a row that has 
 // 2^-14 lose more.  So a row's reference point is kLift below its largest exponent:
 // beside a largest weight of 2^7 or more the small ones keep 2^-32 of it, where
 // beside 1 it would be 2^-25, and many light keys next to a heavy one count.  It
-// moves when an exponent passes 15 (kTop, as bits), so no weight passes 2^15.
+// moves when an exponent passes 15 (kTop, as bits), so no weight passes 2^15.  The sum
+// is of the rounded weights, so that one that is off moves a row towards its value or
+// away from it, and does not scale the row.
 constexpr float kLift = 7.0f;
 constexpr int kTop = 0x41700000;
 
@@ -63,7 +65,9 @@ struct AttnPlan {
     bool both;
 };
 
-// values 1024 + 128 + q of four Q8_0 bytes, as pairs
+// Operands are the cache's values, half(q half(d)): rounded to fp16 because that is what
+// such a cache holds by definition (kv_cache_read returns the same), and what the matrix
+// unit takes.  Q8_0: 1024 + 128 + q of four bytes, as pairs.
 __device__ __forceinline__ h2_t q8_lo(uint32_t w, h2_t d) {
     const h2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
     return (as_h2(nib_pair_lo(w)) - off) * d;
@@ -319,9 +323,9 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // paged_attn_join_kernel joins in order.  The next step's tiles are loaded before
 // the present one is computed, and page numbers 32 steps ahead, a lane each.
 // Bound by the cache's bytes once there are enough of them: four requests of
-// 131072 keys (Q4_0, D = 128, 604 MB) 109 us, 5.5 TB/s (with codes less 8, then times
+// 131072 keys (Q4_0, D = 128, 604 MB) 110 us, 5.5 TB/s (with codes less 8, then times
 // the scale, 6 more: vector instructions count there too); 64 requests of 1 .. 8192
-// keys (Q8_0, 110 MB) 30 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
+// keys (Q8_0, 110 MB) 31 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
 // of descriptor, page table, key and join latencies; drafted tokens and short
 // chunks (two row blocks) by turning codes into fp16 on one wave per SIMD.
 template <int FMT, int D, int NR>
@@ -828,9 +832,9 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
 // double-buffered LDS tile, the codes loaded two tiles ahead; then each wave
 // takes its rows over the tile, 32 x 32 scores at a time.  256 rows share the work
 // of turning codes (128 rows: 1306 us where 256 take 1140).  2048 tokens over 30000
-// keys (D = 128, 972 GFLOP) 1080 us with the join, 0.90 PFLOP/s; counters: the
-// matrix pipe 44% busy, 7.5 vector operations per MFMA, at 1.94 GHz: cycles saved
-// since (2.38 M a CU to 2.03 M) came back as a lower clock, so power bounds it.
+// keys (D = 128, 972 GFLOP) 1067 us with the join, 0.91 PFLOP/s.  Counters: the matrix
+// pipe 44% busy, 8.1 vector operations per MFMA beside it, LDS bank conflicts in 0.23 M
+// of a CU's 1.98 M cycles (V's tile is stored by lanes four rows apart), at 1.9 GHz of 2.2.
 template <int FMT, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
