@@ -349,7 +349,7 @@ M4_API int m4_bridge_kv_cache_read(const m4_kv_cache_t* cache, const m4_kv_batch
  * dim of the rows that see its key, and no others.  Both products are of fp16
  * operands, the cached values and the weights, and are summed in fp32, as are the
  * softmax's sums: 1.6 to 2.8e-4 of the result's norm from the same in 64 bits
- * (the rounding of O alone: 2.1e-4), 2.8 to 4.2e-4 over unrounded q * half(d).  Any number of rows a sequence, from one
+ * (the rounding of O alone: up to 2.1e-4), 2.8 to 4.2e-4 over unrounded q * half(d).  Any number of rows a sequence, from one
  * decoded token to a prompt.  `ws`: m4_bridge_paged_attn_workspace bytes of
  * device memory, 16-byte aligned, whose contents do not matter; calls that may
  * run at the same time need one each.  scale finite.  Codes as above. */
