@@ -359,6 +359,93 @@ M4_API int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv
                                          const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
                                          uint32_t window, void* ws, size_t ws_bytes);
 
+/* ---- trees of drafted tokens over the cache.  The new tokens of a sequence --
+ *      its rows, as far as the call has them -- are the nodes of a tree, numbered
+ *      from the first of them; a node comes behind its parent.  Places in the
+ *      cache are the rows' own, node by node: append them as any rows. ------- */
+
+/* What each row sees of its sequence's new tokens: bit j % 32 of word j / 32 of its
+ * words of `mask` [T][words] for node j; nodes past 32 * words are seen by none.
+ * positions int32 [T]: a node's place in the text, behind its ancestors'. */
+typedef struct {
+    uint32_t* mask;
+    size_t mask_bytes;
+    int32_t* positions;
+    size_t positions_bytes;
+    uint32_t words;
+} m4_draft_tree_t;
+
+/* Fills mask and positions of the batch's rows from their parents (int32 [T], node
+ * numbers; one that is not an earlier node stands for none): a row sees itself and
+ * its ancestors, its position is that of the sequence's first new token plus
+ * their number.  Once a step, for all layers: m4_bridge_kv_cache_append takes the
+ * positions.  Rows behind the last sequence are left.  Codes: -1, -2, -4, -6. */
+M4_API int m4_bridge_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents,
+                                const m4_draft_tree_t* tree);
+
+/* m4_bridge_dispatch_paged_attn where a row sees, of its sequence's new tokens, those
+ * that the mask says (any: not only earlier ones), and all keys before them; with
+ * `window` > 0 those whose position is among the last `window` up to its own
+ * (positions below the first new token's, or past the last one's, count as these;
+ * without a window they may be NULL).  tree NULL: as there, up to itself.
+ * lse (may be NULL): fp32 [T][H] by strides of any size, the natural logarithm of
+ * the sum of exp(scale q . k) over the keys that a row sees, -infinity if none.
+ * The softmax's sum is of unrounded weights here, so the results' last bits differ
+ * from the other call's: 2^-11 of a result at most where few keys count. */
+M4_API int m4_bridge_dispatch_paged_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                              const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
+                                              uint32_t window, const m4_draft_tree_t* tree, const m4_rows_t* lse, void* ws,
+                                              size_t ws_bytes);
+
+/* The path that the model takes down each tree: node 0 (the newest token that is
+ * certain), then again and again the first node whose parent is the last one and
+ * whose token is the model's choice behind it.  parents, tokens, targets int32
+ * [T], targets[i] the model's choice behind row i.  path int32 [T]: a sequence's
+ * rows hold its nodes in order, then -1; count int32 [B]; next int32 [B]: the
+ * choice behind the last of them.  A sequence without rows: 0 and -1. */
+M4_API int m4_bridge_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,
+                                 const int32_t* targets, int32_t* path, int32_t* count, int32_t* next);
+
+/* Keeps of each sequence's new tokens the first count[b] of the list in its rows
+ * of `keep` (int32 [T], node numbers, rising, as m4_bridge_tree_accept writes
+ * them): K and V of node keep[i] move to the place of new token i.  Then the
+ * sequence has kv_len_out[b] keys: those before the tree and count[b] (int32 [B],
+ * may be the batch's kv_len, may be NULL).  Entries that are no nodes, and places
+ * that are not there, move nothing; a list that does not rise leaves the
+ * sequence's new tokens undefined.  Once a layer. */
+M4_API int m4_bridge_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const int32_t* keep,
+                                   const int32_t* count, int32_t* kv_len_out);
+
+/* ---- bounded caches: the attention weight that each key has received -------- */
+
+/* sums, fp32 [num_pages][Hkv][page_size] (16-byte aligned, as the pages lie): adds to
+ * each key's the weights exp(scale q . k - lse) of the batch's rows Q [T][H][D] and
+ * of the H / Hkv query heads of its KV head that see it, as m4_bridge_dispatch_paged_attn
+ * does with the same window; for the batch's new tokens it sets them, whatever
+ * they held.  lse as that call's tree form writes it (append, attend, then weigh).
+ * Products are of fp16 operands, the cached values, summed in fp32; no order changes.
+ * A page that two sequences of a call share: its sums are undefined. */
+M4_API int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
+                                    const m4_rows_t* lse, uint32_t H, float scale, uint32_t window, float* sums,
+                                    size_t sums_bytes);
+
+/* Evicts keys: of each sequence and KV head the first `sinks` places, the last
+ * `recent` and the ones with the largest sums among the others stay, `budget` in all
+ * (at least sinks + recent; equal sums: the lower place; NaN above all numbers), or
+ * all if there are no more.  They are copied in their order, codes, scales and sums,
+ * to the pages of table_out (int32 [B][out_stride], out_pages of a row used, at
+ * least `budget` tokens), whose sequences have kv_len_out[b] keys (int32 [B]);
+ * kept int32 [B][Hkv][budget]: the places that they had, then -1.  The old
+ * pages stay as they are, also where sequences share them; those of table_out are
+ * others, and no two alike.  Heads keep keys of their own, so a place no longer
+ * stands for a position: what is appended next takes explicit positions, and a
+ * window counts places.  Keys on pages that are not there count as gone;
+ * kept ones whose new page is not there are not copied.  q_start is not read (but
+ * not NULL). */
+M4_API int m4_bridge_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, float* sums, size_t sums_bytes,
+                                    const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget,
+                                    uint32_t sinks, uint32_t recent, int32_t* kept, size_t kept_bytes, int32_t* kv_len_out);
+
 /* A transformer block over the cache: m4_bridge_prefill_layer_ex with the
  * batch's rows as its prompt and the paged cache in place of one call's keys --
  * RMSNorm -> Q, K, V -> m4_bridge_kv_cache_append (K and Q turned by `rope`, NULL:
@@ -391,6 +478,24 @@ M4_API int m4_bridge_validate_kv_cache_read(const m4_kv_cache_t* cache, const m4
 M4_API int m4_bridge_validate_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
                                          const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
                                          uint32_t window, const void* ws, size_t ws_bytes);
+M4_API int m4_bridge_validate_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents,
+                                         const m4_draft_tree_t* tree);
+M4_API int m4_bridge_validate_paged_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                              const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
+                                              uint32_t window, const m4_draft_tree_t* tree, const m4_rows_t* lse,
+                                              const void* ws, size_t ws_bytes);
+M4_API int m4_bridge_validate_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents,
+                                          const int32_t* tokens, const int32_t* targets, const int32_t* path,
+                                          const int32_t* count, const int32_t* next);
+M4_API int m4_bridge_validate_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                            const int32_t* keep, const int32_t* count, const int32_t* kv_len_out);
+M4_API int m4_bridge_validate_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
+                                             const m4_rows_t* Q, const m4_rows_t* lse, uint32_t H, float scale,
+                                             uint32_t window, const float* sums, size_t sums_bytes);
+M4_API int m4_bridge_validate_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums,
+                                             size_t sums_bytes, const int32_t* table_out, uint32_t out_pages,
+                                             uint32_t out_stride, uint32_t budget, uint32_t sinks, uint32_t recent,
+                                             const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out);
 
 /* Run subsequent work on `stream` (a hipStream_t, e.g. torch's current
  * stream); NULL restores the bridge's own stream.  Returns 0 or -1. */

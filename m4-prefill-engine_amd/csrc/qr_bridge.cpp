@@ -438,6 +438,10 @@ qr::PagedAttnParams attn_params(const m4_kv_cache_t* c, const m4_kv_batch_t* b, 
     return p;
 }
 
+qr::ValuesView values_view(const m4_rows_t* r) {
+    return {static_cast<float*>(r->ptr), r->token_stride, r->head_stride};
+}
+
 int launched(hipError_t e, const char* what) {
     if (e == hipSuccess) return 0;
     set_error(what, e);
@@ -1016,6 +1020,153 @@ int m4_bridge_dispatch_paged_attn(const m4_kv_cache_t* cache, const m4_kv_batch_
     p.scale = scale;
     p.ws = static_cast<uint8_t*>(ws);
     return launched(qr::launch_paged_attn(p, g_stream), "paged_attn");
+}
+
+int m4_bridge_validate_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const m4_draft_tree_t* tree) {
+    bool empty;
+    return qr::validate_draft_tree(batch, T, parents, tree, &empty);
+}
+
+int m4_bridge_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const m4_draft_tree_t* tree) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_draft_tree(batch, T, parents, tree, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(batch->q_start, batch->kv_len, parents, tree->mask, tree->positions)) return -2;
+    const qr::DraftParams p{batch_view(batch, T), parents, tree->mask, tree->words, tree->positions};
+    return launched(qr::launch_draft_tree(p, g_stream), "draft_tree");
+}
+
+int m4_bridge_validate_paged_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
+                                       const m4_rows_t* O, uint32_t H, float scale, uint32_t window,
+                                       const m4_draft_tree_t* tree, const m4_rows_t* lse, const void* ws, size_t ws_bytes) {
+    bool empty;
+    const int rc = qr::validate_attn_tree(cache, batch, T, Q, O, H, scale, window, tree, lse, ws, &empty);
+    if (rc || empty) return rc;
+    return ws_bytes < m4_bridge_paged_attn_workspace(cache, batch, T, H, window) ? -2 : 0;
+}
+
+int m4_bridge_dispatch_paged_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
+                                       const m4_rows_t* O, uint32_t H, float scale, uint32_t window,
+                                       const m4_draft_tree_t* tree, const m4_rows_t* lse, void* ws, size_t ws_bytes) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_attn_tree(cache, batch, T, Q, O, H, scale, window, tree, lse, ws, &empty);
+    if (rc || empty) return rc;
+    qr::PagedAttnParams p = attn_params(cache, batch, T, H, window);
+    if (ws_bytes < qr::paged_attn_workspace(p)) return -2;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, Q->ptr, O->ptr, ws)) return -2;
+    if (tree && (!dev.owns_all(tree->mask) || (window && !dev.owns_all(tree->positions)))) return -2;
+    if (lse && !dev.owns_all(lse->ptr)) return -2;
+    p.Q = rows_view(Q);
+    p.O = rows_view(O);
+    p.scale = scale;
+    p.ws = static_cast<uint8_t*>(ws);
+    if (tree) p.tree = {tree->mask, tree->words, tree->positions};
+    if (lse) p.lse = values_view(lse);
+    return launched(qr::launch_paged_attn_tree(p, g_stream), "paged_attn_tree");
+}
+
+int m4_bridge_validate_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,
+                                   const int32_t* targets, const int32_t* path, const int32_t* count, const int32_t* next) {
+    bool empty;
+    return qr::validate_tree_accept(batch, T, parents, tokens, targets, path, count, next, &empty);
+}
+
+int m4_bridge_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,
+                          const int32_t* targets, int32_t* path, int32_t* count, int32_t* next) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_tree_accept(batch, T, parents, tokens, targets, path, count, next, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(batch->q_start, batch->kv_len, parents, tokens, targets, path, count, next)) return -2;
+    const qr::AcceptParams p{batch_view(batch, T), parents, tokens, targets, path, count, next};
+    return launched(qr::launch_tree_accept(p, g_stream), "tree_accept");
+}
+
+int m4_bridge_validate_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const int32_t* keep,
+                                     const int32_t* count, const int32_t* kv_len_out) {
+    bool empty;
+    return qr::validate_keep(cache, batch, T, keep, count, kv_len_out, &empty);
+}
+
+int m4_bridge_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const int32_t* keep,
+                            const int32_t* count, int32_t* kv_len_out) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_keep(cache, batch, T, keep, count, kv_len_out, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, keep, count)) return -2;
+    if (kv_len_out && !dev.owns_all(kv_len_out)) return -2;
+    const qr::KeepParams p{cache->D, cache->format, cache_geom(cache), batch_view(batch, T), keep, count, kv_len_out};
+    return launched(qr::launch_kv_keep(p, g_stream), "kv_cache_keep");
+}
+
+int m4_bridge_validate_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
+                                      const m4_rows_t* lse, uint32_t H, float scale, uint32_t window, const float* sums,
+                                      size_t sums_bytes) {
+    bool empty;
+    return qr::validate_weigh(cache, batch, T, Q, lse, H, scale, sums, sums_bytes, &empty);
+}
+
+int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
+                             const m4_rows_t* lse, uint32_t H, float scale, uint32_t window, float* sums,
+                             size_t sums_bytes) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_weigh(cache, batch, T, Q, lse, H, scale, sums, sums_bytes, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, Q->ptr, lse->ptr, sums)) return -2;
+    qr::WeighParams p{};
+    p.Q = rows_view(Q);
+    p.lse = values_view(lse);
+    p.H = H;
+    p.G = H / cache->Hkv;
+    p.D = cache->D;
+    p.format = cache->format;
+    p.scale = scale;
+    p.window = window;
+    p.geom = cache_geom(cache);
+    p.batch = batch_view(batch, T);
+    p.max_new = batch->max_new;
+    p.max_kv = batch->max_kv;
+    p.sums = sums;
+    return launched(qr::launch_kv_weigh(p, g_stream), "kv_cache_weigh");
+}
+
+int m4_bridge_validate_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums,
+                                      size_t sums_bytes, const int32_t* table_out, uint32_t out_pages, uint32_t out_stride,
+                                      uint32_t budget, uint32_t sinks, uint32_t recent, const int32_t* kept,
+                                      size_t kept_bytes, const int32_t* kv_len_out) {
+    bool empty;
+    return qr::validate_evict(cache, batch, sums, sums_bytes, table_out, out_pages, out_stride, budget, sinks, recent, kept,
+                              kept_bytes, kv_len_out, &empty);
+}
+
+int m4_bridge_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, float* sums, size_t sums_bytes,
+                             const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget,
+                             uint32_t sinks, uint32_t recent, int32_t* kept, size_t kept_bytes, int32_t* kv_len_out) {
+    if (!g_initialized) return -1;
+    bool empty;
+    const int rc = qr::validate_evict(cache, batch, sums, sums_bytes, table_out, out_pages, out_stride, budget, sinks, recent,
+                                      kept, kept_bytes, kv_len_out, &empty);
+    if (rc || empty) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    const OnStreamDevice dev;
+    if (!dev.owns_all(cache->pages, batch->kv_len, batch->page_table, sums, table_out, kept, kv_len_out)) return -2;
+    const qr::EvictParams p{cache->D, cache->format, cache_geom(cache), batch_view(batch, 0), batch->max_kv, budget, sinks,
+                            recent, sums, table_out, out_pages, out_stride, kept, kv_len_out};
+    return launched(qr::launch_kv_evict(p, g_stream), "kv_cache_evict");
 }
 
 int m4_bridge_paged_layer(void* X, void* w_attn, void* Wq, void* Wk, void* Wv, void* Wo, void* w_ffn, void* Wg,

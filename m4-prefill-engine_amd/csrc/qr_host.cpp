@@ -154,6 +154,51 @@ int check_rows(const m4_rows_t* r, uint32_t T, uint32_t heads, uint32_t D, bool 
     return 0;
 }
 
+// The rows of a batch alone, where there is no cache.
+int check_rows_of(const m4_kv_batch_t* b, uint32_t T, bool* empty) {
+    if (!b) return -2;
+    if (b->B > 0x7fffffffu || T > kMaxRows) return -4;
+    *empty = b->B == 0 || T == 0;
+    if (*empty) return 0;
+    return !b->q_start || !b->kv_len || misaligned(b->q_start, 4) || misaligned(b->kv_len, 4) ? -2 : 0;
+}
+
+// int32 (or fp32) buffers that have to be there.
+template <typename... P>
+bool all_words(const P*... p) { return (true && ... && (p && !misaligned(p, 4))); }
+
+// One fp32 value per token and head.
+int check_values(const m4_rows_t* r, uint32_t T, uint32_t heads, bool out) {
+    if (!r || !r->ptr || misaligned(r->ptr, 4)) return -2;
+    const int64_t ts = r->token_stride, hs = r->head_stride;
+    if (ts < 0 || hs < 0) return -4;
+    if (out) {  // no two at one place
+        const bool t_inner = T > 1 && (heads <= 1 || ts < hs);
+        const __int128 inner = t_inner ? ts : hs, outer = t_inner ? hs : ts;
+        const uint32_t n_in = t_inner ? T : heads, n_out = t_inner ? heads : T;
+        if (n_in > 1 && inner < 1) return -4;
+        if (n_out > 1 && outer < (n_in > 1 ? inner * (n_in - 1) : 0) + 1) return -4;
+    }
+    const __int128 last = (__int128)(T - 1) * ts + (__int128)(heads - 1) * hs + 1;
+    return (__int128)r->bytes < last * 4 ? -2 : 0;
+}
+
+// Words of a row of a mask: what the bits of as many rows as a call may have need.
+constexpr uint32_t kMaxWords = kMaxRows / 32;
+
+int check_tree(const m4_draft_tree_t* t, uint32_t T, bool positions) {
+    if (!t || !t->mask || misaligned(t->mask, 4) || misaligned(t->positions, 4)) return -2;
+    if (t->words == 0 || t->words > kMaxWords) return -4;
+    if (t->mask_bytes < (size_t)T * t->words * 4) return -2;
+    return positions && (!t->positions || t->positions_bytes < (size_t)T * 4) ? -2 : 0;
+}
+
+// fp32 [num_pages][Hkv][page_size], as the pages lie.
+int check_sums(const m4_kv_cache_t* c, const float* sums, size_t bytes) {
+    if (!sums || misaligned(sums, 16)) return -2;
+    return (unsigned __int128)bytes < (unsigned __int128)c->num_pages * c->Hkv * c->page_size * 4 ? -2 : 0;
+}
+
 int check_rope(const m4_rope_axes_t* r, uint32_t D) {
     if (r->pairs == 0 || r->pairs > M4_ROPE_MAX_PAIRS || r->pairs % 8 || 2 * r->pairs > D) return -4;
     if (r->axes == 0 || r->axes > 256) return -4;
@@ -251,6 +296,71 @@ int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32
     if (int rc = check_rows(O, T, H, cache->D, true)) return rc;
     if (!ws || misaligned(ws, 16)) return -2;
     return 0;
+}
+
+int validate_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* O,
+                       uint32_t H, float scale, uint32_t window, const m4_draft_tree_t* tree, const m4_rows_t* lse,
+                       const void* ws, bool* empty) {
+    if (int rc = validate_attn(cache, batch, T, Q, O, H, scale, ws, empty)) return rc;
+    if (*empty) return 0;
+    if (tree)
+        if (int rc = check_tree(tree, T, window != 0)) return rc;
+    return lse ? check_values(lse, T, H, true) : 0;
+}
+
+int validate_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const m4_draft_tree_t* tree, bool* empty) {
+    *empty = false;
+    if (int rc = check_rows_of(batch, T, empty)) return rc;
+    if (*empty) return 0;
+    if (!all_words(parents)) return -2;
+    return check_tree(tree, T, true);
+}
+
+int validate_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,
+                         const int32_t* targets, const int32_t* path, const int32_t* count, const int32_t* next, bool* empty) {
+    *empty = false;
+    if (int rc = check_rows_of(batch, T, empty)) return rc;
+    if (*empty) return 0;
+    return all_words(parents, tokens, targets, path, count, next) ? 0 : -2;
+}
+
+int validate_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const int32_t* keep,
+                  const int32_t* count, const int32_t* kv_len_out, bool* empty) {
+    *empty = false;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(cache, batch, T, empty)) return rc;
+    if (*empty) return 0;
+    return all_words(keep, count) && !misaligned(kv_len_out, 4) ? 0 : -2;
+}
+
+int validate_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* lse,
+                   uint32_t H, float scale, const float* sums, size_t sums_bytes, bool* empty) {
+    *empty = false;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(cache, batch, T, empty)) return rc;
+    if (H == 0 || H > 0xffffu || H % cache->Hkv || !std::isfinite(scale)) return -4;
+    if (*empty) return 0;
+    if ((uint64_t)T * (H / cache->Hkv) > 0x7fffffffu) return -4;  // rows of a KV head are counted in 32 bits
+    if (int rc = check_rows(Q, T, H, cache->D, false)) return rc;
+    if (int rc = check_values(lse, T, H, false)) return rc;
+    return check_sums(cache, sums, sums_bytes);
+}
+
+int validate_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums, size_t sums_bytes,
+                   const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget, uint32_t sinks,
+                   uint32_t recent, const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out, bool* empty) {
+    *empty = false;
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(cache, batch, 1, empty)) return rc;  // no rows are read, its sequences' keys are
+    if (budget == 0 || budget > 0x7fff0000u || (uint64_t)sinks + recent > budget) return -4;
+    if (*empty) return 0;
+    if (out_pages == 0 || (batch->B > 1 && out_stride < out_pages)) return -4;
+    if ((uint64_t)out_pages * cache->page_size < budget) return -4;
+    if (!all_words(table_out, kept, kv_len_out)) return -2;
+    if ((unsigned __int128)kept_bytes < (unsigned __int128)batch->B * cache->Hkv * budget * 4) return -2;
+    // other pages and lengths than those that are read while they are written
+    if (table_out == batch->page_table || kv_len_out == batch->kv_len) return -2;
+    return check_sums(cache, sums, sums_bytes);
 }
 
 int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rope_axes_t* rope,

@@ -36,6 +36,20 @@ int validate_read(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32
                   bool* empty);
 int validate_attn(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* O,
                   uint32_t H, float scale, const void* ws, bool* empty);
+// lse may be null, and the tree
+int validate_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* O,
+                       uint32_t H, float scale, uint32_t window, const m4_draft_tree_t* tree, const m4_rows_t* lse,
+                       const void* ws, bool* empty);
+int validate_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const m4_draft_tree_t* tree, bool* empty);
+int validate_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,
+                         const int32_t* targets, const int32_t* path, const int32_t* count, const int32_t* next, bool* empty);
+int validate_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const int32_t* keep,
+                  const int32_t* count, const int32_t* kv_len_out, bool* empty);
+int validate_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q, const m4_rows_t* lse,
+                   uint32_t H, float scale, const float* sums, size_t sums_bytes, bool* empty);
+int validate_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums, size_t sums_bytes,
+                   const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget, uint32_t sinks,
+                   uint32_t recent, const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out, bool* empty);
 // all of a layer's arguments but its tensors
 int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rope_axes_t* rope,
                    const int32_t* positions, uint32_t position_stride, int format, uint32_t d_model, uint32_t Hq,

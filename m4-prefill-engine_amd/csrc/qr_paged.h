@@ -87,6 +87,20 @@ struct ReadParams {
 };
 hipError_t launch_kv_read(const ReadParams& p, hipStream_t st);
 
+// One fp32 value per row and head, by strides in elements.
+struct ValuesView {
+    float* p;
+    int64_t ts, hs;
+};
+
+// What each new token sees of its sequence's new tokens: bit j of its words of the
+// mask [T][words] for the j-th of them; places [T]: their positions (for a window).
+struct TreeView {
+    const uint32_t* mask;  // null: those up to itself
+    uint32_t words;
+    const int32_t* places;
+};
+
 struct PagedAttnParams {
     RowsView Q, O;
     uint32_t H, G, D;  // query heads, those of a KV head, head width
@@ -99,8 +113,88 @@ struct PagedAttnParams {
     // a launch's: sequences of that many rows a KV head, [min_rows, max_rows)
     uint32_t min_rows, max_rows;
     uint8_t* ws;
+    // launch_paged_attn_tree only
+    TreeView tree;
+    ValuesView lse;  // p null: not wanted
 };
 size_t paged_attn_workspace(const PagedAttnParams& p);
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st);
+// the same with a tree's mask, and the logarithm of each row's sum of exponentials
+hipError_t launch_paged_attn_tree(const PagedAttnParams& p, hipStream_t st);
+
+
+// ---- trees of drafted tokens ----
+// Masks and places of the batch's new tokens from their parents (launch interface of qr_paged_tree.hip).
+struct DraftParams {
+    BatchView batch;  // no table
+    const int32_t* parents;
+    uint32_t* mask;
+    uint32_t words;
+    int32_t* places;
+};
+hipError_t launch_draft_tree(const DraftParams& p, hipStream_t st);
+
+struct AcceptParams {
+    BatchView batch;  // no table
+    const int32_t *parents, *tokens, *targets;
+    int32_t *path, *count, *next;
+};
+hipError_t launch_tree_accept(const AcceptParams& p, hipStream_t st);
+
+struct KeepParams {
+    uint32_t D;
+    int format;
+    PageGeom geom;
+    BatchView batch;
+    const int32_t *keep, *count;
+    int32_t* len_out;
+};
+hipError_t launch_kv_keep(const KeepParams& p, hipStream_t st);
+
+// ---- bounded caches ----
+struct WeighParams {
+    RowsView Q;
+    ValuesView lse;
+    uint32_t H, G, D;
+    int format;
+    float scale;
+    uint32_t window;
+    PageGeom geom;
+    BatchView batch;
+    uint32_t max_new, max_kv;
+    // a launch's: sequences of that many rows a KV head, [min_rows, max_rows)
+    uint32_t min_rows, max_rows;
+    float* sums;  // [num_pages][Hkv][page]
+};
+hipError_t launch_kv_weigh(const WeighParams& p, hipStream_t st);
+
+struct EvictParams {
+    uint32_t D;
+    int format;
+    PageGeom geom;
+    BatchView batch;  // no rows
+    uint32_t max_kv;
+    uint32_t budget, sinks, recent;
+    float* sums;
+    const int32_t* table_out;
+    uint32_t out_pages, out_stride;
+    int32_t *kept, *len_out;
+};
+hipError_t launch_kv_evict(const EvictParams& p, hipStream_t st);
+
+// The rows of sequence b that a call has, and the position of the first of them.
+struct NewRows {
+    int q0, n, first;
+};
+__host__ __device__ inline NewRows new_rows(const BatchView& v, uint32_t b) {
+    const int T = (int)v.T, start = v.q_start[b], end = v.q_start[b + 1], len = v.kv_len[b];
+    NewRows r;
+    r.q0 = start < 0 ? 0 : (start > T ? T : start);
+    r.n = (end < 0 ? 0 : (end > T ? T : end)) - r.q0;
+    if (r.n < 0) r.n = 0;
+    // rows past T count: those before them keep their positions
+    r.first = r.n ? (len < 0 ? 0 : len) - (end - r.q0) : 0;
+    return r;
+}
 
 }  // namespace qr

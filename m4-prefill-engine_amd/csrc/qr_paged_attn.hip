@@ -9,8 +9,16 @@
 // lane (j, g) gets the scores of keys 16 t + 4 g + r, and takes as its k index
 // 8 g + 4 t + r of V^T the same key.  The contraction runs over dims in the order
 // in which lane group g owns dims D/4 g .. of a key, one run of bytes of the page.
+//
+// QR_PAGED_TREE, a build of its own: the same kernels (TREE) where a mask says which of the
+// new tokens a row sees, and with the logarithm of each row's sum.
 #include "qr_device.h"
 #include "qr_paged.h"
+#include "qr_paged_decode.h"
+
+#ifndef QR_PAGED_TREE
+#define QR_PAGED_TREE 0
+#endif
 
 namespace qr {
 
@@ -65,28 +73,6 @@ struct AttnPlan {
     bool both;
 };
 
-// Operands are the cache's values, half(q half(d)): rounded to fp16 because that is what
-// such a cache holds by definition (kv_cache_read returns the same), and what the matrix
-// unit takes.  Q8_0: 1024 + 128 + q of four bytes, as pairs.
-__device__ __forceinline__ h2_t q8_lo(uint32_t w, h2_t d) {
-    const h2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    return (as_h2(nib_pair_lo(w)) - off) * d;
-}
-__device__ __forceinline__ h2_t q8_hi(uint32_t w, h2_t d) {
-    const h2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    return (as_h2(nib_pair_hi(w)) - off) * d;
-}
-// values c d - 8 d of Q4_0 codes, n8 = -8 d: one instruction, and one rounding as in
-// (c - 8) d since 8 d is exact for scales up to 8188, which fp16 rows do not pass
-template <bool HI>
-__device__ __forceinline__ h2_t q4_pair(uint32_t codes, h2_t d, h2_t n8) {
-    return __builtin_elementwise_fma(code_pair<HI>(codes), d, n8);
-}
-__device__ __forceinline__ h2_t q4_offset(h2_t d) {
-    const h2_t m8 = {(_Float16)-8.0f, (_Float16)-8.0f};
-    return d * m8;
-}
-
 // Smallest V scale (fp16 bits, without the sign) whose values may not be finite: 512,
 // -128 of which is -65536, or 8192, -8 of which is (q4_offset; past what such a cache
 // holds).  A row of fp16 reaches 516 in Q8_0: half(127 half(65504 / 127)) is infinite.
@@ -125,31 +111,6 @@ __device__ __forceinline__ b8_t marks_of(h8_t v) {
 }
 constexpr uint32_t kSeen = 0x4080u;  // bfloat16 4
 
-template <bool ONCE, typename T>
-__device__ __forceinline__ T load_of(const uint8_t* p) {
-    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
-    return *reinterpret_cast<const T*>(p);
-}
-template <int W, bool ONCE>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t w[W]) {
-    if constexpr (W == 1) {
-        w[0] = load_of<ONCE, uint32_t>(p);
-    } else if constexpr (W == 2) {
-        const u2_t a = load_of<ONCE, u2_t>(p);
-        w[0] = a.x;
-        w[1] = a.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < W / 4; i++) {
-            const u4_t a = load_of<ONCE, u4_t>(p + 16 * i);
-            w[4 * i] = a.x;
-            w[4 * i + 1] = a.y;
-            w[4 * i + 2] = a.z;
-            w[4 * i + 3] = a.w;
-        }
-    }
-}
-
 // the same through a buffer resource: a lane's offset and a wave's
 template <int W>
 __device__ __forceinline__ void fetch_words(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff, uint32_t w[W]) {
@@ -171,25 +132,6 @@ __device__ __forceinline__ void fetch_words(__amdgpu_buffer_rsrc_t r, uint32_t o
     }
 }
 
-// K values of dims 8 kk .. 8 kk + 7 of a run of codes
-template <int FMT>
-__device__ __forceinline__ h8_t k_octet(const uint32_t* k, int kk, h2_t d) {
-    h2_t a, b, c, e;
-    if constexpr (FMT == QUANT_Q8_0) {
-        a = q8_lo(k[2 * kk], d);
-        b = q8_hi(k[2 * kk], d);
-        c = q8_lo(k[2 * kk + 1], d);
-        e = q8_hi(k[2 * kk + 1], d);
-    } else {
-        const uint32_t lo = k[kk] & 0x0f0f0f0fu, hi = k[kk] >> 4 & 0x0f0f0f0fu;
-        const h2_t n8 = q4_offset(d);
-        a = q4_pair<false>(lo, d, n8);
-        b = q4_pair<true>(lo, d, n8);
-        c = q4_pair<false>(hi, d, n8);
-        e = q4_pair<true>(hi, d, n8);
-    }
-    return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
-}
 // V values of four keys of dim dt of a run of codes, as two pairs
 template <int FMT>
 __device__ __forceinline__ u2_t v_quad(const uint32_t* v, int dt, u2_t d) {
@@ -314,6 +256,46 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
     return s;
 }
 
+// ---- a mask over the new tokens (TREE) ----
+// Keys before the sequence's first new token are seen by all of its rows, as far as the
+// window reaches; of the new ones a row sees those whose bits are set.
+
+// Position of the sequence's i-th new token: what the caller says, kept within the tree's keys.
+__device__ __forceinline__ int place_of_node(const PagedAttnParams& p, const Seq& s, int i) {
+    return min(max(p.tree.places[s.q0 + i], s.first), s.first + s.n - 1);
+}
+__device__ __forceinline__ int first_seen_by(const PagedAttnParams& p, const Seq& s, int i) {
+    // below zero, too: so may be the places of nodes that have no key, where there are more rows than keys
+    return p.window ? (int)max((int64_t)place_of_node(p, s, i) + 1 - (int64_t)p.window, (int64_t)INT32_MIN) : INT32_MIN;
+}
+// Which of keys key .. key + 3 the row of these mask words sees, as bits; low: the first
+// position that its window holds.
+__device__ __forceinline__ uint32_t sees4(const PagedAttnParams& p, const Seq& s, const uint32_t* mask, int key, int low) {
+    const int node = key - s.first;
+    uint32_t bits = 15;
+    if (node > -4) {
+        const int w = node >> 5;  // -1: the last keys before the tree
+        const uint32_t lo = w < 0 ? 0xffffffffu : ((uint32_t)w < p.tree.words ? mask[w] : 0u);
+        const uint32_t hi = (uint32_t)(w + 1) < p.tree.words ? mask[w + 1] : 0u;
+        bits = (uint32_t)(((uint64_t)hi << 32 | lo) >> (node & 31)) & 15u;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        int at = key + r;
+        const bool there = at < s.keys;
+        if (p.window && there && node + r >= 0) at = place_of_node(p, s, node + r);
+        if (!there || at < low) bits &= ~(1u << r);
+    }
+    return bits;
+}
+// Natural logarithm of a row's sum, from its reference point and its sum beside it.
+__device__ __forceinline__ float lse_of(float m, float l) {
+    return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+__device__ __forceinline__ void put_lse(const PagedAttnParams& p, int row, uint32_t head, float m, float l) {
+    if (p.lse.p) p.lse.p[(int64_t)row * p.lse.ts + (int64_t)head * p.lse.hs] = lse_of(m, l);
+}
+
 // The work is one line: of every sequence, KV head and row tile (an item)
 // kItemCost for its overhead, then its key steps.  A wave takes an even share of
 // the line wherever it begins and ends, so batches of any lengths fill the chip
@@ -328,7 +310,7 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, uint32_t b, uint
 // keys (Q8_0, 110 MB) 31 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
 // of descriptor, page table, key and join latencies; drafted tokens and short
 // chunks (two row blocks) by turning codes into fp16 on one wave per SIMD.
-template <int FMT, int D, int NR>
+template <int FMT, int D, int NR, bool TREE>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
     constexpr int DT = D / 16, KK = D / 32;
@@ -410,6 +392,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         for (int q = 0; q < NR; q++) {
             const uint32_t r = 16 * q + j;
             if (r >= rows) continue;
+            if constexpr (TREE) {
+                const uint32_t f = rt * R + r;
+                if (g == 0) put_lse(p, s.q0 + (int)(f / G), hk * G + f % G, m_run[q], l_run[q]);
+            }
             _Float16* dst = row_of(p.O, r) + g * RUN;
             const float inv = l_run[q] == 0.0f ? 0.0f : 1.0f / l_run[q];
 #pragma unroll
@@ -474,6 +460,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         rows = min(R, (uint32_t)s.n * G - rt * R);
         const int i_first = (int)(rt * R / G), i_last = (int)((rt * R + rows - 1) / G);
         int lim[NR], low[NR];
+        const uint32_t* mask[NR];
         h8_t qf[NR][KK];
 #pragma unroll
         for (int q = 0; q < NR; q++) {
@@ -483,6 +470,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             const uint32_t h = hk * G + f % G;
             lim[q] = last_seen(i);
             low[q] = first_seen(i);
+            mask[q] = nullptr;
+            if constexpr (TREE)
+                if (p.tree.mask) {
+                    mask[q] = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
+                    low[q] = first_seen_by(p, s, i);
+                }
             const _Float16* src = p.Q.p + (int64_t)(s.q0 + i) * p.Q.ts + (int64_t)h * p.Q.hs + g * RUN;
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
@@ -490,8 +483,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                 if (neg) qf[q][kk] = -qf[q][kk];
             }
         }
-        const int lim_min = last_seen(i_first), lim_max = last_seen(i_last);
-        const int low_min = first_seen(i_first), low_max = first_seen(i_last);
+        int lim_min = last_seen(i_first), lim_max = last_seen(i_last);
+        int low_min = first_seen(i_first), low_max = first_seen(i_last);
+        if constexpr (TREE)
+            if (p.tree.mask) {  // all see the keys before the tree, some may see any of its own
+                lim_min = last_seen(-1);
+                lim_max = last_seen(s.n - 1);
+                low_min = first_seen(0);
+                low_max = first_seen(s.n - 1);
+            }
 
 #pragma unroll
         for (int q = 0; q < NR; q++) {
@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         auto step = [&](Tile<FMT, D> tile[2], int u) {
             const int key0 = key_base + u * (int)kStep;
             bool odd = false;  // some row does not see all keys, and some V value may not be finite
+            uint32_t vis[NR];  // TREE: what each row sees of a lane's 8 keys
             f4_t sc[NR][2];
 #pragma unroll
             for (int q = 0; q < NR; q++) sc[q][0] = sc[q][1] = f4_t{};
@@ -554,13 +555,29 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                         large = max(large, e[r] & 0x7fffu);
                     }
                     tile[t].vd = u2_t{e[0] | e[1] << 16, e[2] | e[3] << 16};
+                    if constexpr (TREE) {
 #pragma unroll
-                    for (int q = 0; q < NR; q++)
+                        for (int q = 0; q < NR; q++) {
+                            const int key = key0 + 16 * t + 4 * g;
+                            uint32_t b = 0;
+                            if (tile[t].there && p.tree.mask) b = sees4(p, s, mask[q], key, low[q]);
+                            else if (tile[t].there)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int key = key0 + 16 * t + 4 * g + r;
-                            if (!tile[t].there || key > lim[q] || key < low[q]) sc[q][t][r] = -INFINITY;
+                                for (int r = 0; r < 4; r++) b |= key + r <= lim[q] && key + r >= low[q] ? 1u << r : 0u;
+                            vis[q] = t == 0 ? b : vis[q] | b << 4;
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                if (!(b >> r & 1)) sc[q][t][r] = -INFINITY;
                         }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < NR; q++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const int key = key0 + 16 * t + 4 * g + r;
+                                if (!tile[t].there || key > lim[q] || key < low[q]) sc[q][t][r] = -INFINITY;
+                            }
+                    }
                 }
                 odd = __any(large >= kOddScale<FMT>);
             }
@@ -600,13 +617,24 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                         const f2_t e = {__builtin_amdgcn_exp2f(ex[4 * t + r]), __builtin_amdgcn_exp2f(ex[4 * t + r + 1])};
                         const h2_t pp = __builtin_convertvector(e, h2_t);
                         pk[2 * t + r / 2] = as_u32(pp);
-                        l_run[q] = __builtin_amdgcn_fdot2(pp, one2, l_run[q], false);
+                        // TREE: the logarithm of the sum is wanted to fp32, so its terms are not rounded to
+                        // fp16; O is then off by up to 2^-11 more where few keys count
+                        if constexpr (TREE) l_run[q] += e.x + e.y;
+                        else l_run[q] = __builtin_amdgcn_fdot2(pp, one2, l_run[q], false);
                     }
                 pf[q] = __builtin_bit_cast(h8_t, u4_t{pk[0], pk[1], pk[2], pk[3]});
             }
             if (__builtin_expect(odd, 0)) {
                 auto seen = [&](int q) {
                     u4_t w{};
+                    if constexpr (TREE) {
+                        uint32_t b = vis[q];
+                        asm volatile("" : "+v"(b));
+#pragma unroll
+                        for (int x = 0; x < 8; x++)
+                            if (b >> x & 1) w[x / 2] |= kSeen << (x & 1) * 16;
+                        return __builtin_bit_cast(b8_t, w);
+                    }
                     int l = lim[q] - key0, f = low[q] - key0;
                     asm volatile("" : "+v"(l), "+v"(f));  // formed anew for each dt: kept, registers would spill
 #pragma unroll
@@ -716,7 +744,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 // a row; rows side by side while an item has few parts, else the parts of a row
 // are split over the lane groups, whose sums meet in LDS in a fixed order.
 constexpr uint32_t kJoinBlocks = 512;
-template <int D, int R>
+template <int D, int R, bool TREE>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int L = D / 4, GROUPS = 256 / L, U = 4;
     __shared__ f4_t part_sum[256];
@@ -801,6 +829,8 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
                 if (live && mine0 == 0) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                     const uint32_t f = first + r;
+                    if constexpr (TREE)
+                        if (l4 == 0) put_lse(p, (int)(q0 + f / G), hk * G + f % G, m, l);
                     _Float16* dst = p.O.p + (int64_t)(q0 + f / G) * p.O.ts + (int64_t)(hk * G + f % G) * p.O.hs;
                     const f2_t a = {o.x * inv, o.y * inv}, b = {o.z * inv, o.w * inv};
                     *reinterpret_cast<u2_t*>(dst + 4 * l4) =
@@ -818,8 +848,13 @@ struct Chunk {
 };
 
 // Steps (key tiles of KT) of row tile rt, and its first key.
-template <int KT>
+template <int KT, bool TREE>
 __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq& s, uint32_t tokens, uint32_t rt, int& lo) {
+    if constexpr (TREE)
+        if (p.tree.mask) {  // any row may see any of the new tokens
+            tokens = (uint32_t)s.n;
+            rt = 0;
+        }
     const int64_t first = (int64_t)s.first + rt * tokens;
     const int end = (int)min(first + tokens, (int64_t)s.keys);
     lo = p.window ? (int)min(max(first + 1 - (int64_t)p.window, (int64_t)0), (int64_t)s.keys) / KT * KT : 0;
@@ -835,7 +870,7 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
 // keys (D = 128, 972 GFLOP) 1067 us with the join, 0.91 PFLOP/s.  Counters: the matrix
 // pipe 44% busy, 8.1 vector operations per MFMA beside it, LDS bank conflicts in 0.23 M
 // of a CU's 1.98 M cycles (V's tile is stored by lanes four rows apart), at 1.9 GHz of 2.2.
-template <int FMT, int D, int NW>
+template <int FMT, int D, int NW, bool TREE>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
     constexpr int DT = D / 32, KK = D / 16;
@@ -861,7 +896,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         uint64_t c = 0;
         int lo;
         const uint32_t tiles = ((uint32_t)s.n + tokens - 1) / tokens;
-        for (uint32_t rt = 0; rt < tiles; rt++) c += kChunkCost + steps_of<KT>(p, s, tokens, rt, lo);
+        for (uint32_t rt = 0; rt < tiles; rt++) c += kChunkCost + steps_of<KT, TREE>(p, s, tokens, rt, lo);
         return c;
     };
     const uint32_t per = (p.batch.B + 63) / 64;
@@ -936,7 +971,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         uint32_t rt = 0, steps;
         int lo;
         for (;; rt++) {  // the row tile at this place
-            steps = __builtin_amdgcn_readfirstlane(steps_of<KT>(p, s, tokens, rt, lo));
+            steps = __builtin_amdgcn_readfirstlane(steps_of<KT, TREE>(p, s, tokens, rt, lo));
             if (in_row < kChunkCost + steps) break;
             in_row -= kChunkCost + steps;
         }
@@ -958,11 +993,22 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         auto first_seen = [&](uint32_t r) {
             return p.window ? (int)max((int64_t)s.first + i0 + (int)(r / G) + 1 - (int64_t)p.window, (int64_t)0) : 0;
         };
-        const int lim = last_seen(rc), low = first_seen(rc);
+        int lim = last_seen(rc), low = first_seen(rc);
         // of this wave's rows, and of all
         const uint32_t r0 = min(32u * wave, rows - 1), r1 = min(32u * wave + 31, rows - 1);
-        const int lim0 = last_seen(r0), lim1 = last_seen(r1), low0 = first_seen(r0), low1 = first_seen(r1);
-        const int all0 = last_seen(0), all_low1 = first_seen(rows - 1);
+        int lim0 = last_seen(r0), lim1 = last_seen(r1), low0 = first_seen(r0), low1 = first_seen(r1);
+        int all0 = last_seen(0), all_low1 = first_seen(rows - 1);
+        const uint32_t* mask = nullptr;
+        if constexpr (TREE)
+            if (p.tree.mask) {  // all see the keys before the tree, some may see any of its own
+                const int i = i0 + (int)(rc / G);
+                mask = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
+                low = first_seen_by(p, s, i);
+                all0 = lim0 = min(s.first - 1, s.keys - 1);
+                lim1 = s.keys - 1;
+                low0 = p.window ? (int)max((int64_t)s.first + 1 - (int64_t)p.window, (int64_t)0) : 0;
+                all_low1 = low1 = p.window ? (int)max((int64_t)s.first + s.n - (int64_t)p.window, (int64_t)0) : 0;
+            }
         h8_t qf[KK];
         {
             const _Float16* src = p.Q.p + (int64_t)(s.q0 + (int)(rt * tokens + rc / G)) * p.Q.ts +
@@ -1077,7 +1123,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 const f2_t w = {__builtin_amdgcn_exp2f(ex[e]), __builtin_amdgcn_exp2f(ex[e + 1])};
                 const h2_t pp = __builtin_convertvector(w, h2_t);
                 pk[e >> 1] = as_u32(pp);
-                l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                if constexpr (TREE) l_run += w.x + w.y;  // not rounded, as above
+                else l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
             }
         };
         auto add = [&](const uint8_t* buf, int x, const uint32_t pk[8]) {
@@ -1092,7 +1139,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             }
         };
         // the same where some values may not be finite, and rows do not see all keys
-        auto add_marked = [&](const uint8_t* buf, int x, const uint32_t pk[8], int u) {
+        auto add_marked = [&](const uint8_t* buf, int x, const uint32_t pk[8], int u, uint32_t vis) {
             const int key0 = lo + u * KT + 32 * x;
 #pragma unroll
             for (int t2 = 0; t2 < 2; t2++) {
@@ -1101,7 +1148,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int key = key0 + 16 * t2 + 8 * (e >> 2) + 4 * g + (e & 3);
-                    if ((there[u & 1][2 * x + t2] & 1) && key <= lim && key >= low) seen[e / 2] |= kSeen << (e & 1) * 16;
+                    const bool sees = TREE ? vis >> (8 * t2 + e) & 1 : (there[u & 1][2 * x + t2] & 1) && key <= lim && key >= low;
+                    if (sees) seen[e / 2] |= kSeen << (e & 1) * 16;
                 }
                 const b8_t sf = __builtin_bit_cast(b8_t, seen);
 #pragma unroll
@@ -1158,7 +1206,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                         const f2_t w = {__builtin_amdgcn_exp2f(ex[2 * e]), __builtin_amdgcn_exp2f(ex[2 * e + 1])};
                         const h2_t pp = __builtin_convertvector(w, h2_t);
                         pk[e] = as_u32(pp);
-                        l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                        if constexpr (TREE) l_run += w.x + w.y;
+                        else l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
                     };
                     __builtin_amdgcn_sched_barrier(0);
                     if (x + 1 < UNITS) {
@@ -1204,18 +1253,35 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 const int key0 = k0 + 32 * x;
                 if (key0 > lim1 || key0 + 31 < low0) return;
                 f16v_t sc = scores(buf, x);
+                uint32_t vis = 0xffffu;  // TREE: what the row sees of a lane's 16 keys
                 if (key0 + 31 > lim0 || key0 < low1 || !all_there) {
+                    if constexpr (TREE) {
+                        vis = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int key = key0 + 8 * (e >> 2) + 4 * g + (e & 3);
-                        if (key > lim || key < low || !(there[u & 1][2 * x + (e >> 3)] & 1)) sc[e] = -INFINITY;
+                        for (int y = 0; y < 4; y++) {
+                            const int key = key0 + 8 * y + 4 * g;
+                            if (!(there[u & 1][2 * x + (y >> 1)] & 1)) continue;
+                            if (p.tree.mask) vis |= sees4(p, s, mask, key, low) << 4 * y;
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; e++) vis |= key + e <= lim && key + e >= low ? 1u << (4 * y + e) : 0u;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (!(vis >> e & 1)) sc[e] = -INFINITY;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int key = key0 + 8 * (e >> 2) + 4 * g + (e & 3);
+                            if (key > lim || key < low || !(there[u & 1][2 * x + (e >> 3)] & 1)) sc[e] = -INFINITY;
+                        }
                     }
                 }
                 float ex[16];
                 exponents(sc, ex);
                 uint32_t pk[8];
                 weigh(ex, pk);
-                if (marks) add_marked(buf, x, pk, u);
+                if (marks) add_marked(buf, x, pk, u, vis);
                 else add(buf, x, pk);
             };
             if (__builtin_amdgcn_readfirstlane(some) & 2) {
@@ -1242,6 +1308,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         // lane (j, g): row 32 wave + j, dims 32 t + 8 (e / 4) + 4 g + e % 4
         if (begun && ends) {
             if (r < rows) {
+                if constexpr (TREE)
+                    if (g == 0) put_lse(p, s.q0 + (int)(rt * tokens + r / G), hk * G + r % G, m_run, l_run);
                 const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
                 _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(rt * tokens + r / G)) * p.O.ts + (int64_t)(hk * G + r % G) * p.O.hs;
 #pragma unroll
@@ -1324,10 +1392,14 @@ static size_t ws_bytes(const WorkPlan& w) {
     return (size_t)w.groups * (sizeof(ItemNote) + 2 * slot);
 }
 
+#if !QR_PAGED_TREE
 size_t paged_attn_workspace(const PagedAttnParams& p) {
     const AttnPlan a = plan_of(p);
     return p.D == 64 ? ws_bytes<64>(a.few) + ws_bytes<64>(a.many) : ws_bytes<128>(a.few) + ws_bytes<128>(a.many);
 }
+#endif
+
+constexpr bool kTree = QR_PAGED_TREE != 0;
 
 template <int D, int R>
 static hipError_t launch_join(const PagedAttnParams& p, const WorkPlan& w, hipStream_t st) {
@@ -1340,7 +1412,7 @@ static hipError_t launch_join(const PagedAttnParams& p, const WorkPlan& w, hipSt
     const uint32_t parts = w.groups / w.items, across = R > 32 ? 32 : (parts >= 16 ? 16 : (parts >= 8 ? 8 : 4));
     const uint32_t most = 4 * kJoinBlocks / across;
     const dim3 grid(w.groups < most ? w.groups : most, across);
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, R>), grid, dim3(256), 0, st, p, w.groups);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, R, kTree>), grid, dim3(256), 0, st, p, w.groups);
     return hipGetLastError();
 }
 
@@ -1354,10 +1426,10 @@ static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
         const dim3 grid(a.few.groups), block(64 * kWaves);
         hipError_t e;
         if (a.few.rows == 16) {
-            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1>), grid, block, 0, st, p, a.few.groups);
+            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1, kTree>), grid, block, 0, st, p, a.few.groups);
             e = launch_join<D, 16>(p, a.few, st);
         } else {
-            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2>), grid, block, 0, st, p, a.few.groups);
+            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, kTree>), grid, block, 0, st, p, a.few.groups);
             e = launch_join<D, 32>(p, a.few, st);
         }
         if (e != hipSuccess) return e;
@@ -1369,13 +1441,17 @@ static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
     constexpr int NW = kChunkTile / 32;
     constexpr size_t lds = 2 * 2 * 16 * NW * D * 2;
     static size_t attr[kMaxDevices] = {};  // more than the default 64 KB of LDS
-    const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW>, lds, attr);
+    const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW, kTree>, lds, attr);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW>), dim3(a.many.groups), dim3(64 * NW), lds, st, p, a.many.groups);
+    hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW, kTree>), dim3(a.many.groups), dim3(64 * NW), lds, st, p, a.many.groups);
     return launch_join<D, kChunkTile>(p, a.many, st);
 }
 
+#if QR_PAGED_TREE
+hipError_t launch_paged_attn_tree(const PagedAttnParams& p, hipStream_t st) {
+#else
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) {
+#endif
     if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
     if (p.format == QUANT_Q8_0) return p.D == 64 ? launch_format<QUANT_Q8_0, 64>(p, st) : launch_format<QUANT_Q8_0, 128>(p, st);
     return p.D == 64 ? launch_format<QUANT_Q4_0, 64>(p, st) : launch_format<QUANT_Q4_0, 128>(p, st);

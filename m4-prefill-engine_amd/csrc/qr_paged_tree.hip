@@ -1,0 +1,220 @@
+// qr_paged_tree.hip -- trees of drafted tokens: which nodes each one has before it, the walk
+// that accepts a path of them, and the move of the path's tokens to their places.
+#include "qr_device.h"
+#include "qr_paged.h"
+
+namespace qr {
+
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane) << 32 | (uint32_t)__shfl((int)(uint32_t)v, lane);
+}
+
+// A node's ancestors are itself and its parent's, anc(i) = {i} + anc(parent(i)), and a parent
+// comes before its nodes.  64 nodes at a time, a lane each: pointers are doubled six times, so
+// that every node has its ancestors among the 64 as one word; the lowest of them says where
+// the path leaves the 64, to a node whose row of the mask is there already and is copied.
+// A block a sequence.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) draft_tree_kernel(DraftParams p) {
+    __shared__ uint64_t near_of[64];
+    __shared__ int exit_of[64];
+    const int lane = threadIdx.x & 63;
+    const uint32_t W = p.words;
+    for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
+        const NewRows s = new_rows(p.batch, b);
+        for (int base = 0; base < s.n; base += 64) {
+            const int i = base + lane;
+            int parent = i < s.n ? p.parents[s.q0 + i] : -1;
+            if (parent >= i) parent = -1;
+            if (threadIdx.x < 64) {
+                int jump = parent >= base ? parent - base : -1, leave = parent >= 0 && parent < base ? parent : -1;
+                uint64_t near = (uint64_t)1 << lane;
+#pragma unroll
+                for (int r = 0; r < 6; r++) {
+                    const int at = jump < 0 ? lane : jump;
+                    near |= shfl_u64(near, at);
+                    const int further = __shfl(jump, at);
+                    jump = jump < 0 ? -1 : further;
+                }
+                leave = __shfl(leave, __ffsll((unsigned long long)near) - 1);
+                near_of[lane] = near;
+                exit_of[lane] = leave;
+                if (i < s.n) p.places[s.q0 + i] = (leave >= 0 ? p.places[s.q0 + leave] + 1 : s.first) + __popcll(near) - 1;
+            }
+            __syncthreads();
+            const uint32_t rows = min(s.n - base, 64), own = (uint32_t)base / 32;
+            uint32_t* mask = p.mask + (size_t)s.q0 * W;
+            for (uint32_t x = threadIdx.x; x < rows * W; x += THREADS) {  // W is at most 2^21
+                const uint32_t r = x / W, w = x % W;
+                uint32_t bits = 0;
+                if (w == own) bits = (uint32_t)near_of[r];
+                else if (w == own + 1) bits = (uint32_t)(near_of[r] >> 32);
+                else if (w < own && exit_of[r] >= 0) bits = mask[(size_t)exit_of[r] * W + w];
+                mask[(size_t)base * W + x] = bits;
+            }
+            __syncthreads();  // rows of later nodes copy these
+        }
+    }
+}
+
+hipError_t launch_draft_tree(const DraftParams& p, hipStream_t st) {
+    if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
+    hipLaunchKernelGGL(draft_tree_kernel<256>, dim3(min(p.batch.B, 1u << 20)), dim3(256), 0, st, p);
+    return hipGetLastError();
+}
+
+// From node 0 on, the first node behind the present one that is its child and whose token is
+// the model's choice there.  A wave a sequence, 64 nodes at a time.
+__global__ void __launch_bounds__(64) tree_accept_kernel(AcceptParams p) {
+    const int lane = threadIdx.x;
+    for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
+        const NewRows s = new_rows(p.batch, b);
+        const int32_t *parents = p.parents + s.q0, *tokens = p.tokens + s.q0, *targets = p.targets + s.q0;
+        int count = 0, next = -1;
+        if (s.n > 0) {
+            int cur = 0, base = 0, parent = -1, token = 0, target = 0;
+            auto load = [&](int from) {
+                base = from;
+                const int i = base + lane;
+                parent = i < s.n ? parents[i] : -1;
+                token = i < s.n ? tokens[i] : 0;
+                target = i < s.n ? targets[i] : 0;
+            };
+            load(0);
+            next = __builtin_amdgcn_readlane(target, 0);
+            if (lane == 0) p.path[s.q0] = 0;
+            count = 1;
+            for (;;) {
+                const uint64_t fits = __ballot(parent == cur && token == next && base + lane > cur && base + lane < s.n);
+                if (fits) {
+                    const int at = __ffsll((unsigned long long)fits) - 1;
+                    cur = base + at;
+                    next = __builtin_amdgcn_readlane(target, at);
+                    if (lane == 0) p.path[s.q0 + count] = cur;
+                    count++;
+                    continue;  // its child may be among the same 64
+                }
+                if (base + 64 >= s.n) break;
+                load(base + 64);
+            }
+        }
+        for (int i = count + lane; i < s.n; i += 64) p.path[s.q0 + i] = -1;
+        if (lane == 0) {
+            p.count[b] = count;
+            p.next[b] = next;
+        }
+    }
+}
+
+hipError_t launch_tree_accept(const AcceptParams& p, hipStream_t st) {
+    if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
+    hipLaunchKernelGGL(tree_accept_kernel, dim3(min(p.batch.B, 1u << 20)), dim3(64), 0, st, p);
+    return hipGetLastError();
+}
+
+// New token keep[i] of a sequence becomes its new token i.  Within a head, what a step writes
+// is read by none of the later ones, since keep[i] >= i: a step's tokens are all loaded before
+// any is stored.  A block a sequence, so that its length may be written where it was read.
+// A token of a head is CB / 16 pieces of K codes, CB / 4 of V codes (of four tokens' words each
+// the bytes of one) and one of its scales.
+constexpr int kKeepThreads = 1024, kKeepList = 256;
+template <int FMT, int D>
+__global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(KeepParams p) {
+    constexpr uint32_t CB = FMT == QUANT_Q8_0 ? D : D / 2, NB = D / 32;
+    constexpr uint32_t KP = CB / 16, VP = CB / 4, PIECES = KP + VP + 1, PAIRS = kKeepThreads / PIECES;
+    __shared__ uint32_t src_page[kKeepList], src_slot[kKeepList], dst_page[kKeepList], dst_slot[kKeepList];
+    const uint32_t piece = threadIdx.x % PIECES, pair = threadIdx.x / PIECES;
+    for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
+        const NewRows s = new_rows(p.batch, b);
+        const int len = max(p.batch.kv_len[b], 0), count = min(max(p.count[b], 0), s.n);
+        __syncthreads();  // the length is read
+        if (threadIdx.x == 0 && p.len_out) p.len_out[b] = s.n ? max(s.first + count, 0) : len;
+        for (int base = 0; base < count; base += kKeepList) {
+            const uint32_t tokens = (uint32_t)min(count - base, kKeepList);
+            __syncthreads();
+            if (threadIdx.x < tokens) {
+                const int i = base + (int)threadIdx.x, from = p.keep[s.q0 + i];
+                const uint32_t none = 0xffffffffu;
+                auto place = [&](int node, uint32_t& page, uint32_t& slot) {
+                    const int at = s.first + node;
+                    const uint32_t pi = (uint32_t)at >> p.geom.log2_page;
+                    page = at >= 0 && pi < p.batch.table_pages ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + pi] : none;
+                    if (page >= p.geom.num_pages) page = none;
+                    slot = (uint32_t)at & ((1u << p.geom.log2_page) - 1);
+                };
+                uint32_t sp = none, ss = 0, dp = none, ds = 0;
+                if (from >= 0 && from < s.n && from != i) {
+                    place(from, sp, ss);
+                    place(i, dp, ds);
+                }
+                if (sp == none) dp = none;
+                src_page[threadIdx.x] = sp;
+                src_slot[threadIdx.x] = ss;
+                dst_page[threadIdx.x] = dp;
+                dst_slot[threadIdx.x] = ds;
+            }
+            __syncthreads();
+            const uint64_t pairs = (uint64_t)tokens * p.geom.Hkv;
+            for (uint64_t x0 = 0; x0 < pairs; x0 += PAIRS) {
+                const uint64_t x = x0 + pair;
+                const uint32_t hk = (uint32_t)(x / tokens), t = (uint32_t)(x % tokens);
+                const bool live = pair < PAIRS && x < pairs && dst_page[t] != 0xffffffffu;
+                uint8_t *src = nullptr, *dst = nullptr;
+                uint32_t ss = 0, ds = 0;
+                u4_t v{};
+                if (live) {
+                    src = p.geom.pages + ((size_t)src_page[t] * p.geom.Hkv + hk) * p.geom.head_bytes;
+                    dst = p.geom.pages + ((size_t)dst_page[t] * p.geom.Hkv + hk) * p.geom.head_bytes;
+                    ss = src_slot[t];
+                    ds = dst_slot[t];
+                    if (piece < KP) {
+                        v = *reinterpret_cast<const u4_t*>(src + ss * CB + 16 * piece);
+                    } else if (piece < KP + VP) {
+                        v = *reinterpret_cast<const u4_t*>(src + p.geom.v_off + (ss >> 2) * (4 * CB) + 16 * (piece - KP)) >> (8 * (ss & 3));
+                    } else {
+                        uint32_t h[8] = {};
+#pragma unroll
+                        for (uint32_t j = 0; j < NB; j++) {
+                            h[j] = *reinterpret_cast<const uint16_t*>(src + p.geom.ks_off + (ss * NB + j) * 2);
+                            h[4 + j] = *reinterpret_cast<const uint16_t*>(src + p.geom.vs_off + (((ss >> 2) * NB + j) * 4 + (ss & 3)) * 2);
+                        }
+                        v = u4_t{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
+                    }
+                }
+                __syncthreads();
+                if (!live) continue;
+                if (piece < KP) {
+                    *reinterpret_cast<u4_t*>(dst + ds * CB + 16 * piece) = v;
+                } else if (piece < KP + VP) {
+                    uint8_t* o = dst + p.geom.v_off + (ds >> 2) * (4 * CB) + 16 * (piece - KP) + (ds & 3);
+                    o[0] = (uint8_t)v.x;
+                    o[4] = (uint8_t)v.y;
+                    o[8] = (uint8_t)v.z;
+                    o[12] = (uint8_t)v.w;
+                } else {
+                    const uint32_t h[8] = {v.x, v.x >> 16, v.y, v.y >> 16, v.z, v.z >> 16, v.w, v.w >> 16};
+#pragma unroll
+                    for (uint32_t j = 0; j < NB; j++) {
+                        *reinterpret_cast<uint16_t*>(dst + p.geom.ks_off + (ds * NB + j) * 2) = (uint16_t)h[j];
+                        *reinterpret_cast<uint16_t*>(dst + p.geom.vs_off + (((ds >> 2) * NB + j) * 4 + (ds & 3)) * 2) = (uint16_t)h[4 + j];
+                    }
+                }
+            }
+        }
+    }
+}
+
+hipError_t launch_kv_keep(const KeepParams& p, hipStream_t st) {
+    if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
+    const dim3 grid(min(p.batch.B, 1u << 20)), block(kKeepThreads);
+    if (p.format == QUANT_Q8_0) {
+        if (p.D == 64) hipLaunchKernelGGL((kv_keep_kernel<QUANT_Q8_0, 64>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((kv_keep_kernel<QUANT_Q8_0, 128>), grid, block, 0, st, p);
+    } else {
+        if (p.D == 64) hipLaunchKernelGGL((kv_keep_kernel<QUANT_Q4_0, 64>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((kv_keep_kernel<QUANT_Q4_0, 128>), grid, block, 0, st, p);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace qr

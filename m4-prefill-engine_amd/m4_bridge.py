@@ -93,11 +93,23 @@ SIGNATURES = {
     "m4_bridge_kv_cache_read": ([_VP, _VP, _U32, _VP, _VP], _I),
     "m4_bridge_paged_attn_workspace": ([_VP, _VP, _U32, _U32, _U32], _SZ),
     "m4_bridge_dispatch_paged_attn": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_draft_tree": ([_VP, _U32, _VP, _VP], _I),
+    "m4_bridge_dispatch_paged_attn_tree": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _VP, _VP, _SZ], _I),
+    "m4_bridge_tree_accept": ([_VP, _U32] + [_VP] * 6, _I),
+    "m4_bridge_kv_cache_keep": ([_VP, _VP, _U32, _VP, _VP, _VP], _I),
+    "m4_bridge_kv_cache_weigh": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_kv_cache_evict": ([_VP, _VP, _VP, _SZ, _VP, _U32, _U32, _U32, _U32, _U32, _VP, _SZ, _VP], _I),
     "m4_bridge_paged_layer": ([_VP] * 13 + [_U32, _VP, _VP, _U32, _I, _U32, _U32, _U32, _F, _U32, _I, _F], _I),
     "m4_bridge_validate_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
     "m4_bridge_validate_kv_cache_append": ([_VP, _VP, _U32, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
     "m4_bridge_validate_kv_cache_read": ([_VP, _VP, _U32, _VP, _VP], _I),
     "m4_bridge_validate_paged_attn": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_validate_draft_tree": ([_VP, _U32, _VP, _VP], _I),
+    "m4_bridge_validate_paged_attn_tree": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _VP, _VP, _SZ], _I),
+    "m4_bridge_validate_tree_accept": ([_VP, _U32] + [_VP] * 6, _I),
+    "m4_bridge_validate_kv_cache_keep": ([_VP, _VP, _U32, _VP, _VP, _VP], _I),
+    "m4_bridge_validate_kv_cache_weigh": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
+    "m4_bridge_validate_kv_cache_evict": ([_VP, _VP, _VP, _SZ, _VP, _U32, _U32, _U32, _U32, _U32, _VP, _SZ, _VP], _I),
     "m4_bridge_set_stream": ([_VP], _I),
     "m4_bridge_get_stream": ([], _VP),
     "m4_bridge_last_error": ([], ctypes.c_char_p),
@@ -306,6 +318,42 @@ class RotaryAxes:
             struct = RopeAxesStruct(self.dims // 2, self.axes, int(self.traditional), t.data_ptr(), t.numel())
             held = self._on[device] = (t, struct, ctypes.addressof(struct))
         return held[2]
+
+
+class DraftTreeStruct(ctypes.Structure):
+    """m4_draft_tree_t (include/m4_mlx_bridge.h)."""
+    _fields_ = [("mask", _VP), ("mask_bytes", _SZ), ("positions", _VP), ("positions_bytes", _SZ), ("words", _U32)]
+
+
+class DraftTree:
+    """What each of a call's T rows sees of its sequence's new tokens (m4_draft_tree_t): bit j % 32 of mask[row][j // 32]
+    (int32 [T, words]) for the j-th of them, and each row's position (int32 [T]; None where no window is used).  Any
+    mask will do; HIPBridge.draft_tree fills both from the nodes' parents."""
+
+    def __init__(self, mask, positions=None) -> None:
+        import torch
+
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.int32 or mask.dim() != 2 or not mask.is_contiguous():
+            raise ValueError("mask must be a contiguous int32 tensor [T, words]")
+        if mask.shape[1] == 0:
+            raise ValueError("a mask needs a word a row at least")
+        if positions is not None:
+            _int32("positions", positions, 1)
+            if positions.shape[0] != mask.shape[0]:
+                raise ValueError(f"mask has {mask.shape[0]} rows, positions {positions.shape[0]}")
+        self.mask, self.positions = mask, positions
+        self.T, self.words = mask.shape
+        self.struct = DraftTreeStruct(mask.data_ptr(), mask.nbytes, positions.data_ptr() if positions is not None else None,
+                                      positions.nbytes if positions is not None else 0, self.words)
+        self.ref = ctypes.addressof(self.struct)
+
+    @classmethod
+    def empty(cls, T: int, max_nodes: int, device="cuda") -> "DraftTree":
+        """For T rows of trees with at most `max_nodes` nodes, to be filled."""
+        import torch
+
+        return cls(torch.empty(T, max(1, -(-max_nodes // 32)), dtype=torch.int32, device=device),
+                   torch.empty(T, dtype=torch.int32, device=device))
 
 
 def load_library(path: Optional[Union[str, Path]] = None) -> ctypes.CDLL:
@@ -744,12 +792,121 @@ class HIPBridge:
         """Bytes of workspace that dispatch_paged_attn needs for T rows of H heads."""
         return int(self._lib.m4_bridge_paged_attn_workspace(cache.ref, batch.ref, T, H, window))
 
+    def _lse(self, lse: Any, H: int, T: int, out: bool) -> tuple:
+        """m4_rows_t's words for fp32 [H, T], any strides."""
+        if not isinstance(lse, _torch.Tensor) or lse.dtype is not _torch.float32 or tuple(lse.shape) != (H, T):
+            raise ValueError(f"lse must be an fp32 tensor [{H}, {T}]")
+        hs, ts = lse.stride()
+        if out and T * H and ((T > 1 and ts == 0) or (H > 1 and hs == 0)):
+            raise ValueError("lse has values that share their memory")
+        return lse.data_ptr(), ((T - 1) * ts + (H - 1) * hs + 1) * 4 if T and H else 0, ts, hs
+
+    def _tree(self, tree: "DraftTree", T: int) -> int:
+        if tree.T != T:
+            raise ValueError(f"the tree has {tree.T} rows, the call {T}")
+        return tree.ref
+
+    def _ids(self, name: str, t: Any, n: int) -> int:
+        if not isinstance(t, _torch.Tensor) or t.dtype is not _torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor [{n}]")
+        return t.data_ptr()
+
+    def draft_tree(self, batch: KVBatch, parents, tree: DraftTree) -> int:
+        """Fills `tree` for the batch's rows from their parents, int32 [T]: node numbers within the sequence, -1 for
+        none.  Once a step, for all layers; kv_cache_append takes tree.positions."""
+        if tree.positions is None:
+            raise ValueError("the tree has no positions to fill")
+        at = self._ids("parents", parents, tree.T)
+        self._on_stream_of(parents)
+        ret = self._lib.m4_bridge_draft_tree(batch.ref, tree.T, at, tree.ref)
+        self._check("m4_bridge_draft_tree", ret)
+        self._in_flight_tensors.append((batch, parents, tree))
+        return ret
+
+    def tree_accept(self, batch: KVBatch, parents, tokens, targets, path, count, next_token) -> int:
+        """The model's path down each tree: from node 0 on, the first node behind whose token is the model's choice
+        (`targets`).  All int32: parents, tokens, targets, path [T]; count, next_token [B]."""
+        T, B = parents.shape[0], batch.B
+        ptrs = [self._ids(n, t, T) for n, t in (("parents", parents), ("tokens", tokens), ("targets", targets), ("path", path))]
+        ptrs += [self._ids(n, t, B) for n, t in (("count", count), ("next_token", next_token))]
+        self._on_stream_of(parents)
+        ret = self._lib.m4_bridge_tree_accept(batch.ref, T, *ptrs)
+        self._check("m4_bridge_tree_accept", ret)
+        self._in_flight_tensors.append((batch, parents, tokens, targets, path, count, next_token))
+        return ret
+
+    def kv_cache_keep(self, cache: PagedKVCache, batch: KVBatch, keep, count, kv_len_out=None) -> int:
+        """Of each sequence's new tokens the count[b] that its rows of `keep` [T] name (rising, as tree_accept's path)
+        move to the places of the first; kv_len_out [B] (may be batch.kv_len): what the sequences then hold."""
+        T = keep.shape[0]
+        ptrs = [self._ids("keep", keep, T), self._ids("count", count, batch.B),
+                self._ids("kv_len_out", kv_len_out, batch.B) if kv_len_out is not None else None]
+        self._on_stream_of(keep)
+        ret = self._lib.m4_bridge_kv_cache_keep(cache.ref, batch.ref, T, *ptrs)
+        self._check("m4_bridge_kv_cache_keep", ret)
+        self._in_flight_tensors.append((cache, batch, keep, count, kv_len_out))
+        return ret
+
+    def _sums(self, cache: PagedKVCache, sums: Any) -> tuple:
+        shape = (cache.num_pages, cache.Hkv, cache.page_size)
+        if not isinstance(sums, _torch.Tensor) or sums.dtype is not _torch.float32 or tuple(sums.shape) != shape or not sums.is_contiguous():
+            raise ValueError(f"sums must be a contiguous fp32 tensor {list(shape)}")
+        return sums.data_ptr(), sums.nbytes
+
+    def kv_cache_weigh(self, cache: PagedKVCache, batch: KVBatch, Q, lse, sums, scale: float, token_major: bool = False,
+                       window: int = 0) -> int:
+        """Adds to sums [num_pages, Hkv, page_size] (fp32) the weight that the batch's rows Q [H, T, D] (or [T, H, D]) give
+        each key they see, for the batch's own tokens in place of what was there; lse [H, T] (fp32, any strides) as
+        dispatch_paged_attn writes it for the same rows, scale and window."""
+        q, T, H, Q = self._rows("Q", Q, token_major, None, cache.D, False)
+        z = self._lse(lse, H, T, False)
+        at_sums, held = self._sums(cache, sums)
+        if not 0 <= window < 1 << 32:
+            raise ValueError(f"window={window}")
+        self._on_stream_of(Q)
+        rows = _ROWS2(*q, *z)
+        at = ctypes.addressof(rows)
+        ret = self._lib.m4_bridge_kv_cache_weigh(cache.ref, batch.ref, T, at, at + _ROWS, H, float(scale), window, at_sums, held)
+        self._check("m4_bridge_kv_cache_weigh", ret)
+        self._in_flight_tensors.append((cache, batch, Q, lse, sums))
+        return ret
+
+    def kv_cache_evict(self, cache: PagedKVCache, batch: KVBatch, sums, table_out, kv_len_out, budget: int, sinks: int = 0,
+                       recent: int = 0, kept=None) -> int:
+        """Copies of each sequence and KV head the first `sinks`, the last `recent` and the heaviest other keys by `sums`,
+        `budget` together, to the pages of table_out (int32 [B, pages]), in their order and with their sums.
+        kv_len_out int32 [B]: how many; kept int32 [B, Hkv, budget]: the places that they had, then -1 (None: not
+        wanted).  The caller goes on with table_out and kv_len_out and has the old pages back."""
+        B = batch.B
+        _int32("table_out", table_out, 2)
+        if table_out.shape[0] != B:
+            raise ValueError(f"table_out has {table_out.shape[0]} rows, the batch {B}")
+        for name, v in (("budget", budget), ("sinks", sinks), ("recent", recent)):
+            if not 0 <= v < 1 << 32:
+                raise ValueError(f"{name}={v}")
+        at_sums, held = self._sums(cache, sums)
+        at_len = self._ids("kv_len_out", kv_len_out, B)
+        given = kept  # one made here goes back to the stream that the kernels are on, behind them
+        if kept is None:
+            kept = _torch.empty(B, cache.Hkv, budget, dtype=_torch.int32, device=sums.device)
+        elif kept.dtype is not _torch.int32 or tuple(kept.shape) != (B, cache.Hkv, budget) or not kept.is_contiguous():
+            raise ValueError(f"kept must be a contiguous int32 tensor [{B}, {cache.Hkv}, {budget}]")
+        self._on_stream_of(sums)
+        ret = self._lib.m4_bridge_kv_cache_evict(cache.ref, batch.ref, at_sums, held, table_out.data_ptr(), table_out.shape[1],
+                                                 table_out.stride(0), budget, sinks, recent, kept.data_ptr(), kept.nbytes,
+                                                 at_len)
+        self._check("m4_bridge_kv_cache_evict", ret)
+        self._in_flight_tensors.append((cache, batch, sums, table_out, kv_len_out, given))
+        return ret
+
     def dispatch_paged_attn(self, cache: PagedKVCache, batch: KVBatch, Q, O, scale: float, token_major: bool = False,
-                            o_token_major: bool = False, window: int = 0, workspace=None) -> int:
+                            o_token_major: bool = False, window: int = 0, workspace=None,
+                            tree: Optional[DraftTree] = None, lse=None) -> int:
         """Causal attention of the batch's rows Q [H, T, D] (or [T, H, D]) over their sequences' cached keys (append
         first); O [H, T, D], or [T, H, D] when o_token_major.  `workspace`: a uint8 device tensor of
         paged_attn_workspace bytes, not shared with a call that may run at the same time (None: from torch's
-        allocator, on the current stream)."""
+        allocator, on the current stream).  `tree`: which of its sequence's new tokens a row sees, in place of those up
+        to itself; `lse` [H, T] (fp32, any strides): receives the logarithm of each row's sum of exponentials."""
         q, T, H, Q = self._rows("Q", Q, token_major, None, cache.D, False)
         o, To, _, _ = self._rows("O", O, o_token_major, H, cache.D, True)
         if To != T:
@@ -758,17 +915,30 @@ class HIPBridge:
             raise ValueError(f"window={window}")
         if workspace is not None and not (isinstance(workspace, _torch.Tensor) and workspace.is_contiguous()):
             raise ValueError("workspace must be a contiguous tensor")  # its bytes are counted from its address on
+        at_tree = self._tree(tree, T) if tree is not None else None
+        if tree is not None and window and tree.positions is None:
+            raise ValueError("a window needs the tree's positions")
+        z = self._lse(lse, H, T, True) if lse is not None else None
         self._on_stream_of(Q)
         given = workspace  # one made here goes back to the stream that the kernels are on, behind them
         if workspace is None:
             workspace = _torch.empty(self.paged_attn_workspace(cache, batch, H, T, window), dtype=_torch.uint8,
                                      device=Q.device)
-        rows = _ROWS2(*q, *o)
+        if tree is None and lse is None:
+            rows = _ROWS2(*q, *o)
+            at = ctypes.addressof(rows)
+            ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, T, at, at + _ROWS, H, float(scale), window,
+                                                          workspace.data_ptr(), workspace.nbytes)
+            self._check("m4_bridge_dispatch_paged_attn", ret)
+            self._in_flight_tensors.append((cache, batch, Q, O, given))
+            return ret
+        rows = _ROWS4(*q, *o, *(z or (0, 0, 0, 0)), 0, 0, 0, 0)
         at = ctypes.addressof(rows)
-        ret = self._lib.m4_bridge_dispatch_paged_attn(cache.ref, batch.ref, T, at, at + _ROWS, H, float(scale), window,
-                                                      workspace.data_ptr(), workspace.nbytes)
-        self._check("m4_bridge_dispatch_paged_attn", ret)
-        self._in_flight_tensors.append((cache, batch, Q, O, given))
+        ret = self._lib.m4_bridge_dispatch_paged_attn_tree(cache.ref, batch.ref, T, at, at + _ROWS, H, float(scale), window,
+                                                           at_tree, at + 2 * _ROWS if z else None, workspace.data_ptr(),
+                                                           workspace.nbytes)
+        self._check("m4_bridge_dispatch_paged_attn_tree", ret)
+        self._in_flight_tensors.append((cache, batch, Q, O, given, tree, lse))
         return ret
 
     def paged_layer(self, X, w_attn, Wq, Wk, Wv, Wo, w_ffn, Wg, Wu, Wd, X_out, format, d_model, Hq, N_mlp, attn_scale,
