@@ -444,7 +444,11 @@ M4_API int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batc
  * not NULL). */
 M4_API int m4_bridge_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, float* sums, size_t sums_bytes,
                                     const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget,
-                                    uint32_t sinks, uint32_t recent, int32_t* kept, size_t kept_bytes, int32_t* kv_len_out);
+                                    uint32_t sinks, uint32_t recent, int32_t* kept, size_t kept_bytes, int32_t* kv_len_out,
+                                    void* ws, size_t ws_bytes);
+/* Bytes of its workspace, device memory of any contents, 16-byte aligned; 0 for many or
+ * short sequences (ws may be NULL then).  Calls that may run at the same time need one each. */
+M4_API size_t m4_bridge_kv_evict_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch);
 
 /* A transformer block over the cache: m4_bridge_prefill_layer_ex with the
  * batch's rows as its prompt and the paged cache in place of one call's keys --
@@ -495,7 +499,8 @@ M4_API int m4_bridge_validate_kv_cache_weigh(const m4_kv_cache_t* cache, const m
 M4_API int m4_bridge_validate_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums,
                                              size_t sums_bytes, const int32_t* table_out, uint32_t out_pages,
                                              uint32_t out_stride, uint32_t budget, uint32_t sinks, uint32_t recent,
-                                             const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out);
+                                             const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out,
+                                             const void* ws, size_t ws_bytes);
 
 /* Run subsequent work on `stream` (a hipStream_t, e.g. torch's current
  * stream); NULL restores the bridge's own stream.  Returns 0 or -1. */

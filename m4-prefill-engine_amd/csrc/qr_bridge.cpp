@@ -1144,28 +1144,41 @@ int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* ba
     return launched(qr::launch_kv_weigh(p, g_stream), "kv_cache_weigh");
 }
 
+size_t m4_bridge_kv_evict_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch) {
+    if (!cache || !batch) return 0;
+    qr::EvictParams p{};
+    p.geom.Hkv = cache->Hkv;
+    p.batch.B = batch->B;
+    p.max_kv = batch->max_kv;
+    return qr::kv_evict_workspace(p);
+}
+
 int m4_bridge_validate_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums,
                                       size_t sums_bytes, const int32_t* table_out, uint32_t out_pages, uint32_t out_stride,
                                       uint32_t budget, uint32_t sinks, uint32_t recent, const int32_t* kept,
-                                      size_t kept_bytes, const int32_t* kv_len_out) {
+                                      size_t kept_bytes, const int32_t* kv_len_out, const void* ws, size_t ws_bytes) {
     bool empty;
-    return qr::validate_evict(cache, batch, sums, sums_bytes, table_out, out_pages, out_stride, budget, sinks, recent, kept,
-                              kept_bytes, kv_len_out, &empty);
+    const int rc = qr::validate_evict(cache, batch, sums, sums_bytes, table_out, out_pages, out_stride, budget, sinks, recent,
+                                      kept, kept_bytes, kv_len_out, ws, &empty);
+    if (rc || empty) return rc;
+    const size_t need = m4_bridge_kv_evict_workspace(cache, batch);
+    return need && (!ws || ws_bytes < need) ? -2 : 0;
 }
 
 int m4_bridge_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, float* sums, size_t sums_bytes,
                              const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget,
-                             uint32_t sinks, uint32_t recent, int32_t* kept, size_t kept_bytes, int32_t* kv_len_out) {
+                             uint32_t sinks, uint32_t recent, int32_t* kept, size_t kept_bytes, int32_t* kv_len_out,
+                             void* ws, size_t ws_bytes) {
     if (!g_initialized) return -1;
-    bool empty;
-    const int rc = qr::validate_evict(cache, batch, sums, sums_bytes, table_out, out_pages, out_stride, budget, sinks, recent,
-                                      kept, kept_bytes, kv_len_out, &empty);
-    if (rc || empty) return rc;
+    const int rc = m4_bridge_validate_kv_cache_evict(cache, batch, sums, sums_bytes, table_out, out_pages, out_stride, budget,
+                                                     sinks, recent, kept, kept_bytes, kv_len_out, ws, ws_bytes);
+    if (rc || batch->B == 0) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
     if (!dev.owns_all(cache->pages, batch->kv_len, batch->page_table, sums, table_out, kept, kv_len_out)) return -2;
     const qr::EvictParams p{cache->D, cache->format, cache_geom(cache), batch_view(batch, 0), batch->max_kv, budget, sinks,
-                            recent, sums, table_out, out_pages, out_stride, kept, kv_len_out};
+                            recent, sums, table_out, out_pages, out_stride, kept, kv_len_out, static_cast<uint8_t*>(ws)};
+    if (qr::kv_evict_workspace(p) && !dev.owns_all(ws)) return -2;
     return launched(qr::launch_kv_evict(p, g_stream), "kv_cache_evict");
 }
 

@@ -348,7 +348,7 @@ int validate_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint3
 
 int validate_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums, size_t sums_bytes,
                    const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget, uint32_t sinks,
-                   uint32_t recent, const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out, bool* empty) {
+                   uint32_t recent, const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out, const void* ws, bool* empty) {
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
     if (int rc = check_batch(cache, batch, 1, empty)) return rc;  // no rows are read, its sequences' keys are
@@ -359,7 +359,7 @@ int validate_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const
     if (!all_words(table_out, kept, kv_len_out)) return -2;
     if ((unsigned __int128)kept_bytes < (unsigned __int128)batch->B * cache->Hkv * budget * 4) return -2;
     // other pages and lengths than those that are read while they are written
-    if (table_out == batch->page_table || kv_len_out == batch->kv_len) return -2;
+    if (table_out == batch->page_table || kv_len_out == batch->kv_len || misaligned(ws, 16)) return -2;
     return check_sums(cache, sums, sums_bytes);
 }
 

@@ -49,7 +49,7 @@ int validate_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint3
                    uint32_t H, float scale, const float* sums, size_t sums_bytes, bool* empty);
 int validate_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, const float* sums, size_t sums_bytes,
                    const int32_t* table_out, uint32_t out_pages, uint32_t out_stride, uint32_t budget, uint32_t sinks,
-                   uint32_t recent, const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out, bool* empty);
+                   uint32_t recent, const int32_t* kept, size_t kept_bytes, const int32_t* kv_len_out, const void* ws, bool* empty);
 // all of a layer's arguments but its tensors
 int validate_layer(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rope_axes_t* rope,
                    const int32_t* positions, uint32_t position_stride, int format, uint32_t d_model, uint32_t Hq,

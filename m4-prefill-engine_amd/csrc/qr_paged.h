@@ -179,7 +179,9 @@ struct EvictParams {
     const int32_t* table_out;
     uint32_t out_pages, out_stride;
     int32_t *kept, *len_out;
+    uint8_t* ws;
 };
+size_t kv_evict_workspace(const EvictParams& p);
 hipError_t launch_kv_evict(const EvictParams& p, hipStream_t st);
 
 // The rows of sequence b that a call has, and the position of the first of them.

@@ -272,147 +272,422 @@ hipError_t launch_kv_weigh(const WeighParams& p, hipStream_t st) {
 // kernel finds them, another copies them to pages of their own, so that no copy waits for
 // another and pages that sequences share stay as they are.
 
-// Weights as integers of the same order; 0 for a place that is not there, the top for one that
-// is kept in any case, next to it NaN.
+// Weights as integers of the same order, from 0x007fffff (-infinity) on; 0xffffffff for a place
+// that is kept in any case, next to it NaN; 0 for one that is not there.
 __device__ __forceinline__ uint32_t order_of(float w) {
-    if (w != w) return 0xfffffffeu;
-    const uint32_t u = f32_bits(w == 0.0f ? 0.0f : w);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = f32_bits(w + 0.0f);  // -0 is 0
+    const uint32_t k = u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+    return w != w ? 0xfffffffeu : k;
 }
 
-// A workgroup a sequence and KV head.  The budget-th largest is found digit by digit, eight bits
-// at a time from the top, by counting; then the places at or above it are written in order.
-// Keys stay in LDS where it holds them (as many as expected, up to kHeldKeys), else they are
-// formed again from the sums.
-constexpr int kPickThreads = 1024;
-constexpr uint32_t kHeldKeys = 32768, kCopies = 16;
-__global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(EvictParams p, uint32_t held_keys) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    u4_t* held = reinterpret_cast<u4_t*>(smem);
-    __shared__ uint32_t bins[256 * kCopies];
-    __shared__ uint32_t wave_sum[kPickThreads / 64], found[2];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t pmask = (1u << p.geom.log2_page) - 1;
-    for (uint64_t item = blockIdx.x; item < (uint64_t)p.batch.B * p.geom.Hkv; item += gridDim.x) {
-        const uint32_t b = (uint32_t)(item / p.geom.Hkv), hk = (uint32_t)(item % p.geom.Hkv);
+// The budget-th largest key is found by its leading bits: how many keys have each value of 11
+// bits is counted in LDS (kCopies counters each, against lanes that meet), which names the value
+// that it has.  The keys that share it are few as a rule: up to kList of them are gathered and
+// ranked against each other, more are counted again by the next bits.  Then the places that stay
+// are written in order.  All loops are kept as loops: unrolled, with the keys in registers,
+// most of the 17 KB of code ran once and was waited for (27 us for 64 caches of 8 heads and up to
+// 8192 keys).
+//
+// A workgroup does this for a sequence and KV head, with the keys in LDS (as many as expected,
+// up to kHeld; more are formed again for each sweep).  Where these are few and long, it is done
+// in three launches by a workgroup every kSegment places: each counts its own and leaves the
+// counts (evict_pick_kernel), adds up all and gathers its keys of that value (evict_gather_kernel),
+// and ranks what all have gathered and writes its places (evict_place_kernel).  One request of
+// 131072 keys: 123 us by one workgroup a head.
+constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
+constexpr uint32_t kCopies = 4, kBins = 2048, kList = 1024, kHeld = 24576;
+constexpr uint32_t kSegment = 8192, kGathered = 16384;
+
+// Of a sequence and KV head that is split: the leading bits sought, how many are wanted at or
+// below them, how many have them, how many stay.
+struct alignas(16) PickNote {
+    uint32_t digit, want, share, m;
+};
+// workspace: a note an item, counts [item][segment][kBins] and how many of a segment lie above
+// the bits sought, gathered keys [item][kGathered]
+struct PickSpace {
+    PickNote* notes;
+    uint16_t* counts;
+    uint32_t* above;
+    uint32_t* keys;
+    __host__ __device__ PickSpace(uint8_t* ws, uint64_t items, uint32_t segments) {
+        notes = reinterpret_cast<PickNote*>(ws);
+        keys = reinterpret_cast<uint32_t*>(notes + items);
+        above = keys + items * kGathered;
+        counts = reinterpret_cast<uint16_t*>(above + (items * segments + 3) / 4 * 4);
+    }
+    static size_t bytes(uint64_t items, uint32_t segments) {
+        return items * (sizeof(PickNote) + kGathered * 4) + (items * segments + 3) / 4 * 16 + items * segments * kBins * 2;
+    }
+};
+
+struct PickSeq {
+    uint32_t b, hk, n, last, quads;  // places that the table holds; the first of the last `recent`; n in fours
+    const int32_t* table;
+    __device__ __forceinline__ PickSeq(const EvictParams& p, uint64_t item) {
+        b = (uint32_t)(item / p.geom.Hkv);
+        hk = (uint32_t)(item % p.geom.Hkv);
         const int len = max(p.batch.kv_len[b], 0);
-        const uint32_t n = (uint32_t)min((uint64_t)len, (uint64_t)p.batch.table_pages << p.geom.log2_page);
-        const int64_t last = (int64_t)len - (int64_t)p.recent;  // kept from there on
-        const uint32_t quads = (n + 3) / 4;
-        auto form = [&](uint32_t q) {
-            u4_t k{};
-            const uint32_t page = (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + (4 * q >> p.geom.log2_page)];
-            if (page >= p.geom.num_pages) return k;
-            const f4_t w = *reinterpret_cast<const f4_t*>(p.sums + (((size_t)page * p.geom.Hkv + hk) << p.geom.log2_page) + (4 * q & pmask));
+        n = (uint32_t)min((uint64_t)len, (uint64_t)p.batch.table_pages << p.geom.log2_page);
+        last = (uint32_t)max((int64_t)len - (int64_t)p.recent, (int64_t)0);
+        quads = (n + 3) / 4;
+        table = p.batch.table + (size_t)b * p.batch.table_stride;
+    }
+    // keys of places 4 q .. 4 q + 3
+    __device__ __forceinline__ u4_t keys(const EvictParams& p, uint32_t q) const {
+        const uint32_t page = (uint32_t)table[4 * q >> p.geom.log2_page];
+        if (page >= p.geom.num_pages) return u4_t{};
+        const f4_t w = *reinterpret_cast<const f4_t*>(p.sums + (((size_t)page * p.geom.Hkv + hk) << p.geom.log2_page) +
+                                                      (4 * q & ((1u << p.geom.log2_page) - 1)));
+        u4_t k;
+#pragma unroll
+        for (int e = 0; e < 4; e++) k[e] = order_of(w[e]);
+        if (4 * q < p.sinks || 4 * q + 4 > min(last, n))
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint32_t at = 4 * q + e;
-                if (at < n) k[e] = at < p.sinks || (int64_t)at >= last ? 0xffffffffu : order_of(w[e]);
+                if (4 * q + e < p.sinks || 4 * q + e >= last) k[e] = 0xffffffffu;
+                if (4 * q + e >= n) k[e] = 0;
             }
-            return k;
-        };
-        const bool hold = n <= held_keys;
-        auto keys_of = [&](uint32_t q) { return hold ? held[q] : form(q); };
-        // those that are there
+        return k;
+    }
+    // whether it is split over the workgroups of `segments` segments
+    __device__ __forceinline__ bool split(uint32_t segments) const { return n > 2 * kSegment && n <= segments * kSegment; }
+};
+
+struct PickShared {
+    uint32_t bins[kBins * kCopies];
+    uint32_t list[kList];
+    uint32_t wave_sum[2][kPickWaves], found[3], listed;
+};
+
+__device__ __forceinline__ void clear_bins(PickShared& sh) {
+#pragma unroll 1
+    for (uint32_t x = threadIdx.x; x < kBins * kCopies / 4; x += kPickThreads) reinterpret_cast<u4_t*>(sh.bins)[x] = u4_t{};
+    __syncthreads();
+}
+// How many keys have the values 2 tid and 2 tid + 1.
+__device__ __forceinline__ u2_t bins_of(const PickShared& sh) {
+    const u4_t* v = reinterpret_cast<const u4_t*>(sh.bins) + 2 * threadIdx.x;
+    return u2_t{v[0].x + v[0].y + v[0].z + v[0].w, v[1].x + v[1].y + v[1].z + v[1].w};
+}
+// Of values counted a lane two each: found[0] the one that holds the want-th largest key, found[1] how many
+// of its keys are wanted, found[2] how many it has.  Returns how many keys were counted; with
+// `first` the first value does not count, and nothing is found where the others are at most `want`.
+__device__ __forceinline__ uint32_t find_value(PickShared& sh, u2_t c, uint32_t want, bool first) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (first && tid == 0) c.x = 0;
+    uint32_t above = c.x + c.y;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        const uint32_t y = (uint32_t)__shfl_down((int)above, x);
+        if (lane + x < 64) above += y;
+    }
+    if (lane == 0) sh.wave_sum[0][wave] = above;
+    __syncthreads();
+    uint32_t all = lane < (uint32_t)kPickWaves ? sh.wave_sum[0][lane] : 0, behind = lane > wave ? all : 0;
+#pragma unroll
+    for (int x = 1; x < kPickWaves; x <<= 1) {
+        all += (uint32_t)__shfl_xor((int)all, x);
+        behind += (uint32_t)__shfl_xor((int)behind, x);
+    }
+    all = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
+    above += (uint32_t)__builtin_amdgcn_readfirstlane((int)behind) - c.x - c.y;
+    if (first && all <= want) return all;
+    if (above < want && want <= above + c.x + c.y) {
+        const bool second = want <= above + c.y;
+        sh.found[0] = 2 * tid + second;
+        sh.found[1] = want - above - (second ? 0 : c.y);
+        sh.found[2] = second ? c.y : c.x;
+    }
+    __syncthreads();
+    return all;
+}
+// The want-th largest of `share` keys in the list (1 .. kList): found[0], and found[1] how many of those alike are wanted.
+__device__ __forceinline__ void rank_list(PickShared& sh, uint32_t share, uint32_t want) {
+    const uint32_t tid = threadIdx.x;
+    if (tid < (0u - share & 7)) sh.list[share + tid] = 0;
+    __syncthreads();
+    if (tid / 64 * 64 < share) {
+        const uint32_t k = tid < share ? sh.list[tid] : 0;
+        uint32_t larger = 0, same = 0;
+#pragma unroll 1
+        for (uint32_t x = 0; x < share; x += 8) {
+            const u4_t u = *reinterpret_cast<const u4_t*>(&sh.list[x]), v = *reinterpret_cast<const u4_t*>(&sh.list[x + 4]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                larger += (u[e] > k ? 1 : 0) + (v[e] > k ? 1 : 0);
+                same += (u[e] == k ? 1 : 0) + (v[e] == k ? 1 : 0);
+            }
+        }
+        if (tid < share && larger < want && want <= larger + same) {  // alike in all that are the one sought
+            sh.found[0] = k;
+            sh.found[1] = want - larger;
+        }
+    }
+    __syncthreads();
+}
+// Places of fours q0 .. q1 whose keys lie above `least`, and the first `equal` at it (none
+// where least is 0), written in order; before them are above0 and equal0.  Sums that another
+// stream changes meanwhile give other places, but no more than `room`.
+template <typename KEYS>
+__device__ __forceinline__ void write_places(PickShared& sh, KEYS keys, uint32_t q0, uint32_t q1, uint32_t least, uint32_t equal,
+                                             uint32_t above0, uint32_t equal0, int32_t* out, uint32_t room) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t turn = 0;
+#pragma unroll 1
+    for (; q0 < q1; q0 += kPickThreads, turn ^= 1) {
+        const uint32_t q = q0 + tid;
+        const u4_t k = q < q1 ? keys(q) : u4_t{};
+        // how many lie above it and, in the high half, at it
         uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) mine += k[e] > least ? 1u : (k[e] == least && least ? 0x10000u : 0u);
+        uint32_t before = mine;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t y = (uint32_t)__shfl_up((int)before, x);
+            if (lane >= (uint32_t)x) before += y;
+        }
+        if (lane == 63) sh.wave_sum[turn][wave] = before;
+        __syncthreads();  // the other half may still be read by waves that are behind
+        uint32_t sum = lane < (uint32_t)kPickWaves ? sh.wave_sum[turn][lane] : 0, others = lane < wave ? sum : 0;
+#pragma unroll
+        for (int x = 1; x < kPickWaves; x <<= 1) {
+            sum += (uint32_t)__shfl_xor((int)sum, x);
+            others += (uint32_t)__shfl_xor((int)others, x);
+        }
+        sum = (uint32_t)__builtin_amdgcn_readfirstlane((int)sum);
+        before += (uint32_t)__builtin_amdgcn_readfirstlane((int)others) - mine;
+        uint32_t ne = equal0 + (before >> 16), to = above0 + (before & 0xffffu) + min(ne, equal);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool same = k[e] == least && least, stays = k[e] > least || (same && ne < equal);
+            if (stays && to < room) out[to] = (int32_t)(4 * q + e);
+            to += stays;
+            ne += same;
+        }
+        above0 += sum & 0xffffu;
+        equal0 += sum >> 16;
+    }
+}
+__device__ __forceinline__ void end_places(const EvictParams& p, const PickSeq& s, uint32_t m, int32_t* out) {
+#pragma unroll 1
+    for (uint32_t x = m + threadIdx.x; x < p.budget; x += kPickThreads) out[x] = -1;
+    if (s.hk == 0 && threadIdx.x == 0) p.len_out[s.b] = (int32_t)m;
+}
+
+// From the bits of the key sought above `low`, `prefix`, which `share` of the keys have, to all of
+// them; want: how many of the largest of these are wanted, then of those alike.
+template <typename KEYS>
+__device__ __forceinline__ void settle(PickShared& sh, KEYS keys, uint32_t quads, uint32_t low, uint32_t share, uint32_t& prefix,
+                                       uint32_t& want) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    if (tid == 0) sh.listed = 0;
+    while (low && share > kList) {
+        const uint32_t top = low;
+        low = low == 21 ? 10 : 0;
+        clear_bins(sh);
+#pragma unroll 1
         for (uint32_t q = tid; q < quads; q += kPickThreads) {
-            const u4_t k = form(q);
-            if (hold) held[q] = k;
+            const u4_t k = keys(q);
 #pragma unroll
-            for (int e = 0; e < 4; e++) mine += k[e] != 0;
+            for (int e = 0; e < 4; e++)
+                if (k[e] >> top == prefix) atomicAdd(&sh.bins[(k[e] >> low & ((1u << (top - low)) - 1)) * kCopies + lane % kCopies], 1u);
         }
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) mine += __shfl_xor((int)mine, x);
-        if (lane == 0) wave_sum[wave] = mine;
         __syncthreads();
-        uint32_t there = 0;
+        find_value(sh, bins_of(sh), want, false);
+        prefix = prefix << (top - low) | sh.found[0];
+        want = sh.found[1];
+        share = sh.found[2];
+    }
+    __syncthreads();  // found is read, listed is clear
+    if (!low) return;
+    uint32_t own = 0;
+    asm volatile("" : "+v"(own));  // a lane's own address: lanes that meet are few
+#pragma unroll 1
+    for (uint32_t q = tid; q < quads; q += kPickThreads) {
+        const u4_t k = keys(q);
 #pragma unroll
-        for (int x = 0; x < kPickThreads / 64; x++) there += wave_sum[x];
-        const uint32_t m = min(p.budget, there);
-        uint32_t least = 0, equal = 0;  // kept: above `least`, and the first `equal` at it
-        if (m < there) {
-            uint32_t prefix = 0, want = m;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (uint32_t x = tid; x < 256 * kCopies; x += kPickThreads) bins[x] = 0;
-                __syncthreads();
-                for (uint32_t q = tid; q < quads; q += kPickThreads) {
-                    const u4_t k = keys_of(q);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (k[e] && (shift == 24 || k[e] >> (shift + 8) == prefix)) atomicAdd(&bins[(k[e] >> shift & 255) * kCopies + lane % kCopies], 1u);
-                }
-                __syncthreads();
-                if (tid < 256) {
-                    uint32_t of = 0;
-#pragma unroll
-                    for (uint32_t x = 0; x < kCopies; x++) of += bins[tid * kCopies + (x + tid) % kCopies];
-                    bins[tid * kCopies] = of;
-                }
-                __syncthreads();
-                if (wave == 0) {  // a lane four digits; how many lie above them
-                    uint32_t of[4], sum = 0;
-#pragma unroll
-                    for (int x = 0; x < 4; x++) sum += of[x] = bins[(4 * lane + x) * kCopies];
-                    uint32_t above = sum;
-#pragma unroll
-                    for (int x = 1; x < 64; x <<= 1) {
-                        const uint32_t y = (uint32_t)__shfl_down((int)above, x);
-                        if (lane + x < 64) above += y;
-                    }
-                    above -= sum;
-#pragma unroll
-                    for (int x = 3; x >= 0; x--) {
-                        if (above < want && want <= above + of[x]) {
-                            found[0] = 4 * lane + x;
-                            found[1] = want - above;
-                        }
-                        above += of[x];
-                    }
-                }
-                __syncthreads();
-                prefix = prefix << 8 | found[0];
-                want = found[1];
+        for (int e = 0; e < 4; e++)
+            if (k[e] >> low == prefix) {
+                const uint32_t at = atomicAdd(&sh.listed + own, 1u);
+                if (at < kList) sh.list[at] = k[e];
             }
-            least = prefix;
-            equal = want;
+    }
+    __syncthreads();
+    rank_list(sh, share, want);
+    prefix = sh.found[0];
+    want = sh.found[1];
+}
+
+// All of it by one workgroup; the keys of up to held_keys places are held.
+__device__ __forceinline__ void pick_alone(const EvictParams& p, const PickSeq& s, PickShared& sh, u4_t* held, uint32_t held_keys) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const bool hold = s.n <= held_keys;
+    auto keys_of = [&](uint32_t q) { return hold ? held[q] : s.keys(p, q); };
+    clear_bins(sh);
+#pragma unroll 2
+    for (uint32_t q = tid; q < s.quads; q += kPickThreads) {
+        const u4_t k = s.keys(p, q);
+        if (hold) held[q] = k;
+#pragma unroll
+        for (int e = 0; e < 4; e++) atomicAdd(&sh.bins[(k[e] >> 21) * kCopies + lane % kCopies], 1u);
+    }
+    __syncthreads();
+    // places that are not there have the lowest value to themselves
+    const uint32_t there = find_value(sh, bins_of(sh), p.budget, true);
+    uint32_t least = 0, equal = 0;
+    if (there > p.budget) {
+        least = sh.found[0];
+        equal = sh.found[1];
+        settle(sh, keys_of, s.quads, 21, sh.found[2], least, equal);
+    }
+    int32_t* out = p.kept + ((size_t)s.b * p.geom.Hkv + s.hk) * p.budget;
+    __syncthreads();
+    write_places(sh, keys_of, 0, s.quads, least, equal, 0, 0, out, p.budget);
+    end_places(p, s, min(there, p.budget), out);
+    __syncthreads();
+}
+
+// segments > 1: a workgroup a segment of each item, else one an item.
+__global__ void __launch_bounds__(kPickThreads, 8) evict_pick_kernel(EvictParams p, uint32_t held_keys, uint32_t segments) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ __attribute__((aligned(16))) PickShared sh;
+    const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
+    for (uint64_t x = blockIdx.x; x < items * segments; x += gridDim.x) {
+        const uint64_t item = x / segments;
+        const uint32_t seg = (uint32_t)(x % segments);
+        const PickSeq s(p, item);
+        if (!s.split(segments)) {
+            if (seg == 0) pick_alone(p, s, sh, reinterpret_cast<u4_t*>(smem), held_keys);
+            continue;
         }
-        int32_t* out = p.kept + ((size_t)b * p.geom.Hkv + hk) * p.budget;
-        // counts of those above and at the threshold, 16 bits each
-        uint32_t above0 = 0, equal0 = 0;
-        for (uint32_t q0 = 0; q0 < quads; q0 += kPickThreads) {
-            const uint32_t q = q0 + tid;
-            const u4_t k = q < quads ? keys_of(q) : u4_t{};
-            uint32_t c = 0;
+        clear_bins(sh);
+        const uint32_t q1 = min((seg + 1) * (kSegment / 4), s.quads);
+#pragma unroll 2
+        for (uint32_t q = seg * (kSegment / 4) + threadIdx.x; q < q1; q += kPickThreads) {
+            const u4_t k = s.keys(p, q);
 #pragma unroll
-            for (int e = 0; e < 4; e++) c += (k[e] > least ? 1u : 0u) + (k[e] == least && k[e] ? 0x10000u : 0u);
-            uint32_t incl = c;
-#pragma unroll
-            for (int x = 1; x < 64; x <<= 1) {
-                const uint32_t y = (uint32_t)__shfl_up((int)incl, x);
-                if (lane >= (uint32_t)x) incl += y;
-            }
-            __syncthreads();
-            if (lane == 63) wave_sum[wave] = incl;
-            __syncthreads();
-            uint32_t before = incl - c, all = 0;
-#pragma unroll
-            for (uint32_t x = 0; x < kPickThreads / 64; x++) {
-                if (x < wave) before += wave_sum[x];
-                all += wave_sum[x];
-            }
-            uint32_t na = above0 + (before & 0xffffu), ne = equal0 + (before >> 16);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool a = k[e] > least, at = k[e] == least && k[e];
-                if (a || (at && ne < equal)) out[na + min(ne, equal)] = (int32_t)(4 * q + e);
-                na += a;
-                ne += at;
-            }
-            above0 += all & 0xffffu;
-            equal0 += all >> 16;
+            for (int e = 0; e < 4; e++) atomicAdd(&sh.bins[(k[e] >> 21) * kCopies + threadIdx.x % kCopies], 1u);
         }
-        for (uint32_t x = m + tid; x < p.budget; x += kPickThreads) out[x] = -1;
-        if (hk == 0 && tid == 0) p.len_out[b] = (int32_t)m;
+        __syncthreads();
+        const u2_t c = bins_of(sh);
+        const PickSpace ws(p.ws, items, segments);
+        *reinterpret_cast<uint32_t*>(ws.counts + (item * segments + seg) * kBins + 2 * threadIdx.x) = c.x | c.y << 16;
+        __syncthreads();
+    }
+}
+
+// Sum over the workgroup, by one counter in LDS.
+__device__ __forceinline__ uint32_t sum_of_all(PickShared& sh, uint32_t v) {
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    uint32_t own = 0;
+    asm volatile("" : "+v"(own));
+    if (v) atomicAdd(&sh.listed + own, v);
+    __syncthreads();
+    const uint32_t sum = sh.listed;
+    __syncthreads();
+    return sum;
+}
+
+__global__ void __launch_bounds__(kPickThreads, 8) evict_gather_kernel(EvictParams p, uint32_t segments) {
+    __shared__ __attribute__((aligned(16))) PickShared sh;
+    const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
+    const uint32_t tid = threadIdx.x;
+    const PickSpace ws(p.ws, items, segments);
+    for (uint64_t x = blockIdx.x; x < items * segments; x += gridDim.x) {
+        const uint64_t item = x / segments;
+        const uint32_t seg = (uint32_t)(x % segments);
+        const PickSeq s(p, item);
+        const uint32_t used = (s.n + kSegment - 1) / kSegment;
+        if (!s.split(segments) || seg >= used) continue;
+        const uint16_t* counts = ws.counts + item * segments * kBins;
+        u2_t c{}, mine{};
+#pragma unroll 4
+        for (uint32_t y = 0; y < used; y++) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(counts + (size_t)y * kBins + 2 * tid);
+            const u2_t w = {v & 0xffffu, v >> 16};
+            c += w;
+            if (y == seg) mine = w;
+        }
+        const uint32_t there = find_value(sh, c, p.budget, true);
+        PickNote note{0, 0, 0, there};
+        if (there > p.budget) note = PickNote{sh.found[0], sh.found[1], sh.found[2], p.budget};
+        const uint32_t above = sum_of_all(sh, (2 * tid > note.digit ? mine.x : 0) + (2 * tid + 1 > note.digit ? mine.y : 0));
+        if (tid == 0) {
+            ws.above[item * segments + seg] = above;
+            if (seg == 0) ws.notes[item] = note;
+        }
+        if (note.share == 0 || note.share > kGathered) continue;
+        uint32_t before = 0;
+        for (uint32_t y = tid; y < seg; y += kPickThreads) before += counts[(size_t)y * kBins + note.digit];
+        uint32_t* to = ws.keys + item * kGathered;
+        before = sum_of_all(sh, before);
+        if (tid == 0) sh.listed = 0;
+        __syncthreads();
+        uint32_t own = 0;
+        asm volatile("" : "+v"(own));
+        const uint32_t q1 = min((seg + 1) * (kSegment / 4), s.quads);
+#pragma unroll 2
+        for (uint32_t q = seg * (kSegment / 4) + tid; q < q1; q += kPickThreads) {
+            const u4_t k = s.keys(p, q);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (k[e] >> 21 == note.digit) {
+                    const uint32_t at = before + atomicAdd(&sh.listed + own, 1u);
+                    if (at < kGathered) to[at] = k[e];
+                }
+        }
+        __syncthreads();
+    }
+}
+
+__global__ void __launch_bounds__(kPickThreads, 8) evict_place_kernel(EvictParams p, uint32_t segments) {
+    __shared__ __attribute__((aligned(16))) PickShared sh;
+    const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
+    const uint32_t tid = threadIdx.x;
+    const PickSpace ws(p.ws, items, segments);
+    for (uint64_t x = blockIdx.x; x < items * segments; x += gridDim.x) {
+        const uint64_t item = x / segments;
+        const uint32_t seg = (uint32_t)(x % segments);
+        const PickSeq s(p, item);
+        const uint32_t used = (s.n + kSegment - 1) / kSegment;
+        if (!s.split(segments) || seg >= used) continue;
+        const PickNote note = ws.notes[item];
+        if (note.share > kGathered) {  // too many alike to gather
+            if (seg == 0) pick_alone(p, s, sh, nullptr, 0);
+            continue;
+        }
+        uint32_t least = note.digit, equal = note.want;
+        const uint32_t* gathered = ws.keys + item * kGathered;
+        if (note.share) {
+            auto keys = [&](uint32_t q) {
+                u4_t k = reinterpret_cast<const u4_t*>(gathered)[q];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (4 * q + e >= note.share) k[e] = 0;
+                return k;
+            };
+            settle(sh, keys, (note.share + 3) / 4, 21, note.share, least, equal);
+        }
+        // what the segments before this one have above it and at it
+        uint32_t above = 0, alike = 0, ahead = 0;
+        for (uint32_t y = tid; y < seg; y += kPickThreads) {
+            above += ws.above[item * segments + y];
+            if (note.share) ahead += ws.counts[(item * segments + y) * kBins + note.digit];
+        }
+        ahead = sum_of_all(sh, ahead);
+        for (uint32_t y = tid; y < min(ahead, kGathered); y += kPickThreads) {
+            above += gathered[y] > least;
+            alike += gathered[y] == least;
+        }
+        above = sum_of_all(sh, above);
+        alike = sum_of_all(sh, alike);
+        int32_t* out = p.kept + ((size_t)s.b * p.geom.Hkv + s.hk) * p.budget;
+        write_places(sh, [&](uint32_t q) { return s.keys(p, q); }, seg * (kSegment / 4), min((seg + 1) * (kSegment / 4), s.quads), least,
+                     equal, above, alike, out, p.budget);
+        if (seg == 0) end_places(p, s, note.m, out);
         __syncthreads();
     }
 }
@@ -420,7 +695,7 @@ __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(EvictParams p,
 // Kept token i becomes token i of the other table's pages: 64 of them a workgroup, of one head.
 // Codes of V lie in groups of four tokens, so four sources' bytes make a word; where the last
 // group is not full, the others of its tokens keep their own.
-constexpr uint32_t kCopyTokens = 64;
+constexpr uint32_t kCopyTokens = 128;
 template <int FMT, int D>
 __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, uint32_t tiles) {
     constexpr uint32_t CB = FMT == QUANT_Q8_0 ? D : D / 2, NB = D / 32, KP = CB / 16, VP = CB / 4;
@@ -435,58 +710,80 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, uint32_t
             __syncthreads();
             if (tid < kCopyTokens) {
                 const uint32_t i = t0 + tid, pi = i >> p.geom.log2_page;
-                const int from = i < p.budget ? kept[i] : -1;
+                int from = i < p.budget ? kept[i] : -1;
+                // what the other kernel wrote, unless the caller writes there or to the table meanwhile: nothing outside is read then either
+                uint32_t sp = 0xffffffffu;
+                if (from >= 0 && (uint32_t)from >> p.geom.log2_page < p.batch.table_pages)
+                    sp = (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)from >> p.geom.log2_page)];
+                if (sp >= p.geom.num_pages) from = -1;
                 uint32_t dp = pi < p.out_pages ? (uint32_t)p.table_out[(size_t)b * p.out_stride + pi] : 0xffffffffu;
                 if (dp >= p.geom.num_pages) dp = 0xffffffffu;
                 dst_page[tid] = dp;
                 live[tid] = from >= 0 && dp != 0xffffffffu;
                 if (tid == 0) some = from >= 0;
-                src_page[tid] = from >= 0 ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)from >> p.geom.log2_page)] : dp;
+                src_page[tid] = from >= 0 ? sp : dp;
                 src_slot[tid] = (uint32_t)(from >= 0 ? from : (int)i) & pmask;
             }
             __syncthreads();
             if (!some) break;  // the kept are the first
-            for (uint32_t x = tid; x < kCopyTokens * KP; x += 256) {
-                const uint32_t t = x / KP, u = x % KP;
-                if (!live[t]) continue;
-                *reinterpret_cast<u4_t*>(head_of(dst_page[t]) + ((t0 + t) & pmask) * CB + 16 * u) =
-                    *reinterpret_cast<const u4_t*>(head_of(src_page[t]) + src_slot[t] * CB + 16 * u);
-            }
-            for (uint32_t x = tid; x < kCopyTokens / 4 * VP; x += 256) {
-                const uint32_t t = x / VP * 4, u = x % VP;
-                if (!live[t]) continue;
-                u4_t w[4];
-                uint32_t k[4];
+            // loaded before anything is stored: the compiler cannot tell that the pages are others
+            constexpr int NK = kCopyTokens * KP / 256, NV = kCopyTokens / 4 * VP / 256, NS = kCopyTokens * NB / 256;
+            u4_t kv[NK], vv[NV][4];
+            uint32_t sv[NS], of_k = 0, of_k2 = 0;
+            float sum = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t slot = src_slot[t + e];
-                    k[e] = slot & 3;
-                    w[e] = *reinterpret_cast<const u4_t*>(head_of(src_page[t + e]) + p.geom.v_off + (slot >> 2) * (4 * CB) + 16 * u);
-                }
-                const uint32_t lo = k[0] | (4 + k[1]) << 8 | 0x0c0c0000u, hi = 0x0c0cu | k[2] << 16 | (4 + k[3]) << 24;
+            for (int i = 0; i < NK; i++) {
+                const uint32_t x = tid + 256 * i, t = x / KP, u = x % KP;
+                if (live[t]) kv[i] = *reinterpret_cast<const u4_t*>(head_of(src_page[t]) + src_slot[t] * CB + 16 * u);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const uint32_t x = tid + 256 * i, t = x / VP * 4, u = x % VP;
+                if (live[t])
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        vv[i][e] = *reinterpret_cast<const u4_t*>(head_of(src_page[t + e]) + p.geom.v_off + (src_slot[t + e] >> 2) * (4 * CB) + 16 * u);
+            }
+            // V's scales block by block, K's and the sum a token
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const uint32_t x = tid + 256 * i, t = x % kCopyTokens, y = x / kCopyTokens, ss = src_slot[t];
+                sv[i] = 0;
+                if (live[t]) sv[i] = *reinterpret_cast<const uint16_t*>(head_of(src_page[t]) + p.geom.vs_off + (((ss >> 2) * NB + y) * 4 + (ss & 3)) * 2);
+            }
+            if (tid < kCopyTokens && live[tid]) {
+                const uint32_t* ks = reinterpret_cast<const uint32_t*>(head_of(src_page[tid]) + p.geom.ks_off + src_slot[tid] * (2 * NB));
+                of_k = ks[0];
+                if constexpr (NB == 4) of_k2 = ks[1];
+                sum = p.sums[(((size_t)src_page[tid] * p.geom.Hkv + hk) << p.geom.log2_page) + src_slot[tid]];
+            }
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const uint32_t x = tid + 256 * i, t = x / KP, u = x % KP;
+                if (live[t]) *reinterpret_cast<u4_t*>(head_of(dst_page[t]) + ((t0 + t) & pmask) * CB + 16 * u) = kv[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const uint32_t x = tid + 256 * i, t = x / VP * 4, u = x % VP;
+                if (!live[t]) continue;
+                const uint32_t k0 = src_slot[t] & 3, k1 = src_slot[t + 1] & 3, k2 = src_slot[t + 2] & 3, k3 = src_slot[t + 3] & 3;
+                const uint32_t lo = k0 | (4 + k1) << 8 | 0x0c0c0000u, hi = 0x0c0cu | k2 << 16 | (4 + k3) << 24;
                 u4_t y;
 #pragma unroll
-                for (int d = 0; d < 4; d++) y[d] = perm(w[1][d], w[0][d], lo) | perm(w[3][d], w[2][d], hi);
+                for (int d = 0; d < 4; d++) y[d] = perm(vv[i][1][d], vv[i][0][d], lo) | perm(vv[i][3][d], vv[i][2][d], hi);
                 *reinterpret_cast<u4_t*>(head_of(dst_page[t]) + p.geom.v_off + ((t0 + t) & pmask) / 4 * (4 * CB) + 16 * u) = y;
             }
-            // scales and sums: a token's of K and its sum, and of V block by block
-            for (uint32_t x = tid; x < kCopyTokens * (1 + NB); x += 256) {
-                const uint32_t t = x % kCopyTokens, y = x / kCopyTokens;
-                if (!live[t]) continue;
-                const uint8_t* src = head_of(src_page[t]);
-                uint8_t* dst = head_of(dst_page[t]);
-                const uint32_t ss = src_slot[t], ds = (t0 + t) & pmask;
-                if (y == 0) {
-                    p.sums[(((size_t)dst_page[t] * p.geom.Hkv + hk) << p.geom.log2_page) + ds] =
-                        p.sums[(((size_t)src_page[t] * p.geom.Hkv + hk) << p.geom.log2_page) + ss];
-                    if constexpr (NB == 4)
-                        *reinterpret_cast<u2_t*>(dst + p.geom.ks_off + ds * 8) = *reinterpret_cast<const u2_t*>(src + p.geom.ks_off + ss * 8);
-                    else
-                        *reinterpret_cast<uint32_t*>(dst + p.geom.ks_off + ds * 4) = *reinterpret_cast<const uint32_t*>(src + p.geom.ks_off + ss * 4);
-                } else {
-                    *reinterpret_cast<uint16_t*>(dst + p.geom.vs_off + (((ds >> 2) * NB + y - 1) * 4 + (ds & 3)) * 2) =
-                        *reinterpret_cast<const uint16_t*>(src + p.geom.vs_off + (((ss >> 2) * NB + y - 1) * 4 + (ss & 3)) * 2);
-                }
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const uint32_t x = tid + 256 * i, t = x % kCopyTokens, y = x / kCopyTokens, ds = (t0 + t) & pmask;
+                if (live[t]) *reinterpret_cast<uint16_t*>(head_of(dst_page[t]) + p.geom.vs_off + (((ds >> 2) * NB + y) * 4 + (ds & 3)) * 2) = (uint16_t)sv[i];
+            }
+            if (tid < kCopyTokens && live[tid]) {
+                const uint32_t ds = (t0 + tid) & pmask;
+                uint32_t* ks = reinterpret_cast<uint32_t*>(head_of(dst_page[tid]) + p.geom.ks_off + ds * (2 * NB));
+                ks[0] = of_k;
+                if constexpr (NB == 4) ks[1] = of_k2;
+                p.sums[(((size_t)dst_page[tid] * p.geom.Hkv + hk) << p.geom.log2_page) + ds] = sum;
             }
         }
     }
@@ -500,16 +797,37 @@ static hipError_t launch_copy(const EvictParams& p, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Workgroups for a sequence and KV head: several where there are fewer of these than CUs and the
+// longest is expected to have places for them.
+static uint32_t pick_segments(const EvictParams& p) {
+    const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
+    if (items >= 256 || p.max_kv <= 2 * kSegment) return 1;
+    const uint32_t most = p.max_kv < 0x7fff0000u ? p.max_kv : 0x7fff0000u;
+    return (most + kSegment - 1) / kSegment;
+}
+
+size_t kv_evict_workspace(const EvictParams& p) {
+    const uint32_t segments = pick_segments(p);
+    return segments > 1 ? PickSpace::bytes((uint64_t)p.batch.B * p.geom.Hkv, segments) : 0;
+}
+
 hipError_t launch_kv_evict(const EvictParams& p, hipStream_t st) {
     if (p.batch.B == 0) return hipSuccess;
-    const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
+    const uint32_t segments = pick_segments(p);
+    const uint64_t groups = (uint64_t)p.batch.B * p.geom.Hkv * segments;
+    const uint32_t held = segments > 1 ? 2 * kSegment : (p.max_kv < kHeld ? (p.max_kv + 1023) / 1024 * 1024 : 0);
+    const dim3 grid((uint32_t)(groups < (1u << 20) ? groups : 1u << 20)), block(kPickThreads);
     static size_t attr[kMaxDevices] = {};
-    const uint32_t held = p.max_kv < kHeldKeys ? (p.max_kv + 1023) / 1024 * 1024 : kHeldKeys;
-    hipError_t e = lds_limit_once((const void*)evict_pick_kernel, kHeldKeys * 4, attr);
+    hipError_t e = lds_limit_once((const void*)evict_pick_kernel, kHeld * 4, attr);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(evict_pick_kernel, dim3((uint32_t)(items < (1u << 20) ? items : 1u << 20)), dim3(kPickThreads), held * 4, st, p, held);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(evict_pick_kernel, grid, block, held * 4, st, p, held, segments);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (segments > 1) {
+        hipLaunchKernelGGL(evict_gather_kernel, grid, block, 0, st, p, segments);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        hipLaunchKernelGGL(evict_place_kernel, grid, block, 0, st, p, segments);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     if (p.format == QUANT_Q8_0) return p.D == 64 ? launch_copy<QUANT_Q8_0, 64>(p, st) : launch_copy<QUANT_Q8_0, 128>(p, st);
     return p.D == 64 ? launch_copy<QUANT_Q4_0, 64>(p, st) : launch_copy<QUANT_Q4_0, 128>(p, st);
 }

@@ -98,7 +98,8 @@ SIGNATURES = {
     "m4_bridge_tree_accept": ([_VP, _U32] + [_VP] * 6, _I),
     "m4_bridge_kv_cache_keep": ([_VP, _VP, _U32, _VP, _VP, _VP], _I),
     "m4_bridge_kv_cache_weigh": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
-    "m4_bridge_kv_cache_evict": ([_VP, _VP, _VP, _SZ, _VP, _U32, _U32, _U32, _U32, _U32, _VP, _SZ, _VP], _I),
+    "m4_bridge_kv_cache_evict": ([_VP, _VP, _VP, _SZ, _VP, _U32, _U32, _U32, _U32, _U32, _VP, _SZ, _VP, _VP, _SZ], _I),
+    "m4_bridge_kv_evict_workspace": ([_VP, _VP], _SZ),
     "m4_bridge_paged_layer": ([_VP] * 13 + [_U32, _VP, _VP, _U32, _I, _U32, _U32, _U32, _F, _U32, _I, _F], _I),
     "m4_bridge_validate_rope_axes": ([_VP, _VP, _U32, _VP, _VP, _U32, _U32, _U32], _I),
     "m4_bridge_validate_kv_cache_append": ([_VP, _VP, _U32, _VP, _VP, _VP, _VP, _U32, _VP, _VP, _U32], _I),
@@ -109,7 +110,7 @@ SIGNATURES = {
     "m4_bridge_validate_tree_accept": ([_VP, _U32] + [_VP] * 6, _I),
     "m4_bridge_validate_kv_cache_keep": ([_VP, _VP, _U32, _VP, _VP, _VP], _I),
     "m4_bridge_validate_kv_cache_weigh": ([_VP, _VP, _U32, _VP, _VP, _U32, _F, _U32, _VP, _SZ], _I),
-    "m4_bridge_validate_kv_cache_evict": ([_VP, _VP, _VP, _SZ, _VP, _U32, _U32, _U32, _U32, _U32, _VP, _SZ, _VP], _I),
+    "m4_bridge_validate_kv_cache_evict": ([_VP, _VP, _VP, _SZ, _VP, _U32, _U32, _U32, _U32, _U32, _VP, _SZ, _VP, _VP, _SZ], _I),
     "m4_bridge_set_stream": ([_VP], _I),
     "m4_bridge_get_stream": ([], _VP),
     "m4_bridge_last_error": ([], ctypes.c_char_p),
@@ -871,12 +872,17 @@ class HIPBridge:
         self._in_flight_tensors.append((cache, batch, Q, lse, sums))
         return ret
 
+    def kv_evict_workspace(self, cache: PagedKVCache, batch: KVBatch) -> int:
+        """Bytes of workspace that kv_cache_evict needs; 0 for many or short sequences."""
+        return int(self._lib.m4_bridge_kv_evict_workspace(cache.ref, batch.ref))
+
     def kv_cache_evict(self, cache: PagedKVCache, batch: KVBatch, sums, table_out, kv_len_out, budget: int, sinks: int = 0,
-                       recent: int = 0, kept=None) -> int:
+                       recent: int = 0, kept=None, workspace=None) -> int:
         """Copies of each sequence and KV head the first `sinks`, the last `recent` and the heaviest other keys by `sums`,
         `budget` together, to the pages of table_out (int32 [B, pages]), in their order and with their sums.
         kv_len_out int32 [B]: how many; kept int32 [B, Hkv, budget]: the places that they had, then -1 (None: not
-        wanted).  The caller goes on with table_out and kv_len_out and has the old pages back."""
+        wanted).  `workspace`: a uint8 device tensor of kv_evict_workspace bytes, where these are any, as
+        dispatch_paged_attn's.  The caller goes on with table_out and kv_len_out and has the old pages back."""
         B = batch.B
         _int32("table_out", table_out, 2)
         if table_out.shape[0] != B:
@@ -891,12 +897,19 @@ class HIPBridge:
             kept = _torch.empty(B, cache.Hkv, budget, dtype=_torch.int32, device=sums.device)
         elif kept.dtype is not _torch.int32 or tuple(kept.shape) != (B, cache.Hkv, budget) or not kept.is_contiguous():
             raise ValueError(f"kept must be a contiguous int32 tensor [{B}, {cache.Hkv}, {budget}]")
+        if workspace is not None and not (isinstance(workspace, _torch.Tensor) and workspace.is_contiguous()):
+            raise ValueError("workspace must be a contiguous tensor")
         self._on_stream_of(sums)
+        given_ws = workspace
+        if workspace is None:
+            need = self.kv_evict_workspace(cache, batch)
+            workspace = _torch.empty(need, dtype=_torch.uint8, device=sums.device) if need else None
         ret = self._lib.m4_bridge_kv_cache_evict(cache.ref, batch.ref, at_sums, held, table_out.data_ptr(), table_out.shape[1],
                                                  table_out.stride(0), budget, sinks, recent, kept.data_ptr(), kept.nbytes,
-                                                 at_len)
+                                                 at_len, workspace.data_ptr() if workspace is not None else None,
+                                                 workspace.nbytes if workspace is not None else 0)
         self._check("m4_bridge_kv_cache_evict", ret)
-        self._in_flight_tensors.append((cache, batch, sums, table_out, kv_len_out, given))
+        self._in_flight_tensors.append((cache, batch, sums, table_out, kv_len_out, given, given_ws))
         return ret
 
     def dispatch_paged_attn(self, cache: PagedKVCache, batch: KVBatch, Q, O, scale: float, token_major: bool = False,

@@ -212,6 +212,10 @@ class Bounded(Setup):
     ([5000], 2, 128, 16, 4999, 0, 3, 0),
     ([90] * 70, 1, 64, 16, 40, 2, 9, 90),
     ([40000, 100], 1, 64, 256, 3001, 5, 100, 10 ** 9),       # longer than what is held
+    ([40000, 100, 16384, 16385], 2, 64, 256, 3001, 5, 100, 40000),   # by several workgroups a head, or one
+    ([41000, 30000], 1, 128, 16, 29000, 0, 0, 41000),                # of the second all but a few
+    ([60000, 40000], 1, 64, 64, 35000, 7, 9, 41000),                 # the first longer than expected
+    ([50000], 1, 64, 32, 60000, 0, 0, 50000),                        # all of them
 ])
 def test_evict(bridge, fmt, lens, Hkv, D, P, budget, sinks, recent, max_kv):
     """Every byte of the pages, the sums, the places and the lengths."""
@@ -236,6 +240,30 @@ def test_evict(bridge, fmt, lens, Hkv, D, P, budget, sinks, recent, max_kv):
             tail[s.table_out[b, i // P]][:, token_bytes(s.pages, i % P)] = True
     np.testing.assert_array_equal(np.where(tail, 0, got), np.where(tail, 0, pages))
     np.testing.assert_array_equal(sums.cpu().numpy().view(np.uint32), out.view(np.uint32))
+
+
+@gpu
+@pytest.mark.parametrize("value", ["zero", "few", "near", "nan"])
+@pytest.mark.parametrize("n,max_kv", [(9000, 9000), (45000, 45000), (45000, 1)])
+def test_evict_where_many_are_alike(bridge, value, n, max_kv):
+    """Sums that share all their bits, or most: the lowest places of the equal ones stay."""
+    import torch
+
+    budget = n // 3
+    s = Bounded(Q8_0, [n], [0], 1, 64, 256, seed=n)
+    s.grow(budget)
+    r = s.rng
+    s.sums[:] = {"zero": lambda k: 0.0, "few": lambda k: r.integers(0, 3, k).astype(np.float32),
+                 "near": lambda k: (np.float32(1) + r.integers(0, 4000, k) * np.float32(2.0 ** -23)).astype(np.float32),
+                 "nan": lambda k: np.where(r.random(k) < 0.5, np.float32("nan"), np.float32(1))}[value](s.sums.shape)
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(i32(n)), dev(s.table), 0, max_kv)
+    kept, length = torch.empty(1, 1, budget, dtype=torch.int32, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+    say("alike", value, n, max_kv)
+    bridge.kv_cache_evict(s.cache(), batch, dev(s.sums), dev(s.table_out), length, budget, sinks=3, recent=50, kept=kept)
+    bridge.synchronize()
+    w = s.sums[s.table[0][np.arange(n) // 256], 0, np.arange(n) % 256]
+    np.testing.assert_array_equal(kept.cpu().numpy()[0, 0], chosen(w, np.ones(n, bool), budget, 3, 50, n))
+    assert int(length[0]) == budget
 
 
 @gpu
@@ -406,8 +434,14 @@ def test_refused_evictions(lib, change, code):  # noqa: F811
     """Among them: the old table or its lengths in the place of the new."""
     a, r = Args(), ctypes.addressof
     change(a)
-    assert lib.m4_bridge_validate_kv_cache_evict(r(a.cache), r(a.batch), a.sums, a.held, a.table, a.pages, a.stride, a.budget, a.sinks,
-                                                 a.recent, a.kept, a.room, a.length) == code
+    call = lambda ws, size: lib.m4_bridge_validate_kv_cache_evict(  # noqa: E731
+        r(a.cache), r(a.batch), a.sums, a.held, a.table, a.pages, a.stride, a.budget, a.sinks, a.recent, a.kept, a.room, a.length, ws, size)
+    assert lib.m4_bridge_kv_evict_workspace(r(a.cache), r(a.batch)) == 0 and call(None, 0) == code
+    if code == 0 and a.batch.B:  # long sequences
+        a.batch.max_kv = 50000
+        need = lib.m4_bridge_kv_evict_workspace(r(a.cache), r(a.batch))
+        assert need > 0
+        assert call(0x900000, need) == 0 and call(0x900000, need - 1) == -2 and call(None, need) == -2 and call(0x900008, need) == -2
 
 
 def test_what_a_call_holds_and_refuses(launched):  # noqa: F811
@@ -420,7 +454,7 @@ def test_what_a_call_holds_and_refuses(launched):  # noqa: F811
     assert [c for c in launched.lib.calls if "stream" not in c] == ["m4_bridge_kv_cache_weigh", "m4_bridge_kv_cache_evict"]
     first, second = launched._in_flight_tensors
     assert any(t is sums for t in first) and any(t is sums for t in second)
-    assert second[-1] is None  # `kept` of the call's own goes back to its stream
+    assert second[-2:] == (None, None)  # `kept` and a workspace of the call's own go back to its stream
     n = len(launched.lib.calls)
     for call in (lambda: launched.kv_cache_weigh(cache, batch, x, lse, sums.half(), 0.1),
                  lambda: launched.kv_cache_weigh(cache, batch, x, lse, sums[:3], 0.1),
