@@ -424,7 +424,8 @@ M4_API int m4_bridge_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch
  * does with the same window; for the batch's new tokens it sets them, whatever
  * they held.  lse as that call's tree form writes it (append, attend, then weigh).
  * Products are of fp16 operands, the cached values, summed in fp32; no order changes.
- * A page that two sequences of a call share: its sums are undefined. */
+ * A page that two sequences of a call share: its sums are undefined.  A call without
+ * rows writes nothing.  B x Hkv, and T x H / Hkv, below 2^31. */
 M4_API int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const m4_rows_t* Q,
                                     const m4_rows_t* lse, uint32_t H, float scale, uint32_t window, float* sums,
                                     size_t sums_bytes);

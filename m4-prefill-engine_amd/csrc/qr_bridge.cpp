@@ -1132,10 +1132,11 @@ int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* ba
     p.lse = values_view(lse);
     p.H = H;
     p.G = H / cache->Hkv;
+    p.of_group = qr::divider(p.G);
     p.D = cache->D;
     p.format = cache->format;
     p.scale = scale;
-    p.window = window;
+    p.window = window < 0x80000000u ? window : 0;  // no position is as far
     p.geom = cache_geom(cache);
     p.batch = batch_view(batch, T);
     p.max_new = batch->max_new;

@@ -343,6 +343,7 @@ int validate_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint3
     if ((uint64_t)T * (H / cache->Hkv) > 0x7fffffffu) return -4;  // rows of a KV head are counted in 32 bits
     if (int rc = check_rows(Q, T, H, cache->D, false)) return rc;
     if (int rc = check_values(lse, T, H, false)) return rc;
+    if ((uint64_t)batch->B * cache->Hkv > 0x7fffffffu) return -4;  // as many are counted in 32 bits
     return check_sums(cache, sums, sums_bytes);
 }
 

@@ -152,10 +152,22 @@ struct KeepParams {
 hipError_t launch_kv_keep(const KeepParams& p, hipStream_t st);
 
 // ---- bounded caches ----
+// Division of numbers below 2^31 by a number that is known before, in three instructions.
+struct Divider {
+    uint32_t by, mul, shift;
+};
+inline Divider divider(uint32_t by) {
+    Divider d{by, 0, 0};
+    while ((1ull << d.shift) < by) d.shift++;
+    d.mul = (uint32_t)(((1ull << 32) * ((1ull << d.shift) - by)) / by + 1);
+    return d;
+}
+
 struct WeighParams {
     RowsView Q;
     ValuesView lse;
     uint32_t H, G, D;
+    Divider of_group;
     int format;
     float scale;
     uint32_t window;
@@ -164,6 +176,7 @@ struct WeighParams {
     uint32_t max_new, max_kv;
     // a launch's: sequences of that many rows a KV head, [min_rows, max_rows)
     uint32_t min_rows, max_rows;
+    uint32_t tile_shift;
     float* sums;  // [num_pages][Hkv][page]
 };
 hipError_t launch_kv_weigh(const WeighParams& p, hipStream_t st);

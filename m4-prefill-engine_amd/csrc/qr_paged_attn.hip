@@ -208,27 +208,6 @@ __device__ __forceinline__ float* slot_of(uint8_t* ws, uint32_t groups, uint32_t
     return reinterpret_cast<float*>(ws + (size_t)groups * sizeof(ItemNote) + ((size_t)w * 2 + which) * slot_bytes<D, R>());
 }
 
-// lane `at`'s value, as a wave-uniform one
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int at) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), at) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, at);
-}
-
-// a / b of wave-uniform numbers that nearly always fit in 32 bits, where a
-// division takes a fifth of the time
-__device__ __forceinline__ uint64_t udiv(uint64_t a, uint64_t b) {
-    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
-    return a / b;
-}
-// share w of nw (at most 2^16) of a line of `total`: total w / nw on, in whole
-// places, so that as many items as shares, alike in cost, are not cut
-__device__ __forceinline__ void share_of(uint64_t total, uint32_t nw, uint32_t w, uint64_t& s0, uint64_t& s1) {
-    const uint64_t each = udiv(total, nw);
-    const uint32_t more = (uint32_t)(total - each * nw);
-    s0 = each * w + more * w / nw;
-    s1 = each * (w + 1) + more * (w + 1) / nw;
-}
-
 struct Seq {
     int q0, n, first;     // first row, new tokens, position of the first of them
     int keys, lo;         // keys that the table holds and a row may see, first that one sees (a multiple of kStep)

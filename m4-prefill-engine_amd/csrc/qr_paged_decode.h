@@ -1,4 +1,5 @@
-// qr_paged_decode.h -- the paged cache's codes as fp16 values, for the kernels that multiply by them.
+// qr_paged_decode.h -- the paged cache's codes as fp16 values, for the kernels that multiply by
+// them, and even shares of a line of work.
 #pragma once
 #include "qr_device.h"
 #include "qr_paged.h"
@@ -70,6 +71,27 @@ __device__ __forceinline__ h8_t k_octet(const uint32_t* k, int kk, h2_t d) {
         e = q4_pair<true>(hi, d, n8);
     }
     return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
+}
+
+// lane `at`'s value, as a wave-uniform one
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int at) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), at) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, at);
+}
+
+// a / b of wave-uniform numbers that nearly always fit in 32 bits, where a
+// division takes a fifth of the time
+__device__ __forceinline__ uint64_t udiv(uint64_t a, uint64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
+}
+// share w of nw (at most 2^16) of a line of `total`: total w / nw on, in whole
+// places, so that as many items as shares, alike in cost, are not cut
+__device__ __forceinline__ void share_of(uint64_t total, uint32_t nw, uint32_t w, uint64_t& s0, uint64_t& s1) {
+    const uint64_t each = udiv(total, nw);
+    const uint32_t more = (uint32_t)(total - each * nw);
+    s0 = each * w + more * w / nw;
+    s1 = each * (w + 1) + more * (w + 1) / nw;
 }
 
 }  // namespace qr

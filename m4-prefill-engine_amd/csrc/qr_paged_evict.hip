@@ -30,106 +30,199 @@ __device__ __forceinline__ WeighSeq weigh_seq(const WeighParams& p, uint32_t b) 
     return s;
 }
 
-// The rows (token, query head) of a KV head that see a key are [lo, hi).
+// Row f of a KV head's rows (token, query head): its offset in a view, in elements.
+template <typename VIEW>
+__device__ __forceinline__ int64_t row_offset(const WeighParams& p, const VIEW& v, int q0, uint32_t hk, uint32_t f) {
+    const uint32_t i = (__umulhi(f, p.of_group.mul) + f) >> p.of_group.shift, q = f - i * p.G;
+    return (int64_t)(q0 + (int)i) * v.ts + (int64_t)(hk * p.G + q) * v.hs;
+}
+// The rows of a KV head that see a key are [lo, hi).
 struct RowRange {
     uint32_t lo, hi;
 };
 __device__ __forceinline__ RowRange rows_of(const WeighParams& p, const WeighSeq& s, int key) {
-    const int64_t i = (int64_t)key - s.first;
+    const int i = key - s.first;  // keys past the last row's are not asked for but for a tile's width
     RowRange r;
-    r.lo = (uint32_t)min(max(i, (int64_t)0), (int64_t)s.n) * p.G;
-    r.hi = p.window ? (uint32_t)min(max(i + p.window, (int64_t)0), (int64_t)s.n) * p.G : (uint32_t)s.n * p.G;
+    r.lo = (uint32_t)min(max(i, 0), s.n) * p.G;
+    r.hi = (uint32_t)(p.window ? min(max(i + (int)p.window, 0), s.n) : s.n) * p.G;
     return r;
 }
 
-// Few rows: four waves of 64 keys each, 16 rows at a time.
+// Few rows: a wave takes 64 keys of a KV head at a time, 16 rows at a time.  All work is one line
+// (per sequence and KV head its tiles of 64 keys), of which each wave has an even share,
+// wherever it begins; two tiles' codes are under way while one is computed.  A
+// wave does little more than two tiles in a step of 64 requests, so what it does once counts:
+// the line is counted in 32 bits (a unit is 64 << tile_shift keys, so that any batch fits).
+// 64 requests of up to 8192 keys, 8 KV heads of 128, 8 bit: 20 us (59 MB: 3.0 TB/s); a workgroup
+// for each 256 keys of a head, which a quarter of them found empty: 34.
+constexpr uint32_t kRowWaves = 2048;  // a power of two: two a SIMD
 template <int FMT, int D>
-__global__ void __launch_bounds__(256) weigh_rows_kernel(WeighParams p, uint32_t tiles) {
+__global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
     constexpr int KK = D / 32, RUN = D / 4, W = FMT == QUANT_Q8_0 ? D / 16 : D / 32;
     constexpr uint32_t CB = 4 * W * 4, NB = D / 32;
     const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t hk = blockIdx.x % p.geom.Hkv, G = p.G;
-    const uint32_t pmask = (1u << p.geom.log2_page) - 1;
+    const uint32_t w = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t G = p.G, pmask = (1u << p.geom.log2_page) - 1, unit_shift = 6 + p.tile_shift;
     const float c = p.scale * 1.4426950408889634f;  // log2 units
-    for (uint32_t b = blockIdx.y; b < p.batch.B; b += gridDim.y) {
+
+    auto units_of = [&](const WeighSeq& s) {
+        return (((uint32_t)s.keys + (1u << unit_shift) - 1) >> unit_shift) - ((uint32_t)s.lo >> unit_shift);
+    };
+    const uint32_t per = (p.batch.B + 63) / 64;
+    const uint32_t b_lo = min(lane * per, p.batch.B), b_hi = min(b_lo + per, p.batch.B);
+    uint32_t mine = 0;
+#pragma unroll 1
+    for (uint32_t x = b_lo; x < b_hi; x++) mine += units_of(weigh_seq(p, x)) * p.geom.Hkv;
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = (uint32_t)__shfl_up((int)incl, o);
+        if (lane >= o) incl += x;
+    }
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    const uint32_t waves = gridDim.x * 4, log2_waves = 31 - __builtin_clz(waves);
+    uint32_t cur = (uint32_t)((uint64_t)total * w >> log2_waves);
+    const uint32_t end = (uint32_t)((uint64_t)total * (w + 1) >> log2_waves);
+    if (cur == end) return;
+    const bool here = incl - mine <= cur && cur < incl;
+    uint32_t b = b_lo, off = cur - (incl - mine);
+    if (here)
+#pragma unroll 1
+        for (; b + 1 < b_hi; b++) {
+            const uint32_t all = units_of(weigh_seq(p, b)) * p.geom.Hkv;
+            if (off < all) break;
+            off -= all;
+        }
+    const int at_lane = __ffsll((unsigned long long)__ballot(here)) - 1;
+    b = __builtin_amdgcn_readlane(b, at_lane);
+    off = __builtin_amdgcn_readlane(off, at_lane);
+
+#pragma unroll 1
+    while (cur < end && b < p.batch.B) {
         const WeighSeq s = weigh_seq(p, b);
+        const uint32_t units = units_of(s);
+        if (off >= units * p.geom.Hkv) {
+            b++;
+            off = 0;
+            continue;
+        }
         const uint32_t rows = (uint32_t)s.n * G;
-        for (int64_t k0 = s.lo / (int)kWaveKeys * (int64_t)kWaveKeys + (int64_t)((blockIdx.x / p.geom.Hkv) * 4 + wave) * kWaveKeys; k0 < s.keys;
-             k0 += (int64_t)tiles * 4 * kWaveKeys) {
-            const int key0 = (int)k0;
-            uint32_t page_id = 0xffffffffu;
-            if (lane < 4 && key0 + 16 * lane < s.keys)
-                page_id = (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)(key0 + 16 * lane) >> p.geom.log2_page)];
-            uint32_t page[4], kw[4][W], kd[4];
+        // this share's units of one KV head
+        const uint32_t hk = off / units, u = off - hk * units, nu = min(units - u, end - cur);
+        cur += nu;
+        off += nu;
+        const int first_key = (int)((((uint32_t)s.lo >> unit_shift) + u) << unit_shift);
+        const uint32_t last_key = (uint32_t)first_key + (nu << unit_shift);  // up to 2^31
+        const int key_end = last_key < (uint32_t)s.keys ? (int)last_key : s.keys;
+
+        h8_t qf[KK];
+        float l[4];
+        auto load_rows = [&](uint32_t r0) {
+            const _Float16* src = p.Q.p + row_offset(p, p.Q, s.q0, hk, min(r0 + j, rows - 1)) + g * RUN;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) qf[kk] = *reinterpret_cast<const h8_t*>(src + 8 * kk);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t f = r0 + 4 * g + e;
+                l[e] = INFINITY;  // no such row
+                if (f < rows) l[e] = p.lse.p[row_offset(p, p.lse, s.q0, hk, f)];
+            }
+        };
+        // page numbers of the next 16 tiles, a lane each 16 keys
+        uint32_t ids = 0;
+        int ids_from = first_key - 1024;
+        uint32_t kw[2][4][W], kd[2][4], page[2][4];
+        const uint32_t at_code = j * CB + g * (W * 4), at_scale = p.geom.ks_off + (j * NB + g * NB / 4) * 2;
+        auto fetch = [&](int buf, int key0) {
+            if (key0 - ids_from >= 1024) {
+                ids_from = key0;
+                const int k = key0 + 16 * lane;  // past the last key at most by these
+                ids = k < s.keys ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)k >> p.geom.log2_page)] : 0xffffffffu;
+            }
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                page[t] = __builtin_amdgcn_readlane(page_id, t);
+                page[buf][t] = __builtin_amdgcn_readlane(ids, (key0 - ids_from) / 16 + t);
                 const uint32_t slot = (uint32_t)(key0 + 16 * t) & pmask;
-                const uint8_t* head = p.geom.pages + ((size_t)(page[t] < p.geom.num_pages ? page[t] : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
-                load_words<W, false>(head + (slot + j) * CB + g * (W * 4), kw[t]);
-                kd[t] = *reinterpret_cast<const uint16_t*>(head + p.geom.ks_off + ((slot + j) * NB + g * NB / 4) * 2);
+                const uint8_t* base = p.geom.pages + ((size_t)(page[buf][t] < p.geom.num_pages ? page[buf][t] : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
+                load_words<W, false>(base + slot * CB + at_code, kw[buf][t]);
+                kd[buf][t] = *reinterpret_cast<const uint16_t*>(base + slot * (NB * 2) + at_scale);
             }
+        };
+        // a tile from buffer `buf`, which is filled again with the next but one
+        auto tile = [&](int buf, int key0) {
+            // a lane's key when the sums are written, and what it has so far
+            const uint32_t at = g == 0 ? page[buf][0] : (g == 1 ? page[buf][1] : (g == 2 ? page[buf][2] : page[buf][3]));
+            const int key = key0 + 16 * g + j;
+            float* to = nullptr;
+            float old = 0.0f;
+            if (key < s.keys && at < p.geom.num_pages)
+                to = p.sums + (((size_t)at * p.geom.Hkv + hk) << p.geom.log2_page) + ((uint32_t)key & pmask);
             h8_t kf[4][KK];
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int kk = 0; kk < KK; kk++) kf[t][kk] = k_octet<FMT>(kw[t], kk, as_h2(kd[t] | kd[t] << 16));
-            RowRange see[4];
-#pragma unroll
-            for (int t = 0; t < 4; t++) see[t] = rows_of(p, s, key0 + 16 * t + j);
+                for (int kk = 0; kk < KK; kk++) kf[t][kk] = k_octet<FMT>(kw[buf][t], kk, as_h2(kd[buf][t] | kd[buf][t] << 16));
+            if (to && key < s.first) old = *to;
+            if (key0 + 2 * (int)kWaveKeys < key_end) fetch(buf, key0 + 2 * kWaveKeys);
             float sum[4] = {};
+            const bool whole = key0 + (int)kWaveKeys - 1 <= s.first && !p.window;  // every row sees every key
+#pragma unroll 1
             for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
-                h8_t qf[KK];
-                {
-                    const uint32_t f = min(r0 + j, rows - 1);
-                    const _Float16* src = p.Q.p + (int64_t)(s.q0 + (int)(f / G)) * p.Q.ts + (int64_t)(hk * G + f % G) * p.Q.hs + g * RUN;
-#pragma unroll
-                    for (int kk = 0; kk < KK; kk++) qf[kk] = *reinterpret_cast<const h8_t*>(src + 8 * kk);
-                }
-                float l2[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t f = min(r0 + 4 * g + e, rows - 1);
-                    l2[e] = p.lse.p[(int64_t)(s.q0 + (int)(f / G)) * p.lse.ts + (int64_t)(hk * G + f % G) * p.lse.hs] * 1.4426950408889634f;
-                }
+                if (rows > 16 && (r0 || key0 > first_key)) load_rows(r0);
+                f4_t sc[4];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    f4_t sc{};
+                    sc[t] = f4_t{};
 #pragma unroll
-                    for (int kk = 0; kk < KK; kk++) sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[kk], kf[t][kk], sc, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint32_t f = r0 + 4 * g + e;
-                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -l2[e]));
-                        sum[t] += f >= see[t].lo && f < see[t].hi ? w : 0.0f;
-                    }
+                    for (int kk = 0; kk < KK; kk++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[kk], kf[t][kk], sc[t], 0, 0, 0);
                 }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[t][e] = __builtin_fmaf(sc[t][e], c, l[e] * -1.4426950408889634f);
+                if (!whole)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        const RowRange see = rows_of(p, s, key0 + 16 * t + j);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (r0 + 4 * g + e < see.lo || r0 + 4 * g + e >= see.hi) sc[t][e] = -INFINITY;
+                    }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(sc[t][e]);
             }
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 sum[t] += __shfl_xor(sum[t], 16);
                 sum[t] += __shfl_xor(sum[t], 32);
             }
-            const float mine = g == 0 ? sum[0] : (g == 1 ? sum[1] : (g == 2 ? sum[2] : sum[3]));
-            const uint32_t at = g == 0 ? page[0] : (g == 1 ? page[1] : (g == 2 ? page[2] : page[3]));
-            const int key = key0 + 16 * g + j;
-            if (key < s.keys && at < p.geom.num_pages) {
-                float* to = p.sums + (((size_t)at * p.geom.Hkv + hk) << p.geom.log2_page) + ((uint32_t)key & pmask);
-                *to = key >= s.first ? mine : *to + mine;
-            }
+            if (to) *to = old + (g == 0 ? sum[0] : (g == 1 ? sum[1] : (g == 2 ? sum[2] : sum[3])));
+        };
+        fetch(0, first_key);
+        if (first_key + (int)kWaveKeys < key_end) fetch(1, first_key + kWaveKeys);
+        load_rows(0);
+#pragma unroll 1
+        for (int key0 = first_key; key0 < key_end; key0 += 2 * kWaveKeys) {
+            tile(0, key0);
+            if (key0 + (int)kWaveKeys < key_end) tile(1, key0 + kWaveKeys);
         }
     }
 }
 
 // Many rows: a workgroup's eight waves hold the same 32 NT keys and share the rows, 32 at a
-// time; their sums meet in LDS.
+// time; their sums meet in LDS.  Bound by the matrix and vector units together: 1024 scores are
+// 256 cycles of products (D = 128) and 256 of a fused multiply, an exponential and a sum, and
+// the two add up here whatever the order of the instructions (8 heads, 2048 rows of 32 query
+// heads on 30000 keys: 1.2 M cycles a SIMD, 0.46 M of products, 0.66 M of vector work, 635 us).  With the
+// queries through LDS and 512 keys a workgroup: 670.
 constexpr int kWeighWaves = 8;
 constexpr uint32_t kLseRows = 4096;  // lse staged in LDS at once
 template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighParams p, uint32_t tiles) {
-    constexpr int KK = D / 16, RUN = D / 2, W = FMT == QUANT_Q8_0 ? D / 8 : D / 16;  // a lane: half a key
-    constexpr uint32_t CB = 2 * W * 4, NB = D / 32;
+    constexpr int KK = D / 16, W = FMT == QUANT_Q8_0 ? 2 : 1;  // words of an octet of codes
+    constexpr uint32_t CB = 2 * KK * W * 4, NB = D / 32;
     constexpr int KT = 32 * NT;
     __shared__ __attribute__((aligned(16))) float l2[kLseRows];
     __shared__ float part[kWeighWaves][KT];
@@ -152,12 +245,12 @@ __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighP
                 const uint32_t at = (uint32_t)__shfl((int)page_id, 2 * t + (j >> 4));
                 const uint32_t slot = (uint32_t)(key0 + 32 * t + j) & pmask;
                 const uint8_t* head = p.geom.pages + ((size_t)(at < p.geom.num_pages ? at : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
-                uint32_t kw[W];
-                load_words<W, false>(head + slot * CB + g * (W * 4), kw);
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) {
+                    uint32_t kw[W];
+                    load_words<W, false>(head + slot * CB + (kk + KK * g) * (W * 4), kw);
                     const uint32_t kd = *reinterpret_cast<const uint16_t*>(head + p.geom.ks_off + (slot * NB + g * NB / 2 + kk / 4) * 2);
-                    kf[t][kk] = k_octet<FMT>(kw, kk, as_h2(kd | kd << 16));
+                    kf[t][kk] = k_octet<FMT>(kw, 0, as_h2(kd | kd << 16));
                 }
             }
             float sum[NT] = {};
@@ -171,8 +264,8 @@ __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighP
                 __syncthreads();
                 for (uint32_t x = tid; x < min(kLseRows, (f_hi - f0 + 31) / 32 * 32); x += 64 * kWeighWaves) {
                     const uint32_t f = f0 + x;
-                    l2[x] = f < rows ? p.lse.p[(int64_t)(s.q0 + (int)(f / G)) * p.lse.ts + (int64_t)(hk * G + f % G) * p.lse.hs] * 1.4426950408889634f
-                                     : 0.0f;
+                    const float l = f < rows ? p.lse.p[row_offset(p, p.lse, s.q0, hk, f)] : 0.0f;
+                    l2[x] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;  // a row that sees nothing gives nothing
                 }
                 __syncthreads();
                 const uint32_t f1 = min(f0 + kLseRows, f_hi);
@@ -180,7 +273,7 @@ __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighP
                     h8_t qf[KK];
                     {
                         const uint32_t f = min(r0 + j, rows - 1);
-                        const _Float16* src = p.Q.p + (int64_t)(s.q0 + (int)(f / G)) * p.Q.ts + (int64_t)(hk * G + f % G) * p.Q.hs + g * RUN;
+                        const _Float16* src = p.Q.p + row_offset(p, p.Q, s.q0, hk, f) + D / 2 * g;
 #pragma unroll
                         for (int kk = 0; kk < KK; kk++) qf[kk] = *reinterpret_cast<const h8_t*>(src + 8 * kk);
                     }
@@ -246,8 +339,13 @@ static hipError_t launch_weigh(WeighParams p, hipStream_t st) {
     p.min_rows = 0;
     p.max_rows = both ? kWeighChunk : 0xffffffffu;
     if (!chunks || both) {
-        const uint32_t tiles = tiles_of(4 * kWaveKeys);
-        hipLaunchKernelGGL((weigh_rows_kernel<FMT, D>), dim3(tiles * p.geom.Hkv, across), dim3(256), 0, st, p, tiles);
+        const uint64_t heads = (uint64_t)p.batch.B * p.geom.Hkv, cap = (uint64_t)p.batch.table_pages << p.geom.log2_page;
+        p.tile_shift = 0;
+        while (heads * ((cap >> (6 + p.tile_shift)) + 1) >= 1ull << 31 && p.tile_shift < 24) p.tile_shift++;
+        const uint64_t tiles = (keys + kWaveKeys - 1) / kWaveKeys;
+        uint32_t groups = 1;  // a power of two
+        while (4ull * groups < kRowWaves && 4ull * groups < heads * tiles) groups *= 2;
+        hipLaunchKernelGGL((weigh_rows_kernel<FMT, D>), dim3(groups), dim3(256), 0, st, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !chunks) return e;
     }

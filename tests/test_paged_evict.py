@@ -126,6 +126,36 @@ def test_weigh_out_of_range(bridge, fmt, kernels, scale):
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("B,H,Hkv,P,pages,window", [
+    (70, 6, 2, 16, 0, 0),               # more sequences than a wave has lanes
+    (150, 7, 1, 32, 0, 33),
+    (16, 16, 16, 256, 2 ** 21, 0),      # a table for so many keys that two tiles are counted as one
+    (16, 16, 16, 256, 2 ** 21, 90),
+])
+def test_weigh_many_sequences(bridge, fmt, B, H, Hkv, P, pages, window):
+    import torch
+
+    D = 64
+    lens = [(37 * b) % 401 + (b % 5 > 0) if b % 7 else 0 for b in range(B)]
+    new = [min(n, b % 4) for b, n in enumerate(lens)]
+    s = Setup(fmt, lens, new, Hkv, D, P, seed=B + P)
+    table = dev(s.table)
+    if pages:
+        table = torch.full((B, pages), -1, dtype=torch.int32, device="cuda")
+        table[:, :s.table.shape[1]] = dev(s.table)
+    q = half(s.rng, H, s.T, D)
+    sums = s.rng.random((s.num_pages, Hkv, P)).astype(np.float32)
+    lse = s.rng.standard_normal((H, s.T)).astype(np.float32) + 4
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), table, max_new=max(new), max_kv=max(lens))
+    got = dev(sums)
+    say("weigh many sequences", fmt, B, H, Hkv, P, pages, window)
+    bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(lse), got, 0.125, window=window)
+    bridge.synchronize()
+    close(got.cpu().numpy(), *weighed(s, sums, q, lse, lens, s.q_start, window, 0.125), "sums")
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_weights_of_a_row_add_up_to_one(bridge, fmt):
     """Attention hands its lse over: what the rows of a call give all keys is 1 for each row and query head."""
     import torch
@@ -417,7 +447,7 @@ class Args:
     (lambda a: None, 0), (set_("sums", 0), -2), (set_("sums", 0x500004), -2), (set_("held", 511), -2), (set_("lse.ptr", 0), -2),
     (set_("lse.bytes", 316), -2), (set_("lse.token_stride", 0), 0), (set_("lse.head_stride", -1), -4), (set_("rows.ptr", 0x300004), -2),
     (set_("rows.bytes", 100), -2), (set_("H", 9), -4), (set_("scale", float("inf")), -4), (set_("cache.format", 2), -3),
-    (set_("batch.table_pages", 0), -4), (set_("T", 0), 0), (set_("batch.B", 0), 0)])
+    (set_("batch.table_pages", 0), -4), (set_("T", 0), 0), (set_("batch.B", 0), 0), (set_("batch.B", 2 ** 30), -4)])
 def test_refused_weights(lib, change, code):  # noqa: F811
     a, r = Args(), ctypes.addressof
     change(a)
