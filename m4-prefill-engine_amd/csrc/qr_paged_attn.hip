@@ -247,24 +247,29 @@ __device__ __forceinline__ int first_seen_by(const PagedAttnParams& p, const Seq
     // below zero, too: so may be the places of nodes that have no key, where there are more rows than keys
     return p.window ? (int)max((int64_t)place_of_node(p, s, i) + 1 - (int64_t)p.window, (int64_t)INT32_MIN) : INT32_MIN;
 }
-// Which of keys key .. key + 3 the row of these mask words sees, as bits; low: the first
-// position that its window holds.
-__device__ __forceinline__ uint32_t sees4(const PagedAttnParams& p, const Seq& s, const uint32_t* mask, int key, int low) {
-    const int node = key - s.first;
-    uint32_t bits = 15;
-    if (node > -4) {
-        const int w = node >> 5;  // -1: the last keys before the tree
-        const uint32_t lo = w < 0 ? 0xffffffffu : ((uint32_t)w < p.tree.words ? mask[w] : 0u);
-        const uint32_t hi = (uint32_t)(w + 1) < p.tree.words ? mask[w + 1] : 0u;
-        bits = (uint32_t)(((uint64_t)hi << 32 | lo) >> (node & 31)) & 15u;
-    }
+// Word w of a row's mask: all of it before the tree, nothing behind.
+__device__ __forceinline__ uint32_t mask_word(const PagedAttnParams& p, const uint32_t* mask, int w) {
+    return w < 0 ? 0xffffffffu : ((uint32_t)w < p.tree.words ? mask[w] : 0u);
+}
+// Which of 32 keys from `key` on the row sees, as bits, of the words at (key - s.first) >> 5 and
+// behind it.  The words of many keys are read before the first is used: read
+// where they are, one after the other, they took half of the time of a call for the trees of 16
+// requests.
+__device__ __forceinline__ uint32_t seen32(const Seq& s, int key, uint32_t lo, uint32_t hi) {
+    const int there = s.keys - key;
+    const uint32_t bits = (uint32_t)(((uint64_t)hi << 32 | lo) >> ((key - s.first) & 31));
+    return there >= 32 ? bits : (there <= 0 ? 0u : bits & ((1u << there) - 1));
+}
+// Of these, 4 from key + at on, the ones in the row's window (low: the first position that it holds).
+__device__ __forceinline__ uint32_t quad_of(const PagedAttnParams& p, const Seq& s, uint32_t seen, int key, int at, int low) {
+    uint32_t bits = seen >> at & 15u;
+    if (p.window)
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        int at = key + r;
-        const bool there = at < s.keys;
-        if (p.window && there && node + r >= 0) at = place_of_node(p, s, node + r);
-        if (!there || at < low) bits &= ~(1u << r);
-    }
+        for (int r = 0; r < 4; r++) {
+            int pos = key + at + r;
+            if (pos >= s.first && pos < s.keys) pos = place_of_node(p, s, pos - s.first);
+            if (pos < low) bits &= ~(1u << r);
+        }
     return bits;
 }
 // Natural logarithm of a row's sum, from its reference point and its sum beside it.
@@ -509,6 +514,14 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             const int key0 = key_base + u * (int)kStep;
             bool odd = false;  // some row does not see all keys, and some V value may not be finite
             uint32_t vis[NR];  // TREE: what each row sees of a lane's 8 keys
+            uint32_t seen32_of[NR];
+            if constexpr (TREE)
+#pragma unroll
+                for (int q = 0; q < NR; q++) {
+                    seen32_of[q] = 0xffffffffu;
+                    const int w = (key0 - s.first) >> 5;
+                    if (p.tree.mask && key0 + 31 > lim_min) seen32_of[q] = seen32(s, key0, mask_word(p, mask[q], w), mask_word(p, mask[q], w + 1));
+                }
             f4_t sc[NR][2];
 #pragma unroll
             for (int q = 0; q < NR; q++) sc[q][0] = sc[q][1] = f4_t{};
@@ -539,7 +552,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                         for (int q = 0; q < NR; q++) {
                             const int key = key0 + 16 * t + 4 * g;
                             uint32_t b = 0;
-                            if (tile[t].there && p.tree.mask) b = sees4(p, s, mask[q], key, low[q]);
+                            if (tile[t].there && p.tree.mask) b = quad_of(p, s, seen32_of[q], key0, 16 * t + 4 * g, low[q]);
                             else if (tile[t].there)
 #pragma unroll
                                 for (int r = 0; r < 4; r++) b |= key + r <= lim[q] && key + r >= low[q] ? 1u << r : 0u;
@@ -977,12 +990,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         const uint32_t r0 = min(32u * wave, rows - 1), r1 = min(32u * wave + 31, rows - 1);
         int lim0 = last_seen(r0), lim1 = last_seen(r1), low0 = first_seen(r0), low1 = first_seen(r1);
         int all0 = last_seen(0), all_low1 = first_seen(rows - 1);
-        const uint32_t* mask = nullptr;
         if constexpr (TREE)
             if (p.tree.mask) {  // all see the keys before the tree, some may see any of its own
-                const int i = i0 + (int)(rc / G);
-                mask = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
-                low = first_seen_by(p, s, i);
                 all0 = lim0 = min(s.first - 1, s.keys - 1);
                 lim1 = s.keys - 1;
                 low0 = p.window ? (int)max((int64_t)s.first + 1 - (int64_t)p.window, (int64_t)0) : 0;
@@ -1228,7 +1237,19 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 }
                 return;
             }
-            auto unit = [&](int x, bool marks) {
+            uint32_t words[UNITS + 1];  // TREE: of the row's mask
+            int win = low;  // the first position of the row's window
+            if constexpr (TREE)
+                if (p.tree.mask) {
+                    uint32_t row = rc;
+                    asm volatile("" : "+v"(row));  // what follows is formed anew: kept, more registers would spill
+                    const int i = i0 + (int)(row / G);
+                    const uint32_t* mask = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
+                    win = first_seen_by(p, s, i);
+#pragma unroll
+                    for (int x = 0; x <= UNITS; x++) words[x] = mask_word(p, mask, ((k0 - s.first) >> 5) + x);
+                }
+            auto unit = [&](int x, bool marks, uint32_t lo_word, uint32_t hi_word) {
                 const int key0 = k0 + 32 * x;
                 if (key0 > lim1 || key0 + 31 < low0) return;
                 f16v_t sc = scores(buf, x);
@@ -1236,11 +1257,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 if (key0 + 31 > lim0 || key0 < low1 || !all_there) {
                     if constexpr (TREE) {
                         vis = 0;
+                        const uint32_t seen = seen32(s, key0, lo_word, hi_word);
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             const int key = key0 + 8 * y + 4 * g;
                             if (!(there[u & 1][2 * x + (y >> 1)] & 1)) continue;
-                            if (p.tree.mask) vis |= sees4(p, s, mask, key, low) << 4 * y;
+                            if (p.tree.mask) vis |= quad_of(p, s, seen, key0, 8 * y + 4 * g, win) << 4 * y;
                             else
 #pragma unroll
                                 for (int e = 0; e < 4; e++) vis |= key + e <= lim && key + e >= low ? 1u << (4 * y + e) : 0u;
@@ -1265,11 +1287,21 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             };
             if (__builtin_amdgcn_readfirstlane(some) & 2) {
 #pragma unroll 1
-                for (int x = 0; x < UNITS; x++) unit(x, true);
+                for (int x = 0; x < UNITS; x++) {
+                    uint32_t lo_word = 0, hi_word = 0;
+                    if constexpr (TREE)
+#pragma unroll
+                        for (int y = 0; y < UNITS; y++)
+                            if (x == y) {
+                                lo_word = words[y];
+                                hi_word = words[y + 1];
+                            }
+                    unit(x, true, lo_word, hi_word);
+                }
                 return;
             }
 #pragma unroll
-            for (int x = 0; x < UNITS; x++) unit(x, false);
+            for (int x = 0; x < UNITS; x++) unit(x, false, TREE ? words[x] : 0u, TREE ? words[x + 1] : 0u);
         };
 
         fetch(u0);
