@@ -1,5 +1,7 @@
 // qr_paged_evict.hip -- a bounded cache: the attention weight that each cached key has
 // received, and eviction of the lightest.
+#include <algorithm>
+
 #include "qr_device.h"
 #include "qr_paged.h"
 #include "qr_paged_decode.h"
@@ -36,16 +38,13 @@ __device__ __forceinline__ int64_t row_offset(const WeighParams& p, const VIEW& 
     const uint32_t i = (__umulhi(f, p.of_group.mul) + f) >> p.of_group.shift, q = f - i * p.G;
     return (int64_t)(q0 + (int)i) * v.ts + (int64_t)(hk * p.G + q) * v.hs;
 }
-// The rows of a KV head that see a key are [lo, hi).
-struct RowRange {
-    uint32_t lo, hi;
+// The new tokens that see a key are [lo, hi).
+struct Range {
+    int lo, hi;
 };
-__device__ __forceinline__ RowRange rows_of(const WeighParams& p, const WeighSeq& s, int key) {
-    const int i = key - s.first;  // keys past the last row's are not asked for but for a tile's width
-    RowRange r;
-    r.lo = (uint32_t)min(max(i, 0), s.n) * p.G;
-    r.hi = (uint32_t)(p.window ? min(max(i + (int)p.window, 0), s.n) : s.n) * p.G;
-    return r;
+__device__ __forceinline__ Range tokens_of(const WeighParams& p, const WeighSeq& s, int key) {
+    const int i = key - s.first;  // keys past the last token's are not asked for but for a tile's width
+    return Range{min(max(i, 0), s.n), p.window ? min(max(i + (int)p.window, 0), s.n) : s.n};
 }
 
 // Few rows: a wave takes 64 keys of a KV head at a time, 16 rows at a time.  All work is one line
@@ -183,10 +182,10 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
                 if (!whole)
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
-                        const RowRange see = rows_of(p, s, key0 + 16 * t + j);
+                        const Range see = tokens_of(p, s, key0 + 16 * t + j);
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (r0 + 4 * g + e < see.lo || r0 + 4 * g + e >= see.hi) sc[t][e] = -INFINITY;
+                            if (r0 + 4 * g + e < see.lo * G || r0 + 4 * g + e >= see.hi * G) sc[t][e] = -INFINITY;
                     }
 #pragma unroll
                 for (int t = 0; t < 4; t++)
@@ -211,31 +210,90 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
     }
 }
 
-// Many rows: a workgroup's eight waves hold the same 32 NT keys and share the rows, 32 at a
-// time; their sums meet in LDS.  Bound by the matrix and vector units together: 1024 scores are
-// 256 cycles of products (D = 128) and 256 of a fused multiply, an exponential and a sum, and
-// the two add up here whatever the order of the instructions (8 heads, 2048 rows of 32 query
-// heads on 30000 keys: 1.2 M cycles a SIMD, 0.46 M of products, 0.66 M of vector work, 635 us).  With the
-// queries through LDS and 512 keys a workgroup: 670.
-constexpr int kWeighWaves = 8;
-constexpr uint32_t kLseRows = 4096;  // lse staged in LDS at once
-template <int FMT, int D, int NT>
-__global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighParams p, uint32_t tiles) {
+// Many rows: a workgroup's waves hold the same 32 NT keys and share the rows, 32 at a time, which
+// each brings into LDS of its own by loads of whole rows (operands straight from the rows
+// touch 64 lines a load; a row's address by division and 64-bit products cost as much as a
+// tile's weights, so all offsets are formed once); their sums meet in LDS.  A tile's products run
+// beside the exponentials of the one before.  8 heads, 2048 rows of 32 query heads on 30000 keys of
+// 128: 545 us, 0.89 PFLOP/s.  By itself that loop takes 350 cycles a tile of 32 x 32 (256 of products,
+// 256 of fused multiplies, exponentials and sums, at 1.65 GHz under this load), 390 us; bringing
+// the rows (3.8 GB through the L2s) costs 100 more.
+template <int FMT, int D, int NT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams p) {
     constexpr int KK = D / 16, W = FMT == QUANT_Q8_0 ? 2 : 1;  // words of an octet of codes
     constexpr uint32_t CB = 2 * KK * W * 4, NB = D / 32;
     constexpr int KT = 32 * NT;
-    __shared__ __attribute__((aligned(16))) float l2[kLseRows];
-    __shared__ float part[kWeighWaves][KT];
+    constexpr uint32_t U = D / 8, BLOCK = 32 * D * 2, LOADS = BLOCK / 1024;  // 16-byte units of a row; bytes of 32 rows
+    extern __shared__ __attribute__((aligned(16))) uint8_t qs[];             // a wave's 32 rows
+    __shared__ __attribute__((aligned(16))) float l2[WAVES][32];
+    __shared__ float lse[WAVES][64];  // as it is, twice
+    __shared__ __attribute__((aligned(16))) int rel_of[32];
+    // what each lane loads of 32 rows, and where a row's lse is, from their first row on (bytes)
+    __shared__ int64_t q_off[LOADS * 64], l_off[32];
+    __shared__ float part[WAVES][KT];
     const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t hk = blockIdx.x % p.geom.Hkv, G = p.G;
     const uint32_t pmask = (1u << p.geom.log2_page) - 1;
-    const float c = p.scale * 1.4426950408889634f;
-    for (uint32_t b = blockIdx.y; b < p.batch.B; b += gridDim.y) {
+    const float c = p.scale * 1.4426950408889634f;  // log2 units
+    // 32 rows: some tokens' heads of the group, or of one token 32 at a time, so that what
+    // follows is a whole number of tokens on
+    const int heads = (int)min(G, 32u), tokens = 32 / heads, subs = (int)(G + 31) / 32;
+    const int rel = min(j / heads, tokens), head = j - rel * heads;
+    // unit u of row r sits at u ^ swz(r): no two of 16 rows in the same banks
+    auto swz = [](uint32_t r) -> uint32_t { return U == 16 ? (r & 15u) : (r >> 1 & 7u); };
+    uint8_t* block = qs + wave * BLOCK;
+    const uint32_t q_at = j * (U * 16) + 16 * (g ^ swz(j));
+    // rows behind the last token's, where 32 are no whole tokens, are its own again and weigh nothing
+    for (uint32_t x = tid; x < LOADS * 64; x += 64 * WAVES) {
+        const uint32_t r = x / U;
+        const int t = min((int)r / heads, tokens);
+        q_off[x] = ((int64_t)min(t, tokens - 1) * p.Q.ts + (int64_t)((int)r - t * heads) * p.Q.hs) * 2 + 16 * (x % U ^ swz(r));
+    }
+    if (tid < 32) {
+        rel_of[tid] = rel < tokens ? rel : 0x40000000;
+        l_off[tid] = ((int64_t)min(rel, tokens - 1) * p.lse.ts + (int64_t)head * p.lse.hs) * 4;
+    }
+    __syncthreads();
+    for (uint32_t b = blockIdx.x / p.geom.Hkv; b < p.batch.B; b += gridDim.x / p.geom.Hkv) {
         const WeighSeq s = weigh_seq(p, b);
-        const uint32_t rows = (uint32_t)s.n * G;
-        for (int64_t k0 = s.lo / KT * (int64_t)KT + (int64_t)(blockIdx.x / p.geom.Hkv) * KT; k0 < s.keys; k0 += (int64_t)tiles * KT) {
+        const int64_t k_lo = s.lo / KT * (int64_t)KT + (int64_t)blockIdx.y * KT;
+        if (k_lo >= s.keys) continue;
+        for (int64_t k0 = k_lo; k0 < s.keys; k0 += (int64_t)gridDim.y * KT) {
             const int key0 = (int)k0;
+            // tokens that see some of these keys, and those that see them all
+            const Range first_key = tokens_of(p, s, key0), last_key = tokens_of(p, s, key0 + KT - 1);
+            const int i_lo = first_key.lo + (int)wave * tokens, i_hi = last_key.hi;
+            auto from_head = [&](int sub) { return min(32 * sub, (int)G - heads); };  // the last ones: some again
+            // rows straight into LDS, each load a run of whole ones
+            auto bring = [&](int i, int sub) {
+                const int64_t row = s.q0 + i, h = hk * G + from_head(sub);
+                const uint64_t q = reinterpret_cast<uint64_t>(p.Q.p + row * p.Q.ts + h * p.Q.hs);
+                const uint64_t l = reinterpret_cast<uint64_t>(p.lse.p + row * p.lse.ts + h * p.lse.hs);
+                const int there = s.n - i;
+                const bool all = there >= tokens;  // else again the last token's where there is none
+                const int64_t l_at = all ? l_off[j] : ((int64_t)min(rel, there - 1) * p.lse.ts + (int64_t)head * p.lse.hs) * 4;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(l + l_at),
+                                                 (__attribute__((address_space(3))) void*)lse[wave], 4, 0, 0);
+                int of = lane;
+                asm volatile("" : "+v"(of));
+                auto load = [&](uint32_t n, int64_t at) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(q + at),
+                                                     (__attribute__((address_space(3))) void*)(block + n * 1024), 16, 0, 0);
+                };
+                if (all) {
+#pragma unroll
+                    for (uint32_t n = 0; n < LOADS; n++) load(n, q_off[n * 64 + of]);
+                } else {
+#pragma unroll 1
+                    for (uint32_t n = 0; n < LOADS; n++) {
+                        const uint32_t r = (n * 64 + of) / U;
+                        const int t = min(rel_of[r], tokens);
+                        load(n, ((int64_t)min(t, there - 1) * p.Q.ts + (int64_t)((int)r - t * heads) * p.Q.hs) * 2 + 16 * (of % U ^ swz(r)));
+                    }
+                }
+            };
+            if (i_lo < i_hi) bring(i_lo, 0);
             uint32_t page_id = 0xffffffffu;
             if (lane < 2 * NT && key0 + 16 * lane < s.keys)
                 page_id = (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)(key0 + 16 * lane) >> p.geom.log2_page)];
@@ -244,61 +302,72 @@ __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighP
             for (int t = 0; t < NT; t++) {
                 const uint32_t at = (uint32_t)__shfl((int)page_id, 2 * t + (j >> 4));
                 const uint32_t slot = (uint32_t)(key0 + 32 * t + j) & pmask;
-                const uint8_t* head = p.geom.pages + ((size_t)(at < p.geom.num_pages ? at : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
+                const uint8_t* head_of = p.geom.pages + ((size_t)(at < p.geom.num_pages ? at : 0) * p.geom.Hkv + hk) * p.geom.head_bytes;
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) {
                     uint32_t kw[W];
-                    load_words<W, false>(head + slot * CB + (kk + KK * g) * (W * 4), kw);
-                    const uint32_t kd = *reinterpret_cast<const uint16_t*>(head + p.geom.ks_off + (slot * NB + g * NB / 2 + kk / 4) * 2);
+                    load_words<W, false>(head_of + slot * CB + (2 * kk + g) * (W * 4), kw);
+                    const uint32_t kd = *reinterpret_cast<const uint16_t*>(head_of + p.geom.ks_off + (slot * NB + kk / 2) * 2);
                     kf[t][kk] = k_octet<FMT>(kw, 0, as_h2(kd | kd << 16));
                 }
             }
             float sum[NT] = {};
-            // rows that see some of these keys, and those that see them all
-            const RowRange first_key = rows_of(p, s, key0), last_key = rows_of(p, s, key0 + KT - 1);
-            const uint32_t f_lo = first_key.lo / 32 * 32, f_hi = last_key.hi;
-            RowRange see[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) see[t] = rows_of(p, s, key0 + 32 * t + j);
-            for (uint32_t f0 = f_lo; f0 < f_hi; f0 += kLseRows) {
-                __syncthreads();
-                for (uint32_t x = tid; x < min(kLseRows, (f_hi - f0 + 31) / 32 * 32); x += 64 * kWeighWaves) {
-                    const uint32_t f = f0 + x;
-                    const float l = f < rows ? p.lse.p[row_offset(p, p.lse, s.q0, hk, f)] : 0.0f;
-                    l2[x] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;  // a row that sees nothing gives nothing
+            int i = i_lo, sub = 0;
+#pragma unroll 1
+            while (i < i_hi && sub < subs) {
+                int i_next = i + tokens * WAVES, sub_next = sub;
+                if (i_next >= i_hi) {
+                    i_next = i_lo;
+                    sub_next++;
                 }
-                __syncthreads();
-                const uint32_t f1 = min(f0 + kLseRows, f_hi);
-                for (uint32_t r0 = f0 + 32 * wave; r0 < f1; r0 += 32 * kWeighWaves) {
-                    h8_t qf[KK];
-                    {
-                        const uint32_t f = min(r0 + j, rows - 1);
-                        const _Float16* src = p.Q.p + row_offset(p, p.Q, s.q0, hk, f) + D / 2 * g;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // these rows have landed
+                // a row that sees nothing gives nothing, nor one that is not there or not of this turn
+                const bool live = rel < min(tokens, s.n - i) && from_head(sub) + head >= 32 * sub;
+                const float mine = lse[wave][lane];
+                if (g == 0) l2[wave][j] = mine == -INFINITY || !live ? INFINITY : mine * 1.4426950408889634f;
+                h8_t qf[KK];
 #pragma unroll
-                        for (int kk = 0; kk < KK; kk++) qf[kk] = *reinterpret_cast<const h8_t*>(src + 8 * kk);
+                for (int kk = 0; kk < KK; kk++) qf[kk] = *reinterpret_cast<const h8_t*>(block + (q_at ^ 32u * kk));
+                float l[16];
+#pragma unroll
+                for (int y = 0; y < 4; y++) *reinterpret_cast<f4_t*>(l + 4 * y) = *reinterpret_cast<const f4_t*>(&l2[wave][8 * y + 4 * g]);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and are read: the next ones may take their place
+                if (sub_next < subs) bring(i_next, sub_next);
+                if (i >= last_key.lo && min(i + tokens, s.n) <= first_key.hi) {
+                    // all see all: a tile's scores while those before them are weighed
+                    f16v_t sc[2];
+#pragma unroll
+                    for (int t = 0; t <= NT; t++) {
+                        if (t < NT) sc[t & 1] = f16v_t{};
+#pragma unroll
+                        for (int kk = 0; kk < KK; kk++) {
+                            if (t < NT) sc[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[kk], kf[t][kk], sc[t & 1], 0, 0, 0);
+                            if (t > 0)
+#pragma unroll
+                                for (int e = kk * 16 / KK; e < (kk + 1) * 16 / KK; e++)
+                                    sum[t - 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[(t - 1) & 1][e], c, -l[e]));
+                            if (t > 0) __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
-                    float l[16];
-#pragma unroll
-                    for (int y = 0; y < 4; y++) *reinterpret_cast<f4_t*>(l + 4 * y) = *reinterpret_cast<const f4_t*>(&l2[r0 - f0 + 8 * y + 4 * g]);
-                    const bool whole = r0 >= last_key.lo && r0 + 32 <= first_key.hi;
+                } else {
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
                         f16v_t sc{};
 #pragma unroll
                         for (int kk = 0; kk < KK; kk++) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[kk], kf[t][kk], sc, 0, 0, 0);
-                        if (whole) {
+                        int key = key0 + 32 * t + j;
+                        asm volatile("" : "+v"(key));  // formed anew: kept, these ranges would spill
+                        const Range see = tokens_of(p, s, key);
 #pragma unroll
-                            for (int e = 0; e < 16; e++) sum[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -l[e]));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const uint32_t f = r0 + 4 * g + 8 * (e >> 2) + (e & 3);
-                                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -l[e]));
-                                sum[t] += f >= see[t].lo && f < see[t].hi ? w : 0.0f;
-                            }
+                        for (int e = 0; e < 16; e++) {
+                            const int at = i + rel_of[8 * (e >> 2) + 4 * g + (e & 3)];
+                            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -l[e]));
+                            sum[t] += at >= see.lo && at < see.hi ? w : 0.0f;
                         }
                     }
                 }
+                i = i_next;
+                sub = sub_next;
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -306,11 +375,11 @@ __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighP
                 if (g == 0) part[wave][32 * t + j] = sum[t];
             }
             __syncthreads();
-            for (int x = tid; x < KT; x += 64 * kWeighWaves) {
+            for (int x = tid; x < KT; x += 64 * WAVES) {
                 const int key = key0 + x;
                 float mine = 0.0f;
 #pragma unroll
-                for (int v = 0; v < kWeighWaves; v++) mine += part[v][x];
+                for (int v = 0; v < WAVES; v++) mine += part[v][x];
                 const uint32_t at = key < s.keys ? (uint32_t)p.batch.table[(size_t)b * p.batch.table_stride + ((uint32_t)key >> p.geom.log2_page)] : 0xffffffffu;
                 if (at < p.geom.num_pages) {
                     float* to = p.sums + (((size_t)at * p.geom.Hkv + hk) << p.geom.log2_page) + ((uint32_t)key & pmask);
@@ -324,6 +393,10 @@ __global__ void __launch_bounds__(64 * kWeighWaves, 2) weigh_chunk_kernel(WeighP
 
 // Rows of a KV head from which a sequence is the chunk kernel's.
 constexpr uint32_t kWeighChunk = 128;
+// 128 keys to four waves where there are as many workgroups as the chip holds, else 64 to eight.
+// us of the two: 8 prompts of 2048 (D = 128, 1024 workgroups of the first kind) 188 / 240, four of
+// them 118 / 125, two 103 / 69; 512 rows on 8192 keys (512) 57 / 73; D = 64: 8 prompts 139 / 127, two 80 / 45.
+constexpr uint64_t kWeighGroups = 512;
 
 template <int FMT, int D>
 static hipError_t launch_weigh(WeighParams p, hipStream_t st) {
@@ -331,11 +404,6 @@ static hipError_t launch_weigh(WeighParams p, hipStream_t st) {
     uint64_t keys = p.max_kv ? p.max_kv : 1;
     if (p.window && keys > (uint64_t)p.window + p.max_new) keys = (uint64_t)p.window + p.max_new;
     const bool chunks = rows >= kWeighChunk, both = chunks && p.batch.T < (uint64_t)p.batch.B * p.max_new && p.batch.B > 1;
-    const uint32_t across = p.batch.B < 65535 ? p.batch.B : 65535;
-    auto tiles_of = [&](uint32_t of) {  // of the longest sequence, no more workgroups than a launch may have
-        const uint64_t t = (keys + of - 1) / of, most = (1u << 24) / p.geom.Hkv;
-        return (uint32_t)(t < most ? t : most);
-    };
     p.min_rows = 0;
     p.max_rows = both ? kWeighChunk : 0xffffffffu;
     if (!chunks || both) {
@@ -351,10 +419,22 @@ static hipError_t launch_weigh(WeighParams p, hipStream_t st) {
     }
     p.min_rows = both ? kWeighChunk : 0;
     p.max_rows = 0xffffffffu;
-    constexpr int NT = 4;
-    const uint32_t tiles = tiles_of(32 * NT);
-    hipLaunchKernelGGL((weigh_chunk_kernel<FMT, D, NT>), dim3(tiles * p.geom.Hkv, across), dim3(64 * kWeighWaves), 0, st, p, tiles);
-    return hipGetLastError();
+    const uint64_t heads = (uint64_t)p.batch.B * p.geom.Hkv, most = std::max(1u << 20, p.geom.Hkv) / p.geom.Hkv * p.geom.Hkv;
+    auto launch = [&](auto kernel, uint32_t tile, uint32_t waves, size_t (&attr)[kMaxDevices]) {
+        const size_t lds = (size_t)waves * 32 * D * 2;
+        const hipError_t e = lds_limit_once((const void*)kernel, lds, attr);
+        if (e != hipSuccess) return e;
+        // the tiles that most rows see first, of all sequences
+        const dim3 grid((uint32_t)std::min(heads, most), (uint32_t)std::min((keys + tile - 1) / tile, (uint64_t)65535));
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), lds, st, p);
+        return hipGetLastError();
+    };
+    if ((keys + 127) / 128 * heads >= kWeighGroups) {
+        static size_t attr[kMaxDevices] = {};
+        return launch(weigh_chunk_kernel<FMT, D, 4, 4>, 128, 4, attr);
+    }
+    static size_t attr[kMaxDevices] = {};
+    return launch(weigh_chunk_kernel<FMT, D, 2, 8>, 64, 8, attr);
 }
 
 hipError_t launch_kv_weigh(const WeighParams& p, hipStream_t st) {

@@ -155,6 +155,34 @@ def test_weigh_many_sequences(bridge, fmt, B, H, Hkv, P, pages, window):
 
 
 @gpu
+@pytest.mark.parametrize("kernels", ["rows", "chunks"])
+@pytest.mark.parametrize("G", [1, 2, 3, 7, 12, 16, 17, 31, 32, 33, 40, 64, 71])
+@pytest.mark.parametrize("window", [0, 40])
+def test_weigh_groups(bridge, kernels, G, window):
+    """Query heads that share a KV head, any number: what belongs to no row weighs nothing, though its values are."""
+    D, P, Hkv, lens, new = 128, 32, 2, [170, 33, 5, 64], [70, 20, 5, 1]
+    s = Setup(Q8_0, lens, new, Hkv, D, P, seed=G)
+    q = half(s.rng, G * Hkv, s.T, D)
+    q[:, 60] = np.inf   # a row of the first sequence: NaN or infinity for the keys that it sees, and none else
+    sums = s.rng.random((s.num_pages, Hkv, P)).astype(np.float32)
+    lse = s.rng.standard_normal((G * Hkv, s.T)).astype(np.float32) + 4
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), dev(s.table), **EXPECTED[kernels])
+    got, clean = dev(sums), dev(sums)
+    say("weigh groups", kernels, G, window)
+    bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(lse), got, 0.09, window=window)
+    q[:, 60] = 0.5
+    bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(lse), clean, 0.09, window=window)
+    bridge.synchronize()
+    want, bound = weighed(s, sums, q, lse, lens, s.q_start, window, 0.09)
+    close(clean.cpu().numpy(), want, bound, "sums")
+    seen = np.zeros(sums.shape, bool)  # by that row: token 60 of positions 100 .. 169
+    for k in range(max(0, 160 - window + 1) if window else 0, 161):
+        seen[s.table[0, k // P], :, k % P] = True
+    got = got.cpu().numpy()
+    assert np.isfinite(got[~seen]).all() and (got[~seen] == clean.cpu().numpy()[~seen]).all()
+
+
+@gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_weights_of_a_row_add_up_to_one(bridge, fmt):
     """Attention hands its lse over: what the rows of a call give all keys is 1 for each row and query head."""
