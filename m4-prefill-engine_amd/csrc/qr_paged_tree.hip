@@ -12,44 +12,85 @@ __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
 // A node's ancestors are itself and its parent's, anc(i) = {i} + anc(parent(i)), and a parent
 // comes before its nodes.  64 nodes at a time, a lane each: pointers are doubled six times, so
 // that every node has its ancestors among the 64 as one word; the lowest of them says where
-// the path leaves the 64, to a node whose row of the mask is there already and is copied.
-// A block a sequence.
+// the path leaves the 64, to an earlier node or to none.
+struct Near {
+    uint64_t bits;
+    int exit;
+};
+__device__ __forceinline__ Near near_of(int parent, int base, int lane) {
+    int jump = parent >= base ? parent - base : -1;
+    const int leave = parent >= 0 && parent < base ? parent : -1;
+    uint64_t near = (uint64_t)1 << lane;
+#pragma unroll
+    for (int r = 0; r < 6; r++) {
+        const int at = jump < 0 ? lane : jump;
+        near |= shfl_u64(near, at);
+        const int further = __shfl(jump, at);
+        jump = jump < 0 ? -1 : further;
+    }
+    return Near{near, __shfl(leave, __ffsll((unsigned long long)near) - 1)};
+}
+
+// A block a sequence.  Up to kHeldNodes the words of all its 64s are formed side by side and kept
+// in LDS; then a thread follows each node's path from 64 to 64 and writes its row.  Longer trees
+// take one 64 after the other, whose rows copy the rest from those that are there already (300
+// nodes of 64 requests so: 10.5 us, a round trip to memory for each 64; in LDS 4.5).
+constexpr int kHeldNodes = 2048;
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) draft_tree_kernel(DraftParams p) {
-    __shared__ uint64_t near_of[64];
-    __shared__ int exit_of[64];
-    const int lane = threadIdx.x & 63;
+    __shared__ uint64_t near[kHeldNodes];
+    __shared__ int leave[kHeldNodes];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t W = p.words;
     for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
         const NewRows s = new_rows(p.batch, b);
-        for (int base = 0; base < s.n; base += 64) {
-            const int i = base + lane;
-            int parent = i < s.n ? p.parents[s.q0 + i] : -1;
-            if (parent >= i) parent = -1;
-            if (threadIdx.x < 64) {
-                int jump = parent >= base ? parent - base : -1, leave = parent >= 0 && parent < base ? parent : -1;
-                uint64_t near = (uint64_t)1 << lane;
-#pragma unroll
-                for (int r = 0; r < 6; r++) {
-                    const int at = jump < 0 ? lane : jump;
-                    near |= shfl_u64(near, at);
-                    const int further = __shfl(jump, at);
-                    jump = jump < 0 ? -1 : further;
+        uint32_t* mask = p.mask + (size_t)s.q0 * W;
+        auto parent_of = [&](int i) {
+            const int parent = i < s.n ? p.parents[s.q0 + i] : -1;
+            return parent < i ? parent : -1;
+        };
+        if (s.n <= kHeldNodes) {
+            for (int base = 64 * wave; base < s.n; base += THREADS) {
+                const Near at = near_of(parent_of(base + lane), base, lane);
+                near[base + lane] = at.bits;
+                leave[base + lane] = at.exit;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < s.n; i += THREADS) {
+                uint32_t* row = mask + (size_t)i * W;
+                int cur = i, depth = 0;
+                for (uint32_t w = i / 64 * 2 + 2; w < W; w++) row[w] = 0;
+                for (int x = i / 64; x >= 0; x--) {
+                    uint64_t bits = 0;
+                    if (cur >= 64 * x) {  // else the path passes these by
+                        bits = near[cur];
+                        cur = leave[cur];
+                        depth += __popcll(bits);
+                    }
+                    if (2u * x < W) row[2 * x] = (uint32_t)bits;
+                    if (2 * x + 1u < W) row[2 * x + 1] = (uint32_t)(bits >> 32);
                 }
-                leave = __shfl(leave, __ffsll((unsigned long long)near) - 1);
-                near_of[lane] = near;
-                exit_of[lane] = leave;
-                if (i < s.n) p.places[s.q0 + i] = (leave >= 0 ? p.places[s.q0 + leave] + 1 : s.first) + __popcll(near) - 1;
+                p.places[s.q0 + i] = s.first + depth - 1;
+            }
+            __syncthreads();
+            continue;
+        }
+        for (int base = 0; base < s.n; base += 64) {
+            const int i = base + lane, parent = parent_of(i);
+            if (wave == 0) {
+                const Near at = near_of(parent, base, lane);
+                near[lane] = at.bits;
+                leave[lane] = at.exit;
+                if (i < s.n) p.places[s.q0 + i] = (at.exit >= 0 ? p.places[s.q0 + at.exit] + 1 : s.first) + __popcll(at.bits) - 1;
             }
             __syncthreads();
             const uint32_t rows = min(s.n - base, 64), own = (uint32_t)base / 32;
-            uint32_t* mask = p.mask + (size_t)s.q0 * W;
             for (uint32_t x = threadIdx.x; x < rows * W; x += THREADS) {  // W is at most 2^21
                 const uint32_t r = x / W, w = x % W;
                 uint32_t bits = 0;
-                if (w == own) bits = (uint32_t)near_of[r];
-                else if (w == own + 1) bits = (uint32_t)(near_of[r] >> 32);
-                else if (w < own && exit_of[r] >= 0) bits = mask[(size_t)exit_of[r] * W + w];
+                if (w == own) bits = (uint32_t)near[r];
+                else if (w == own + 1) bits = (uint32_t)(near[r] >> 32);
+                else if (w < own && leave[r] >= 0) bits = mask[(size_t)leave[r] * W + w];
                 mask[(size_t)base * W + x] = bits;
             }
             __syncthreads();  // rows of later nodes copy these

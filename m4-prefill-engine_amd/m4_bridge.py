@@ -808,7 +808,7 @@ class HIPBridge:
         return tree.ref
 
     def _ids(self, name: str, t: Any, n: int) -> int:
-        if not isinstance(t, _torch.Tensor) or t.dtype is not _torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        if not isinstance(t, _torch.Tensor) or t.dtype is not _torch.int32 or t.shape != (n,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor [{n}]")
         return t.data_ptr()
 

@@ -173,6 +173,15 @@ def test_draft_tree(bridge, sizes, back, words):
 
 
 @gpu
+@pytest.mark.parametrize("sizes,back,words", [
+    ([2048, 70], 3, 64), ([2049, 70], 3, 65), ([2047, 2050], 5000, 65),  # about the most whose words are held together
+    ([2048], 1, 3), ([3000], 1, 3), ([1000], 2, 0x41), ([2100], 2, 0x61),
+])
+def test_draft_tree_of_many_nodes(bridge, sizes, back, words):
+    test_draft_tree(bridge, sizes, back, words)
+
+
+@gpu
 @pytest.mark.parametrize("starts", [(-3, 4, 9), (0, 2, 40), (-2 ** 31, 3, 2 ** 31 - 1), (5, 3, 7), (9, 9, 9)])
 def test_rows_that_a_call_has_are_the_nodes(bridge, starts):
     """Starts below zero and past the rows: the nodes are the rows there are, from the first of them on; a sequence whose
