@@ -123,8 +123,9 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t f = r0 + 4 * g + e;
-                l[e] = INFINITY;  // no such row
+                l[e] = INFINITY;  // no such row, or one that sees nothing
                 if (f < rows) l[e] = p.lse.p[row_offset(p, p.lse, s.q0, hk, f)];
+                if (l[e] == -INFINITY) l[e] = INFINITY;
             }
         };
         // page numbers of the next 16 tiles, a lane each 16 keys

@@ -183,6 +183,61 @@ def test_weigh_groups(bridge, kernels, G, window):
 
 
 @gpu
+@pytest.mark.parametrize("kernels", ["rows", "chunks"])
+@pytest.mark.parametrize("window", [0, 25])
+def test_rows_without_a_sum_weigh_nothing(bridge, kernels, window):
+    """lse -infinity, whether or not the row sees keys; +infinity too."""
+    lens, new, H, Hkv, D, P = [200, 60], [70, 60], 8, 2, 64, 16
+    s = Setup(Q8_0, lens, new, Hkv, D, P, seed=31)
+    q = half(s.rng, H, s.T, D)
+    sums = s.rng.random((s.num_pages, Hkv, P)).astype(np.float32)
+    lse = s.rng.standard_normal((H, s.T)).astype(np.float32) + 4
+    none = s.rng.random((H, s.T)) < 0.4
+    given = np.where(none, np.where(s.rng.random((H, s.T)) < 0.8, -np.inf, np.inf), lse).astype(np.float32)
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), dev(s.table), **EXPECTED[kernels])
+    got = dev(sums)
+    say("weigh without a sum", kernels, window)
+    bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(given), got, 0.1, window=window)
+    bridge.synchronize()
+    want, bound = weighed(s, sums, q, np.where(none, np.float32(1e5), lse), lens, s.q_start, window, 0.1)
+    close(got.cpu().numpy(), want, bound, "sums")
+
+
+@gpu
+def test_pages_past_4_gib(bridge):
+    """The same bits from pages that lie past 4 GiB of a cache as from its first ones."""
+    import torch
+
+    lens, new, H, Hkv, D, P, budget = [700, 90, 333], [40, 9, 64], 16, 8, 128, 256, 128
+    s = Bounded(Q8_0, lens, new, Hkv, D, P, seed=77)
+    s.grow(budget)
+    few, pages = s.cache(), dev(s.pages.raw)
+    far = (1 << 32) // (few.pages.numel() // s.num_pages) + 7
+    many = m4_bridge.PagedKVCache(Q8_0, far + s.num_pages, P, Hkv, D)
+    many.pages.view(far + s.num_pages, -1)[far:] = pages.view(s.num_pages, -1)
+    q, parents = dev(half(s.rng, H, s.T, D)), dev(np.concatenate([np.arange(n, dtype=np.int32) - 1 for n in new]))
+    keep = dev(np.concatenate([np.minimum(2 * np.arange(n), n).astype(np.int32) for n in new]))
+    count, results = dev(np.array([n // 2 for n in new], np.int32)), []
+    for cache, at in ((few, 0), (many, far)):
+        batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), dev(s.table + at), max(new), max(lens))
+        tree, O, lse = m4_bridge.DraftTree.empty(s.T, max(new)), torch.empty_like(q), torch.empty(H, s.T, device="cuda")
+        sums = torch.zeros(cache.num_pages, Hkv, P, device="cuda")
+        kept, length = i32(*[0] * (len(lens) * Hkv * budget)).reshape(len(lens), Hkv, budget), dev(i32(*[0] * len(lens)))
+        kept = dev(kept)
+        say("pages past 4 GiB", at)
+        bridge.draft_tree(batch, parents, tree)
+        bridge.dispatch_paged_attn(cache, batch, q, O, 0.09, tree=tree, lse=lse)
+        bridge.kv_cache_keep(cache, batch, keep, count)
+        bridge.kv_cache_weigh(cache, batch, q, lse, sums, 0.09)
+        bridge.kv_cache_evict(cache, batch, sums, dev(s.table_out + at), length, budget, sinks=3, recent=20, kept=kept)
+        bridge.synchronize()
+        raw = cache.pages.view(cache.num_pages, -1)[at:at + s.num_pages]
+        results.append([x.clone().view(torch.uint8) for x in (O, lse, sums[at:at + s.num_pages].contiguous(), kept, length, raw.contiguous())])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_weights_of_a_row_add_up_to_one(bridge, fmt):
     """Attention hands its lse over: what the rows of a call give all keys is 1 for each row and query head."""
