@@ -277,6 +277,7 @@ def evicted(s, raw, sums, lens, table, table_out, budget, sinks, recent):
     """(pages, sums, kept, lengths) after an eviction."""
     pages, out = raw.copy(), sums.copy()
     kept, length = np.full((len(lens), s.Hkv, budget), -1, np.int32), np.zeros(len(lens), np.int32)
+    at_slot = np.array([token_bytes(s.pages, x) for x in range(s.P)])
     for b, L in enumerate(lens):
         n = min(max(int(L), 0), table.shape[1] * s.P)
         at = table[b, np.arange(n) // s.P]
@@ -286,11 +287,11 @@ def evicted(s, raw, sums, lens, table, table_out, budget, sinks, recent):
             places = chosen(w, there, budget, sinks, recent, int(L))
             kept[b, h, :places.size] = places
             length[b] = places.size
-            for i, p in enumerate(places):
-                to = table_out[b, i // s.P]
-                if 0 <= to < s.num_pages:
-                    pages[to, h, token_bytes(s.pages, i % s.P)] = raw[at[p], h, token_bytes(s.pages, p % s.P)]
-                    out[to, h, i % s.P] = sums[at[p], h, p % s.P]
+            i = np.arange(places.size)
+            to = table_out[b, i // s.P]
+            i, p, to = (x[(to >= 0) & (to < s.num_pages)] for x in (i, places, to))
+            pages[to[:, None], h, at_slot[i % s.P]] = raw[at[p][:, None], h, at_slot[p % s.P]]
+            out[to, h, i % s.P] = sums[at[p], h, p % s.P]
     return pages, out, kept, length
 
 
