@@ -15,7 +15,8 @@ from test_paged_tree import attend, host, i32, launched, lib, rows_of, set_, tok
 
 gpu = pytest.mark.gpu
 # what is expected of the lengths chooses the kernels; the results hold for any
-EXPECTED = {"rows": {"max_new": 1, "max_kv": 1}, "chunks": {"max_new": 10 ** 6, "max_kv": 400}, "both": {"max_new": 2 ** 20, "max_kv": 10 ** 4}}
+EXPECTED = {"rows": {"max_new": 1, "max_kv": 1}, "chunks": {"max_new": 10 ** 6, "max_kv": 400}, "both": {"max_new": 2 ** 20, "max_kv": 10 ** 4},
+            "wide": {"max_new": 10 ** 6, "max_kv": 2 * 10 ** 6}}
 
 
 # ---- weights received -----------------------------------------------------------------------------------------------
@@ -101,7 +102,22 @@ def test_weigh(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("kernels", ["rows", "chunks", "both"])
+@pytest.mark.parametrize("lens,new,H,Hkv,D,P,window", [
+    ([1], [1], 1, 1, 64, 16, 0),
+    ([260, 131], [61, 100], 6, 2, 128, 64, 0),
+    ([260, 131, 700], [61, 100, 513], 6, 2, 128, 256, 50),
+    ([1200, 40], [1100, 1], 5, 1, 128, 16, 0),
+    ([1200, 40, 90], [1100, 1, 90], 5, 1, 64, 16, 300),
+    ([1500, 0, 513, 512], [3, 0, 513, 31], 8, 2, 64, 32, 0),
+    ([1100, 1029], [200, 1029], 3, 1, 128, 16, 600),
+])
+def test_weigh_as_if_long(bridge, fmt, lens, new, H, Hkv, D, P, window):
+    test_weigh(bridge, fmt, lens, new, H, Hkv, D, P, window, "wide")
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kernels", ["rows", "chunks", "both", "wide"])
 @pytest.mark.parametrize("scale", [-0.125, 0.0, 0.3])
 def test_weigh_out_of_range(bridge, fmt, kernels, scale):
     """Starts outside the rows, lengths past the table, more rows than keys, pages that are not there, rows that see
@@ -155,7 +171,7 @@ def test_weigh_many_sequences(bridge, fmt, B, H, Hkv, P, pages, window):
 
 
 @gpu
-@pytest.mark.parametrize("kernels", ["rows", "chunks"])
+@pytest.mark.parametrize("kernels", ["rows", "chunks", "wide"])
 @pytest.mark.parametrize("G", [1, 2, 3, 7, 12, 16, 17, 31, 32, 33, 40, 64, 71])
 @pytest.mark.parametrize("window", [0, 40])
 def test_weigh_groups(bridge, kernels, G, window):
@@ -183,7 +199,7 @@ def test_weigh_groups(bridge, kernels, G, window):
 
 
 @gpu
-@pytest.mark.parametrize("kernels", ["rows", "chunks"])
+@pytest.mark.parametrize("kernels", ["rows", "chunks", "wide"])
 @pytest.mark.parametrize("window", [0, 25])
 def test_rows_without_a_sum_weigh_nothing(bridge, kernels, window):
     """lse -infinity, whether or not the row sees keys; +infinity too."""
