@@ -123,9 +123,8 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t f = r0 + 4 * g + e;
-                l[e] = INFINITY;  // no such row, or one that sees nothing
+                l[e] = INFINITY;  // no such row
                 if (f < rows) l[e] = p.lse.p[row_offset(p, p.lse, s.q0, hk, f)];
-                if (l[e] == -INFINITY) l[e] = INFINITY;
             }
         };
         // page numbers of the next 16 tiles, a lane each 16 keys
@@ -176,10 +175,13 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 #pragma unroll
                     for (int kk = 0; kk < KK; kk++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[kk], kf[t][kk], sc[t], 0, 0, 0);
                 }
+                float less[4];  // a row that sees nothing gives nothing (asked here: the products do not wait for lse)
+#pragma unroll
+                for (int e = 0; e < 4; e++) less[e] = l[e] == -INFINITY ? -INFINITY : l[e] * -1.4426950408889634f;
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[t][e] = __builtin_fmaf(sc[t][e], c, l[e] * -1.4426950408889634f);
+                    for (int e = 0; e < 4; e++) sc[t][e] = __builtin_fmaf(sc[t][e], c, less[e]);
                 if (!whole)
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
