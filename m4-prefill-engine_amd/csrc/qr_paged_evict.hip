@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 // touch 64 lines a load; a row's address by division and 64-bit products cost as much as a
 // tile's weights, so all offsets are formed once); their sums meet in LDS.  A tile's products run
 // beside the exponentials of the one before.  8 heads, 2048 rows of 32 query heads on 30000 keys of
-// 128: 545 us, 0.89 PFLOP/s.  By itself that loop takes 350 cycles a tile of 32 x 32 (256 of products,
+// 128: 535 us, 0.91 PFLOP/s.  By itself that loop takes 350 cycles a tile of 32 x 32 (256 of products,
 // 256 of fused multiplies, exponentials and sums, at 1.65 GHz under this load), 390 us; bringing
 // the rows (3.8 GB through the L2s) costs 100 more.
 template <int FMT, int D, int NT, int WAVES>
@@ -342,15 +342,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams 
 #pragma unroll
                     for (int t = 0; t <= NT; t++) {
                         if (t < NT) sc[t & 1] = f16v_t{};
+                        float of_rows = 0.0f;  // apart from what there is: many small terms
 #pragma unroll
                         for (int kk = 0; kk < KK; kk++) {
                             if (t < NT) sc[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[kk], kf[t][kk], sc[t & 1], 0, 0, 0);
                             if (t > 0)
 #pragma unroll
                                 for (int e = kk * 16 / KK; e < (kk + 1) * 16 / KK; e++)
-                                    sum[t - 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[(t - 1) & 1][e], c, -l[e]));
+                                    of_rows += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[(t - 1) & 1][e], c, -l[e]));
                             if (t > 0) __builtin_amdgcn_sched_barrier(0);
                         }
+                        if (t > 0) sum[t - 1] += of_rows;
                     }
                 } else {
 #pragma unroll
