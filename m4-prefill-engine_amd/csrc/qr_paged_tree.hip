@@ -105,7 +105,8 @@ hipError_t launch_draft_tree(const DraftParams& p, hipStream_t st) {
 }
 
 // From node 0 on, the first node behind the present one that is its child and whose token is
-// the model's choice there.  A wave a sequence, 64 nodes at a time.
+// the model's choice there.  A wave a sequence, 64 nodes at a time: a child of the present node is
+// one ballot, so what it takes is the loads (26 nodes 1.7 us, 64 requests of 64 nodes 3.8).
 __global__ void __launch_bounds__(64) tree_accept_kernel(AcceptParams p) {
     const int lane = threadIdx.x;
     for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
@@ -157,7 +158,8 @@ hipError_t launch_tree_accept(const AcceptParams& p, hipStream_t st) {
 // is read by none of the later ones, since keep[i] >= i: a step's tokens are all loaded before
 // any is stored.  A block a sequence, so that its length may be written where it was read.
 // A token of a head is CB / 16 pieces of K codes, CB / 4 of V codes (of four tokens' words each
-// the bytes of one) and one of its scales.
+// the bytes of one) and one of its scales.  Few bytes, each behind its page number: 64 requests with
+// some nodes kept of 64 (8 heads of 128, 8 bit) 9 us, one 2.3.
 constexpr int kKeepThreads = 1024, kKeepList = 256;
 template <int FMT, int D>
 __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(KeepParams p) {
