@@ -373,6 +373,26 @@ def test_evict(bridge, fmt, lens, Hkv, D, P, budget, sinks, recent, max_kv):
 
 
 @gpu
+@pytest.mark.parametrize("lens,Hkv,D,P,budget,sinks,recent,max_kv", [
+    ([512, 511, 510, 257, 256, 255, 64, 1, 0], 3, 64, 16, 100, 3, 40, 512),
+    ([512, 513, 90, 2000, 4], 2, 64, 32, 300, 0, 1, 512),                       # some longer than expected
+    ([500, 20], 1, 128, 64, 512, 0, 0, 500),                                    # all of them
+    ([80 + b % 9 for b in range(130)], 2, 64, 16, 1, 0, 1, 89),
+    ([(911 * b) % 1025 for b in range(140)], 8, 64, 64, 33, 2, 5, 1024),        # many, and longer
+    ([(911 * b) % 1025 for b in range(140)] + [3000], 8, 64, 64, 700, 0, 0, 600),
+])
+def test_evict_of_short_sequences(bridge, lens, Hkv, D, P, budget, sinks, recent, max_kv):
+    test_evict(bridge, Q8_0, lens, Hkv, D, P, budget, sinks, recent, max_kv)
+
+
+@gpu
+@pytest.mark.parametrize("value", ["zero", "few", "near", "nan"])
+@pytest.mark.parametrize("n,max_kv", [(512, 512), (300, 300), (1000, 300), (512, 513)])
+def test_evict_where_many_of_few_are_alike(bridge, value, n, max_kv):
+    test_evict_where_many_are_alike(bridge, value, n, max_kv)
+
+
+@gpu
 @pytest.mark.parametrize("value", ["zero", "few", "near", "nan"])
 @pytest.mark.parametrize("n,max_kv", [(9000, 9000), (45000, 45000), (45000, 1)])
 def test_evict_where_many_are_alike(bridge, value, n, max_kv):
