@@ -13,7 +13,7 @@
 // QR_PAGED_TREE, a build of its own: the same kernels (TREE) where a mask says which of the
 // new tokens a row sees, and with the logarithm of each row's sum.  Only tiles that hold new
 // tokens ask the mask.  H = 32, Hkv = 8, D = 128: trees of 64 nodes over 16 requests of 200 ..
-// 8192 keys (Q8_0) 73 us and the join 15, of 61 nodes over four of 131072 (Q4_0) 620, 0.84 PFLOP/s.
+// 8192 keys (Q8_0) 70 us and the join 15, of 61 nodes over four of 131072 (Q4_0) 594, 0.88 PFLOP/s.
 #include "qr_device.h"
 #include "qr_paged.h"
 #include "qr_paged_decode.h"
@@ -855,21 +855,31 @@ __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq
     return end <= lo ? 1u : (uint32_t)(end - lo + KT - 1) / KT;
 }
 
+// A tile in LDS: K a row a key, V^T a row a dim, 16 bytes between the rows: what is read, a row
+// a lane, meets in no bank, and a lane's addresses are one base and constants.  V is stored a few rows
+// apart; neighbours change places in every other 16 rows, so that half as many meet.
+template <int D, int KT>
+struct ChunkLds {
+    static constexpr uint32_t key = D * 2 + 16, dim = KT * 2 + 16, keys = KT * key, tile = keys + D * dim;
+    static __device__ constexpr uint32_t dim_at(uint32_t r) { return (r ^ (r >> 4 & 1)) * dim; }
+};
+
 // A workgroup of NW waves takes 32 NW rows (whole tokens' query heads) and an even
 // share of the line of all row tiles' key tiles, as above.  Key tiles of 16 NW
 // keys: every thread turns 32 bytes of K and of V codes (Q4_0: 16) into fp16 in a
 // double-buffered LDS tile, the codes loaded two tiles ahead; then each wave
 // takes its rows over the tile, 32 x 32 scores at a time.  256 rows share the work
 // of turning codes (128 rows: 1306 us where 256 take 1140).  2048 tokens over 30000
-// keys (D = 128, 972 GFLOP) 1067 us with the join, 0.91 PFLOP/s.  Counters: the matrix
-// pipe 44% busy, 8.1 vector operations per MFMA beside it, LDS bank conflicts in 0.23 M
-// of a CU's 1.98 M cycles (V's tile is stored by lanes four rows apart), at 1.9 GHz of 2.2.
+// keys (D = 128, 972 GFLOP) 1029 us with the join, 0.94 PFLOP/s.  Counters: the matrix
+// pipe 47% busy, 7.7 vector operations per MFMA beside it, LDS bank conflicts in 0.12 M
+// of a CU's 1.90 M cycles (V's tile is stored by lanes four rows apart), at 1.8 GHz of 2.4, to
+// which the clock falls under this load.
 template <int FMT, int D, int NW, bool TREE>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
     constexpr int DT = D / 32, KK = D / 16;
-    constexpr int KU = D / 8, VU = KT / 8;       // 16-byte units of a K row (a key), of a V^T row (a dim)
-    constexpr int KB = KT * D * 2, TB = 2 * KB;  // bytes of a K tile, of a tile
+    using L = ChunkLds<D, KT>;
+    constexpr uint32_t KS = L::key, VS = L::dim, KB = L::keys, TB = L::tile;
     constexpr int RUN = D / 4;                   // dims of a K task: a quarter of a key
     constexpr int DV = D / 32;                   // dims of a V task: 8 keys of each
     constexpr int KW = FMT == QUANT_Q8_0 ? RUN / 4 : RUN / 8, VW = FMT == QUANT_Q8_0 ? DV : DV / 2;
@@ -929,18 +939,14 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
     if (neg) c = -c;
     c = fmaxf(c, 1.17549435e-38f);
 
-    // Unit u of row r of a tile sits at u ^ swz(r).  A row's units differ from one
-    // base by the exclusive or of 16 times their number: the bases alone are kept
-    // (hidden from the compiler, which would keep every sum).
-    auto swz = [](int units, uint32_t r) -> uint32_t { return units == 16 ? (r & 15u) : ((r ^ (r >> 3)) & 7u); };
-    auto place = [&](int units, uint32_t r, uint32_t u) { return r * (units * 16u) + 16u * (u ^ swz(units, r & 31u)); };
-    uint32_t kof = place(KU, (uint32_t)j, (uint32_t)g), vof = place(VU, (uint32_t)j, (uint32_t)g);
+    uint32_t kof = j * KS + 16 * g, vof = L::dim_at(j) + 16 * g;
     // tasks: K, a quarter of key 16 wave + lane / 4; V, dims DV (lane % 32) .. of
     // unit 2 wave + lane / 32, i.e. keys 16 wave + 4 g + {0 .. 3, 8 .. 11}
     const uint32_t kkey = lane >> 2, kq = lane & 3, vdim = DV * (uint32_t)j;
-    uint32_t kst = place(KU, 16 * wave + kkey, kq * (RUN / 8)), vst = place(VU, vdim, 2 * wave + g);
+    uint32_t kst = (16 * wave + kkey) * KS + kq * (RUN / 8) * 16, vst = vdim * VS + (2 * wave + g) * 16;
     uint32_t kld = kkey * CB + kq * (KW * 4), vld = p.geom.v_off + g * (4 * CB) + vdim * (4 * CB / D);
     uint32_t ksl = p.geom.ks_off + (kkey * NB + kq * NB / 4) * 2, vsl = p.geom.vs_off + (g * NB + vdim / 32) * 8;
+    const uint32_t swap = vdim >> 4 & 1 ? VS : 0;  // dim_at
     const h2_t one2 = {(_Float16)1.0f, (_Float16)1.0f};
 
     f16v_t o[DT];
@@ -1047,7 +1053,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             const h2_t d = as_h2(kd | kd << 16);
 #pragma unroll
             for (int kk = 0; kk < RUN / 8; kk++)
-                *reinterpret_cast<h8_t*>(buf + (kst ^ 16u * kk)) = k_octet<FMT>(kw, kk, d);
+                *reinterpret_cast<h8_t*>(buf + kst + 16u * kk) = k_octet<FMT>(kw, kk, d);
             int odd = 0;
             if (k0 + KT - 1 > all0 || k0 < all_low1 || !mine_there) {
                 // not all rows see all of the tile's keys: V scales of keys that none sees are cleared
@@ -1068,17 +1074,17 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
 #pragma unroll
             for (int x = 0; x < DV; x++) {
                 const u2_t a = v_quad<FMT>(vw[0], x, vd[0]), e = v_quad<FMT>(vw[1], x, vd[1]);
-                *reinterpret_cast<u4_t*>(buf + KB + x * (VU * 16) + (vst ^ 16u * x)) = u4_t{a.x, a.y, e.x, e.y};
+                *reinterpret_cast<u4_t*>(buf + KB + vst + x * VS + (x & 1 ? -swap : swap)) = u4_t{a.x, a.y, e.x, e.y};
             }
         };
 
         // ---- this wave's rows over a tile, 32 keys (a unit) at a time ----
         auto scores = [&](const uint8_t* buf, int x) {
-            const uint8_t* kb = buf + x * 32 * (KU * 16);
+            const uint8_t* kb = buf + x * 32 * KS;
             f16v_t sc{};
 #pragma unroll
             for (int kk = 0; kk < KK; kk++)
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8_t*>(kb + (kof ^ 32u * kk)), qf[kk], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8_t*>(kb + kof + 32u * kk), qf[kk], sc, 0, 0, 0);
             return sc;
         };
         // Exponents of a unit's weights, beside the reference point; whether that has to
@@ -1123,7 +1129,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 const h8_t pf = __builtin_bit_cast(h8_t, u4_t{pk[4 * t2], pk[4 * t2 + 1], pk[4 * t2 + 2], pk[4 * t2 + 3]});
 #pragma unroll
                 for (int t = 0; t < DT; t++) {
-                    const h8_t va = *reinterpret_cast<const h8_t*>(buf + KB + t * 32 * (VU * 16) + (vof ^ 32u * (2 * x + t2)));
+                    const h8_t va = *reinterpret_cast<const h8_t*>(buf + KB + vof + L::dim_at(32 * t) + 32u * (2 * x + t2));
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pf, o[t], 0, 0, 0);
                 }
             }
@@ -1144,7 +1150,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 const b8_t sf = __builtin_bit_cast(b8_t, seen);
 #pragma unroll
                 for (int t = 0; t < DT; t++) {
-                    const h8_t va = *reinterpret_cast<const h8_t*>(buf + KB + t * 32 * (VU * 16) + (vof ^ 32u * (2 * x + t2)));
+                    const h8_t va = *reinterpret_cast<const h8_t*>(buf + KB + vof + L::dim_at(32 * t) + 32u * (2 * x + t2));
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(marks_of<false>(va), sf, o[t], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(marks_of<true>(va), sf, o[t], 0, 0, 0);
@@ -1172,10 +1178,10 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 // matrix pipe leaves the transcendental unit free), the next one's exponents
                 // beside this one's values.
                 auto key = [&](int x, int kk) {
-                    return *reinterpret_cast<const h8_t*>(buf + x * 32 * (KU * 16) + (kof ^ 32u * kk));
+                    return *reinterpret_cast<const h8_t*>(buf + kof + x * 32 * KS + 32u * kk);
                 };
                 auto value = [&](int x, int i) {
-                    return *reinterpret_cast<const h8_t*>(buf + KB + (i % DT) * 32 * (VU * 16) + (vof ^ 32u * (2 * x + i / DT)));
+                    return *reinterpret_cast<const h8_t*>(buf + KB + vof + L::dim_at(32 * (i % DT)) + 32u * (2 * x + i / DT));
                 };
                 constexpr int NV = 2 * DT;
                 h8_t kf[4], vf[4];
@@ -1311,9 +1317,9 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         if (u0 + 1 < u1) fetch(u0 + 1);
         __syncthreads();
         for (int u = u0; u < u1; u++) {
+            attend(u);  // before the next tile is turned: a share's second tile has that long to come
             if (u + 1 < u1) fill(u + 1);
             if (u + 2 < u1) fetch(u + 2);
-            attend(u);
             __syncthreads();
         }
 
@@ -1422,8 +1428,18 @@ static hipError_t launch_join(const PagedAttnParams& p, const WorkPlan& w, hipSt
     // where items have many parts.  us of the whole call with 4 / 16 of them: 64 tokens
     // over 16384 keys (32 parts an item) 82 / 42, one token 27 / 23, 64 requests (one
     // part) 34 / 40.
-    const uint32_t parts = w.groups / w.items, across = R > 32 ? 32 : (parts >= 16 ? 16 : (parts >= 8 ? 8 : 4));
-    const uint32_t most = 4 * kJoinBlocks / across;
+    const uint32_t parts = w.groups / w.items;
+    uint32_t across = parts >= 16 ? 16 : (parts >= 8 ? 8 : 4), most = 4 * kJoinBlocks / across;
+    if (R > 32) {
+        // As many blocks as an item's rows are taken side by side, and some for each item.  us of the
+        // kernel with 64 x 32 blocks / so: 10 items of 25 parts 45 / 19, 32 of 8 12.1 / 9.5, 128 of two 15 / 15.
+        constexpr uint32_t groups = 256 / (D / 4);
+        uint32_t split = 1;
+        while (split < groups && parts > 4 * split) split *= 2;
+        across = R * split / groups;
+        most = 8;
+        while (most < 64 && (most < w.items || most * across < 4 * kJoinBlocks)) most *= 2;
+    }
     const dim3 grid(w.groups < most ? w.groups : most, across);
     hipLaunchKernelGGL((paged_attn_join_kernel<D, R, kTree>), grid, dim3(256), 0, st, p, w.groups);
     return hipGetLastError();
@@ -1452,7 +1468,7 @@ static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
     p.min_rows = a.both ? cut : 0;
     p.max_rows = 0xffffffffu;
     constexpr int NW = kChunkTile / 32;
-    constexpr size_t lds = 2 * 2 * 16 * NW * D * 2;
+    constexpr size_t lds = 2 * ChunkLds<D, 16 * NW>::tile;
     static size_t attr[kMaxDevices] = {};  // more than the default 64 KB of LDS
     const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW, kTree>, lds, attr);
     if (e != hipSuccess) return e;
