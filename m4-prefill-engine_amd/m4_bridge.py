@@ -795,7 +795,7 @@ class HIPBridge:
 
     def _lse(self, lse: Any, H: int, T: int, out: bool) -> tuple:
         """m4_rows_t's words for fp32 [H, T], any strides."""
-        if not isinstance(lse, _torch.Tensor) or lse.dtype is not _torch.float32 or tuple(lse.shape) != (H, T):
+        if not isinstance(lse, _torch.Tensor) or lse.dtype is not _torch.float32 or lse.shape != (H, T):
             raise ValueError(f"lse must be an fp32 tensor [{H}, {T}]")
         hs, ts = lse.stride()
         if out and T * H and ((T > 1 and ts == 0) or (H > 1 and hs == 0)):
@@ -850,7 +850,7 @@ class HIPBridge:
 
     def _sums(self, cache: PagedKVCache, sums: Any) -> tuple:
         shape = (cache.num_pages, cache.Hkv, cache.page_size)
-        if not isinstance(sums, _torch.Tensor) or sums.dtype is not _torch.float32 or tuple(sums.shape) != shape or not sums.is_contiguous():
+        if not isinstance(sums, _torch.Tensor) or sums.dtype is not _torch.float32 or sums.shape != shape or not sums.is_contiguous():
             raise ValueError(f"sums must be a contiguous fp32 tensor {list(shape)}")
         return sums.data_ptr(), sums.nbytes
 
@@ -895,7 +895,7 @@ class HIPBridge:
         given = kept  # one made here goes back to the stream that the kernels are on, behind them
         if kept is None:
             kept = _torch.empty(B, cache.Hkv, budget, dtype=_torch.int32, device=sums.device)
-        elif kept.dtype is not _torch.int32 or tuple(kept.shape) != (B, cache.Hkv, budget) or not kept.is_contiguous():
+        elif kept.dtype is not _torch.int32 or kept.shape != (B, cache.Hkv, budget) or not kept.is_contiguous():
             raise ValueError(f"kept must be a contiguous int32 tensor [{B}, {cache.Hkv}, {budget}]")
         if workspace is not None and not (isinstance(workspace, _torch.Tensor) and workspace.is_contiguous()):
             raise ValueError("workspace must be a contiguous tensor")
