@@ -408,7 +408,11 @@ static hipError_t launch_weigh(WeighParams p, hipStream_t st) {
     const uint64_t rows = (uint64_t)(p.max_new ? p.max_new : 1) * p.G;
     uint64_t keys = p.max_kv ? p.max_kv : 1;
     if (p.window && keys > (uint64_t)p.window + p.max_new) keys = (uint64_t)p.window + p.max_new;
-    const bool chunks = rows >= kWeighChunk, both = chunks && p.batch.T < (uint64_t)p.batch.B * p.max_new && p.batch.B > 1;
+    // Sequences of few rows among others are the rows kernel's, if there can be any: with as many rows as all
+    // but one could have, the last has the rest (three prompts of 809 .. 1739 tokens 41 us, with a launch of the
+    // other in vain 45).
+    const uint64_t others = (uint64_t)(p.batch.B - 1) * p.max_new, least = (kWeighChunk + p.G - 1) / p.G;
+    const bool chunks = rows >= kWeighChunk, both = chunks && p.batch.B > 1 && p.batch.T < others + least;
     p.min_rows = 0;
     p.max_rows = both ? kWeighChunk : 0xffffffffu;
     if (!chunks || both) {

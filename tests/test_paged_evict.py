@@ -16,7 +16,8 @@ from test_paged_tree import attend, host, i32, launched, lib, rows_of, set_, tok
 gpu = pytest.mark.gpu
 # what is expected of the lengths chooses the kernels; the results hold for any
 EXPECTED = {"rows": {"max_new": 1, "max_kv": 1}, "chunks": {"max_new": 10 ** 6, "max_kv": 400}, "both": {"max_new": 2 ** 20, "max_kv": 10 ** 4},
-            "wide": {"max_new": 10 ** 6, "max_kv": 2 * 10 ** 6}}
+            "wide": {"max_new": 10 ** 6, "max_kv": 2 * 10 ** 6},
+            "alone": {"max_new": 200, "max_kv": 500}, "wide alone": {"max_new": 200, "max_kv": 10 ** 6}}
 
 
 # ---- weights received -----------------------------------------------------------------------------------------------
@@ -113,6 +114,18 @@ def test_weigh(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels):
 ])
 def test_weigh_as_if_long(bridge, fmt, lens, new, H, Hkv, D, P, window):
     test_weigh(bridge, fmt, lens, new, H, Hkv, D, P, window, "wide")
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kernels", ["alone", "wide alone"])
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("lens,new,H,Hkv,D,P", [
+    ([700, 40, 90, 300], [600, 1, 3, 300], 8, 2, 64, 16),    # more rows than three could have, so the fourth is held to be long
+    ([900, 333, 0, 5], [700, 1, 0, 5], 5, 1, 128, 32),
+])
+def test_weigh_where_all_seem_long(bridge, fmt, kernels, window, lens, new, H, Hkv, D, P):
+    test_weigh(bridge, fmt, lens, new, H, Hkv, D, P, window, kernels)
 
 
 @gpu
