@@ -13,7 +13,7 @@
 // QR_PAGED_TREE, a build of its own: the same kernels (TREE) where a mask says which of the
 // new tokens a row sees, and with the logarithm of each row's sum.  Only tiles that hold new
 // tokens ask the mask.  H = 32, Hkv = 8, D = 128: trees of 64 nodes over 16 requests of 200 ..
-// 8192 keys (Q8_0) 70 us and the join 15, of 61 nodes over four of 131072 (Q4_0) 594, 0.88 PFLOP/s.
+// 8192 keys (Q8_0) 64 us and the join 14, of 61 nodes over four of 131072 (Q4_0) 594, 0.88 PFLOP/s.
 #include "qr_device.h"
 #include "qr_paged.h"
 #include "qr_paged_decode.h"
@@ -876,6 +876,9 @@ struct ChunkLds {
 // which the clock falls under this load.
 template <int FMT, int D, int NW, bool TREE>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
+    // a row tile's share beside its steps: with trees, whose last steps ask the mask, more (16 requests of
+    // 64 nodes with 1 / 2 / 3 / 4 / 5, join included: 92 / 84 / 78 / 78 / 78 us)
+    constexpr uint32_t COST = TREE ? 4 : kChunkCost;
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
     constexpr int DT = D / 32, KK = D / 16;
     using L = ChunkLds<D, KT>;
@@ -900,7 +903,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         uint64_t c = 0;
         int lo;
         const uint32_t tiles = ((uint32_t)s.n + tokens - 1) / tokens;
-        for (uint32_t rt = 0; rt < tiles; rt++) c += kChunkCost + steps_of<KT, TREE>(p, s, tokens, rt, lo);
+        for (uint32_t rt = 0; rt < tiles; rt++) c += COST + steps_of<KT, TREE>(p, s, tokens, rt, lo);
         return c;
     };
     const uint32_t per = (p.batch.B + 63) / 64;
@@ -972,15 +975,15 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         int lo;
         for (;; rt++) {  // the row tile at this place
             steps = __builtin_amdgcn_readfirstlane(steps_of<KT, TREE>(p, s, tokens, rt, lo));
-            if (in_row < kChunkCost + steps) break;
-            in_row -= kChunkCost + steps;
+            if (in_row < COST + steps) break;
+            in_row -= COST + steps;
         }
-        const uint32_t line = kChunkCost + steps, o0 = (uint32_t)in_row;
+        const uint32_t line = COST + steps, o0 = (uint32_t)in_row;
         const uint32_t o1 = (uint32_t)min((uint64_t)line, o0 + (s1 - cur));
         cur += o1 - o0;
         off += o1 - o0;
-        if (o1 <= kChunkCost) continue;
-        const int u0 = (int)(o0 > kChunkCost ? o0 - kChunkCost : 0), u1 = (int)(o1 - kChunkCost);
+        if (o1 <= COST) continue;
+        const int u0 = (int)(o0 > COST ? o0 - COST : 0), u1 = (int)(o1 - COST);
         const bool begun = u0 == 0, ends = u1 == (int)steps;
 
         // ---- rows ----
