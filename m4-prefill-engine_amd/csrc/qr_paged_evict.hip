@@ -771,9 +771,10 @@ __global__ void __launch_bounds__(kPickThreads, 8) evict_pick_kernel(EvictParams
 // request of 260 keys and 4 heads 6.8 / 5.4, 3840 items of up to 89 keys 53 / 6.0; with four fours 2400
 // of up to 900 39 / 14, but 512 of them 11.0 / 12.7 and 8 of them 7.6 / 8.3.
 constexpr uint32_t kShortKeys = 512, kShortItems = 1024;
-// HELD: all keys are in registers; else (sequences longer than expected) they are formed again for each count.
+// HELD: all keys are in registers; else (sequences longer than expected) they are formed again, and the
+// value is found eight bits at a time by counts in LDS.
 template <uint32_t FOURS, bool HELD>
-__device__ __forceinline__ void pick_short(const EvictParams& p, const PickSeq& s, uint32_t lane) {
+__device__ __forceinline__ void pick_short(const EvictParams& p, const PickSeq& s, uint32_t lane, uint32_t (&bins)[256]) {
     u4_t held[FOURS];
     if constexpr (HELD)
 #pragma unroll
@@ -797,7 +798,40 @@ __device__ __forceinline__ void pick_short(const EvictParams& p, const PickSeq& 
     };
     const uint32_t there = reach(1);
     uint32_t least = 0, equal = 0;
-    if (there > p.budget) {
+    if (!HELD && there > p.budget) {
+        equal = p.budget;
+#pragma unroll 1
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            *reinterpret_cast<u4_t*>(&bins[4 * lane]) = u4_t{};
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            each([&](uint32_t, u4_t k) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (shift == 24 || k[e] >> (shift + 8 & 31) == least) atomicAdd(&bins[k[e] >> shift & 255], 1u);
+            });
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            const u4_t c = *reinterpret_cast<const u4_t*>(&bins[4 * lane]);
+            const uint32_t mine = c.x + c.y + c.z + c.w;
+            uint32_t above = mine;
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) {
+                const uint32_t y = (uint32_t)__shfl_down((int)above, x);
+                if (lane + x < 64) above += y;
+            }
+            above -= mine;
+            // one lane has it among its four
+            uint32_t digit = 4 * lane + 3, left = equal - above;
+#pragma unroll
+            for (int e = 3; e > 0; e--)
+                if (digit == 4 * lane + e && left > c[e]) {
+                    left -= c[e];
+                    digit--;
+                }
+            const int at = __ffsll((unsigned long long)__ballot(above < equal && equal <= above + mine)) - 1;
+            least = least << 8 | (uint32_t)__builtin_amdgcn_readlane((int)digit, max(at, 0));
+            equal = (uint32_t)__builtin_amdgcn_readlane((int)left, max(at, 0));
+        }
+    } else if (there > p.budget) {
         bool exact = false;  // as many reach it as are wanted: no need to know it better
 #pragma unroll 1
         for (uint32_t bit = 0x80000000u; bit && !exact; bit >>= 1) {
@@ -840,12 +874,13 @@ __device__ __forceinline__ void pick_short(const EvictParams& p, const PickSeq& 
 
 template <uint32_t FOURS>
 __global__ void __launch_bounds__(256) evict_pick_short_kernel(EvictParams p) {
+    __shared__ __attribute__((aligned(16))) uint32_t bins[4][256];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
     for (uint64_t item = (uint64_t)blockIdx.x * 4 + wave; item < items; item += (uint64_t)gridDim.x * 4) {
         const PickSeq s(p, item);
-        if (s.n <= 256 * FOURS) pick_short<FOURS, true>(p, s, lane);
-        else pick_short<FOURS, false>(p, s, lane);
+        if (s.n <= 256 * FOURS) pick_short<FOURS, true>(p, s, lane, bins[wave]);
+        else pick_short<FOURS, false>(p, s, lane, bins[wave]);
     }
 }
 
