@@ -44,7 +44,9 @@ struct Range {
 };
 __device__ __forceinline__ Range tokens_of(const WeighParams& p, const WeighSeq& s, int key) {
     const int i = key - s.first;  // keys past the last token's are not asked for but for a tile's width
-    return Range{min(max(i, 0), s.n), p.window ? min(max(i + (int)p.window, 0), s.n) : s.n};
+    // i + window tokens, as far as there are as many: windows reach 2^31 - 1, so it is not formed where it is more
+    const int w = (int)p.window;
+    return Range{min(max(i, 0), s.n), p.window && i < s.n - w ? max(i + w, 0) : s.n};
 }
 
 // Few rows: a wave takes 64 keys of a KV head at a time, 16 rows at a time.  All work is one line

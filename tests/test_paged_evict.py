@@ -233,6 +233,32 @@ def test_rows_without_a_sum_weigh_nothing(bridge, kernels, window):
 
 
 @gpu
+@pytest.mark.parametrize("kernels", ["rows", "chunks", "both", "wide", "wide alone"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 60, 2 ** 31, 2 ** 32 - 1])
+def test_weigh_with_the_widest_windows(bridge, kernels, window):
+    """Windows that reach past every key, with which tokens behind the first still see what is before them; and a length
+    whose positions are as far as the window."""
+    import torch
+
+    lens, new, H, Hkv, D, P = [64, 200, 80, 160], [64, 70, 1, 130], 8, 2, 64, 16
+    s = Setup(Q8_0, lens, new, Hkv, D, P, seed=7)
+    q = half(s.rng, H, s.T, D)
+    lse = s.rng.standard_normal((H, s.T)).astype(np.float32) + 4
+    sums = s.rng.random((s.num_pages, Hkv, P)).astype(np.float32)
+    for far in (False, True):
+        length = i32(64, 200, 2 ** 31 - 1 if far else 80, 160)  # keys past the table are not there
+        batch = m4_bridge.KVBatch(dev(s.q_start), dev(length), dev(s.table), **EXPECTED[kernels])
+        got, without = dev(sums), dev(sums)
+        say("weigh with a window of", window, kernels, far)
+        bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(lse), got, 0.125, window=window)
+        bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(lse), without, 0.125)
+        bridge.synchronize()
+        close(got.cpu().numpy(), *weighed(s, sums, q, lse, length, s.q_start, window, 0.125), "sums")
+        if not far or window >= 2 ** 31 - 1:
+            assert torch.equal(got, without)  # the same terms in the same order
+
+
+@gpu
 def test_pages_past_4_gib(bridge):
     """The same bits from pages that lie past 4 GiB of a cache as from its first ones."""
     import torch
