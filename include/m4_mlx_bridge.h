@@ -423,7 +423,7 @@ M4_API int m4_bridge_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch
  * of the H / Hkv query heads of its KV head that see it, as m4_bridge_dispatch_paged_attn
  * does with the same window; for the batch's new tokens it sets them, whatever
  * they held.  lse as that call's tree form writes it (append, attend, then weigh; a
- * row whose lse is -infinity gives nothing).
+ * row whose lse is infinite gives nothing, whatever its Q holds).
  * Products are of fp16 operands, the cached values, summed in fp32; no order changes.
  * A page that two sequences of a call share: its sums are undefined.  A call without
  * rows writes nothing.  B x Hkv, and T x H / Hkv, below 2^31. */

@@ -57,6 +57,7 @@ __device__ __forceinline__ Range tokens_of(const WeighParams& p, const WeighSeq&
 // 64 requests of up to 8192 keys, 8 KV heads of 128, 8 bit: 20 us (59 MB: 3.0 TB/s); a workgroup
 // for each 256 keys of a head, which a quarter of them found empty: 34.
 constexpr uint32_t kRowWaves = 2048;  // a power of two: two a SIMD
+constexpr float kNoRow = 1e38f;  // lse of a row that is not there: its weights are 0, as those of an infinite one
 template <int FMT, int D>
 __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
     constexpr int KK = D / 32, RUN = D / 4, W = FMT == QUANT_Q8_0 ? D / 16 : D / 32;
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t f = r0 + 4 * g + e;
-                l[e] = INFINITY;  // no such row
+                l[e] = kNoRow;
                 if (f < rows) l[e] = p.lse.p[row_offset(p, p.lse, s.q0, hk, f)];
             }
         };
@@ -180,10 +181,18 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
                 float less[4];  // a row that sees nothing gives nothing (asked here: the products do not wait for lse)
 #pragma unroll
                 for (int e = 0; e < 4; e++) less[e] = l[e] == -INFINITY ? -INFINITY : l[e] * -1.4426950408889634f;
+                // its products may be NaN or infinite, and so may those of what is no row, which is the last one again
+                const bool without = __any(fminf(fminf(less[0], less[1]), fminf(less[2], less[3])) == -INFINITY);
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) sc[t][e] = __builtin_fmaf(sc[t][e], c, less[e]);
+                if (without)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (less[e] <= -kNoRow) sc[t][e] = -INFINITY;
                 if (!whole)
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
@@ -222,9 +231,10 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 // beside the exponentials of the one before.  8 heads, 2048 rows of 32 query heads on 30000 keys of
 // 128: 535 us, 0.91 PFLOP/s.  By itself that loop takes 350 cycles a tile of 32 x 32 (256 of products,
 // 256 of fused multiplies, exponentials and sums, at 1.65 GHz under this load), 390 us; bringing
-// the rows (3.8 GB through the L2s) costs 100 more.
+// the rows (3.8 GB through the L2s) costs 100 more.  Eight waves of D = 64 are held to the 128
+// registers with which two workgroups fit a CU.
 template <int FMT, int D, int NT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams p) {
+__global__ void __launch_bounds__(64 * WAVES, D == 64 && NT == 2 ? 4 : 2) weigh_chunk_kernel(WeighParams p) {
     constexpr int KK = D / 16, W = FMT == QUANT_Q8_0 ? 2 : 1;  // words of an octet of codes
     constexpr uint32_t CB = 2 * KK * W * 4, NB = D / 32;
     constexpr int KT = 32 * NT;
@@ -232,7 +242,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams 
     extern __shared__ __attribute__((aligned(16))) uint8_t qs[];             // a wave's 32 rows
     __shared__ __attribute__((aligned(16))) float l2[WAVES][32];
     __shared__ float lse[WAVES][64];  // as it is, twice
-    __shared__ __attribute__((aligned(16))) int rel_of[32];
+    __shared__ __attribute__((aligned(16))) int at_of[WAVES][32];  // tokens from the first of the 32 rows on, far for one that gives nothing
+    __shared__ int rel_of[32];
     // what each lane loads of 32 rows, and where a row's lse is, from their first row on (bytes)
     __shared__ int64_t q_off[LOADS * 64], l_off[32];
     __shared__ float part[WAVES][KT];
@@ -329,7 +340,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams 
                 // a row that sees nothing gives nothing, nor one that is not there or not of this turn
                 const bool live = rel < min(tokens, s.n - i) && from_head(sub) + head >= 32 * sub;
                 const float mine = lse[wave][lane];
-                if (g == 0) l2[wave][j] = mine == -INFINITY || !live ? INFINITY : mine * 1.4426950408889634f;
+                const bool without = fabsf(mine) == INFINITY;
+                if (g == 0) {
+                    l2[wave][j] = without || !live ? INFINITY : mine * 1.4426950408889634f;
+                    at_of[wave][j] = without || !live ? 0x40000000 : rel;
+                }
                 h8_t qf[KK];
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) qf[kk] = *reinterpret_cast<const h8_t*>(block + (q_at ^ 32u * kk));
@@ -338,8 +353,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams 
                 for (int y = 0; y < 4; y++) *reinterpret_cast<f4_t*>(l + 4 * y) = *reinterpret_cast<const f4_t*>(&l2[wave][8 * y + 4 * g]);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and are read: the next ones may take their place
                 if (sub_next < subs) bring(i_next, sub_next);
-                if (i >= last_key.lo && min(i + tokens, s.n) <= first_key.hi) {
-                    // all see all: a tile's scores while those before them are weighed
+                if (i >= last_key.lo && min(i + tokens, s.n) <= first_key.hi && !__any(without)) {
+                    // all see all: a tile's scores while those before them are weighed (a row of an infinite lse
+                    // may hold anything, so it is left out by choice: infinity less infinity would be NaN)
                     f16v_t sc[2];
 #pragma unroll
                     for (int t = 0; t <= NT; t++) {
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) weigh_chunk_kernel(WeighParams 
                         const Range see = tokens_of(p, s, key);
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            const int at = i + rel_of[8 * (e >> 2) + 4 * g + (e & 3)];
+                            const int at = i + at_of[wave][8 * (e >> 2) + 4 * g + (e & 3)];
                             const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -l[e]));
                             sum[t] += at >= see.lo && at < see.hi ? w : 0.0f;
                         }

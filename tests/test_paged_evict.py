@@ -259,6 +259,45 @@ def test_weigh_with_the_widest_windows(bridge, kernels, window):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kernels", ["rows", "chunks", "wide"])
+@pytest.mark.parametrize("H", [8, 10, 66])
+@pytest.mark.parametrize("window", [0, 25])
+def test_rows_without_a_sum_weigh_nothing_whatever_they_hold(bridge, fmt, kernels, H, window):
+    """Rows of a padded batch that nothing but their lse marks: NaN and infinities in them reach no key; nor do keys that
+    are infinite (65504 in Q8_0) where no other row sees them."""
+    import torch
+
+    lens, new, Hkv, D, P = [200, 60, 300, 90, 33], [70, 60, 5, 1, 33], 2, 64, 16
+    s = Setup(fmt, lens, new, Hkv, D, P, seed=32)
+    k, v = half(s.rng, 2, 64), half(s.rng, 2, 64)
+    k[:, 3] = 65504
+    (kq, kd), (vq, vd) = ref.quantize(fmt, k), ref.quantize(fmt, v)
+    for p in (0, 17, 32):  # of the last sequence, none of whose rows has a sum
+        s.pages.write(s.table[4, p // P], p % P, kq, kd, vq, vd)
+    q = half(s.rng, H, s.T, D)
+    sums = s.rng.random((s.num_pages, Hkv, P)).astype(np.float32)
+    lse = s.rng.standard_normal((H, s.T)).astype(np.float32) + 4
+    none = s.rng.random((H, s.T)) < 0.3
+    none[:, 69:75] = True       # the last row of a sequence and the first of the next
+    none[:, s.q_start[3]:] = True
+    lse[none] = -np.inf
+    odd = q.copy()
+    odd[none] = np.array([np.nan, np.inf, -np.inf, 65504], np.float16)[s.rng.integers(0, 4, (int(none.sum()), D))]
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), dev(s.table), **EXPECTED[kernels])
+    got, clean = dev(sums), dev(sums)
+    say("weigh rows without a sum that hold anything", fmt, kernels, H, window)
+    bridge.kv_cache_weigh(s.cache(), batch, dev(odd), dev(lse), got, 0.1, window=window)
+    q[none] = 0
+    bridge.kv_cache_weigh(s.cache(), batch, dev(q), dev(lse), clean, 0.1, window=window)
+    bridge.synchronize()
+    assert torch.equal(got, clean)
+    s.k[4] = np.zeros_like(s.k[4])
+    want, bound = weighed(s, sums, q, np.where(none, np.float32(1e5), lse), lens, s.q_start, window, 0.1)
+    close(got.cpu().numpy(), want, bound, "sums")
+
+
+@gpu
 def test_pages_past_4_gib(bridge):
     """The same bits from pages that lie past 4 GiB of a cache as from its first ones."""
     import torch
