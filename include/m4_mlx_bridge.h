@@ -402,7 +402,8 @@ M4_API int m4_bridge_dispatch_paged_attn_tree(const m4_kv_cache_t* cache, const 
  * whose token is the model's choice behind it.  parents, tokens, targets int32
  * [T], targets[i] the model's choice behind row i.  path int32 [T]: a sequence's
  * rows hold its nodes in order, then -1; count int32 [B]; next int32 [B]: the
- * choice behind the last of them.  A sequence without rows: 0 and -1. */
+ * choice behind the last of them.  A sequence without rows: 0 and -1; so all of them
+ * where T is 0, whose other pointers, and those of the two that are not wanted, may be NULL. */
 M4_API int m4_bridge_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,
                                  const int32_t* targets, int32_t* path, int32_t* count, int32_t* next);
 
@@ -412,7 +413,8 @@ M4_API int m4_bridge_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const i
  * sequence has kv_len_out[b] keys: those before the tree and count[b] (int32 [B],
  * may be the batch's kv_len, may be NULL).  Entries that are no nodes, and places
  * that are not there, move nothing; a list that does not rise leaves the
- * sequence's new tokens undefined.  Once a layer. */
+ * sequence's new tokens undefined.  Once a layer.  T = 0 needs nothing but the cache's
+ * description and, for kv_len_out, the batch's kv_len, which it gets. */
 M4_API int m4_bridge_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T, const int32_t* keep,
                                    const int32_t* count, int32_t* kv_len_out);
 

@@ -1085,7 +1085,8 @@ int m4_bridge_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t*
     if (rc || empty) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
-    if (!dev.owns_all(batch->q_start, batch->kv_len, parents, tokens, targets, path, count, next)) return -2;
+    if (T && !dev.owns_all(batch->q_start, batch->kv_len, parents, tokens, targets, path, count, next)) return -2;
+    if (T == 0 && ((count && !dev.owns_all(count)) || (next && !dev.owns_all(next)))) return -2;
     const qr::AcceptParams p{batch_view(batch, T), parents, tokens, targets, path, count, next};
     return launched(qr::launch_tree_accept(p, g_stream), "tree_accept");
 }
@@ -1104,8 +1105,8 @@ int m4_bridge_kv_cache_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* bat
     if (rc || empty) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
     const OnStreamDevice dev;
-    if (!dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, keep, count)) return -2;
-    if (kv_len_out && !dev.owns_all(kv_len_out)) return -2;
+    if (T && !dev.owns_all(cache->pages, batch->q_start, batch->kv_len, batch->page_table, keep, count)) return -2;
+    if (kv_len_out && !dev.owns_all(batch->kv_len, kv_len_out)) return -2;
     const qr::KeepParams p{cache->D, cache->format, cache_geom(cache), batch_view(batch, T), keep, count, kv_len_out};
     return launched(qr::launch_kv_keep(p, g_stream), "kv_cache_keep");
 }

@@ -320,7 +320,11 @@ int validate_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* 
                          const int32_t* targets, const int32_t* path, const int32_t* count, const int32_t* next, bool* empty) {
     *empty = false;
     if (int rc = check_rows_of(batch, T, empty)) return rc;
-    if (*empty) return 0;
+    if (batch->B == 0) return 0;
+    if (T == 0) {  // what the sequences get, where it is wanted
+        *empty = !count && !next;
+        return misaligned(count, 4) || misaligned(next, 4) ? -2 : 0;
+    }
     return all_words(parents, tokens, targets, path, count, next) ? 0 : -2;
 }
 
@@ -329,7 +333,11 @@ int validate_keep(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32
     *empty = false;
     if (int rc = check_cache(cache)) return rc;
     if (int rc = check_batch(cache, batch, T, empty)) return rc;
-    if (*empty) return 0;
+    if (batch->B == 0) return 0;
+    if (T == 0) {  // the lengths, where they are wanted
+        *empty = !kv_len_out;
+        return *empty || all_words(kv_len_out, batch->kv_len) ? 0 : -2;
+    }
     return all_words(keep, count) && !misaligned(kv_len_out, 4) ? 0 : -2;
 }
 

@@ -104,13 +104,16 @@ hipError_t launch_draft_tree(const DraftParams& p, hipStream_t st) {
     return hipGetLastError();
 }
 
+// A call without rows has results for its sequences all the same, and needs nothing else: q_start may be null then.
+__device__ __forceinline__ NewRows rows_if_any(const BatchView& v, uint32_t b) { return v.T ? new_rows(v, b) : NewRows{0, 0, 0}; }
+
 // From node 0 on, the first node behind the present one that is its child and whose token is
 // the model's choice there.  A wave a sequence, 64 nodes at a time: a child of the present node is
 // one ballot, so what it takes is the loads (26 nodes 1.7 us, 64 requests of 64 nodes 3.8).
 __global__ void __launch_bounds__(64) tree_accept_kernel(AcceptParams p) {
     const int lane = threadIdx.x;
     for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
-        const NewRows s = new_rows(p.batch, b);
+        const NewRows s = rows_if_any(p.batch, b);
         const int32_t *parents = p.parents + s.q0, *tokens = p.tokens + s.q0, *targets = p.targets + s.q0;
         int count = 0, next = -1;
         if (s.n > 0) {
@@ -141,15 +144,15 @@ __global__ void __launch_bounds__(64) tree_accept_kernel(AcceptParams p) {
             }
         }
         for (int i = count + lane; i < s.n; i += 64) p.path[s.q0 + i] = -1;
-        if (lane == 0) {
-            p.count[b] = count;
-            p.next[b] = next;
+        if (lane == 0) {  // null in a call without rows alone
+            if (p.count) p.count[b] = count;
+            if (p.next) p.next[b] = next;
         }
     }
 }
 
 hipError_t launch_tree_accept(const AcceptParams& p, hipStream_t st) {
-    if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
+    if (p.batch.B == 0) return hipSuccess;
     hipLaunchKernelGGL(tree_accept_kernel, dim3(min(p.batch.B, 1u << 20)), dim3(64), 0, st, p);
     return hipGetLastError();
 }
@@ -168,8 +171,8 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(KeepParams p) {
     __shared__ uint32_t src_page[kKeepList], src_slot[kKeepList], dst_page[kKeepList], dst_slot[kKeepList];
     const uint32_t piece = threadIdx.x % PIECES, pair = threadIdx.x / PIECES;
     for (uint32_t b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
-        const NewRows s = new_rows(p.batch, b);
-        const int len = max(p.batch.kv_len[b], 0), count = min(max(p.count[b], 0), s.n);
+        const NewRows s = rows_if_any(p.batch, b);
+        const int len = max(p.batch.kv_len[b], 0), count = s.n ? min(max(p.count[b], 0), s.n) : 0;
         __syncthreads();  // the length is read
         if (threadIdx.x == 0 && p.len_out) p.len_out[b] = s.n ? max(s.first + count, 0) : len;
         for (int base = 0; base < count; base += kKeepList) {
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(KeepParams p) {
 }
 
 hipError_t launch_kv_keep(const KeepParams& p, hipStream_t st) {
-    if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
+    if (p.batch.B == 0) return hipSuccess;
     const dim3 grid(min(p.batch.B, 1u << 20)), block(kKeepThreads);
     if (p.format == QUANT_Q8_0) {
         if (p.D == 64) hipLaunchKernelGGL((kv_keep_kernel<QUANT_Q8_0, 64>), grid, block, 0, st, p);

@@ -381,6 +381,44 @@ def test_tree_accept(bridge, sizes, back, vocabulary):
     np.testing.assert_array_equal(path.cpu().numpy(), want)
 
 
+@gpu
+def test_calls_without_rows_say_so(bridge):
+    """T = 0: every sequence is one without rows, for each of which the header says what it gets."""
+    import torch
+
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    s = Setup(Q8_0, [40, 0, 60], [0, 0, 0], 2, 64, 16, seed=4)
+    lens = dev(i32(40, 0, -3))
+    batch = m4_bridge.KVBatch(dev(i32(0, 5, 9, 12)), lens, dev(s.table), 1, 1)
+    count, nxt, out = z(3) + 9, z(3) + 9, z(3) + 9
+    cache = s.cache()
+    bridge.tree_accept(batch, z(0), z(0), z(0), z(0), count, nxt)
+    bridge.kv_cache_keep(cache, batch, z(0), count, out)
+    bridge.synchronize()
+    assert count.tolist() == [0] * 3 and nxt.tolist() == [-1] * 3 and out.tolist() == [40, 0, 0]
+    bridge.kv_cache_keep(cache, batch, z(0), count, batch.kv_len)
+    bridge.kv_cache_keep(cache, batch, z(0), count)
+    bridge.synchronize()
+    assert batch.kv_len.tolist() == [40, 0, 0]
+    np.testing.assert_array_equal(cache.pages.cpu().numpy(), s.pages.raw)
+
+
+def test_refused_without_rows(lib):
+    """T = 0 needs nothing of the rows, and takes what it is given to write for the sequences."""
+    a, r = Args(), ctypes.addressof
+    accept = lambda *p: lib.m4_bridge_validate_tree_accept(r(a.batch), 0, None, None, None, None, *p)  # noqa: E731
+    assert accept(0x700000, 0x710000) == 0 and accept(None, None) == 0 and accept(0x700000, None) == 0
+    assert accept(0x700001, 0x710000) == -2 and accept(0x700000, 0x710002) == -2
+    keep = lambda *p: lib.m4_bridge_validate_kv_cache_keep(r(a.cache), r(a.batch), 0, *p)  # noqa: E731
+    assert keep(None, None, None) == 0 and keep(None, None, 0x700000) == 0 and keep(None, None, 0x700002) == -2
+    a.batch.kv_len = 0
+    assert keep(None, None, None) == 0 and keep(None, None, 0x700000) == -2 and accept(0x700000, 0x710000) == 0
+    a.batch.kv_len = 0x2001
+    assert keep(None, None, 0x700000) == -2
+    a.batch.B = 0
+    assert keep(None, None, 0x700000) == 0 and accept(0x700001, None) == 0
+
+
 def token_bytes(pages, slot):
     """Where a token's bytes lie in a head's share of a page."""
     ak, av, aks, avs = pages._places(slot)
