@@ -1148,9 +1148,10 @@ int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batch_t* ba
 
 size_t m4_bridge_kv_evict_workspace(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch) {
     if (!cache || !batch) return 0;
+    if (qr::kv_cache_bytes(cache->format, cache->num_pages, cache->page_size, cache->Hkv, cache->D) == 0) return 0;
     qr::EvictParams p{};
-    p.geom.Hkv = cache->Hkv;
-    p.batch.B = batch->B;
+    p.geom = cache_geom(cache);
+    p.batch = batch_view(batch, 0);
     p.max_kv = batch->max_kv;
     return qr::kv_evict_workspace(p);
 }

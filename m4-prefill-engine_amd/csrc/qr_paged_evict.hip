@@ -1124,12 +1124,13 @@ static hipError_t launch_copy(const EvictParams& p, hipStream_t st) {
 }
 
 // Workgroups for a sequence and KV head: several where there are fewer of these than CUs and the
-// longest is expected to have places for them.
+// longest is expected to have places for them.  No more than its row of the table has, whatever is
+// expected: 4 KB of workspace each.
 static uint32_t pick_segments(const EvictParams& p) {
     const uint64_t items = (uint64_t)p.batch.B * p.geom.Hkv;
     if (items >= 256 || p.max_kv <= 2 * kSegment) return 1;
-    const uint32_t most = p.max_kv < 0x7fff0000u ? p.max_kv : 0x7fff0000u;
-    return (most + kSegment - 1) / kSegment;
+    const uint64_t held = std::max((uint64_t)p.batch.table_pages << p.geom.log2_page, (uint64_t)2 * kSegment + 1);
+    return (uint32_t)((std::min((uint64_t)p.max_kv, held) + kSegment - 1) / kSegment);
 }
 
 size_t kv_evict_workspace(const EvictParams& p) {

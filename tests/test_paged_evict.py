@@ -672,6 +672,26 @@ def test_refused_evictions(lib, change, code):  # noqa: F811
         assert call(0x900000, need) == 0 and call(0x900000, need - 1) == -2 and call(None, need) == -2 and call(0x900008, need) == -2
 
 
+@pytest.mark.parametrize("B,Hkv", [(1, 1), (2, 4), (31, 8)])
+def test_workspace_of_evictions_goes_by_the_table(lib, B, Hkv):  # noqa: F811
+    """Expectations may be any number: the workspace is for as many keys as the table holds, however many are expected."""
+    a, r = Args(), ctypes.addressof
+    a.batch.B, a.cache.Hkv, a.cache.page_size = B, Hkv, 256
+
+    def need(pages, max_kv):
+        a.batch.table_pages = a.batch.table_stride = pages
+        a.batch.max_kv = max_kv
+        return lib.m4_bridge_kv_evict_workspace(r(a.cache), r(a.batch))
+
+    for pages in (157, 1024, 0x7fff00):  # 40192 keys, 2^18, all that positions reach
+        keys = pages * 256
+        for max_kv in (keys + 1, max(keys, 10 ** 9), 2 ** 32 - 1):
+            assert need(pages, max_kv) == need(pages, keys) > 0
+        assert need(pages, 16384) == 0 and need(pages, 16385) <= need(pages, keys)
+    for max_kv in (16385, 10 ** 6, 10 ** 9, 2 ** 32 - 1):  # a table for fewer keys than are worth several workgroups
+        assert need(4, max_kv) <= need(0x7fff00, 16385)
+
+
 def test_what_a_call_holds_and_refuses(launched):  # noqa: F811
     import torch
 
