@@ -522,6 +522,30 @@ def test_evict_out_of_range(bridge, fmt):
     np.testing.assert_array_equal(sums.cpu().numpy().view(np.uint32), want.view(np.uint32))
 
 
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,budget,P,max_kv", [
+    ([300, 1, 2, 3, 5, 66, 0, 203], 63, 16, 300), ([300, 127, 129, 130, 131, 90], 130, 16, 5000), ([700, 6, 257], 257, 256, 700),
+    ([400, 21], 3, 32, 2 ** 31)])
+def test_evict_leaves_what_lies_behind(bridge, fmt, D, lens, budget, P, max_kv):
+    """Every byte, those of a last group of four that is not full among them; any length may be expected."""
+    import torch
+
+    s = Bounded(fmt, lens, [0] * len(lens), 2, D, P, seed=budget + D)
+    s.grow(budget)
+    cache, sums = s.cache(), dev(s.sums)
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), dev(s.table), 0, max_kv)
+    length = torch.empty(len(lens), dtype=torch.int32, device="cuda")
+    say("what lies behind", fmt, D, lens, budget, P, max_kv)
+    bridge.kv_cache_evict(cache, batch, sums, dev(s.table_out), length, budget, sinks=1, recent=2)
+    bridge.synchronize()
+    pages, out, _, n = evicted(s, s.pages.raw, s.sums, lens, s.table, s.table_out, budget, 1, 2)
+    np.testing.assert_array_equal(length.cpu().numpy(), n)
+    np.testing.assert_array_equal(cache.pages.cpu().numpy(), pages)
+    np.testing.assert_array_equal(sums.cpu().numpy().view(np.uint32), out.view(np.uint32))
+
+
 # ---- steps as they are used -----------------------------------------------------------------------------------------
 
 class Steps:
