@@ -389,9 +389,10 @@ M4_API int m4_bridge_draft_tree(const m4_kv_batch_t* batch, uint32_t T, const in
  * (positions below the first new token's, or past the last one's, count as these;
  * without a window they may be NULL).  tree NULL: as there, up to itself.
  * lse (may be NULL): fp32 [T][H] by strides of any size, the natural logarithm of
- * the sum of exp(scale q . k) over the keys that a row sees, -infinity if none.
- * The softmax's sum is of unrounded weights here, so the results' last bits differ
- * from the other call's: 2^-11 of a result at most where few keys count. */
+ * the sum of exp(scale q . k) over the keys that a row sees, -infinity if none, of
+ * unrounded weights.  O is divided by the sum of the rounded ones as in the other
+ * call, and differs from its results by their rounding at most; with neither tree nor lse
+ * it is that call. */
 M4_API int m4_bridge_dispatch_paged_attn_tree(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, uint32_t T,
                                               const m4_rows_t* Q, const m4_rows_t* O, uint32_t H, float scale,
                                               uint32_t window, const m4_draft_tree_t* tree, const m4_rows_t* lse, void* ws,

@@ -1068,7 +1068,8 @@ int m4_bridge_dispatch_paged_attn_tree(const m4_kv_cache_t* cache, const m4_kv_b
     p.ws = static_cast<uint8_t*>(ws);
     if (tree) p.tree = {tree->mask, tree->words, tree->positions};
     if (lse) p.lse = values_view(lse);
-    return launched(qr::launch_paged_attn_tree(p, g_stream), "paged_attn_tree");
+    const auto launch = tree ? qr::launch_paged_attn_tree : lse ? qr::launch_paged_attn_lse : qr::launch_paged_attn;
+    return launched(launch(p, g_stream), "paged_attn_tree");
 }
 
 int m4_bridge_validate_tree_accept(const m4_kv_batch_t* batch, uint32_t T, const int32_t* parents, const int32_t* tokens,

@@ -96,7 +96,7 @@ struct ValuesView {
 // What each new token sees of its sequence's new tokens: bit j of its words of the
 // mask [T][words] for the j-th of them; places [T]: their positions (for a window).
 struct TreeView {
-    const uint32_t* mask;  // null: those up to itself
+    const uint32_t* mask;
     uint32_t words;
     const int32_t* places;
 };
@@ -113,13 +113,13 @@ struct PagedAttnParams {
     // a launch's: sequences of that many rows a KV head, [min_rows, max_rows)
     uint32_t min_rows, max_rows;
     uint8_t* ws;
-    // launch_paged_attn_tree only
-    TreeView tree;
-    ValuesView lse;  // p null: not wanted
+    TreeView tree;   // launch_paged_attn_tree only
+    ValuesView lse;  // and launch_paged_attn_lse; p null: not wanted
 };
 size_t paged_attn_workspace(const PagedAttnParams& p);
 hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st);
-// the same with a tree's mask, and the logarithm of each row's sum of exponentials
+// the same with the logarithm of each row's sum of exponentials, and with a tree's mask (lse or none)
+hipError_t launch_paged_attn_lse(const PagedAttnParams& p, hipStream_t st);
 hipError_t launch_paged_attn_tree(const PagedAttnParams& p, hipStream_t st);
 
 

@@ -10,10 +10,11 @@
 // 8 g + 4 t + r of V^T the same key.  The contraction runs over dims in the order
 // in which lane group g owns dims D/4 g .. of a key, one run of bytes of the page.
 //
-// QR_PAGED_TREE, a build of its own: the same kernels (TREE) where a mask says which of the
-// new tokens a row sees, and with the logarithm of each row's sum.  Only tiles that hold new
-// tokens ask the mask.  H = 32, Hkv = 8, D = 128: trees of 64 nodes over 16 requests of 200 ..
-// 8192 keys (Q8_0) 64 us and the join 14, of 61 nodes over four of 131072 (Q4_0) 594, 0.88 PFLOP/s.
+// QR_PAGED_TREE, builds of their own: the same kernels with the logarithm of each row's sum (2: LSE), and
+// where a mask says which of the new tokens a row sees (1: TREE, with LSE and without).  Only
+// tiles that hold new tokens ask the mask.  H = 32, Hkv = 8, D = 128: trees of 64 nodes over 16 requests of 200 ..
+// 8192 keys (Q8_0) 65 us and the join 14 with lse, of 61 nodes over four of 131072 (Q4_0) 635, 0.83
+// PFLOP/s, without lse 609.
 #include "qr_device.h"
 #include "qr_paged.h"
 #include "qr_paged_decode.h"
@@ -204,7 +205,9 @@ __host__ __device__ constexpr size_t slot_bytes() {
     return (size_t)R * (D + 2) * 4;
 }
 // workspace: a note per workgroup, then two slots per workgroup of partial rows
-// (O [R][D], reference points [R], sums [R], fp32)
+// (O [R][D], reference points [R], sums [R], fp32).  TREE and LSE: rows divided by their sums,
+// the logarithms of these [R] and of the sums of unrounded weights [R], to base 2, in
+// place of reference points and sums, so that the same slot holds both.
 template <int D, int R>
 __device__ __forceinline__ float* slot_of(uint8_t* ws, uint32_t groups, uint32_t w, int which) {
     return reinterpret_cast<float*>(ws + (size_t)groups * sizeof(ItemNote) + ((size_t)w * 2 + which) * slot_bytes<D, R>());
@@ -274,12 +277,13 @@ __device__ __forceinline__ uint32_t quad_of(const PagedAttnParams& p, const Seq&
         }
     return bits;
 }
-// Natural logarithm of a row's sum, from its reference point and its sum beside it.
-__device__ __forceinline__ float lse_of(float m, float l) {
-    return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-}
-__device__ __forceinline__ void put_lse(const PagedAttnParams& p, int row, uint32_t head, float m, float l) {
-    if (p.lse.p) p.lse.p[(int64_t)row * p.lse.ts + (int64_t)head * p.lse.hs] = lse_of(m, l);
+// LSE: a row has two sums.  O is divided by that of the weights as they are in the product, rounded to
+// fp16, as without; the logarithm is of the unrounded ones, since it is fp32.  (The second takes 16
+// additions every 32 keys: four requests of 131072 keys and 61 nodes 609 us without lse, 638 with.)
+// To base 2, from a reference point and the sum beside it:
+__device__ __forceinline__ float log2_of(float m, float l) { return l == 0.0f ? kNone : m + __builtin_amdgcn_logf(l); }
+__device__ __forceinline__ void put_lse(const PagedAttnParams& p, int row, uint32_t head, float z) {
+    p.lse.p[(int64_t)row * p.lse.ts + (int64_t)head * p.lse.hs] = z == kNone ? -INFINITY : z * 0.6931471805599453f;
 }
 
 // The work is one line: of every sequence, KV head and row tile (an item)
@@ -296,7 +300,7 @@ __device__ __forceinline__ void put_lse(const PagedAttnParams& p, int row, uint3
 // keys (Q8_0, 110 MB) 31 us, 24 of them this kernel; one of 1000 keys 12 us, a chain
 // of descriptor, page table, key and join latencies; drafted tokens and short
 // chunks (two row blocks) by turning codes into fp16 on one wave per SIMD.
-template <int FMT, int D, int NR, bool TREE>
+template <int FMT, int D, int NR, bool TREE, bool LSE>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr uint32_t R = 16 * NR;
     constexpr int DT = D / 16, KK = D / 32;
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
     ItemNote* note = reinterpret_cast<ItemNote*>(p.ws) + blockIdx.x;
     // rows of waves 1 .. 3 that finish or carry on an item of the wave before them
     __shared__ __attribute__((aligned(16))) f4_t xo[kWaves - 1][NR][DT][64];
-    __shared__ float xs[kWaves - 1][NR][64][2];
+    __shared__ float xs[kWaves - 1][NR][64][LSE ? 3 : 2];
     __shared__ int head_of[kWaves];  // 0: none, 1: it ends in that wave's share, 2: it goes on
 
     // ---- this wave's share [s0, s1) and the item in which it begins ----
@@ -363,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 
     // the item at work: its rows, and their running state
     f4_t o[NR][DT];
-    float m_run[NR], l_run[NR];
+    float m_run[NR], l_run[NR], z_run[NR];  // z_run: LSE, the sum of unrounded weights
     Seq s{};
     uint32_t hk = 0, rt = 0, rows = 0;
     bool open = false, begun = false;  // it goes on in the next wave's share; its first step was here
@@ -378,9 +382,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         for (int q = 0; q < NR; q++) {
             const uint32_t r = 16 * q + j;
             if (r >= rows) continue;
-            if constexpr (TREE) {
+            if constexpr (LSE) {
                 const uint32_t f = rt * R + r;
-                if (g == 0) put_lse(p, s.q0 + (int)(f / G), hk * G + f % G, m_run[q], l_run[q]);
+                if (g == 0) put_lse(p, s.q0 + (int)(f / G), hk * G + f % G, log2_of(m_run[q], z_run[q]));
             }
             _Float16* dst = row_of(p.O, r) + g * RUN;
             const float inv = l_run[q] == 0.0f ? 0.0f : 1.0f / l_run[q];
@@ -399,14 +403,19 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         for (int q = 0; q < NR; q++) {
             const uint32_t r = 16 * q + j;
             if (r >= rows) continue;
+            if constexpr (TREE || LSE) {
+                const float inv = l_run[q] == 0.0f ? 0.0f : 1.0f / l_run[q];
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[q][dt] *= inv;
+            }
 #pragma unroll
             for (int e = 0; e < RUN; e += 4)
                 *reinterpret_cast<f4_t*>(slot + r * D + g * RUN + e) =
                     f4_t{o[q][e % DT][e / DT], o[q][(e + 1) % DT][(e + 1) / DT], o[q][(e + 2) % DT][(e + 2) / DT],
                          o[q][(e + 3) % DT][(e + 3) / DT]};
             if (g == 0) {
-                slot[R * D + r] = m_run[q];
-                slot[R * D + R + r] = l_run[q];
+                slot[R * D + r] = TREE || LSE ? log2_of(m_run[q], l_run[q]) : m_run[q];
+                if (LSE || !TREE) slot[R * D + R + r] = LSE ? log2_of(m_run[q], z_run[q]) : l_run[q];
             }
         }
     };
@@ -457,11 +466,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             lim[q] = last_seen(i);
             low[q] = first_seen(i);
             mask[q] = nullptr;
-            if constexpr (TREE)
-                if (p.tree.mask) {
-                    mask[q] = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
-                    low[q] = first_seen_by(p, s, i);
-                }
+            if constexpr (TREE) {
+                mask[q] = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
+                low[q] = first_seen_by(p, s, i);
+            }
             const _Float16* src = p.Q.p + (int64_t)(s.q0 + i) * p.Q.ts + (int64_t)h * p.Q.hs + g * RUN;
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
@@ -471,18 +479,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         }
         int lim_min = last_seen(i_first), lim_max = last_seen(i_last);
         int low_min = first_seen(i_first), low_max = first_seen(i_last);
-        if constexpr (TREE)
-            if (p.tree.mask) {  // all see the keys before the tree, some may see any of its own
-                lim_min = last_seen(-1);
-                lim_max = last_seen(s.n - 1);
-                low_min = first_seen(0);
-                low_max = first_seen(s.n - 1);
-            }
+        if constexpr (TREE) {  // all see the keys before the tree, some may see any of its own
+            lim_min = last_seen(-1);
+            lim_max = last_seen(s.n - 1);
+            low_min = first_seen(0);
+            low_max = first_seen(s.n - 1);
+        }
 
 #pragma unroll
         for (int q = 0; q < NR; q++) {
             m_run[q] = kNone;
-            l_run[q] = 0.0f;
+            l_run[q] = z_run[q] = 0.0f;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) o[q][dt] = f4_t{};
         }
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                 for (int q = 0; q < NR; q++) {
                     seen32_of[q] = 0xffffffffu;
                     const int w = (key0 - s.first) >> 5;
-                    if (p.tree.mask && key0 + 31 > lim_min) seen32_of[q] = seen32(s, key0, mask_word(p, mask[q], w), mask_word(p, mask[q], w + 1));
+                    if (key0 + 31 > lim_min) seen32_of[q] = seen32(s, key0, mask_word(p, mask[q], w), mask_word(p, mask[q], w + 1));
                 }
             f4_t sc[NR][2];
 #pragma unroll
@@ -552,12 +559,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     if constexpr (TREE) {
 #pragma unroll
                         for (int q = 0; q < NR; q++) {
-                            const int key = key0 + 16 * t + 4 * g;
-                            uint32_t b = 0;
-                            if (tile[t].there && p.tree.mask) b = quad_of(p, s, seen32_of[q], key0, 16 * t + 4 * g, low[q]);
-                            else if (tile[t].there)
-#pragma unroll
-                                for (int r = 0; r < 4; r++) b |= key + r <= lim[q] && key + r >= low[q] ? 1u << r : 0u;
+                            const uint32_t b = tile[t].there ? quad_of(p, s, seen32_of[q], key0, 16 * t + 4 * g, low[q]) : 0u;
                             vis[q] = t == 0 ? b : vis[q] | b << 4;
 #pragma unroll
                             for (int r = 0; r < 4; r++)
@@ -598,6 +600,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                     const float alpha = __builtin_amdgcn_exp2f(m_run[q] - m_new);
                     m_run[q] = m_new;
                     l_run[q] *= alpha;
+                    if constexpr (LSE) z_run[q] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) o[q][dt] *= alpha;
 #pragma unroll
@@ -611,10 +614,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                         const f2_t e = {__builtin_amdgcn_exp2f(ex[4 * t + r]), __builtin_amdgcn_exp2f(ex[4 * t + r + 1])};
                         const h2_t pp = __builtin_convertvector(e, h2_t);
                         pk[2 * t + r / 2] = as_u32(pp);
-                        // TREE: the logarithm of the sum is wanted to fp32, so its terms are not rounded to
-                        // fp16; O is then off by up to 2^-11 more where few keys count
-                        if constexpr (TREE) l_run[q] += e.x + e.y;
-                        else l_run[q] = __builtin_amdgcn_fdot2(pp, one2, l_run[q], false);
+                        l_run[q] = __builtin_amdgcn_fdot2(pp, one2, l_run[q], false);
+                        if constexpr (LSE) z_run[q] += e.x + e.y;
                     }
                 pf[q] = __builtin_bit_cast(h8_t, u4_t{pk[0], pk[1], pk[2], pk[3]});
             }
@@ -677,6 +678,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
         for (int q = 0; q < NR; q++) {
             l_run[q] += __shfl_xor(l_run[q], 16);
             l_run[q] += __shfl_xor(l_run[q], 32);
+            if constexpr (LSE) {
+                z_run[q] += __shfl_xor(z_run[q], 16);
+                z_run[q] += __shfl_xor(z_run[q], 32);
+            }
         }
         const bool ends = u0 + nu == s.steps;
         begun = u0 == 0;
@@ -690,6 +695,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
                 for (int dt = 0; dt < DT; dt++) xo[wave - 1][q][dt][lane] = o[q][dt];
                 xs[wave - 1][q][lane][0] = m_run[q];
                 xs[wave - 1][q][lane][1] = l_run[q];
+                if constexpr (LSE) xs[wave - 1][q][lane][2] = z_run[q];
             }
             if (lane == 0) head_of[wave] = ends ? 1 : 2;
             open = false;  // the wave before gathers it
@@ -711,6 +717,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
             const float fa = __builtin_amdgcn_exp2f(m_run[q] - m), fb = __builtin_amdgcn_exp2f(m2 - m);
             m_run[q] = m;
             l_run[q] = l_run[q] * fa + l2 * fb;
+            if constexpr (LSE) z_run[q] = z_run[q] * fa + xs[v - 1][q][lane][2] * fb;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) o[q][dt] = o[q][dt] * fa + xo[v - 1][q][dt][lane] * fb;
         }
@@ -738,7 +745,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnParams p, u
 // a row; rows side by side while an item has few parts, else the parts of a row
 // are split over the lane groups, whose sums meet in LDS in a fixed order.
 constexpr uint32_t kJoinBlocks = 512;
-template <int D, int R, bool TREE>
+template <int D, int R, bool TREE, bool LSE>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p, uint32_t groups) {
     constexpr int L = D / 4, GROUPS = 256 / L, U = 4;
     __shared__ f4_t part_sum[256];
@@ -775,11 +782,12 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
                 const uint32_t r = r0 + group / split;
                 const bool live = r < rows;
                 // reference points and sums, a lane each part, and the first rows, all under way together
-                float m = kNone, l = 0.0f, mk[U];
+                float m = kNone, l = 0.0f, z = kNone, mk[U];
                 f4_t v[U], o{};
                 if (live && l4 < parts) {
                     m = slot(l4)[R * D + r];
-                    l = slot(l4)[R * D + R + r];
+                    l = TREE || LSE ? 1.0f : slot(l4)[R * D + R + r];
+                    if constexpr (LSE) z = slot(l4)[R * D + R + r];
                 }
 #pragma unroll
                 for (int i = 0; i < U; i++) {
@@ -794,7 +802,12 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
                 if (live)
                     for (uint32_t k = l4 + L; k < parts; k += L) {
                         const float m2 = slot(k)[R * D + r], m_new = fmaxf(m, m2);
-                        l = l * __builtin_amdgcn_exp2f(m - m_new) + slot(k)[R * D + R + r] * __builtin_amdgcn_exp2f(m2 - m_new);
+                        const float l2 = TREE && !LSE ? 0.0f : slot(k)[R * D + R + r];
+                        l = l * __builtin_amdgcn_exp2f(m - m_new) + (TREE || LSE ? 1.0f : l2) * __builtin_amdgcn_exp2f(m2 - m_new);
+                        if constexpr (LSE) {
+                            const float z_new = fmaxf(z, l2);
+                            z = log2_of(z_new, __builtin_amdgcn_exp2f(z - z_new) + __builtin_amdgcn_exp2f(l2 - z_new));
+                        }
                         m = m_new;
                     }
                 const float m_lane = m;
@@ -803,6 +816,12 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
                 l *= __builtin_amdgcn_exp2f(m_lane - m);
 #pragma unroll
                 for (int x = L / 2; x >= 1; x >>= 1) l += __shfl_xor(l, x);
+                if constexpr (LSE) {  // beside the same reference point, of which they are a rounding away
+                    float sum = z == kNone ? 0.0f : __builtin_amdgcn_exp2f(z - m);
+#pragma unroll
+                    for (int x = L / 2; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+                    z = log2_of(m, sum);
+                }
 #pragma unroll
                 for (int i = 0; i < U; i++)
                     if (live && mine0 + i * split < parts) o += v[i] * __builtin_amdgcn_exp2f(mk[i] - m);
@@ -823,8 +842,8 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p,
                 if (live && mine0 == 0) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                     const uint32_t f = first + r;
-                    if constexpr (TREE)
-                        if (l4 == 0) put_lse(p, (int)(q0 + f / G), hk * G + f % G, m, l);
+                    if constexpr (LSE)
+                        if (l4 == 0) put_lse(p, (int)(q0 + f / G), hk * G + f % G, z);
                     _Float16* dst = p.O.p + (int64_t)(q0 + f / G) * p.O.ts + (int64_t)(hk * G + f % G) * p.O.hs;
                     const f2_t a = {o.x * inv, o.y * inv}, b = {o.z * inv, o.w * inv};
                     *reinterpret_cast<u2_t*>(dst + 4 * l4) =
@@ -844,11 +863,10 @@ struct Chunk {
 // Steps (key tiles of KT) of row tile rt, and its first key.
 template <int KT, bool TREE>
 __device__ __forceinline__ uint32_t steps_of(const PagedAttnParams& p, const Seq& s, uint32_t tokens, uint32_t rt, int& lo) {
-    if constexpr (TREE)
-        if (p.tree.mask) {  // any row may see any of the new tokens
-            tokens = (uint32_t)s.n;
-            rt = 0;
-        }
+    if constexpr (TREE) {  // any row may see any of the new tokens
+        tokens = (uint32_t)s.n;
+        rt = 0;
+    }
     const int64_t first = (int64_t)s.first + rt * tokens;
     const int end = (int)min(first + tokens, (int64_t)s.keys);
     lo = p.window ? (int)min(max(first + 1 - (int64_t)p.window, (int64_t)0), (int64_t)s.keys) / KT * KT : 0;
@@ -874,11 +892,13 @@ struct ChunkLds {
 // pipe 47% busy, 7.7 vector operations per MFMA beside it, LDS bank conflicts in 0.12 M
 // of a CU's 1.90 M cycles (V's tile is stored by lanes four rows apart), at 1.8 GHz of 2.4, to
 // which the clock falls under this load.
-template <int FMT, int D, int NW, bool TREE>
+template <int FMT, int D, int NW, bool TREE, bool LSE>
 __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnParams p, uint32_t groups) {
     // a row tile's share beside its steps: with trees, whose last steps ask the mask, more (16 requests of
-    // 64 nodes with 1 / 2 / 3 / 4 / 5, join included: 92 / 84 / 78 / 78 / 78 us)
-    constexpr uint32_t COST = TREE ? 4 : kChunkCost;
+    // 64 nodes with 1 / 2 / 3 / 4 / 5, join included: 92 / 84 / 78 / 78 / 78 us).  Causal calls with lse
+    // with 2 / 3 / 4: four chunks of 512 over 4096 keys 189 / 180 / 177, 512 rows among 31 single tokens
+    // 80 / 78 / 71, a prompt of 2048 95 / 98 / 96, eight of them 425 / 424 / 437
+    constexpr uint32_t COST = TREE || LSE ? 4 : kChunkCost;
     constexpr int R = 32 * NW, KT = 16 * NW, UNITS = KT / 32;
     constexpr int DT = D / 32, KK = D / 16;
     using L = ChunkLds<D, KT>;
@@ -953,7 +973,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
     const h2_t one2 = {(_Float16)1.0f, (_Float16)1.0f};
 
     f16v_t o[DT];
-    float m_run = kNone, l_run = 0.0f;
+    float m_run = kNone, l_run = 0.0f, z_run = 0.0f;  // z_run: LSE, as above
     Seq s{};
     uint64_t row_cost = 0;  // of a KV head of the sequence at work
     uint32_t at_b = 0xffffffffu;
@@ -1001,13 +1021,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         const uint32_t r0 = min(32u * wave, rows - 1), r1 = min(32u * wave + 31, rows - 1);
         int lim0 = last_seen(r0), lim1 = last_seen(r1), low0 = first_seen(r0), low1 = first_seen(r1);
         int all0 = last_seen(0), all_low1 = first_seen(rows - 1);
-        if constexpr (TREE)
-            if (p.tree.mask) {  // all see the keys before the tree, some may see any of its own
-                all0 = lim0 = min(s.first - 1, s.keys - 1);
-                lim1 = s.keys - 1;
-                low0 = p.window ? (int)max((int64_t)s.first + 1 - (int64_t)p.window, (int64_t)0) : 0;
-                all_low1 = low1 = p.window ? (int)max((int64_t)s.first + s.n - (int64_t)p.window, (int64_t)0) : 0;
-            }
+        if constexpr (TREE) {  // all see the keys before the tree, some may see any of its own
+            all0 = lim0 = min(s.first - 1, s.keys - 1);
+            lim1 = s.keys - 1;
+            low0 = p.window ? (int)max((int64_t)s.first + 1 - (int64_t)p.window, (int64_t)0) : 0;
+            all_low1 = low1 = p.window ? (int)max((int64_t)s.first + s.n - (int64_t)p.window, (int64_t)0) : 0;
+        }
         h8_t qf[KK];
         {
             const _Float16* src = p.Q.p + (int64_t)(s.q0 + (int)(rt * tokens + rc / G)) * p.Q.ts +
@@ -1019,7 +1038,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             }
         }
         m_run = kNone;
-        l_run = 0.0f;
+        l_run = z_run = 0.0f;
 #pragma unroll
         for (int t = 0; t < DT; t++) o[t] = f16v_t{};
 
@@ -1102,6 +1121,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
                 m_run = m_new;
                 l_run *= alpha;
+                if constexpr (LSE) z_run *= alpha;
 #pragma unroll
                 for (int t = 0; t < DT; t++) o[t] *= alpha;
 #pragma unroll
@@ -1122,8 +1142,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                 const f2_t w = {__builtin_amdgcn_exp2f(ex[e]), __builtin_amdgcn_exp2f(ex[e + 1])};
                 const h2_t pp = __builtin_convertvector(w, h2_t);
                 pk[e >> 1] = as_u32(pp);
-                if constexpr (TREE) l_run += w.x + w.y;  // not rounded, as above
-                else l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                if constexpr (LSE) z_run += w.x + w.y;
             }
         };
         auto add = [&](const uint8_t* buf, int x, const uint32_t pk[8]) {
@@ -1205,8 +1225,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                         const f2_t w = {__builtin_amdgcn_exp2f(ex[2 * e]), __builtin_amdgcn_exp2f(ex[2 * e + 1])};
                         const h2_t pp = __builtin_convertvector(w, h2_t);
                         pk[e] = as_u32(pp);
-                        if constexpr (TREE) l_run += w.x + w.y;
-                        else l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                        l_run = __builtin_amdgcn_fdot2(pp, one2, l_run, false);
+                        if constexpr (LSE) z_run += w.x + w.y;
                     };
                     __builtin_amdgcn_sched_barrier(0);
                     if (x + 1 < UNITS) {
@@ -1250,16 +1270,15 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             }
             uint32_t words[UNITS + 1];  // TREE: of the row's mask
             int win = low;  // the first position of the row's window
-            if constexpr (TREE)
-                if (p.tree.mask) {
-                    uint32_t row = rc;
-                    asm volatile("" : "+v"(row));  // what follows is formed anew: kept, more registers would spill
-                    const int i = i0 + (int)(row / G);
-                    const uint32_t* mask = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
-                    win = first_seen_by(p, s, i);
+            if constexpr (TREE) {
+                uint32_t row = rc;
+                asm volatile("" : "+v"(row));  // what follows is formed anew: kept, more registers would spill
+                const int i = i0 + (int)(row / G);
+                const uint32_t* mask = p.tree.mask + (size_t)(s.q0 + i) * p.tree.words;
+                win = first_seen_by(p, s, i);
 #pragma unroll
-                    for (int x = 0; x <= UNITS; x++) words[x] = mask_word(p, mask, ((k0 - s.first) >> 5) + x);
-                }
+                for (int x = 0; x <= UNITS; x++) words[x] = mask_word(p, mask, ((k0 - s.first) >> 5) + x);
+            }
             auto unit = [&](int x, bool marks, uint32_t lo_word, uint32_t hi_word) {
                 const int key0 = k0 + 32 * x;
                 if (key0 > lim1 || key0 + 31 < low0) return;
@@ -1271,12 +1290,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                         const uint32_t seen = seen32(s, key0, lo_word, hi_word);
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
-                            const int key = key0 + 8 * y + 4 * g;
                             if (!(there[u & 1][2 * x + (y >> 1)] & 1)) continue;
-                            if (p.tree.mask) vis |= quad_of(p, s, seen, key0, 8 * y + 4 * g, win) << 4 * y;
-                            else
-#pragma unroll
-                                for (int e = 0; e < 4; e++) vis |= key + e <= lim && key + e >= low ? 1u << (4 * y + e) : 0u;
+                            vis |= quad_of(p, s, seen, key0, 8 * y + 4 * g, win) << 4 * y;
                         }
 #pragma unroll
                         for (int e = 0; e < 16; e++)
@@ -1327,11 +1342,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
         }
 
         l_run += __shfl_xor(l_run, 32);
+        if constexpr (LSE) z_run += __shfl_xor(z_run, 32);
         // lane (j, g): row 32 wave + j, dims 32 t + 8 (e / 4) + 4 g + e % 4
         if (begun && ends) {
             if (r < rows) {
-                if constexpr (TREE)
-                    if (g == 0) put_lse(p, s.q0 + (int)(rt * tokens + r / G), hk * G + r % G, m_run, l_run);
+                if constexpr (LSE)
+                    if (g == 0) put_lse(p, s.q0 + (int)(rt * tokens + r / G), hk * G + r % G, log2_of(m_run, z_run));
                 const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
                 _Float16* dst = p.O.p + (int64_t)(s.q0 + (int)(rt * tokens + r / G)) * p.O.ts + (int64_t)(hk * G + r % G) * p.O.hs;
 #pragma unroll
@@ -1345,6 +1361,11 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
             }
         } else {
             float* slot = slot_of<D, R>(p.ws, groups, blockIdx.x, begun ? 1 : 0);
+            if constexpr (TREE || LSE) {
+                const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+#pragma unroll
+                for (int t = 0; t < DT; t++) o[t] *= inv;
+            }
             if (r < rows) {
 #pragma unroll
                 for (int t = 0; t < DT; t++)
@@ -1353,8 +1374,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_attn_chunk_kernel(PagedAttnP
                         *reinterpret_cast<f4_t*>(slot + r * D + 32 * t + 8 * q + 4 * g) =
                             f4_t{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]};
                 if (g == 0) {
-                    slot[R * D + r] = m_run;
-                    slot[R * D + R + r] = l_run;
+                    slot[R * D + r] = TREE || LSE ? log2_of(m_run, l_run) : m_run;
+                    if (LSE || !TREE) slot[R * D + R + r] = LSE ? log2_of(m_run, z_run) : l_run;
                 }
             }
             if (tid == 0) {
@@ -1421,9 +1442,9 @@ size_t paged_attn_workspace(const PagedAttnParams& p) {
 }
 #endif
 
-constexpr bool kTree = QR_PAGED_TREE != 0;
+constexpr bool kTree = QR_PAGED_TREE == 1;
 
-template <int D, int R>
+template <int D, int R, bool LSE>
 static hipError_t launch_join(const PagedAttnParams& p, const WorkPlan& w, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1444,11 +1465,11 @@ static hipError_t launch_join(const PagedAttnParams& p, const WorkPlan& w, hipSt
         while (most < 64 && (most < w.items || most * across < 4 * kJoinBlocks)) most *= 2;
     }
     const dim3 grid(w.groups < most ? w.groups : most, across);
-    hipLaunchKernelGGL((paged_attn_join_kernel<D, R, kTree>), grid, dim3(256), 0, st, p, w.groups);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D, R, kTree, LSE>), grid, dim3(256), 0, st, p, w.groups);
     return hipGetLastError();
 }
 
-template <int FMT, int D>
+template <int FMT, int D, bool LSE>
 static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
     const AttnPlan a = plan_of(p);
     constexpr uint32_t cut = kChunkTile / 2;
@@ -1458,11 +1479,11 @@ static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
         const dim3 grid(a.few.groups), block(64 * kWaves);
         hipError_t e;
         if (a.few.rows == 16) {
-            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1, kTree>), grid, block, 0, st, p, a.few.groups);
-            e = launch_join<D, 16>(p, a.few, st);
+            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1, kTree, LSE>), grid, block, 0, st, p, a.few.groups);
+            e = launch_join<D, 16, LSE>(p, a.few, st);
         } else {
-            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, kTree>), grid, block, 0, st, p, a.few.groups);
-            e = launch_join<D, 32>(p, a.few, st);
+            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, kTree, LSE>), grid, block, 0, st, p, a.few.groups);
+            e = launch_join<D, 32, LSE>(p, a.few, st);
         }
         if (e != hipSuccess) return e;
     }
@@ -1473,20 +1494,25 @@ static hipError_t launch_format(PagedAttnParams p, hipStream_t st) {
     constexpr int NW = kChunkTile / 32;
     constexpr size_t lds = 2 * ChunkLds<D, 16 * NW>::tile;
     static size_t attr[kMaxDevices] = {};  // more than the default 64 KB of LDS
-    const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW, kTree>, lds, attr);
+    const hipError_t e = lds_limit_once((const void*)paged_attn_chunk_kernel<FMT, D, NW, kTree, LSE>, lds, attr);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW, kTree>), dim3(a.many.groups), dim3(64 * NW), lds, st, p, a.many.groups);
-    return launch_join<D, kChunkTile>(p, a.many, st);
+    hipLaunchKernelGGL((paged_attn_chunk_kernel<FMT, D, NW, kTree, LSE>), dim3(a.many.groups), dim3(64 * NW), lds, st, p, a.many.groups);
+    return launch_join<D, kChunkTile, LSE>(p, a.many, st);
 }
 
-#if QR_PAGED_TREE
-hipError_t launch_paged_attn_tree(const PagedAttnParams& p, hipStream_t st) {
-#else
-hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) {
-#endif
+template <bool LSE>
+static hipError_t launch(const PagedAttnParams& p, hipStream_t st) {
     if (p.batch.B == 0 || p.batch.T == 0) return hipSuccess;
-    if (p.format == QUANT_Q8_0) return p.D == 64 ? launch_format<QUANT_Q8_0, 64>(p, st) : launch_format<QUANT_Q8_0, 128>(p, st);
-    return p.D == 64 ? launch_format<QUANT_Q4_0, 64>(p, st) : launch_format<QUANT_Q4_0, 128>(p, st);
+    if (p.format == QUANT_Q8_0) return p.D == 64 ? launch_format<QUANT_Q8_0, 64, LSE>(p, st) : launch_format<QUANT_Q8_0, 128, LSE>(p, st);
+    return p.D == 64 ? launch_format<QUANT_Q4_0, 64, LSE>(p, st) : launch_format<QUANT_Q4_0, 128, LSE>(p, st);
 }
+
+#if QR_PAGED_TREE == 1
+hipError_t launch_paged_attn_tree(const PagedAttnParams& p, hipStream_t st) { return p.lse.p ? launch<true>(p, st) : launch<false>(p, st); }
+#elif QR_PAGED_TREE == 2
+hipError_t launch_paged_attn_lse(const PagedAttnParams& p, hipStream_t st) { return launch<true>(p, st); }
+#else
+hipError_t launch_paged_attn(const PagedAttnParams& p, hipStream_t st) { return launch<false>(p, st); }
+#endif
 
 }  // namespace qr

@@ -352,6 +352,48 @@ def test_masks_and_positions_out_of_range(bridge, fmt, kernels):
             close(O[:, a:a + n].cpu().numpy(), o, ob, f"sequence {b}, window {window}")
 
 
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,new,kernels", [
+    ([40, 9, 33], [5, 9, 1], "rows"), ([900, 333, 2000], [40, 3, 16], "rows"), ([300, 65, 900], [40, 60, 90], "chunks"),
+    ([2300, 65, 900], [40, 3, 90], "both")])
+def test_weights_of_a_row_are_one_together(bridge, fmt, D, lens, new, kernels):
+    """Where all keys of a sequence have one value, that is the result, to the last bit, whatever the weights: what O is
+    divided by is the sum of the weights as the product with V took them.  fp32 sums are off by (keys + 8) 2^-24 at most,
+    2^-12.8, which is less than half a step of any fp16 value, 2^-12 of it or more, so O's rounding takes it back."""
+    import torch
+
+    H, Hkv, P = 16, 2, 16
+    s = Trees(fmt, lens, new, Hkv, D, P, seed=len(lens) + D + sum(new))
+    tree = s.masks("any")
+    value = np.zeros((H, s.T, D), np.float16)
+    for b, (L, n, a) in enumerate(zip(lens, new, s.q_start)):
+        v = (s.rng.integers(1, 8, (Hkv, D)) * 0.25).astype(np.float16)  # 0.25 .. 1.75
+        k = half(s.rng, L, Hkv, D)
+        (kq, kd), (vq, vd) = ref.quantize(fmt, k), ref.quantize(fmt, v)
+        held = ref.values(vq, vd)
+        s.v[b] = np.repeat(held[:, None], L, 1)
+        s.k[b] = ref.values(kq, kd).transpose(1, 0, 2)
+        for p in range(L):
+            s.pages.write(s.table[b, p // P], p % P, kq[p], kd[p], vq, vd)
+        value[:, a:a + n] = np.repeat(held, H // Hkv, 0)[:, None]
+    q = (3 * half(s.rng, H, s.T, D)).astype(np.float16)
+    cache = s.cache()
+    batch = m4_bridge.KVBatch(dev(s.q_start), dev(np.array(lens, np.int32)), dev(s.table), **KERNELS[kernels])
+    for kw in ({}, {"lse": torch.empty(H, s.T, device="cuda")}, {"tree": tree}, {"tree": tree, "lse": torch.empty(H, s.T, device="cuda")}):
+        O = torch.full((H, s.T, D), 6.0, dtype=torch.float16, device="cuda")
+        say("one together", fmt, D, lens, new, kernels, sorted(kw))
+        bridge.dispatch_paged_attn(cache, batch, dev(q), O, D ** -0.5, **kw)
+        bridge.synchronize()
+        want = value.copy()
+        if "tree" in kw:  # rows that see nothing
+            for b, (L, n, a) in enumerate(zip(lens, new, s.q_start)):
+                if L == n:
+                    want[:, a:a + n][:, s.bits[b].sum(-1) == 0] = 0
+        np.testing.assert_array_equal(O.cpu().numpy(), want)
+
+
 # ---- the accepted path ----------------------------------------------------------------------------------------------
 
 @gpu
