@@ -444,7 +444,8 @@ M4_API int m4_bridge_kv_cache_weigh(const m4_kv_cache_t* cache, const m4_kv_batc
  * pages stay as they are, also where sequences share them; those of table_out are
  * others, and no two alike.  Heads keep keys of their own, so a place no longer
  * stands for a position: what is appended next takes explicit positions, and a
- * window counts places.  Keys on pages that are not there count as gone;
+ * window counts places.  Those of m4_bridge_draft_tree are formed from kv_len, so they are
+ * places then: attention takes them as they are, an append with what was evicted added.  Keys on pages that are not there count as gone;
  * kept ones whose new page is not there are not copied.  q_start is not read (but
  * not NULL). */
 M4_API int m4_bridge_kv_cache_evict(const m4_kv_cache_t* cache, const m4_kv_batch_t* batch, float* sums, size_t sums_bytes,

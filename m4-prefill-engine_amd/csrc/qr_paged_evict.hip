@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(256, 2) weigh_rows_kernel(WeighParams p) {
 // touch 64 lines a load; a row's address by division and 64-bit products cost as much as a
 // tile's weights, so all offsets are formed once); their sums meet in LDS.  A tile's products run
 // beside the exponentials of the one before.  8 heads, 2048 rows of 32 query heads on 30000 keys of
-// 128: 535 us, 0.91 PFLOP/s.  By itself that loop takes 350 cycles a tile of 32 x 32 (256 of products,
+// 128: 540 us, 0.90 PFLOP/s.  By itself that loop takes 350 cycles a tile of 32 x 32 (256 of products,
 // 256 of fused multiplies, exponentials and sums, at 1.65 GHz under this load), 390 us; bringing
 // the rows (3.8 GB through the L2s) costs 100 more.  Eight waves of D = 64 are held to the 128
 // registers with which two workgroups fit a CU.
